@@ -49,6 +49,7 @@ extern "C" {
 /* ---- device status word bits (set by kernels, read by the host) -------- */
 #define BIO_DEV_TIMEOUT 1     /* a bounded mbarrier wait gave up             */
 #define BIO_DEV_INDEX 2       /* an index operand was out of range           */
+#define BIO_DEV_PAGES 4       /* a page pool had too few free pages          */
 
 /* ---- dtypes ------------------------------------------------------------ */
 #define BIO_F32 0
@@ -374,6 +375,150 @@ BIO_API int bio_attention(const bio_attn_args* args, void* stream);
  * varlen_scaled_dot_product_attention_batch_invariant
  * (batch_invariant_ops.py:1216-1344). */
 BIO_API int bio_attention_varlen(const bio_attn_args* args, void* stream);
+
+/* Prefill attention with a sliding window and sink tokens.  Query i sits at
+ * position p = i + (lk - lq) (the last query at the last key); it sees key j
+ * iff j <= p and (j > p - window or j < sinks).  window >= 1, sinks >= 0.
+ * Rows that see no key produce zeros.  Operands, strides, grouped-query
+ * sharing, alignment and batch invariance as bio_attention (causal and mask
+ * fields must be 0); work grows with lq * (window + sinks), not lq * lk.  Keys
+ * and values that a row does not see never reach it, whatever they hold.  No
+ * counterpart in the reference (its SDPA, batch_invariant_ops.py:1148-1213,
+ * would need the mask as a tensor and visits every key). */
+BIO_API int bio_attention_window(const bio_attn_args* args, int64_t window, int64_t sinks,
+                                 void* stream);
+
+/* The same over packed sequences (cu_q / cu_k as in bio_attention_varlen, no
+ * workspace): sequence s aligns its last query to its last key.  Query tokens
+ * outside every sequence, and the rows of sequences with invalid offsets
+ * (BIO_DEV_INDEX), are left as they are: the caller zeroes o first. */
+BIO_API int bio_attention_window_varlen(const bio_attn_args* args, int64_t window, int64_t sinks,
+                                        void* stream);
+
+/* ---- paged key/value cache ------------------------------------------------
+ * A pool holds `pages` pages of page_size tokens for each of `layers` layers:
+ * K element (layer, page, head, slot, c) at k + layer*k_sl + page*k_sp +
+ * head*k_sh + slot*k_st + c, V alike with dv columns.  A table maps sequences
+ * to pages: token t of row r lives in page page_table[r*t_sr + t/page_size],
+ * slot t % page_size; -1 marks "no page".  ref_counts[page] counts the table
+ * entries that hold the page (0 = free); seq_lens[r] is the row's length.
+ * Everything lives on the device and is updated there, without a host
+ * synchronisation.  No counterpart in the reference, which keeps no cache. */
+typedef struct bio_kv_pool {
+  int32_t dtype, device;
+  void* k;
+  void* v;
+  int64_t layers, pages, kv_heads, page_size;
+  int64_t k_sl, k_sp, k_sh, k_st;
+  int64_t v_sl, v_sp, v_sh, v_st;
+  int64_t d, dv;
+} bio_kv_pool;
+
+typedef struct bio_kv_table {
+  int32_t* page_table;
+  int64_t t_sr;        /* elements between rows of page_table               */
+  int64_t rows, width; /* sequences, pages per sequence at most             */
+  int32_t* seq_lens;   /* [rows]; not used by append and compact            */
+  int32_t* ref_counts; /* [pages]; not used by append                       */
+  int64_t pages, page_size;
+  int32_t device, pad;
+} bio_kv_table;
+
+/* Writes tokens' keys and values into their pages: token t (k + t*k_st +
+ * h*k_sh, v alike) goes to position positions[t] of row rows[t].  A negative
+ * position is skipped; a row, position or page out of range raises
+ * BIO_DEV_INDEX and is skipped.  pool->layers must be 1.  Two tokens for one
+ * place leave either. */
+BIO_API int bio_kv_append(const bio_kv_pool* pool, const bio_kv_table* table, const void* k,
+                          int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                          const int32_t* rows, const int32_t* positions, int64_t tokens,
+                          void* stream);
+
+/* Bytes of device workspace (4-byte aligned) for the calls below on n rows of
+ * a table over `pages` pages. */
+BIO_API int64_t bio_kv_workspace(int64_t n, int64_t pages);
+
+/* Grows row rows[i] to new_lens[i] tokens: it takes the lowest free pages (in
+ * the order of i, then of the row's columns), whose counts become 1.  A length
+ * that is not larger leaves the row as it is.  Rows that are out of range or
+ * repeated, and lengths beyond the table's width, raise BIO_DEV_INDEX and are
+ * skipped; when the pool runs out (BIO_DEV_PAGES) a row ends with the pages
+ * that it got. */
+BIO_API int bio_kv_extend(const bio_kv_table* table, const int32_t* rows, const int32_t* new_lens,
+                          int64_t n, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Releases the pages of rows[0..n): counts go down by one, entries become -1,
+ * lengths 0. */
+BIO_API int bio_kv_free(const bio_kv_table* table, const int32_t* rows, int64_t n, void* stream);
+
+/* Releases the pages of rows[0..n) that lie wholly outside the sinks and the
+ * window of the row's newest token (token t with t >= sinks and t < len -
+ * window): such entries become -1; bio_paged_attention with this window and
+ * these sinks never reads them.  Lengths stay. */
+BIO_API int bio_kv_evict(const bio_kv_table* table, const int32_t* rows, int64_t n, int64_t window,
+                         int64_t sinks, void* stream);
+
+/* Branches row dst[i] off row src[i]: what dst[i] held is released, whole
+ * pages are shared (counts up by one), the tokens of a last partial page are
+ * copied, for every layer, into the lowest free page (in the order of i), and
+ * the length is taken over.  Rows out of range, rows that appear twice in dst
+ * or in both lists, raise BIO_DEV_INDEX and are skipped; without a free page
+ * (BIO_DEV_PAGES) the branch ends at the last whole page. */
+BIO_API int bio_kv_fork(const bio_kv_pool* pool, const bio_kv_table* table, const int32_t* src,
+                        const int32_t* dst, int64_t n, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+
+/* Copies the pages in use (count > 0) to the front of another pool, in the
+ * order of their numbers, and writes the table and the counts that go with
+ * them (entries without a page -1, counts of unused pages 0).  The pools
+ * agree in everything but their strides and number of pages and must not
+ * overlap; the tables agree in rows and width.  Pages that the other pool has
+ * no room for are dropped (BIO_DEV_PAGES). */
+BIO_API int bio_kv_compact(const bio_kv_pool* pool, const bio_kv_table* table,
+                           const bio_kv_pool* out_pool, const bio_kv_table* out_table,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of one new token per sequence over a paged cache (one layer).
+ * Query b [heads][d] attends to the first seq_lens[r] tokens of row r = rows[b]
+ * (r = b without rows); with window > 0 only to tokens j with j >= len -
+ * window or j < sinks.  Output [batch][heads][dv].  Rows of length 0 give
+ * zeros.  Rows, lengths or page numbers out of range raise BIO_DEV_INDEX and
+ * give zeros.  Slots beyond the length and tokens outside the window never
+ * reach the result, whatever they hold.
+ *
+ * Split: the n visible tokens of a row are cut into pieces whose size is a
+ * function of n alone; each piece gives a maximum, a sum and an unnormalised
+ * output in fp32, which are joined in the order of the pieces.  A row's bits
+ * therefore depend on its own length and values only.  d, dv <= 256; strides
+ * in elements, the innermost dimension contiguous. */
+typedef struct bio_paged_attn_args {
+  int32_t dtype, device;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  int64_t q_sb, q_sh;
+  int64_t k_sp, k_sh, k_st;
+  int64_t v_sp, v_sh, v_st;
+  int64_t o_sb, o_sh;
+  int64_t batch, heads, kv_heads;
+  int64_t pages, page_size;
+  const int32_t* page_table;
+  int64_t t_sr, table_rows, table_width;
+  const int32_t* seq_lens; /* [table_rows]                       */
+  const int32_t* rows;     /* [batch], or NULL                   */
+  int64_t window, sinks;   /* window 0: every token is visible   */
+  int32_t d, dv;
+  float scale;
+  int32_t pad;
+} bio_paged_attn_args;
+
+/* Workspace bytes that bio_paged_attention needs for these sizes (pure; the
+ * pointers are not looked at).  The workspace is 16-byte aligned device
+ * memory; it may be NULL when 0 bytes are needed. */
+BIO_API int64_t bio_paged_attention_workspace(const bio_paged_attn_args* args);
+BIO_API int bio_paged_attention(const bio_paged_attn_args* args, void* workspace,
+                                int64_t workspace_bytes, void* stream);
 
 /* ---- mixture of experts ---------------------------------------------------
  * The expert GEMMs themselves run through bio_gemm (one fixed-schedule GEMM

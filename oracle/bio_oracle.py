@@ -10,7 +10,9 @@ citations are ``file:line`` into that project).  It is imported only by
 Parity is pinned: ``tests/test_oracle_golden.py`` checks every function here
 against golden vectors produced by running the reference itself (its Triton
 kernels under ``TRITON_INTERPRET=1``, its CPU MoE branch) with
-``tests/golden/make_golden.py``.
+``tests/golden/make_golden.py``.  The paged cache at the end has no
+counterpart there; ``tests/test_paged_cpu.py`` checks it against dense
+attention.
 
 All functions take and return torch tensors; inputs of any dtype/device are
 copied to CPU float64 first.  Outputs are float64 (callers compare against
@@ -373,3 +375,134 @@ def topk_routing(logits, k):
     order = torch.argsort(-l64, dim=-1, stable=True)[:, :k]
     vals = torch.gather(l64, 1, order)
     return torch.softmax(vals, dim=-1), order
+
+
+# ---------------------------------------------------------------------------
+# Paged key/value cache and the attentions around it (no counterpart in the
+# reference): float64, one row at a time, invisible keys never touched
+# ---------------------------------------------------------------------------
+def visible_keys(position: int, window: int | None, sinks: int) -> torch.Tensor:
+    """Keys that the query at ``position`` sees, in order."""
+    keys = torch.arange(max(position + 1, 0))
+    if window is None:
+        return keys
+    return keys[(keys > position - window) | (keys < sinks)]
+
+
+def _attend_row(q, k, v, scale):
+    """q [H, D], k [n, Hkv, D], v [n, Hkv, Dv] -> [H, Dv]; no key gives zeros."""
+    h, hk = q.shape[0], k.shape[1]
+    if k.shape[0] == 0:
+        return torch.zeros(h, v.shape[2], dtype=torch.float64)
+    s = torch.einsum("gad,ngd->gan", q.view(hk, h // hk, -1), k) * scale
+    return torch.einsum("gan,ngd->gad", torch.softmax(s, -1), v).reshape(h, -1)
+
+
+def paged_attention(q, k_pages, v_pages, table, lens, window=None, sinks=0, scale=None, rows=None):
+    """One new token per row over a paged cache (paged_attention_decode_batch_invariant)."""
+    q, k_pages, v_pages = (t.double().cpu() for t in (q, k_pages, v_pages))
+    table, lens = table.long().cpu(), lens.tolist()
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    page = k_pages.shape[2]
+    out = []
+    for b, r in enumerate(rows.tolist() if rows is not None else range(q.shape[0])):
+        keys = visible_keys(lens[r] - 1, window, sinks)
+        at, slot = table[r, keys // page], keys % page
+        out.append(_attend_row(q[b], k_pages[at, :, slot], v_pages[at, :, slot], scale))
+    return torch.stack(out)
+
+
+def window_attention(q, k, v, window, sinks=0, scale=None):
+    """q [B, H, Lq, D], k/v [B, Hkv, Lk, D|Dv] (sliding_window_attention_batch_invariant)."""
+    q, k, v = (t.double().cpu() for t in (q, k, v))
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    b, h, lq, _ = q.shape
+    out = torch.zeros(b, h, lq, v.shape[-1], dtype=torch.float64)
+    for i in range(lq):
+        keys = visible_keys(i + k.shape[2] - lq, window, sinks)
+        for j in range(b):
+            out[j, :, i] = _attend_row(q[j, :, i], k[j, :, keys].transpose(0, 1),
+                                       v[j, :, keys].transpose(0, 1), scale)
+    return out
+
+
+class PageBook:
+    """The bookkeeping of a paged cache on plain lists: what
+    paged_kv_extend/free/evict/fork/compact must reproduce exactly, and the
+    token moves of a fork and of a compaction."""
+
+    def __init__(self, table, lens, refs, page_size):
+        self.table, self.lens, self.refs = table.tolist(), lens.tolist(), refs.tolist()
+        self.page = page_size
+
+    def _take(self):
+        for p, n in enumerate(self.refs):
+            if n == 0:
+                self.refs[p] = 1
+                return p
+        return None
+
+    def _release(self, r, c):
+        if self.table[r][c] >= 0:
+            self.refs[self.table[r][c]] -= 1
+        self.table[r][c] = -1
+
+    def extend(self, rows, new_lens):
+        for r, n in zip(rows, new_lens):
+            have = -(-self.lens[r] // self.page)
+            for c in range(have, -(-n // self.page)):
+                p = self._take()
+                if p is None:
+                    n = min(n, c * self.page)
+                    break
+                self.table[r][c] = p
+            self.lens[r] = max(self.lens[r], n)
+
+    def free(self, rows):
+        for r in rows:
+            for c in range(len(self.table[r])):
+                self._release(r, c)
+            self.lens[r] = 0
+
+    def evict(self, rows, window, sinks):
+        for r in rows:
+            for c in range(len(self.table[r])):
+                if c * self.page >= sinks and (c + 1) * self.page <= self.lens[r] - window:
+                    self._release(r, c)
+
+    def fork(self, src, dst):
+        """Returns the copies: (from page, to page, tokens)."""
+        copies = []
+        for d in dst:
+            for c in range(len(self.table[d])):
+                self._release(d, c)
+        for s, d in zip(src, dst):
+            full = self.lens[s] // self.page
+            for c in range(full):
+                self.table[d][c] = self.table[s][c]
+                if self.table[s][c] >= 0:
+                    self.refs[self.table[s][c]] += 1
+        for s, d in zip(src, dst):
+            full, part = divmod(self.lens[s], self.page)
+            self.lens[d] = self.lens[s]
+            if part:
+                p = self._take()
+                if p is None:
+                    self.lens[d] = full * self.page
+                else:
+                    self.table[d][full] = p
+                    copies.append((self.table[s][full], p, part))
+        return copies
+
+    def compact(self, pages):
+        """Returns the pages that move, in their new order."""
+        live = [p for p, n in enumerate(self.refs) if n > 0]
+        new = {p: i for i, p in enumerate(live) if i < pages}
+        self.table = [[new.get(p, -1) for p in row] for row in self.table]
+        self.refs = [self.refs[p] for p in live[:pages]] + [0] * (pages - len(live[:pages]))
+        return live[:pages]
+
+    def state(self):
+        return (torch.tensor(self.table, dtype=torch.int32),
+                torch.tensor(self.lens, dtype=torch.int32),
+                torch.tensor(self.refs, dtype=torch.int32))

@@ -28,10 +28,22 @@ from .batch_invariant_ops import (
     rms_norm_batch_invariant,
     scaled_dot_product_attention_batch_invariant,
     set_batch_invariant_mode,
+    sliding_window_attention_batch_invariant,
     softmax,
     varlen_scaled_dot_product_attention_batch_invariant,
+    varlen_sliding_window_attention_batch_invariant,
 )
 from .moe import deterministic_token_choice_moe
+from .paged import (
+    PagedKVCache,
+    paged_attention_decode_batch_invariant,
+    paged_kv_append,
+    paged_kv_compact,
+    paged_kv_evict,
+    paged_kv_extend,
+    paged_kv_fork,
+    paged_kv_free,
+)
 
 __version__ = "0.2.0"
 
@@ -63,4 +75,15 @@ __all__ = [
     "rms_norm_batch_invariant",
     "gated_linear_batch_invariant",
     "linear_residual_batch_invariant",
+    # a paged key/value cache and the attention that fills and reads it
+    "sliding_window_attention_batch_invariant",
+    "varlen_sliding_window_attention_batch_invariant",
+    "paged_attention_decode_batch_invariant",
+    "PagedKVCache",
+    "paged_kv_append",
+    "paged_kv_extend",
+    "paged_kv_fork",
+    "paged_kv_free",
+    "paged_kv_evict",
+    "paged_kv_compact",
 ]

@@ -216,3 +216,71 @@ def varlen(q, k, v, cu_q, cu_k, *, is_causal, causal_name, scale):
         _lib.load().bio_attention_varlen(ctypes.byref(a), _lib.stream_of(q)), "bio_attention_varlen"
     )
     return out
+
+
+def _window_args(q, k, v, out, q_s, k_s, v_s, o_s, batch, heads, kv_heads, lq, lk, scale):
+    a = _AttnArgs()
+    a.dtype = _lib.DTYPE_CODE[q.dtype]
+    a.device = q.device.index
+    a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.q_sb, a.q_sh, a.q_st = q_s
+    a.k_sb, a.k_sh, a.k_st = k_s
+    a.v_sb, a.v_sh, a.v_st = v_s
+    a.o_sb, a.o_sh, a.o_st = o_s
+    a.batch, a.heads, a.kv_heads = batch, heads, kv_heads
+    a.lq, a.lk, a.d, a.dv = lq, lk, q.shape[-1], v.shape[-1]
+    a.scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    return a
+
+
+def window(q, k, v, window, sinks, scale):
+    """q [..., H, Lq, D], k [..., Hkv, Lk, D], v [..., Hkv, Lk, Dv] -> [..., H, Lq, Dv]."""
+    lead = q.shape[:-3]
+    h, lq, d = q.shape[-3:]
+    hkv, lk, dv = k.shape[-3], k.shape[-2], v.shape[-1]
+    nb = math.prod(lead)
+    q4 = _dim_contiguous(q.reshape(nb, h, lq, d))
+    k4 = _dim_contiguous(k.reshape(nb, hkv, lk, d))
+    v4 = _dim_contiguous(v.reshape(nb, hkv, lk, dv))
+    # token-major like the output of sdpa
+    out = torch.empty((nb, lq, h, dv), device=q.device, dtype=q.dtype).transpose(1, 2)
+    if out.numel() == 0:
+        return out.reshape(*lead, h, lq, dv)
+    a = _window_args(q4, k4, v4, out, q4.stride()[:3], k4.stride()[:3], v4.stride()[:3],
+                     out.stride()[:3], nb, h, hkv, lq, lk, scale)
+    seen = min(lk, window + sinks)
+    with tracing.span("window_attention", f"bio_attention_window [B={nb}, H={h}/{hkv}, Lq={lq}, "
+                      f"Lk={lk}, D={d}/{dv}, window={window}, sinks={sinks}]",
+                      2.0 * nb * h * lq * seen * (d + dv),
+                      q.element_size() * (q4.numel() + k4.numel() + v4.numel() + out.numel()),
+                      q.element_size()):
+        _lib.check(_lib.load().bio_attention_window(ctypes.byref(a), window, sinks,
+                                                    _lib.stream_of(q)), "bio_attention_window")
+    return out.reshape(*lead, h, lq, dv)
+
+
+def window_varlen(q, k, v, cu_q, cu_k, window, sinks, scale):
+    """Packed q [1, Tq, H, D], k/v [1, Tk, Hkv, D|Dv] -> [1, Tq, H, Dv]."""
+    _, tq, h, _ = q.shape
+    _, tk, hkv, _ = k.shape
+    dv = v.shape[3]
+    q3, k3, v3 = _dim_contiguous(q[0]), _dim_contiguous(k[0]), _dim_contiguous(v[0])
+    out = torch.zeros((1, tq, h, dv), device=q.device, dtype=q.dtype)
+    if out.numel() == 0 or cu_q.numel() == 1:
+        return out
+    cu_k = cu_k.to(cu_q.dtype) if cu_k.dtype != cu_q.dtype else cu_k
+    cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+    by_token = lambda t: (0, t.stride(1), t.stride(0))  # noqa: E731
+    a = _window_args(q3, k3, v3, out, by_token(q3), by_token(k3), by_token(v3), by_token(out[0]),
+                     1, h, hkv, tq, tk, scale)
+    a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    a.cu_is64 = 1 if cu_q.dtype == torch.int64 else 0
+    a.nseq = cu_q.numel() - 1
+    with tracing.span("window_attention", f"bio_attention_window_varlen [T={tq}/{tk}, H={h}/{hkv}, "
+                      f"window={window}, sinks={sinks}]", 0,
+                      q.element_size() * (q3.numel() + k3.numel() + v3.numel() + out.numel()),
+                      q.element_size()):
+        _lib.check(_lib.load().bio_attention_window_varlen(ctypes.byref(a), window, sinks,
+                                                           _lib.stream_of(q)),
+                   "bio_attention_window_varlen")
+    return out

@@ -32,6 +32,7 @@ NOALLOC_SCRATCH_BYTES = 32 << 20
 
 BIO_DEV_TIMEOUT = 1
 BIO_DEV_INDEX = 2
+BIO_DEV_PAGES = 4
 
 BIO_GEMM_BIAS_PER_ROW = 1
 BIO_GEMM_GATE_GELU_TANH = 2
@@ -119,6 +120,19 @@ SIGNATURES: dict[str, tuple] = {
     "bio_conv_transpose_scatter": (ctypes.c_int, [_I32, _P, _P, _P, _P, _I64, _I32, _P]),
     "bio_attention": (ctypes.c_int, [_P, _P]),
     "bio_attention_varlen": (ctypes.c_int, [_P, _P]),
+    "bio_attention_window": (ctypes.c_int, [_P, _I64, _I64, _P]),
+    "bio_attention_window_varlen": (ctypes.c_int, [_P, _I64, _I64, _P]),
+    "bio_kv_append": (
+        ctypes.c_int, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P],
+    ),
+    "bio_kv_workspace": (_I64, [_I64, _I64]),
+    "bio_kv_extend": (ctypes.c_int, [_P, _P, _P, _I64, _P, _I64, _P]),
+    "bio_kv_free": (ctypes.c_int, [_P, _P, _I64, _P]),
+    "bio_kv_evict": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _P]),
+    "bio_kv_fork": (ctypes.c_int, [_P, _P, _P, _P, _I64, _P, _I64, _P]),
+    "bio_kv_compact": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _P]),
+    "bio_paged_attention_workspace": (_I64, [_P]),
+    "bio_paged_attention": (ctypes.c_int, [_P, _P, _I64, _P]),
     "bio_silu_mul": (ctypes.c_int, [_I32, _P, _P, _P, _I64, _I32, _P]),
     "bio_moe_route_sum": (
         ctypes.c_int,

@@ -418,6 +418,95 @@ def varlen_scaled_dot_product_attention_batch_invariant(
 
 
 # ---------------------------------------------------------------------------
+# Sliding-window attention (not in the reference)
+# ---------------------------------------------------------------------------
+def _check_window(query, key, value, window, sinks, heads_dim, tokens_dim):
+    if query.dtype != key.dtype or query.dtype != value.dtype:
+        raise ValueError("query, key, and value must have the same dtype")
+    if query.dtype not in _FLOAT_TYPES:
+        raise ValueError(f"unsupported sliding-window attention dtype: {query.dtype}")
+    if key.shape[heads_dim] != value.shape[heads_dim] or (
+            key.shape[tokens_dim] != value.shape[tokens_dim]):
+        raise ValueError("key and value token and head dimensions must match")
+    if query.shape[-1] != key.shape[-1]:
+        raise ValueError("query and key head dimensions must match")
+    if query.shape[-1] == 0 or value.shape[-1] == 0:
+        raise ValueError("head dimensions must not be zero")
+    if key.shape[heads_dim] == 0 or query.shape[heads_dim] % key.shape[heads_dim]:
+        raise ValueError("query heads must be divisible by key/value heads")
+    if not 1 <= window <= 2147483647:
+        raise ValueError("window must be at least 1 and fit in 32 bits")
+    if not 0 <= sinks <= 2147483647:
+        raise ValueError("sinks must not be negative and fit in 32 bits")
+    _attn._check_head_dims(query.shape[-1], value.shape[-1])
+
+
+def sliding_window_attention_batch_invariant(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    window: int,
+    sinks: int = 0,
+    *,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """Causal attention with a sliding window and sink tokens.
+
+    ``query [..., H, Lq, D]``, ``key [..., Hkv, Lk, D]``, ``value [..., Hkv, Lk,
+    Dv]`` with H a multiple of Hkv.  The queries are the last Lq of Lk tokens
+    (a whole prompt, or a chunk behind tokens already cached): query i at
+    position p = i + Lk - Lq sees key j iff j <= p and (j > p - window or
+    j < sinks).  Rows that see no key give zeros; keys that a row does not see
+    never reach it, whatever they hold.  The work grows with Lq * (window +
+    sinks).  A row's bits depend on its own query, keys and values only.  An
+    addition: the reference's SDPA (:1148-1213) would need the mask as a tensor
+    and visits every key."""
+    if query.ndim < 3 or key.ndim != query.ndim or value.ndim != query.ndim:
+        raise ValueError("query, key, and value must be [..., heads, tokens, head_dim]")
+    if query.shape[:-3] != key.shape[:-3] or query.shape[:-3] != value.shape[:-3]:
+        raise ValueError("query, key, and value batch dimensions must match")
+    _check_window(query, key, value, window, sinks, -3, -2)
+    _require_cuda(query, key, value)
+    return _attn.window(query, key, value, window, sinks, scale)
+
+
+def varlen_sliding_window_attention_batch_invariant(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    cumulative_seqlen_q: torch.Tensor,
+    cumulative_seqlen_kv: torch.Tensor,
+    window: int,
+    sinks: int = 0,
+    *,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """``sliding_window_attention_batch_invariant`` over sequence-packed
+    ``[1, T, H, D]`` inputs (prompts of different lengths): each sequence is
+    evaluated by itself, its last query at its last key.  Offsets are read on
+    the device; tokens outside every sequence, and sequences with invalid
+    offsets (``BIO_DEV_INDEX``), give zeros."""
+    if query.ndim != 4 or key.ndim != 4 or value.ndim != 4:
+        raise ValueError("varlen attention expects rank-4 query, key, and value")
+    if query.shape[0] != 1 or key.shape[0] != 1 or value.shape[0] != 1:
+        raise ValueError("varlen attention expects sequence-packed batch size 1")
+    _check_window(query, key, value, window, sinks, 2, 1)
+    if cumulative_seqlen_q.ndim != 1 or cumulative_seqlen_kv.ndim != 1:
+        raise ValueError("cumulative sequence lengths must be rank 1")
+    integer_dtypes = {torch.int32, torch.int64}
+    if (cumulative_seqlen_q.dtype not in integer_dtypes
+            or cumulative_seqlen_kv.dtype not in integer_dtypes):
+        raise ValueError("cumulative sequence lengths must use int32 or int64")
+    if cumulative_seqlen_q.numel() != cumulative_seqlen_kv.numel():
+        raise ValueError("query and KV cumulative sequence counts must match")
+    if cumulative_seqlen_q.numel() == 0:
+        raise ValueError("cumulative sequence lengths must start at zero")
+    _require_cuda(query, key, value, cumulative_seqlen_q, cumulative_seqlen_kv)
+    return _attn.window_varlen(query, key, value, cumulative_seqlen_q, cumulative_seqlen_kv,
+                               window, sinks, scale)
+
+
+# ---------------------------------------------------------------------------
 # Reductions (reference :1347-1597, :1633-1651)
 # ---------------------------------------------------------------------------
 def mean_dim(

@@ -1,0 +1,724 @@
+// Pages of a key/value cache: writing new tokens, growing, freeing and
+// branching sequences, and moving the pages in use into another pool.
+//
+// All of it is data movement and integer bookkeeping on the device (page
+// table, lengths, reference counts), with no host synchronisation.  Page
+// numbers never depend on the order in which threads run: reference counts
+// change by integer atomics, which commute, and free pages are handed out in
+// the order of their numbers by one block that scans the counts.
+//
+// Not in the reference, which keeps no cache between calls.
+#include "bio_common.cuh"
+
+namespace bio {
+
+struct KvPool {
+  char* k;
+  char* v;
+  int64_t layers, pages;
+  int heads, page_size;
+  int64_t k_sl, k_sp, k_sh, k_st;  // bytes
+  int64_t v_sl, v_sp, v_sh, v_st;
+  int k_row, v_row;                // bytes of one token of one head
+};
+
+struct KvTable {
+  int32_t* table;
+  int64_t t_sr;
+  int64_t rows, width;
+  int32_t* lens;
+  int32_t* refs;
+  int64_t pages;
+  int page_size;
+  int* status;
+};
+
+// A later kernel of a chain starts while the one before it drains, and waits
+// here until that one's writes are visible.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_start_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ bool in_pool(int page, int64_t pages) {
+  return page >= 0 && page < pages;
+}
+
+// ---------------------------------------------------------------------------
+// append: one warp per token, V-wide loads, the token's keys then its values
+// ---------------------------------------------------------------------------
+constexpr int kAppendWarps = 4;
+
+template <typename V>
+__global__ void __launch_bounds__(kAppendWarps * 32)
+    kv_append_kernel(const KvPool pool, const KvTable tb, const char* __restrict__ k, int64_t k_st,
+                     int64_t k_sh, const char* __restrict__ v, int64_t v_st, int64_t v_sh,
+                     const int32_t* __restrict__ rows, const int32_t* __restrict__ positions,
+                     int64_t tokens) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  const int row = rows[t], pos = positions[t];
+  if (pos < 0) return;
+  const int col = pos / pool.page_size, slot = pos - col * pool.page_size;
+  const bool in = row >= 0 && row < tb.rows && col < tb.width;
+  const int page = in ? tb.table[row * tb.t_sr + col] : -1;
+  if (!in_pool(page, pool.pages)) {
+    if (lane == 0) raise_status(tb.status, BIO_DEV_INDEX);
+    return;
+  }
+  const unsigned vk = pool.k_row / sizeof(V), vv = pool.v_row / sizeof(V);
+  const unsigned nk = vk * pool.heads, n = nk + vv * pool.heads;
+  const char* ks = k + t * k_st;
+  const char* vs = v + t * v_st;
+  char* kd = pool.k + page * pool.k_sp + slot * pool.k_st;
+  char* vd = pool.v + page * pool.v_sp + slot * pool.v_st;
+  constexpr int U = 4;  // loads in flight per lane
+  for (unsigned i0 = lane; i0 < n; i0 += 32 * U) {
+    V val[U];
+    char* to[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned i = i0 + 32 * u;
+      to[u] = nullptr;
+      if (i >= n) continue;
+      const bool key = i < nk;
+      const unsigned j = key ? i : i - nk, w = key ? vk : vv;
+      const unsigned h = j / w, c = (j - h * w) * sizeof(V);
+      val[u] = *reinterpret_cast<const V*>((key ? ks + h * k_sh : vs + h * v_sh) + c);
+      to[u] = (key ? kd + h * pool.k_sh : vd + h * pool.v_sh) + c;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (to[u] != nullptr) *reinterpret_cast<V*>(to[u]) = val[u];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// free and evict: one block per listed row
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+
+// Whether row rows[i] appears earlier in the list (block-wide answer).
+__device__ __forceinline__ bool seen_before(const int32_t* rows, int64_t i) {
+  const int r = rows[i];
+  int hit = 0;
+  for (int64_t j = threadIdx.x; j < i; j += blockDim.x) hit |= rows[j] == r;
+  return __syncthreads_or(hit) != 0;
+}
+
+// window < 0: release everything and set the length to 0.
+__global__ void __launch_bounds__(kRowThreads)
+    kv_release_kernel(const KvTable tb, const int32_t* __restrict__ rows, int64_t window,
+                      int64_t sinks) {
+  const int64_t i = blockIdx.x;
+  const int r = rows[i];
+  const bool bad = r < 0 || r >= tb.rows;
+  if (seen_before(rows, i) || bad) {
+    if (threadIdx.x == 0) raise_status(tb.status, BIO_DEV_INDEX);
+    return;
+  }
+  int64_t lo = 0, hi = tb.width;  // columns [lo, hi) go
+  if (window >= 0) {
+    const int64_t p = tb.page_size, gone = static_cast<int64_t>(tb.lens[r]) - window;
+    lo = (sinks + p - 1) / p;
+    hi = gone > 0 ? min(tb.width, gone / p) : 0;
+  }
+  for (int64_t c = lo + threadIdx.x; c < hi; c += blockDim.x) {
+    int32_t* e = tb.table + r * tb.t_sr + c;
+    if (in_pool(*e, tb.pages)) atomicSub(&tb.refs[*e], 1);
+    *e = -1;
+  }
+  if (window < 0 && threadIdx.x == 0) tb.lens[r] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// fork, first kernel: one block per branch.  Releases and shares change
+// different rows' entries, and the counts by atomics, so all branches run at
+// once.  want[i]: 1 page for a partial last page, 0 none, -1 skipped.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(kRowThreads)
+    kv_fork_table_kernel(const KvTable tb, const int32_t* __restrict__ src,
+                         const int32_t* __restrict__ dst, int64_t n, int32_t* __restrict__ want) {
+  chain_start_next();
+  const int64_t i = blockIdx.x;
+  const int s = src[i], d = dst[i];
+  int bad = s < 0 || s >= tb.rows || d < 0 || d >= tb.rows;
+  for (int64_t j = threadIdx.x; j < n; j += blockDim.x)
+    bad |= src[j] == d || (j != i && dst[j] == d);
+  const int64_t len = bad ? 0 : tb.lens[s];
+  bad |= len < 0 || len > tb.width * tb.page_size;
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) {
+      want[i] = -1;
+      raise_status(tb.status, BIO_DEV_INDEX);
+    }
+    return;
+  }
+  const int64_t full = len / tb.page_size;
+  for (int64_t c = threadIdx.x; c < tb.width; c += blockDim.x) {
+    int32_t* e = tb.table + d * tb.t_sr + c;
+    const int old = *e;
+    int now = c < full ? tb.table[s * tb.t_sr + c] : -1;
+    if (now >= tb.pages) {
+      raise_status(tb.status, BIO_DEV_INDEX);
+      now = -1;
+    }
+    if (in_pool(old, tb.pages)) atomicSub(&tb.refs[old], 1);
+    if (now >= 0) atomicAdd(&tb.refs[now], 1);
+    *e = now < 0 ? -1 : now;
+  }
+  if (threadIdx.x == 0) {
+    const bool part = len % tb.page_size != 0;
+    const bool held = part && in_pool(tb.table[s * tb.t_sr + full], tb.pages);
+    if (part && !held) raise_status(tb.status, BIO_DEV_INDEX);
+    want[i] = held ? 1 : 0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// One block hands out the lowest free pages: request i's columns first(i) ..
+// first(i) + want[i] of its row take the next ones in order.  The block scans
+// the counts 4096 at a time and stops when every request is served.
+// ---------------------------------------------------------------------------
+constexpr int kScanThreads = 1024;
+
+// Exclusive sum over the block; *total gets the sum.  Two barriers.
+__device__ __forceinline__ int block_scan(int x, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  const int ws = lane < kScanThreads / 32 ? warp_sums[lane] : 0;
+  int wi = ws;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, wi, o);
+    if (lane >= o) wi += y;
+  }
+  *total = __shfl_sync(0xffffffffu, wi, 31);
+  const int base = __shfl_sync(0xffffffffu, wi - ws, warp);
+  __syncthreads();
+  return base + inc - x;
+}
+
+template <bool FORK>
+__global__ void __launch_bounds__(kScanThreads)
+    kv_assign_kernel(const KvTable tb, const int32_t* __restrict__ src,
+                     const int32_t* __restrict__ rows, const int32_t* __restrict__ new_lens,
+                     int64_t n, int32_t* __restrict__ want, int32_t* __restrict__ first_of) {
+  // rows: the rows that grow (dst of a fork).  want[i], then the running sum
+  // before request i in first_of[i]; first_of[n] is the number of pages asked.
+  __shared__ int sums[32];
+  if (FORK) {
+    chain_start_next();
+    chain_wait();
+  }
+  const int64_t P = tb.page_size;
+  int asked = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += kScanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    int w = 0;
+    if (i < n) {
+      if (FORK) {
+        w = want[i];
+      } else {
+        const int r = rows[i], want_len = new_lens[i];
+        bool bad = r < 0 || r >= tb.rows || want_len < 0 || want_len > tb.width * P;
+        for (int64_t j = 0; j < i; ++j) bad |= rows[j] == r;
+        const int64_t len = bad ? 0 : tb.lens[r];
+        bad |= len < 0 || len > tb.width * P;
+        if (bad) raise_status(tb.status, BIO_DEV_INDEX);
+        w = bad ? -1 : static_cast<int>(max(static_cast<int64_t>(0),
+                                            (want_len + P - 1) / P - (len + P - 1) / P));
+        want[i] = w;
+      }
+      w = max(w, 0);
+    }
+    int total;
+    const int before = block_scan(w, sums, &total);
+    if (i < n) first_of[i] = asked + before;
+    asked += total;
+  }
+  if (threadIdx.x == 0) first_of[n] = asked;
+  __syncthreads();
+  auto first_column = [&](int64_t i) -> int64_t {
+    return FORK ? tb.lens[src[i]] / P : (tb.lens[rows[i]] + P - 1) / P;
+  };
+  int found = 0;
+  for (int64_t p0 = 0; p0 < tb.pages && found < asked; p0 += 4 * kScanThreads) {
+    const int64_t p = p0 + 4 * threadIdx.x;
+    bool free_page[4];
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      free_page[u] = p + u < tb.pages && tb.refs[p + u] == 0;
+      mine += free_page[u];
+    }
+    int total;
+    int rank = found + block_scan(mine, sums, &total);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (!free_page[u]) continue;
+      if (rank < asked) {
+        int64_t lo = 0, hi = n;  // the last request that starts at or before rank
+        while (hi - lo > 1) {
+          const int64_t mid = (lo + hi) >> 1;
+          if (first_of[mid] <= rank) lo = mid; else hi = mid;
+        }
+        tb.table[rows[lo] * tb.t_sr + first_column(lo) + rank - first_of[lo]] =
+            static_cast<int32_t>(p + u);
+        tb.refs[p + u] = 1;
+      }
+      ++rank;
+    }
+    found += total;
+  }
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < n; i += kScanThreads) {
+    const int w = want[i];
+    if (w < 0) continue;
+    const int got = max(0, min(w, found - first_of[i]));
+    const int64_t room = (first_column(i) + got) * P;
+    if (got < w) raise_status(tb.status, BIO_DEV_PAGES);
+    const int r = rows[i];
+    const int64_t len = FORK ? tb.lens[src[i]] : new_lens[i];
+    const int64_t now = min(len, room);
+    if (FORK) {
+      tb.lens[r] = static_cast<int32_t>(now);
+    } else if (now > tb.lens[r]) {
+      tb.lens[r] = static_cast<int32_t>(now);
+    }
+  }
+}
+
+// fork, last kernel: block (i, layer, K or V) copies the tokens of the partial page.
+template <typename V>
+__global__ void __launch_bounds__(kRowThreads)
+    kv_fork_copy_kernel(const KvPool pool, const KvTable tb, const int32_t* __restrict__ src,
+                        const int32_t* __restrict__ dst, const int32_t* __restrict__ want) {
+  chain_wait();
+  const int64_t per = 2 * pool.layers;
+  const int64_t i = blockIdx.x / per, layer = (blockIdx.x % per) >> 1;
+  const bool key = (blockIdx.x % per & 1) == 0;
+  if (want[i] <= 0) return;
+  const int s = src[i], d = dst[i];
+  const int len = tb.lens[s], part = len % pool.page_size;
+  if (tb.lens[d] != len) return;  // the pool had no page left
+  const int64_t full = len / pool.page_size;
+  const int64_t from = tb.table[s * tb.t_sr + full], to = tb.table[d * tb.t_sr + full];
+  const int64_t sl = key ? pool.k_sl : pool.v_sl, sp = key ? pool.k_sp : pool.v_sp;
+  const int64_t sh = key ? pool.k_sh : pool.v_sh, st = key ? pool.k_st : pool.v_st;
+  char* base = (key ? pool.k : pool.v) + layer * sl;
+  const unsigned w = (key ? pool.k_row : pool.v_row) / sizeof(V);
+  const unsigned run = w * part, n = run * pool.heads;
+  constexpr int U = 4;
+  for (unsigned i0 = threadIdx.x; i0 < n; i0 += kRowThreads * U) {
+    V val[U];
+    int64_t off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned x = i0 + kRowThreads * u;
+      off[u] = -1;
+      if (x >= n) continue;
+      const unsigned h = x / run, y = x - h * run, slot = y / w;
+      off[u] = h * sh + slot * st + (y - slot * w) * sizeof(V);
+      val[u] = *reinterpret_cast<const V*>(base + from * sp + off[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (off[u] >= 0) *reinterpret_cast<V*>(base + to * sp + off[u]) = val[u];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// compact, first kernel: new number of every page in use (its rank), the list
+// of pages in use, and the new counts.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(kScanThreads)
+    kv_rank_kernel(const int32_t* __restrict__ refs, int64_t pages, int32_t* __restrict__ out_refs,
+                   int64_t out_pages, int32_t* __restrict__ rank_of, int32_t* __restrict__ in_use,
+                   int* status) {
+  // rank_of[pages], in_use[1 + pages]: in_use[0] the number of pages that move
+  __shared__ int sums[32];
+  chain_start_next();
+  int64_t found = 0;
+  for (int64_t p0 = 0; p0 < pages; p0 += 4 * kScanThreads) {
+    const int64_t p = p0 + 4 * threadIdx.x;
+    int ref[4], mine = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      ref[u] = p + u < pages ? refs[p + u] : 0;
+      mine += ref[u] > 0;
+    }
+    int total;
+    int64_t rank = found + block_scan(mine, sums, &total);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (p + u >= pages) continue;
+      const bool moves = ref[u] > 0 && rank < out_pages;
+      rank_of[p + u] = moves ? static_cast<int32_t>(rank) : -1;
+      if (moves) {
+        in_use[1 + rank] = static_cast<int32_t>(p + u);
+        out_refs[rank] = ref[u];
+      }
+      rank += ref[u] > 0;
+    }
+    found += total;
+  }
+  if (found > out_pages && threadIdx.x == 0) raise_status(status, BIO_DEV_PAGES);
+  const int64_t moved = min(found, out_pages);
+  if (threadIdx.x == 0) in_use[0] = static_cast<int32_t>(moved);
+  for (int64_t p = moved + threadIdx.x; p < out_pages; p += kScanThreads) out_refs[p] = 0;
+}
+
+// compact, second kernel: the table, then the pages.  A block copies pieces of
+// U * kRowThreads vectors; piece x belongs to page x / pieces of one layer's K
+// or V.  `runs` contiguous runs of `run` vectors make a page.
+struct KvCopySide {
+  const char* from;
+  char* to;
+  int64_t from_sl, from_sp, from_s1, from_s2, to_sl, to_sp, to_s1, to_s2;  // bytes
+  unsigned n1, n2, run;  // a page: n1 x n2 runs of `run` vectors
+};
+
+template <typename V>
+__global__ void __launch_bounds__(kRowThreads)
+    kv_compact_kernel(const KvCopySide ks, const KvCopySide vs, int64_t layers, const KvTable tb,
+                      const KvTable out, const int32_t* __restrict__ rank_of,
+                      const int32_t* __restrict__ in_use) {
+  chain_wait();
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * kRowThreads;
+  for (int64_t x = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
+       x < tb.rows * tb.width; x += threads) {
+    const int64_t r = x / tb.width, c = x - r * tb.width;
+    const int page = tb.table[r * tb.t_sr + c];
+    if (page >= tb.pages) raise_status(tb.status, BIO_DEV_INDEX);
+    out.table[r * out.t_sr + c] = in_pool(page, tb.pages) ? rank_of[page] : -1;
+  }
+  constexpr int U = 8;
+  constexpr unsigned kPiece = U * kRowThreads;
+  const int64_t moved = in_use[0];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const KvCopySide& c = side == 0 ? ks : vs;
+    const unsigned per = c.n1 * c.n2 * c.run;  // vectors of a page
+    const unsigned pieces = (per + kPiece - 1) / kPiece;
+    const int64_t work = layers * moved * pieces;
+    for (int64_t x = blockIdx.x; x < work; x += gridDim.x) {
+      const int64_t pg = x / pieces;
+      const unsigned at = static_cast<unsigned>(x - pg * pieces) * kPiece;
+      const int64_t layer = pg / moved, rank = pg - layer * moved;
+      const char* from = c.from + layer * c.from_sl + in_use[1 + rank] * c.from_sp;
+      char* to = c.to + layer * c.to_sl + rank * c.to_sp;
+      V val[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const unsigned y = at + u * kRowThreads + threadIdx.x;
+        if (y >= per) continue;
+        const unsigned r = y / c.run, i1 = r / c.n2, i2 = r - i1 * c.n2;
+        val[u] = *reinterpret_cast<const V*>(from + i1 * c.from_s1 + i2 * c.from_s2 +
+                                             (y - r * c.run) * sizeof(V));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const unsigned y = at + u * kRowThreads + threadIdx.x;
+        if (y >= per) continue;
+        const unsigned r = y / c.run, i1 = r / c.n2, i2 = r - i1 * c.n2;
+        *reinterpret_cast<V*>(to + i1 * c.to_s1 + i2 * c.to_s2 + (y - r * c.run) * sizeof(V)) =
+            val[u];
+      }
+    }
+  }
+}
+
+}  // namespace bio
+
+namespace {
+
+int elem_bytes(int32_t dtype) {
+  return dtype == BIO_F32 ? 4 : (dtype == BIO_F16 || dtype == BIO_BF16) ? 2 : 0;
+}
+
+constexpr int64_t kMaxInt = 2147483647;
+
+int check_pool(const bio_kv_pool* p) {
+  if (p == nullptr) return BIO_ERR_ARG;
+  if (elem_bytes(p->dtype) == 0) return BIO_ERR_DTYPE;
+  if (p->layers < 0 || p->pages < 0 || p->pages > kMaxInt || p->kv_heads < 1 ||
+      p->kv_heads > 65536 || p->page_size < 1 || p->page_size > 65536 || p->d < 1 ||
+      p->d > 65536 || p->dv < 1 || p->dv > 65536)
+    return BIO_ERR_SHAPE;
+  // vectors of a page are counted in 32 bits
+  if (p->kv_heads * p->page_size > (1 << 28) / (p->d > p->dv ? p->d : p->dv)) return BIO_ERR_SHAPE;
+  if (p->layers > 0 && p->pages > 0 && (p->k == nullptr || p->v == nullptr)) return BIO_ERR_ARG;
+  return BIO_OK;
+}
+
+int check_table(const bio_kv_table* t, bool lens, bool refs) {
+  if (t == nullptr) return BIO_ERR_ARG;
+  if (t->rows < 0 || t->rows > kMaxInt || t->width < 0 || t->width > kMaxInt || t->pages < 0 ||
+      t->pages > kMaxInt || t->page_size < 1 || t->page_size > 65536)
+    return BIO_ERR_SHAPE;
+  if (t->rows > 0 && t->width > 0 && t->page_table == nullptr) return BIO_ERR_ARG;
+  if (lens && t->rows > 0 && t->seq_lens == nullptr) return BIO_ERR_ARG;
+  if (refs && t->pages > 0 && t->ref_counts == nullptr) return BIO_ERR_ARG;
+  return BIO_OK;
+}
+
+bio::KvPool pool_view(const bio_kv_pool* p) {
+  const int64_t e = elem_bytes(p->dtype);
+  bio::KvPool v;
+  v.k = static_cast<char*>(p->k);
+  v.v = static_cast<char*>(p->v);
+  v.layers = p->layers;
+  v.pages = p->pages;
+  v.heads = static_cast<int>(p->kv_heads);
+  v.page_size = static_cast<int>(p->page_size);
+  v.k_sl = p->k_sl * e; v.k_sp = p->k_sp * e; v.k_sh = p->k_sh * e; v.k_st = p->k_st * e;
+  v.v_sl = p->v_sl * e; v.v_sp = p->v_sp * e; v.v_sh = p->v_sh * e; v.v_st = p->v_st * e;
+  v.k_row = static_cast<int>(p->d * e);
+  v.v_row = static_cast<int>(p->dv * e);
+  return v;
+}
+
+bio::KvTable table_view(const bio_kv_table* t) {
+  bio::KvTable v;
+  v.table = t->page_table;
+  v.t_sr = t->t_sr;
+  v.rows = t->rows;
+  v.width = t->width;
+  v.lens = t->seq_lens;
+  v.refs = t->ref_counts;
+  v.pages = t->pages;
+  v.page_size = static_cast<int>(t->page_size);
+  v.status = bio_host::status_word(t->device);
+  return v;
+}
+
+// Widest vector (16, 8, 4 or 2 bytes) that every one of these byte offsets is a multiple of.
+struct Width {
+  uint64_t bits = 16;
+  void add(const void* p) { bits |= reinterpret_cast<uint64_t>(p); }
+  void add(int64_t n) { bits |= static_cast<uint64_t>(n); }
+  void add(const bio::KvPool& p) {
+    add(p.k); add(p.v);
+    add(p.k_sl); add(p.k_sp); add(p.k_sh); add(p.k_st); add(p.k_row);
+    add(p.v_sl); add(p.v_sp); add(p.v_sh); add(p.v_st); add(p.v_row);
+  }
+  int bytes() const { return static_cast<int>(bits & (~bits + 1)); }
+};
+
+// Launch that may overlap the end of the kernel before it on the stream; the
+// kernel waits for that one itself (chain_wait).
+template <typename... P, typename... A>
+int launch_chained(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t s,
+                   A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return bio_host::launch_status(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+}
+
+template <typename F>
+int with_width(int bytes, F f) {
+  switch (bytes) {
+    case 16: return f(uint4{});
+    case 8: return f(uint2{});
+    case 4: return f(uint32_t{});
+    case 2: return f(uint16_t{});
+    default: return BIO_ERR_ALIGN;  // a pointer that no element can have
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int bio_kv_append(const bio_kv_pool* pool, const bio_kv_table* table, const void* k, int64_t k_st,
+                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int32_t* rows,
+                  const int32_t* positions, int64_t tokens, void* stream) {
+  int st = check_pool(pool);
+  if (st == BIO_OK) st = check_table(table, false, false);
+  if (st != BIO_OK) return st;
+  if (pool->layers != 1 || table->page_size != pool->page_size || tokens < 0) return BIO_ERR_SHAPE;
+  if (tokens == 0) return BIO_OK;
+  if (k == nullptr || v == nullptr || rows == nullptr || positions == nullptr) return BIO_ERR_ARG;
+  const int64_t blocks = (tokens + bio::kAppendWarps - 1) / bio::kAppendWarps;
+  if (blocks > kMaxInt) return BIO_ERR_SHAPE;
+  st = bio_host::ensure_device(pool->device);
+  if (st != BIO_OK) return st;
+  const bio::KvPool p = pool_view(pool);
+  const bio::KvTable t = table_view(table);
+  const int64_t e = elem_bytes(pool->dtype);
+  Width w;
+  w.add(p);
+  w.add(k); w.add(v);
+  w.add(k_st * e); w.add(k_sh * e); w.add(v_st * e); w.add(v_sh * e);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return with_width(w.bytes(), [&](auto vec) {
+    using V = decltype(vec);
+    bio::kv_append_kernel<V><<<static_cast<unsigned>(blocks), bio::kAppendWarps * 32, 0, s>>>(
+        p, t, static_cast<const char*>(k), k_st * e, k_sh * e, static_cast<const char*>(v),
+        v_st * e, v_sh * e, rows, positions, tokens);
+    return bio_host::launch_status(cudaGetLastError());
+  });
+}
+
+int64_t bio_kv_workspace(int64_t n, int64_t pages) {
+  if (n < 0 || pages < 0 || n > kMaxInt || pages > kMaxInt) return 0;
+  const int64_t rows = 2 * n + 1, moved = 2 * pages + 1;
+  return 4 * (rows > moved ? rows : moved);
+}
+
+int bio_kv_extend(const bio_kv_table* table, const int32_t* rows, const int32_t* new_lens,
+                  int64_t n, void* workspace, int64_t workspace_bytes, void* stream) {
+  int st = check_table(table, true, true);
+  if (st != BIO_OK) return st;
+  if (n < 0 || n > kMaxInt) return BIO_ERR_SHAPE;
+  if (n == 0) return BIO_OK;
+  if (rows == nullptr || new_lens == nullptr || workspace == nullptr) return BIO_ERR_ARG;
+  if (workspace_bytes < 4 * (2 * n + 1)) return BIO_ERR_SCRATCH;
+  st = bio_host::ensure_device(table->device);
+  if (st != BIO_OK) return st;
+  int32_t* ws = static_cast<int32_t*>(workspace);
+  bio::kv_assign_kernel<false><<<1, bio::kScanThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      table_view(table), nullptr, rows, new_lens, n, ws, ws + n);
+  return bio_host::launch_status(cudaGetLastError());
+}
+
+static int release(const bio_kv_table* table, const int32_t* rows, int64_t n, int64_t window,
+                   int64_t sinks, void* stream) {
+  int st = check_table(table, true, true);
+  if (st != BIO_OK) return st;
+  if (n < 0 || n > kMaxInt) return BIO_ERR_SHAPE;
+  if (n == 0) return BIO_OK;
+  if (rows == nullptr) return BIO_ERR_ARG;
+  st = bio_host::ensure_device(table->device);
+  if (st != BIO_OK) return st;
+  bio::kv_release_kernel<<<static_cast<unsigned>(n), bio::kRowThreads, 0,
+                           static_cast<cudaStream_t>(stream)>>>(table_view(table), rows, window,
+                                                                sinks);
+  return bio_host::launch_status(cudaGetLastError());
+}
+
+int bio_kv_free(const bio_kv_table* table, const int32_t* rows, int64_t n, void* stream) {
+  return release(table, rows, n, -1, 0, stream);
+}
+
+int bio_kv_evict(const bio_kv_table* table, const int32_t* rows, int64_t n, int64_t window,
+                 int64_t sinks, void* stream) {
+  if (window < 1 || window > kMaxInt || sinks < 0 || sinks > kMaxInt) return BIO_ERR_ARG;
+  return release(table, rows, n, window, sinks, stream);
+}
+
+int bio_kv_fork(const bio_kv_pool* pool, const bio_kv_table* table, const int32_t* src,
+                const int32_t* dst, int64_t n, void* workspace, int64_t workspace_bytes,
+                void* stream) {
+  int st = check_pool(pool);
+  if (st == BIO_OK) st = check_table(table, true, true);
+  if (st != BIO_OK) return st;
+  if (table->page_size != pool->page_size || table->pages != pool->pages || n < 0)
+    return BIO_ERR_SHAPE;
+  if (n == 0) return BIO_OK;
+  if (src == nullptr || dst == nullptr || workspace == nullptr) return BIO_ERR_ARG;
+  if (n > kMaxInt / 2 || pool->layers > kMaxInt / 2 / n) return BIO_ERR_SHAPE;
+  if (workspace_bytes < 4 * (2 * n + 1)) return BIO_ERR_SCRATCH;
+  st = bio_host::ensure_device(pool->device);
+  if (st != BIO_OK) return st;
+  const bio::KvPool p = pool_view(pool);
+  const bio::KvTable t = table_view(table);
+  int32_t* ws = static_cast<int32_t*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  bio::kv_fork_table_kernel<<<static_cast<unsigned>(n), bio::kRowThreads, 0, s>>>(t, src, dst, n,
+                                                                                  ws);
+  st = bio_host::launch_status(cudaGetLastError());
+  if (st != BIO_OK) return st;
+  st = launch_chained(bio::kv_assign_kernel<true>, 1, bio::kScanThreads, s, t, src, dst,
+                      static_cast<const int32_t*>(nullptr), n, ws, ws + n);
+  if (st != BIO_OK || pool->layers == 0) return st;
+  Width w;
+  w.add(p);
+  return with_width(w.bytes(), [&](auto vec) {
+    using V = decltype(vec);
+    return launch_chained(bio::kv_fork_copy_kernel<V>, static_cast<unsigned>(2 * n * p.layers),
+                          bio::kRowThreads, s, p, t, src, dst, ws);
+  });
+}
+
+int bio_kv_compact(const bio_kv_pool* pool, const bio_kv_table* table, const bio_kv_pool* out_pool,
+                   const bio_kv_table* out_table, void* workspace, int64_t workspace_bytes,
+                   void* stream) {
+  int st = check_pool(pool);
+  if (st == BIO_OK) st = check_pool(out_pool);
+  if (st == BIO_OK) st = check_table(table, false, true);
+  if (st == BIO_OK) st = check_table(out_table, false, true);
+  if (st != BIO_OK) return st;
+  if (pool->dtype != out_pool->dtype) return BIO_ERR_DTYPE;
+  if (pool->layers != out_pool->layers || pool->kv_heads != out_pool->kv_heads ||
+      pool->page_size != out_pool->page_size || pool->d != out_pool->d ||
+      pool->dv != out_pool->dv || table->rows != out_table->rows ||
+      table->width != out_table->width || table->pages != pool->pages ||
+      out_table->pages != out_pool->pages || pool->device != out_pool->device)
+    return BIO_ERR_SHAPE;
+  if (workspace == nullptr) return BIO_ERR_ARG;
+  if (workspace_bytes < 4 * (2 * pool->pages + 1)) return BIO_ERR_SCRATCH;
+  st = bio_host::ensure_device(pool->device);
+  if (st != BIO_OK) return st;
+  const int sms = bio_host::sm_count(pool->device);
+  if (sms <= 0) return BIO_ERR_LAUNCH;
+  const bio::KvPool p = pool_view(pool), q = pool_view(out_pool);
+  const bio::KvTable t = table_view(table), o = table_view(out_table);
+  int32_t* rank_of = static_cast<int32_t*>(workspace);
+  int32_t* in_use = rank_of + pool->pages;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  bio::kv_rank_kernel<<<1, bio::kScanThreads, 0, s>>>(t.refs, t.pages, o.refs, o.pages, rank_of,
+                                                      in_use, t.status);
+  st = bio_host::launch_status(cudaGetLastError());
+  if (st != BIO_OK) return st;
+  Width w;
+  w.add(p);
+  w.add(q);
+  return with_width(w.bytes(), [&](auto vec) {
+    using V = decltype(vec);
+    auto side = [&](bool key) {
+      bio::KvCopySide c;
+      c.from = key ? p.k : p.v;
+      c.to = key ? q.k : q.v;
+      c.from_sl = key ? p.k_sl : p.v_sl; c.to_sl = key ? q.k_sl : q.v_sl;
+      c.from_sp = key ? p.k_sp : p.v_sp; c.to_sp = key ? q.k_sp : q.v_sp;
+      c.from_s1 = key ? p.k_sh : p.v_sh; c.to_s1 = key ? q.k_sh : q.v_sh;
+      c.from_s2 = key ? p.k_st : p.v_st; c.to_s2 = key ? q.k_st : q.v_st;
+      const int64_t row = key ? p.k_row : p.v_row;
+      c.n1 = p.heads;
+      c.n2 = p.page_size;
+      c.run = static_cast<unsigned>(row / sizeof(V));
+      if (c.from_s2 == row && c.to_s2 == row) {  // a head's tokens lie together
+        c.run *= c.n2;
+        c.n2 = 1;
+        if (c.from_s1 == row * p.page_size && c.to_s1 == c.from_s1) {  // and the heads do
+          c.run *= c.n1;
+          c.n1 = 1;
+        }
+      }
+      return c;
+    };
+    return launch_chained(bio::kv_compact_kernel<V>, static_cast<unsigned>(sms * 4),
+                          bio::kRowThreads, s, side(true), side(false), p.layers, t, o,
+                          static_cast<const int32_t*>(rank_of),
+                          static_cast<const int32_t*>(in_use));
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,219 @@
+"""Sliding-window attention with sink tokens against the 64-bit oracle.
+
+Tolerances are those of tests/test_paged_attention_gpu.py: |out - oracle| <=
+v* (4 u + 2^-24 (2 D S + 2 n + 8)) per element, and 2 u in the norm for 16-bit
+types."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import batch_invariant_ops as bio
+from batch_invariant_ops import _lib
+from oracle import bio_oracle
+
+pytestmark = pytest.mark.gpu
+
+UNIT = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
+DTYPES = tuple(UNIT)
+
+
+def make(b, h, hk, lq, lk, d, dv=None, dtype=torch.bfloat16, seed=0, spread=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    q = spread * torch.randn(b, lq, h, d, generator=gen, device="cuda")
+    k = torch.randn(b, lk, hk, d, generator=gen, device="cuda")
+    v = torch.randn(b, lk, hk, dv or d, generator=gen, device="cuda")
+    return [t.to(dtype).transpose(1, 2) for t in (q, k, v)]
+
+
+def bound_of(q, k, v, scale=None):
+    """One bound for all rows, from the largest values that any of them sees."""
+    u, d = UNIT[q.dtype], q.shape[-1]
+    scale = d ** -0.5 if scale is None else abs(scale)
+    k, v = torch.nan_to_num(k.double(), 0, 0, 0), torch.nan_to_num(v.double(), 0, 0, 0)
+    k = k.abs().repeat_interleave(q.shape[1] // k.shape[1], 1)
+    reach = scale * (q.double().abs() @ k.transpose(-1, -2)).max().item()
+    return v.abs().max().item() * (4 * u + 2.0**-24 * (2 * d * reach + 2 * k.shape[2] + 8))
+
+
+def check(out, q, k, v, window, sinks, scale=None):
+    ref = bio_oracle.window_attention(q, k, v, window, sinks, scale)
+    got = out.double().cpu()
+    assert got.shape == ref.shape and out.dtype == q.dtype
+    err = (got - ref).abs().max().item()
+    assert err <= bound_of(q, k, v, scale), f"{err} > {bound_of(q, k, v, scale)}"
+    if q.dtype != torch.float32 and ref.norm() > 0:
+        assert ((got - ref).norm() / ref.norm()).item() <= 2 * UNIT[q.dtype]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,hk,lq,lk,d,window,sinks", [
+    (1, 1, 1, 1, 1, 64, 1, 0),
+    (2, 4, 2, 1, 300, 128, 100, 4),      # one token behind a cache
+    (1, 2, 1, 7, 7, 64, 3, 1),
+    (1, 2, 2, 127, 127, 128, 16, 4),
+    (1, 2, 1, 128, 128, 64, 64, 0),
+    (1, 2, 1, 129, 129, 128, 128, 2),
+    (2, 3, 1, 255, 300, 64, 129, 5),
+    (1, 2, 1, 257, 257, 128, 1, 0),      # each token sees itself
+    (1, 4, 2, 400, 400, 128, 1000, 0),   # plain causal
+    (1, 2, 1, 520, 1100, 64, 257, 130),  # more sinks than a block
+    (1, 2, 1, 300, 900, 128, 64, 700),   # the sinks reach into the window
+    (1, 8, 1, 333, 333, 256, 100, 4),
+    (1, 4, 2, 200, 260, 72, 50, 3),
+    (1, 2, 1, 190, 190, 96, 31, 9),
+    (1, 2, 1, 140, 140, 8, 20, 1),
+    (1, 2, 1, 70, 70, 33, 20, 1),
+    (1, 2, 1, 70, 90, 200, 20, 1),
+    (3, 2, 2, 40, 20, 64, 8, 2),         # more queries than keys: the first see nothing
+    (1, 2, 1, 30, 0, 64, 8, 2),          # no key at all
+    (1, 16, 2, 64, 640, 64, 256, 16),
+])
+def test_matches_the_oracle(b, h, hk, lq, lk, d, window, sinks, dtype):
+    q, k, v = make(b, h, hk, lq, lk, d, dtype=dtype, seed=lq + d)
+    out = bio.sliding_window_attention_batch_invariant(q, k, v, window, sinks)
+    if lk == 0:
+        assert torch.equal(out, torch.zeros_like(out))
+        return
+    check(out, q, k, v, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,dv", [(64, 128), (128, 64), (256, 64), (40, 256), (24, 17)])
+def test_value_dim_of_its_own(d, dv, dtype):
+    q, k, v = make(1, 4, 2, 150, 200, d, dv, dtype=dtype, seed=dv)
+    check(bio.sliding_window_attention_batch_invariant(q, k, v, 64, 4), q, k, v, 64, 4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 128, 256, 80))
+@pytest.mark.parametrize("window,sinks", [(1, 0), (100, 0), (128, 4), (300, 140)])
+def test_hidden_values_never_reach_a_row(window, sinks, d, dtype):
+    """One key in the middle holds infinities and NaN: the rows that do not see
+    it keep their exact bits, the others show it."""
+    lk, bad = 700, 333
+    q, k, v = make(1, 2, 1, lk, lk, d, dtype=dtype, seed=window)
+    clean = bio.sliding_window_attention_batch_invariant(q, k, v, window, sinks)
+    k, v = k.clone(), v.clone()
+    k[:, :, bad, 0] = float("inf")
+    v[:, :, bad, 1:] = float("nan")
+    out = bio.sliding_window_attention_batch_invariant(q, k, v, window, sinks)
+    i = torch.arange(lk, device="cuda")
+    sees = (i >= bad) & ((i < bad + window) | (bad < sinks))
+    hidden = ~sees
+    err = (out[:, :, hidden].double() - clean[:, :, hidden].double()).abs().max().item()
+    # finite, and the same values up to the order of the sums
+    assert err <= 2 * bound_of(q, k, v)
+    # a score of +inf shows up; one of -inf has weight 0 (and alone gives a zero row)
+    shows = sees & (q[0, :, :, 0] > 0)
+    assert torch.isnan(out[0][shows][:, 1:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_extreme_scores(dtype):
+    q, k, v = make(1, 4, 2, 300, 300, 64, dtype=dtype, seed=9, spread=100.0)
+    q[:, 1] = 0
+    check(bio.sliding_window_attention_batch_invariant(q, k, v, 90, 4), q, k, v, 90, 4)
+    check(bio.sliding_window_attention_batch_invariant(q, k, v, 90, 4, scale=-0.02), q, k, v, 90, 4,
+          -0.02)
+    check(bio.sliding_window_attention_batch_invariant(q, k, v, 90, 4, scale=0.0), q, k, v, 90, 4,
+          0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 128, 256, 33))
+def test_a_row_does_not_depend_on_the_batch(d, dtype):
+    q, k, v = make(5, 4, 2, 300, 420, d, dtype=dtype, seed=d)
+    full = bio.sliding_window_attention_batch_invariant(q, k, v, 130, 4)
+    for b in range(5):
+        alone = bio.sliding_window_attention_batch_invariant(q[b:b + 1], k[b:b + 1], v[b:b + 1],
+                                                             130, 4)
+        assert torch.equal(alone, full[b:b + 1])
+    # heads are independent too
+    pair = bio.sliding_window_attention_batch_invariant(q[:, 2:], k[:, 1:], v[:, 1:], 130, 4)
+    assert torch.equal(pair, full[:, 2:])
+    for _ in range(3):
+        assert torch.equal(bio.sliding_window_attention_batch_invariant(q, k, v, 130, 4), full)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_leading_dims_strides_and_odd_offsets(dtype):
+    q, k, v = make(6, 4, 2, 100, 100, 64, dtype=dtype)
+    out = bio.sliding_window_attention_batch_invariant(q, k, v, 40, 4)
+    lead = bio.sliding_window_attention_batch_invariant(
+        q.reshape(2, 3, 4, 100, 64), k.reshape(2, 3, 2, 100, 64), v.reshape(2, 3, 2, 100, 64),
+        40, 4)
+    assert torch.equal(lead.reshape(6, 4, 100, 64), out)
+    assert torch.equal(bio.sliding_window_attention_batch_invariant(
+        q[0], k[0], v[0], 40, 4), out[0])
+    fused = torch.zeros(6, 100, 8, 67, dtype=dtype, device="cuda")
+    fused[:, :, :4, 3:] = q.transpose(1, 2)
+    fused[:, :, 4:6, 3:] = k.transpose(1, 2)
+    fused[:, :, 6:, 3:] = v.transpose(1, 2)
+    f = fused[..., 3:].transpose(1, 2)
+    assert torch.equal(bio.sliding_window_attention_batch_invariant(
+        f[:, :4], f[:, 4:6], f[:, 6:], 40, 4), out)
+    assert bio.sliding_window_attention_batch_invariant(q[:0], k[:0], v[:0], 4).shape == (
+        0, 4, 100, 64)
+    assert bio.sliding_window_attention_batch_invariant(q[:, :, :0], k, v, 4).shape == (
+        6, 4, 0, 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 128, 256, 72))
+@pytest.mark.parametrize("index", (torch.int32, torch.int64))
+def test_packed_equals_dense(d, dtype, index):
+    lens_q, lens_k = [1, 130, 0, 300, 5, 257, 20], [1, 130, 40, 500, 700, 257, 0]
+    parts = [make(1, 4, 2, a, b, d, dtype=dtype, seed=a + b) for a, b in zip(lens_q, lens_k)]
+    q, k, v = (torch.cat([p[i].transpose(1, 2) for p in parts], 1) for i in range(3))
+    off = lambda x: torch.tensor([0, *x], device="cuda").cumsum(0).to(index)  # noqa: E731
+    out = bio.varlen_sliding_window_attention_batch_invariant(q, k, v, off(lens_q), off(lens_k),
+                                                              100, 4)
+    for part, got in zip(parts, out.split(lens_q, 1)):
+        if part[0].shape[2] == 0:
+            continue
+        want = bio.sliding_window_attention_batch_invariant(*part, 100, 4).transpose(1, 2)
+        assert torch.equal(got, want)
+
+
+def test_packed_neighbours_do_not_leak():
+    """NaN in the next sequence's keys and values."""
+    q, k, v = make(1, 2, 1, 300, 300, 64)
+    q, k, v = (t.transpose(1, 2).contiguous() for t in (q, k, v))
+    cu = torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+    out = bio.varlen_sliding_window_attention_batch_invariant(q, k, v, cu, cu, 64, 2)
+    k[:, 100:], v[:, 100:] = float("nan"), float("nan")
+    got = bio.varlen_sliding_window_attention_batch_invariant(q, k, v, cu, cu, 64, 2)
+    assert torch.equal(got[:, :100], out[:, :100])
+
+
+def test_packed_bad_offsets_and_uncovered_tokens():
+    q, k, v = (t.transpose(1, 2).contiguous() for t in make(1, 2, 1, 300, 300, 64))
+    cu = torch.tensor([0, 100, 200], dtype=torch.int32, device="cuda")
+    out = bio.varlen_sliding_window_attention_batch_invariant(q, k, v, cu, cu, 64, 2)
+    assert torch.equal(out[:, 200:], torch.zeros_like(out[:, 200:]))
+    assert _lib.device_status() == 0
+    bad_k = torch.tensor([0, 100, 5000], dtype=torch.int32, device="cuda")
+    got = bio.varlen_sliding_window_attention_batch_invariant(q, k, v, cu, bad_k, 64, 2)
+    assert torch.equal(got[:, :100], out[:, :100])
+    assert torch.equal(got[:, 100:], torch.zeros_like(got[:, 100:]))
+    assert _lib.device_status() == _lib.BIO_DEV_INDEX
+    _lib.clear_device_status()
+
+
+def test_streams_and_graphs():
+    q, k, v = make(2, 4, 2, 300, 300, 128)
+    want = bio.sliding_window_attention_batch_invariant(q, k, v, 100, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = bio.sliding_window_attention_batch_invariant(q, k, v, 100, 4)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = bio.sliding_window_attention_batch_invariant(q, k, v, 100, 4)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, want)
