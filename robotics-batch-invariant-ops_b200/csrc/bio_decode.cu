@@ -11,6 +11,8 @@
 // batch.  Scores are kept in units of log2 (scale * log2(e) goes into q).
 //
 // Not in the reference, which keeps no cache between calls.
+#include <mutex>
+
 #include "bio_common.cuh"
 
 namespace bio {
@@ -248,6 +250,446 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 }
 
 // ---------------------------------------------------------------------------
+// 16-bit kernel: cp.async into swizzled shared memory, m16n8k16 products.
+//
+// Four warps share an item (one piece of one row for 8 * NH query heads of one
+// KV head); warp w takes the 16-token tiles w, w + 4, ....  Every warp has its
+// own ring of S stages, each a tile's keys, values and the item's queries, and
+// refills a stage as soon as it has used it, across item borders, so the loads
+// never wait for the arithmetic.  Per tile:
+//   S^T [16 keys x 8 heads] = K [16 x d] Q^T     A: ldmatrix, B: ldmatrix of Q
+//   p = 2^(s - m) in the accumulator layout, rounded to T; movmatrix turns its
+//   8 x 8 halves into the B operand of
+//   O^T [d x 8 heads] += V^T [d x 16] P^T        A: ldmatrix.trans
+// Keys are the 16-row side, so a group of 8 heads fills the 8-column side
+// exactly and m, l and the rescale factors of a head pair sit in the lane that
+// holds that pair of O.  The cache is read once at a few flops per byte: what
+// bounds it is HBM, not the products (m16n8k16 covers 2048 products per
+// instruction; the tcgen05 tile of 128 rows would be 15/16 padding here).
+// ---------------------------------------------------------------------------
+constexpr int kMmaWarps = 4;
+constexpr int kTile = 16;         // tokens of a tile
+constexpr int kListRows = 1024;   // rows whose piece counts fit in shared memory
+
+template <int DP, int NH>
+struct PagedSmem {
+  static constexpr int kRow = DP * 2;                       // bytes of a token's row
+  static constexpr int kStage = 2 * kTile * kRow + 8 * NH * kRow;
+  static constexpr int kPitch = DP + 4;                     // floats, spreads the banks
+  static constexpr int kPart = kMmaWarps * 8 * NH * kPitch * 4;
+  static constexpr int kList = (kListRows + 4) * 4;
+  static constexpr int kMisc = kMmaWarps * 8 * NH * 8 + 64 * 4 + kList;
+  // two CTAs per SM where two stages fit, else one with as many as fit
+  static constexpr int kTwo = (113 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
+  static constexpr int kOne = (226 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
+  static constexpr int kCtas = kTwo >= 2 ? 2 : 1;
+  static constexpr int kStages = kTwo >= 2 ? (kTwo > 4 ? 4 : kTwo) : (kOne > 6 ? 6 : kOne);
+  static constexpr int kBytes = kPart + kMisc + kMmaWarps * kStages * kStage;
+  static_assert(kStages >= 2, "a ring needs two stages");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t mov_trans(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4],
+                                                        uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4],
+                                                 uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two probabilities rounded to T, and their rounded values for the sum.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b, float& ra, float& rb);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b, float& ra, float& rb) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  ra = __low2float(v);
+  rb = __high2float(v);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b, float& ra, float& rb) {
+  const __half2 v = __floats2half2_rn(a, b);
+  ra = __low2float(v);
+  rb = __high2float(v);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+struct PagedItem {
+  int64_t b;       // query
+  Visible z;
+  int hg;          // KV head * blocks of heads + block
+  int64_t piece, pieces;
+  int64_t u0;      // first token of the piece
+  int tokens;
+};
+
+template <typename T, int DP, int NH>
+__global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
+    paged_mma_kernel(const PagedParams p, int64_t batch, int list) {
+  using L = PagedSmem<DP, NH>;
+  constexpr int S = L::kStages, HB = 8 * NH;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* ring = smem;
+  float* part = reinterpret_cast<float*>(ring + kMmaWarps * S * L::kStage);
+  float2* part_ml = reinterpret_cast<float2*>(part + L::kPart / 4);
+  int* misc = reinterpret_cast<int*>(part_ml + kMmaWarps * HB);  // [0..31] stage flags, [32..] bad
+  int* first = misc + 64;          // list: items before row b, [batch + 1]
+  int* scan = misc + 40;           // list: sums of the four warps
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hblocks = (p.group + HB - 1) / HB;
+  const int hgs = p.kv_heads * hblocks;
+
+  // columns past d / dv are never written by the copies: zero the ring once
+  if (p.d < DP || p.dv < DP) {
+    uint4* z = reinterpret_cast<uint4*>(ring);
+    for (int i = threadIdx.x; i < kMmaWarps * S * L::kStage / 16; i += blockDim.x)
+      z[i] = make_uint4(0, 0, 0, 0);
+  }
+  auto pieces_of = [&](const Visible& z) -> int64_t {
+    const int c = piece_tokens(z.n);
+    const int64_t k = (z.n + c - 1) / c;
+    return k > 1 ? k : 1;  // an empty or refused row has one item, which writes zeros
+  };
+  int64_t total = 1;
+  if (list) {
+    // items of every row, as a running sum in shared memory
+    int carry = 0;
+    for (int64_t b0 = 0; b0 < batch; b0 += blockDim.x) {
+      const int64_t b = b0 + threadIdx.x;
+      const int mine = b < batch ? static_cast<int>(pieces_of(visible_of(p, b))) * hgs : 0;
+      int inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      if (lane == 31) scan[warp] = inc;
+      __syncthreads();
+      int base = carry, sum = 0;
+#pragma unroll
+      for (int w = 0; w < kMmaWarps; ++w) {
+        if (w < warp) base += scan[w];
+        sum += scan[w];
+      }
+      if (b < batch) first[b] = base + inc - mine;
+      carry += sum;
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) first[batch] = carry;
+    total = carry;
+  }
+  __syncthreads();
+
+  // item number -> what to do; without a list the block has one item
+  auto decode = [&](int64_t item, PagedItem& it) {
+    int64_t rest;
+    if (list) {
+      int lo = 0, hi = static_cast<int>(batch);
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= item) lo = mid; else hi = mid;
+      }
+      it.b = lo;
+      rest = item - first[lo];
+      it.hg = static_cast<int>(rest % hgs);
+      it.piece = rest / hgs;
+    } else {
+      rest = blockIdx.x;
+      it.piece = rest % p.max_pieces;
+      rest /= p.max_pieces;
+      it.hg = static_cast<int>(rest % hgs);
+      it.b = rest / hgs;
+    }
+    it.z = visible_of(p, it.b);
+    const int c = piece_tokens(it.z.n);
+    it.pieces = pieces_of(it.z);
+    it.u0 = it.piece * c;
+    it.tokens = static_cast<int>(max(static_cast<int64_t>(0),
+                                     min(static_cast<int64_t>(c), it.z.n - it.u0)));
+  };
+
+  // ------------------------------------------------------------- producer side
+  // the next tile to fetch: its item, its number, and its tokens' pages
+  const uint32_t my_ring = smem_u32(ring) + warp * (S * L::kStage);
+  int64_t in_item = list ? blockIdx.x : 0;
+  PagedItem in;
+  decode(in_item, in);
+  const bool dead = !list && in.piece >= in.pieces;
+  if (dead) return;
+  int in_tile = warp;
+  bool in_done = in_item >= total;
+  int in_page = -1, in_slot = 0;  // of token `lane` of the tile (lanes 0..15)
+  auto look_up = [&]() {
+    while (!in_done && in_tile * kTile >= in.tokens) {
+      in_item += gridDim.x;
+      if (!list || in_item >= total) {
+        in_done = true;
+      } else {
+        decode(in_item, in);
+        in_tile = warp;
+      }
+    }
+    in_page = -1;
+    if (!in_done && lane < kTile && in_tile * kTile + lane < in.tokens) {
+      const int64_t u = in.u0 + in_tile * kTile + lane;
+      const int64_t pos = u < in.z.sinks ? u : u + in.z.skip;
+      const int col = static_cast<int>(pos / p.page_size);
+      in_slot = static_cast<int>(pos - static_cast<int64_t>(col) * p.page_size);
+      in_page = p.table[in.z.row * p.t_sr + col];
+      if (in_page < 0 || in_page >= p.pages) in_page = -2;  // refused
+    }
+  };
+  const unsigned kc = p.d / 8, vc = p.dv / 8;  // 16-byte chunks of a row
+  auto fetch = [&](int stage) {
+    if (!in_done) {
+      const uint32_t dst = my_ring + stage * L::kStage;
+      const int hk = in.hg / hblocks;
+      const char* kb = static_cast<const char*>(p.k) + hk * p.k_sh * 2;
+      const char* vb = static_cast<const char*>(p.v) + hk * p.v_sh * 2;
+      const int lost = __any_sync(0xffffffffu, in_page == -2);
+      if (lane == 0) misc[warp * 8 + stage] = lost;
+      // DP / 8 chunks per row: a warp covers `rows` rows per step
+      constexpr int kChunks = DP / 8;
+      constexpr int kRows = kChunks >= 32 ? 1 : 32 / kChunks;
+      const unsigned ch = lane % kChunks;
+#pragma unroll
+      for (int r0 = 0; r0 < kTile; r0 += kRows) {
+        const int r = r0 + lane / kChunks;
+        const int page = __shfl_sync(0xffffffffu, in_page, r);
+        const int slot = __shfl_sync(0xffffffffu, in_slot, r);
+        const bool on = page >= 0;
+        const uint32_t d = dst + r * L::kRow + ((ch ^ (r & 7)) << 4);
+        const char* ks = on ? kb + (page * p.k_sp + slot * p.k_st) * 2 + ch * 16 : kb;
+        const char* vs = on ? vb + (page * p.v_sp + slot * p.v_st) * 2 + ch * 16 : vb;
+        if (ch < kc) cp_async16(d, ks, on);
+        if (ch < vc) cp_async16(d + kTile * L::kRow, vs, on);
+      }
+      if (in_tile == warp) {  // the item's queries travel with its first tile
+        const int h0 = hk * p.group + (in.hg - hk * hblocks) * HB;
+        const int nh = min(HB, p.group - (in.hg - hk * hblocks) * HB);
+        const char* qb = static_cast<const char*>(p.q) + (in.b * p.q_sb + h0 * p.q_sh) * 2;
+#pragma unroll
+        for (int r0 = 0; r0 < HB; r0 += kRows) {
+          const int r = r0 + lane / kChunks;
+          const uint32_t d = dst + 2 * kTile * L::kRow + r * L::kRow + ((ch ^ (r & 7)) << 4);
+          if (ch < kc) cp_async16(d, r < nh ? qb + r * p.q_sh * 2 + ch * 16 : qb, r < nh);
+        }
+      }
+      in_tile += kMmaWarps;
+      look_up();
+    }
+    cp_async_commit();
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < S; ++s) fetch(s);
+
+  // ------------------------------------------------------------- consumer side
+  const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
+  int stage = 0;
+  for (int64_t item = list ? blockIdx.x : 0; item < total; item += gridDim.x) {
+    PagedItem it;
+    decode(item, it);
+    const int hk = it.hg / hblocks, hb = it.hg - hk * hblocks;
+    const int h0 = hk * p.group + hb * HB, nh = min(HB, p.group - hb * HB);
+    int bad = it.z.row < 0;
+    float m[NH][2], l[NH][2], o[DP / 16][NH][4];
+    uint32_t qf[DP / 16][NH][2];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
+    }
+    for (int tile = warp; tile * kTile < it.tokens; tile += kMmaWarps) {
+      cp_async_wait<S - 1>();
+      __syncwarp();
+      const uint32_t sk = my_ring + stage * L::kStage;
+      const uint32_t sv = sk + kTile * L::kRow, sq = sv + kTile * L::kRow;
+      bad |= misc[warp * 8 + stage];
+      if (tile == warp) {
+        // B operand: heads in rows of 8, four 8-dim chunks per ldmatrix
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int t = 0; t < DP / 16; t += 2) {
+            uint32_t r[4];
+            const int row = n * 8 + (lane & 7), ch = t * 2 + (lane >> 3);
+            ldsm_x4(sq + row * L::kRow + ((ch ^ (row & 7)) << 4), r);
+            qf[t][n][0] = r[0];
+            qf[t][n][1] = r[1];
+            qf[t + 1][n][0] = r[2];
+            qf[t + 1][n][1] = r[3];
+          }
+      }
+      float s[NH][4];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) {
+        if (t < ksteps) {
+          uint32_t a[4];
+          const int row = lane & 15, ch = t * 2 + (lane >> 4);
+          ldsm_x4(sk + row * L::kRow + ((ch ^ (row & 7)) << 4), a);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma16816<T>(s[n], a, qf[t][n][0], qf[t][n][1]);
+        }
+      }
+      // rows of s: keys lane / 4 and lane / 4 + 8; columns: heads 2 (lane % 4) + {0, 1}
+      const int left = it.tokens - tile * kTile;
+      const bool on0 = (lane >> 2) < left, on1 = (lane >> 2) + 8 < left;
+      uint32_t pf[NH][2];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float s0 = on0 ? s[n][e] * p.scale_log2 : -INFINITY;
+          const float s1 = on1 ? s[n][2 + e] * p.scale_log2 : -INFINITY;
+          float top = fmaxf(s0, s1);
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          top = fmaxf(top, m[n][e]);
+          f[e] = m[n][e] == -INFINITY ? 0.f : exp2f(m[n][e] - top);
+          m[n][e] = top;
+          s[n][e] = s0 == -INFINITY ? 0.f : exp2f(s0 - top);
+          s[n][2 + e] = s1 == -INFINITY ? 0.f : exp2f(s1 - top);
+        }
+        float r00, r01, r10, r11;
+        pf[n][0] = mov_trans(pack2<T>(s[n][0], s[n][1], r00, r01));
+        pf[n][1] = mov_trans(pack2<T>(s[n][2], s[n][3], r10, r11));
+        l[n][0] = l[n][0] * f[0] + (r00 + r10);
+        l[n][1] = l[n][1] * f[1] + (r01 + r11);
+        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) {
+            o[t][n][0] *= f[0];
+            o[t][n][1] *= f[1];
+            o[t][n][2] *= f[0];
+            o[t][n][3] *= f[1];
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) {
+        if (t < vsteps) {
+          uint32_t a[4];
+          const int i = lane >> 3, row = (lane & 7) + (i & 2) * 4, ch = t * 2 + (i & 1);
+          ldsm_x4_t(sv + row * L::kRow + ((ch ^ (row & 7)) << 4), a);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma16816<T>(o[t][n], a, pf[n][0], pf[n][1]);
+        }
+      }
+      __syncwarp();
+      fetch(stage);
+      stage = stage + 1 == S ? 0 : stage + 1;
+    }
+    // ------------------------------------------------------- the item's result
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+        const int h = n * 8 + 2 * (lane & 3) + e;
+        if (lane < 4) part_ml[warp * HB + h] = make_float2(m[n][e], l[n][e]);
+        float* row = part + (warp * HB + h) * L::kPitch + (lane >> 2);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+          if (t < vsteps) {
+            row[t * 16] = o[t][n][e];
+            row[t * 16 + 8] = o[t][n][2 + e];
+          }
+        }
+      }
+    }
+    bad = __syncthreads_or(bad);
+    if (bad && threadIdx.x == 0) raise_status(p.status, BIO_DEV_INDEX);
+    const int quads = p.dv / 4;
+    for (int i = threadIdx.x; i < nh * quads; i += blockDim.x) {
+      const int h = i / quads, e = (i - h * quads) * 4;
+      float top = -INFINITY, w[kMmaWarps], sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < kMmaWarps; ++x) top = fmaxf(top, part_ml[x * HB + h].x);
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int x = 0; x < kMmaWarps; ++x) {
+        const float2 ml = part_ml[x * HB + h];
+        w[x] = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+        sum = fmaf(ml.y, w[x], sum);
+        const float4 a =
+            *reinterpret_cast<const float4*>(part + (x * HB + h) * L::kPitch + e);
+        y.x = fmaf(a.x, w[x], y.x);
+        y.y = fmaf(a.y, w[x], y.y);
+        y.z = fmaf(a.z, w[x], y.z);
+        y.w = fmaf(a.w, w[x], y.w);
+      }
+      const int64_t bh = it.b * p.heads + h0 + h;
+      if (it.pieces == 1) {
+        const bool none = bad || sum == 0.f;
+        T* out = static_cast<T*>(p.o) + it.b * p.o_sb + (h0 + h) * p.o_sh + e;
+        out[0] = from_f32<T>(none ? 0.f : y.x / sum);
+        out[1] = from_f32<T>(none ? 0.f : y.y / sum);
+        out[2] = from_f32<T>(none ? 0.f : y.z / sum);
+        out[3] = from_f32<T>(none ? 0.f : y.w / sum);
+      } else {
+        *reinterpret_cast<float4*>(p.acc + (bh * p.max_pieces + it.piece) * p.dvp + e) = y;
+        if (e == 0) p.ml[bh * p.max_pieces + it.piece] = make_float2(top, bad ? -1.f : sum);
+      }
+    }
+    __syncthreads();  // the partial results are free for the next item
+  }
+  cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------------------
 // Joins the pieces of one (row, head): weights e^(m_i - max m), eight warps
 // take the pieces i = warp, warp + 8, ... and are added in order.
 // ---------------------------------------------------------------------------
@@ -374,6 +816,44 @@ int dispatch_simt(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   return wide ? launch_simt<T, 1, 16, VEC>(p, batch, s) : launch_simt<T, 1, 8, VEC>(p, batch, s);
 }
 
+template <typename T, int DP, int NH>
+int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
+  using L = bio::PagedSmem<DP, NH>;
+  static std::once_flag once[bio_host::kMaxDevices];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= bio_host::kMaxDevices)
+    return BIO_ERR_LAUNCH;
+  cudaError_t set = cudaSuccess;
+  std::call_once(once[device], [&] {
+    set = cudaFuncSetAttribute(bio::paged_mma_kernel<T, DP, NH>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  });
+  if (set != cudaSuccess) return BIO_ERR_LAUNCH;
+  const int64_t slots = static_cast<int64_t>(bio_host::sm_count(device)) * L::kCtas;
+  const int64_t items =
+      batch * p.kv_heads * ((p.group + 8 * NH - 1) / (8 * NH)) * p.max_pieces;
+  // A block per possible item when they run in a few rounds: blocks of pieces
+  // that a row does not have end at once.  Beyond, every block builds the list
+  // of the items that exist and walks it.
+  const bool list = items > 4 * slots && batch <= bio::kListRows;
+  const int64_t grid = list ? slots : items;
+  if (slots <= 0) return BIO_ERR_LAUNCH;
+  bio::paged_mma_kernel<T, DP, NH>
+      <<<static_cast<unsigned>(grid), bio::kMmaWarps * 32, L::kBytes, s>>>(p, batch, list ? 1 : 0);
+  return bio_host::launch_status(cudaGetLastError());
+}
+
+template <typename T>
+int dispatch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
+  const int dim = p.d > p.dv ? p.d : p.dv;
+  // 16 heads at once halve the cache traffic of wide groups; at 256 columns
+  // their partial results would not leave room for the ring
+  if (dim > 128) return launch_mma<T, 256, 1>(p, batch, s);
+  if (dim > 64)
+    return p.group > 8 ? launch_mma<T, 128, 2>(p, batch, s) : launch_mma<T, 128, 1>(p, batch, s);
+  return p.group > 8 ? launch_mma<T, 64, 2>(p, batch, s) : launch_mma<T, 64, 1>(p, batch, s);
+}
+
 template <typename T>
 int run(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   int st;
@@ -384,7 +864,11 @@ int run(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
     st = bits % 16 == 0 ? dispatch_simt<T, true>(p, batch, s)
                         : dispatch_simt<T, false>(p, batch, s);
   } else {
-    st = dispatch_simt<T, false>(p, batch, s);
+    const uint64_t bits = reinterpret_cast<uint64_t>(p.q) | reinterpret_cast<uint64_t>(p.k) |
+                          reinterpret_cast<uint64_t>(p.v) |
+                          2 * static_cast<uint64_t>(p.q_sb | p.q_sh | p.k_sp | p.k_sh | p.k_st |
+                                                    p.v_sp | p.v_sh | p.v_st | p.d | p.dv);
+    st = bits % 16 == 0 ? dispatch_mma<T>(p, batch, s) : dispatch_simt<T, false>(p, batch, s);
   }
   if (st != BIO_OK || p.max_pieces == 1) return st;
   cudaLaunchConfig_t cfg = {};
