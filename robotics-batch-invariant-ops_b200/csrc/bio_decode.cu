@@ -1,17 +1,20 @@
 // Attention of one new token per sequence over a paged key/value cache.
 //
-// For query head h of row b, with the n tokens that its window leaves visible,
-//   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q.k_j,  m = max s_j.
-// The visible tokens are cut into pieces of piece_tokens(n) tokens.  One block
-// takes one piece of one row for the query heads that share a KV head (each
-// key and value is read once for all of them) and leaves the piece's maximum,
-// sum and unnormalised output in fp32; a second kernel joins the pieces in
-// their order.  A row that fits in one piece is finished by the first kernel.
-// The piece size depends on n alone, so a row's bits do not depend on the
-// batch.  Scores are kept in units of log2 (scale * log2(e) goes into q).
+// For query head h of row b, with the tokens V that its window leaves visible,
+//   o = sum_V e^(s_j - m) v_j / sum_V e^(s_j - m),  s_j = scale q.k_j,  m = max s_j.
+// A row's cache is a list of 16-token tiles (those with a visible token), cut
+// into pieces of piece_tiles() tiles.  One block takes one piece of one row for
+// the query heads that share a KV head (each key and value is read once for
+// all of them) and leaves the piece's maximum, sum and unnormalised output in
+// fp32; a second kernel joins the pieces in their order.  A row that fits in
+// one piece is finished by the first kernel.  Tiles and pieces depend on the
+// row's own length and window alone, so its bits do not depend on the batch.
+// Scores are kept in units of log2 (the scale carries log2(e)).
 //
 // Not in the reference, which keeps no cache between calls.
+#include <algorithm>
 #include <mutex>
+#include <numeric>
 
 #include "bio_common.cuh"
 
@@ -28,7 +31,9 @@ struct PagedParams {
   const int32_t* table;
   const int32_t* lens;
   const int32_t* rows;
-  int64_t window, sinks;
+  int window, sinks;   // window 0: everything is visible
+  int max_len;         // tokens that a row of the table can hold
+  int box_rows;        // tokens of a TMA box: gcd(page size, tile)
   float scale_log2;
   int64_t max_pieces;  // most pieces that any row can have
   int dvp;             // floats between partial outputs
@@ -37,38 +42,50 @@ struct PagedParams {
   int* status;
 };
 
-// Tokens of a piece of a row that sees n tokens.  Short pieces spread one
-// sequence over the SMs; long rows take longer ones, since every piece costs a
-// write and a read of its fp32 output.
-__host__ __device__ __forceinline__ int piece_tokens(int64_t n) {
-  return n <= 1024 ? 64 : n <= 8192 ? 128 : n <= 32768 ? 256 : 512;
+constexpr int kTile = 16;  // tokens of a tile
+
+// Tiles of a piece of a row of n tiles.  Short pieces spread one sequence over
+// the SMs; long rows take longer ones, since every piece costs a write and a
+// read of its fp32 output.
+__host__ __device__ __forceinline__ int piece_tiles(int n) {
+  return n <= 64 ? 4 : n <= 512 ? 8 : n <= 2048 ? 16 : 32;
 }
 
-// What row b sees: tokens u = 0..n-1, token u at position u < sinks ? u : u + skip.
+__host__ __device__ __forceinline__ int pieces_of(int tiles) {
+  const int c = piece_tiles(tiles);
+  return (tiles + c - 1) / c;
+}
+
+// What a row sees: token j with j < len and (j < sinks or j >= start).  Tile t
+// of the row is the tile t < head ? t : t + jump of its tokens.  Positions fit
+// in 32 bits: the table's width times the page size does.
 struct Visible {
-  int64_t row;  // row of the table, -1 if refused
-  int64_t n, sinks, skip;
+  int row;  // row of the table, -1 if refused
+  int len, sinks, start;
+  int head, jump, tiles;
+  __device__ __forceinline__ int base(int t) const { return (t < head ? t : t + jump) * kTile; }
+  __device__ __forceinline__ bool sees(int j) const {
+    return j < len && (j < sinks || j >= start);
+  }
 };
 
-__device__ __forceinline__ Visible visible_of(const PagedParams& p, int64_t b) {
+// The row of query b and its length; (-1, 0) if one of them is out of range.
+__device__ __forceinline__ int2 row_of(const PagedParams& p, int64_t b) {
+  const int row = p.rows != nullptr ? p.rows[b] : static_cast<int>(b);
+  if (row < 0 || row >= p.table_rows) return make_int2(-1, 0);
+  const int len = p.lens[row];
+  return len < 0 || len > p.max_len ? make_int2(-1, 0) : make_int2(row, len);
+}
+
+__device__ __forceinline__ Visible visible_of(const PagedParams& p, int2 row_len) {
   Visible z;
-  z.row = p.rows != nullptr ? p.rows[b] : b;
-  z.n = z.sinks = z.skip = 0;
-  if (z.row < 0 || z.row >= p.table_rows) {
-    z.row = -1;
-    return z;
-  }
-  const int64_t len = p.lens[z.row];
-  if (len < 0 || len > p.table_width * p.page_size) {
-    z.row = -1;
-    return z;
-  }
-  z.n = len;
-  if (p.window > 0 && p.window < len) {
-    z.sinks = min(p.sinks, len - p.window);
-    z.skip = len - p.window - z.sinks;
-    z.n = p.window + z.sinks;
-  }
+  z.row = row_len.x;
+  z.len = row_len.y;
+  z.start = p.window > 0 && p.window < z.len ? z.len - p.window : 0;
+  z.sinks = min(p.sinks, z.start);
+  z.head = z.sinks / kTile + (z.sinks % kTile != 0);
+  z.jump = max(0, z.start / kTile - z.head);
+  z.tiles = z.len / kTile + (z.len % kTile != 0) - z.jump;
   return z;
 }
 
@@ -133,9 +150,8 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
   const int h0 = hk * p.group + hb * HB;              // first query head
   const int nh = min(HB, p.group - hb * HB);
 
-  const Visible z = visible_of(p, b);
-  const int c = piece_tokens(z.n);
-  const int64_t pieces = (z.n + c - 1) / c;
+  const Visible z = visible_of(p, row_of(p, b));
+  const int c = piece_tiles(z.tiles), pieces = pieces_of(z.tiles);
   if (piece > 0 && piece >= pieces) return;
   int bad = z.row < 0;
 
@@ -158,18 +174,18 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
   }
   const T* kb = static_cast<const T*>(p.k) + hk * p.k_sh;
   const T* vb = static_cast<const T*>(p.v) + hk * p.v_sh;
-  const int64_t u1 = min(z.n, (piece + 1) * c);
-  for (int64_t u0 = piece * c + warp * kKeys; u0 < u1; u0 += kSimtWarps * kKeys) {
-    const int64_t u = u0 + sub;
-    const int64_t pos = u < z.sinks ? u : u + z.skip;
-    const int64_t col = pos / p.page_size;
-    bool on = u < u1;
+  const int t0 = static_cast<int>(piece) * c, left = min(c, z.tiles - t0) * kTile;
+  for (int x0 = warp * kKeys; x0 < left; x0 += kSimtWarps * kKeys) {
+    const int x1 = x0 + sub;  // kKeys divides the tile: all of them lie in one
+    const int pos = z.base(t0 + x1 / kTile) + x1 % kTile;
+    const int col = pos / p.page_size;
+    bool on = z.sees(pos);
     const int page = on ? p.table[z.row * p.t_sr + col] : 0;
     if (page < 0 || page >= p.pages) {
       bad = 1;
       on = false;
     }
-    const int64_t slot = pos - col * p.page_size;
+    const int slot = pos - col * p.page_size;
     float kx[kLaneDims], vx[kLaneDims];
     load_dims<T, LPK, VEC>(kb + page * p.k_sp + slot * p.k_st, li, p.d, on, kx);
     load_dims<T, LPK, VEC>(vb + page * p.v_sp + slot * p.v_st, li, p.dv, on, vx);
@@ -250,13 +266,14 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 }
 
 // ---------------------------------------------------------------------------
-// 16-bit kernel: cp.async into swizzled shared memory, m16n8k16 products.
+// 16-bit kernel: TMA into swizzled shared memory, m16n8k16 products.
 //
 // Four warps share an item (one piece of one row for 8 * NH query heads of one
-// KV head); warp w takes the 16-token tiles w, w + 4, ....  Every warp has its
+// KV head); warp w takes the piece's tiles w, w + 4, ....  Every warp has its
 // own ring of S stages, each a tile's keys, values and the item's queries, and
 // refills a stage as soon as it has used it, across item borders, so the loads
-// never wait for the arithmetic.  Per tile:
+// never wait for the arithmetic.  A tile is fetched in boxes of 64 columns by
+// R tokens, R = gcd(page size, 16), so a box never leaves its page.  Per tile:
 //   S^T [16 keys x 8 heads] = K [16 x d] Q^T     A: ldmatrix, B: ldmatrix of Q
 //   p = 2^(s - m) in the accumulator layout, rounded to T; movmatrix turns its
 //   8 x 8 halves into the B operand of
@@ -266,40 +283,34 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 // holds that pair of O.  The cache is read once at a few flops per byte: what
 // bounds it is HBM, not the products (m16n8k16 covers 2048 products per
 // instruction; the tcgen05 tile of 128 rows would be 15/16 padding here).
+// Loads by TMA rather than per lane: copying a tile lane by lane took more
+// instructions than the arithmetic (1080 against about 350 per tile, and
+// 636 us against the time below on 128 rows of 1..8192 tokens).
 // ---------------------------------------------------------------------------
 constexpr int kMmaWarps = 4;
-constexpr int kTile = 16;         // tokens of a tile
 constexpr int kListRows = 1024;   // rows whose piece counts fit in shared memory
 
 template <int DP, int NH>
 struct PagedSmem {
-  static constexpr int kRow = DP * 2;                       // bytes of a token's row
-  static constexpr int kStage = 2 * kTile * kRow + 8 * NH * kRow;
+  static constexpr int kBlocks = DP / 64;                   // 64-column blocks
+  static constexpr int kKv = kTile * 128 * kBlocks;         // keys (or values) of a tile
+  static constexpr int kQ = 8 * NH * 128 * kBlocks;
+  static constexpr int kStage = 2 * kKv + kQ;
   static constexpr int kPitch = DP + 4;                     // floats, spreads the banks
   static constexpr int kPart = kMmaWarps * 8 * NH * kPitch * 4;
-  static constexpr int kList = (kListRows + 4) * 4;
-  static constexpr int kMisc = kMmaWarps * 8 * NH * 8 + 64 * 4 + kList;
+  static constexpr int kList = (3 * kListRows + 4) * 4;
+  static constexpr int kBars = kMmaWarps * 8 * 8;
+  static constexpr int kMisc = kBars + kMmaWarps * 8 * NH * 8 + 64 * 4 + kList;
   // two CTAs per SM where two stages fit, else one with as many as fit
-  static constexpr int kTwo = (113 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
-  static constexpr int kOne = (226 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
+  static constexpr int kTwo = (112 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
+  static constexpr int kOne = (225 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
   static constexpr int kCtas = kTwo >= 2 ? 2 : 1;
   static constexpr int kStages = kTwo >= 2 ? (kTwo > 4 ? 4 : kTwo) : (kOne > 6 ? 6 : kOne);
-  static constexpr int kBytes = kPart + kMisc + kMmaWarps * kStages * kStage;
-  static_assert(kStages >= 2, "a ring needs two stages");
+  static constexpr int kBytes = 1024 + kPart + kMisc + kMmaWarps * kStages * kStage;
+  static_assert(kStages >= 2 && kStages <= 8, "a ring needs two stages");
+  static_assert(kStage % 1024 == 0, "the swizzle counts from 1024-byte borders");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(on ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -315,6 +326,13 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ uint32_t mov_trans(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// 2^x on the special-function unit (PTX ex2.approx: 2 ulp, 2^-inf = 0).
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -357,50 +375,57 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b, float& ra, f
 }
 
 struct PagedItem {
-  int64_t b;       // query
   Visible z;
+  int b;           // query
   int hg;          // KV head * blocks of heads + block
-  int64_t piece, pieces;
-  int64_t u0;      // first token of the piece
-  int tokens;
+  int piece, pieces;
+  int t0, tiles;   // of the piece
 };
 
 template <typename T, int DP, int NH>
 __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
-    paged_mma_kernel(const PagedParams p, int64_t batch, int list) {
+    paged_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const PagedParams p, int64_t batch,
+                     int list) {
   using L = PagedSmem<DP, NH>;
   constexpr int S = L::kStages, HB = 8 * NH;
-  extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* ring = smem;
+  extern __shared__ uint8_t smem[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
   float* part = reinterpret_cast<float*>(ring + kMmaWarps * S * L::kStage);
   float2* part_ml = reinterpret_cast<float2*>(part + L::kPart / 4);
-  int* misc = reinterpret_cast<int*>(part_ml + kMmaWarps * HB);  // [0..31] stage flags, [32..] bad
-  int* first = misc + 64;          // list: items before row b, [batch + 1]
-  int* scan = misc + 40;           // list: sums of the four warps
+  uint64_t* bars = reinterpret_cast<uint64_t*>(part_ml + kMmaWarps * HB);  // [warps][8]
+  int* misc = reinterpret_cast<int*>(bars + kMmaWarps * 8);  // [0..31] a stage's refused pages
+  int2* rows = reinterpret_cast<int2*>(misc + 64);  // table row and length of query b
+  int* first = misc + 64 + 2 * kListRows;           // list: items before query b, [batch + 1]
+  int* scan = misc + 40;                            // list: sums of the four warps
+  volatile int* abort_flag = misc + 48;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hblocks = (p.group + HB - 1) / HB;
   const int hgs = p.kv_heads * hblocks;
 
-  // columns past d / dv are never written by the copies: zero the ring once
-  if (p.d < DP || p.dv < DP) {
-    uint4* z = reinterpret_cast<uint4*>(ring);
-    for (int i = threadIdx.x; i < kMmaWarps * S * L::kStage / 16; i += blockDim.x)
-      z[i] = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kMmaWarps * 8; ++i) mbar_init(&bars[i], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
-  auto pieces_of = [&](const Visible& z) -> int64_t {
-    const int c = piece_tokens(z.n);
-    const int64_t k = (z.n + c - 1) / c;
-    return k > 1 ? k : 1;  // an empty or refused row has one item, which writes zeros
-  };
-  int64_t total = 1;
+  // an empty or refused row has one item, which writes zeros
+  int total = 1;
   if (list) {
     // items of every row, as a running sum in shared memory
     int carry = 0;
-    for (int64_t b0 = 0; b0 < batch; b0 += blockDim.x) {
-      const int64_t b = b0 + threadIdx.x;
-      const int mine = b < batch ? static_cast<int>(pieces_of(visible_of(p, b))) * hgs : 0;
+    for (int b0 = 0; b0 < batch; b0 += blockDim.x) {
+      const int b = b0 + threadIdx.x;
+      int mine = 0;
+      if (b < batch) {
+        rows[b] = row_of(p, b);
+        mine = max(1, pieces_of(visible_of(p, rows[b]).tiles)) * hgs;
+      }
       int inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -421,50 +446,53 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
     }
     if (threadIdx.x == 0) first[batch] = carry;
     total = carry;
+  } else if (threadIdx.x == 0) {
+    rows[0] = row_of(p, blockIdx.x / (static_cast<unsigned>(p.max_pieces) * hgs));
   }
   __syncthreads();
 
   // item number -> what to do; without a list the block has one item
-  auto decode = [&](int64_t item, PagedItem& it) {
-    int64_t rest;
+  auto decode = [&](int item, PagedItem& it) {
+    unsigned rest;
+    int slot = 0;
     if (list) {
-      int lo = 0, hi = static_cast<int>(batch);
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= item) lo = mid; else hi = mid;
+      int hi = static_cast<int>(batch);
+      while (hi - slot > 1) {
+        const int mid = (slot + hi) >> 1;
+        if (first[mid] <= item) slot = mid; else hi = mid;
       }
-      it.b = lo;
-      rest = item - first[lo];
-      it.hg = static_cast<int>(rest % hgs);
+      it.b = slot;
+      rest = item - first[slot];
       it.piece = rest / hgs;
+      it.hg = rest - it.piece * hgs;
     } else {
-      rest = blockIdx.x;
-      it.piece = rest % p.max_pieces;
-      rest /= p.max_pieces;
-      it.hg = static_cast<int>(rest % hgs);
+      rest = blockIdx.x / static_cast<unsigned>(p.max_pieces);
+      it.piece = blockIdx.x - rest * static_cast<unsigned>(p.max_pieces);
       it.b = rest / hgs;
+      it.hg = rest - it.b * hgs;
     }
-    it.z = visible_of(p, it.b);
-    const int c = piece_tokens(it.z.n);
-    it.pieces = pieces_of(it.z);
-    it.u0 = it.piece * c;
-    it.tokens = static_cast<int>(max(static_cast<int64_t>(0),
-                                     min(static_cast<int64_t>(c), it.z.n - it.u0)));
+    it.z = visible_of(p, rows[slot]);
+    const int c = piece_tiles(it.z.tiles);
+    it.pieces = max(1, pieces_of(it.z.tiles));
+    it.t0 = it.piece * c;
+    it.tiles = max(0, min(c, it.z.tiles - it.t0));
   };
 
   // ------------------------------------------------------------- producer side
-  // the next tile to fetch: its item, its number, and its tokens' pages
-  const uint32_t my_ring = smem_u32(ring) + warp * (S * L::kStage);
-  int64_t in_item = list ? blockIdx.x : 0;
+  // the next tile to fetch: its item, its number, and its groups' pages
+  uint8_t* my_ring = ring + warp * (S * L::kStage);
+  uint64_t* my_bars = bars + warp * 8;
+  int in_item = list ? blockIdx.x : 0;
   PagedItem in;
   decode(in_item, in);
-  const bool dead = !list && in.piece >= in.pieces;
-  if (dead) return;
+  if (!list && in.piece >= in.pieces) return;
   int in_tile = warp;
   bool in_done = in_item >= total;
-  int in_page = -1, in_slot = 0;  // of token `lane` of the tile (lanes 0..15)
+  const int groups = kTile / p.box_rows, group_mask = groups - 1;
+  int in_page = 0, in_slot = 0;  // of group `lane` of the tile (lanes below groups)
+  bool in_held = false;          // the group has a visible token
   auto look_up = [&]() {
-    while (!in_done && in_tile * kTile >= in.tokens) {
+    while (!in_done && in_tile >= in.tiles) {
       in_item += gridDim.x;
       if (!list || in_item >= total) {
         in_done = true;
@@ -473,56 +501,55 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
         in_tile = warp;
       }
     }
-    in_page = -1;
-    if (!in_done && lane < kTile && in_tile * kTile + lane < in.tokens) {
-      const int64_t u = in.u0 + in_tile * kTile + lane;
-      const int64_t pos = u < in.z.sinks ? u : u + in.z.skip;
-      const int col = static_cast<int>(pos / p.page_size);
-      in_slot = static_cast<int>(pos - static_cast<int64_t>(col) * p.page_size);
-      in_page = p.table[in.z.row * p.t_sr + col];
-      if (in_page < 0 || in_page >= p.pages) in_page = -2;  // refused
+    in_held = false;
+    if (!in_done && lane < groups) {
+      const int pos = in.z.base(in.t0 + in_tile) + lane * p.box_rows;
+      // visible in [pos, pos + box_rows): before the sinks' end, or from start to the length
+      in_held = pos < in.z.sinks || (pos < in.z.len && pos + p.box_rows > in.z.start);
+      if (in_held) {
+        const int col = pos / p.page_size;
+        in_slot = pos - col * p.page_size;
+        // not looked at before the next fetch, so that nobody waits for it here
+        in_page = p.table[in.z.row * p.t_sr + col];
+      }
     }
   };
-  const unsigned kc = p.d / 8, vc = p.dv / 8;  // 16-byte chunks of a row
+  const int kc = (p.d + 63) / 64, vc = (p.dv + 63) / 64;  // 64-column boxes of a row
+  int issued = 0;  // tiles fetched so far
   auto fetch = [&](int stage) {
-    if (!in_done) {
-      const uint32_t dst = my_ring + stage * L::kStage;
-      const int hk = in.hg / hblocks;
-      const char* kb = static_cast<const char*>(p.k) + hk * p.k_sh * 2;
-      const char* vb = static_cast<const char*>(p.v) + hk * p.v_sh * 2;
-      const int lost = __any_sync(0xffffffffu, in_page == -2);
-      if (lane == 0) misc[warp * 8 + stage] = lost;
-      // DP / 8 chunks per row: a warp covers `rows` rows per step
-      constexpr int kChunks = DP / 8;
-      constexpr int kRows = kChunks >= 32 ? 1 : 32 / kChunks;
-      const unsigned ch = lane % kChunks;
-#pragma unroll
-      for (int r0 = 0; r0 < kTile; r0 += kRows) {
-        const int r = r0 + lane / kChunks;
-        const int page = __shfl_sync(0xffffffffu, in_page, r);
-        const int slot = __shfl_sync(0xffffffffu, in_slot, r);
-        const bool on = page >= 0;
-        const uint32_t d = dst + r * L::kRow + ((ch ^ (r & 7)) << 4);
-        const char* ks = on ? kb + (page * p.k_sp + slot * p.k_st) * 2 + ch * 16 : kb;
-        const char* vs = on ? vb + (page * p.v_sp + slot * p.v_st) * 2 + ch * 16 : vb;
-        if (ch < kc) cp_async16(d, ks, on);
-        if (ch < vc) cp_async16(d + kTile * L::kRow, vs, on);
-      }
-      if (in_tile == warp) {  // the item's queries travel with its first tile
+    if (in_done) return;
+    ++issued;
+    const bool refused = in_held && (in_page < 0 || in_page >= p.pages);
+    const int lost = __any_sync(0xffffffffu, refused);
+    const int page = in_held && !refused ? in_page : -1;
+    const int boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+    const int hk = in.hg / hblocks;
+    uint8_t* dst = my_ring + stage * L::kStage;
+    const bool query = in_tile == warp;  // the item's queries travel with its first tile
+    if (lane == 0) {
+      misc[warp * 8 + stage] = lost;
+      mbar_arrive_expect_tx(&my_bars[stage], boxes * (kc + vc) * p.box_rows * 128 +
+                                                 (query ? kc * HB * 128 : 0));
+      if (query) {
         const int h0 = hk * p.group + (in.hg - hk * hblocks) * HB;
-        const int nh = min(HB, p.group - (in.hg - hk * hblocks) * HB);
-        const char* qb = static_cast<const char*>(p.q) + (in.b * p.q_sb + h0 * p.q_sh) * 2;
-#pragma unroll
-        for (int r0 = 0; r0 < HB; r0 += kRows) {
-          const int r = r0 + lane / kChunks;
-          const uint32_t d = dst + 2 * kTile * L::kRow + r * L::kRow + ((ch ^ (r & 7)) << 4);
-          if (ch < kc) cp_async16(d, r < nh ? qb + r * p.q_sh * 2 + ch * 16 : qb, r < nh);
-        }
+        for (int c = 0; c < kc; ++c)
+          tma_load_4d(dst + 2 * L::kKv + c * HB * 128, &tmQ, &my_bars[stage], c * 64, h0, in.b, 0);
       }
-      in_tile += kMmaWarps;
-      look_up();
     }
-    cp_async_commit();
+    __syncwarp();
+    for (int x0 = 0; x0 < groups * (kc + vc); x0 += 32) {
+      const int x = x0 + lane, g = x & group_mask, c = x / groups;
+      const int pg = __shfl_sync(0xffffffffu, page, g);
+      const int slot = __shfl_sync(0xffffffffu, in_slot, g);
+      if (pg >= 0 && c < kc + vc) {
+        const bool key = c < kc;
+        const int cb = key ? c : c - kc;
+        tma_load_4d(dst + (key ? 0 : L::kKv) + cb * (kTile * 128) + g * p.box_rows * 128,
+                    key ? &tmK : &tmV, &my_bars[stage], cb * 64, slot, hk, pg);
+      }
+    }
+    in_tile += kMmaWarps;
+    look_up();
   };
   look_up();
 #pragma unroll
@@ -530,8 +557,15 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
 
   // ------------------------------------------------------------- consumer side
   const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
-  int stage = 0;
-  for (int64_t item = list ? blockIdx.x : 0; item < total; item += gridDim.x) {
+  const uint32_t ring32 = smem_u32(my_ring);
+  int stage = 0, used = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  // byte offset of (row r, 16-byte chunk ch) in 64-column blocks of `rows` rows
+  auto chunk = [](int r, int ch, int rows) -> uint32_t {
+    return (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+  };
+  for (int item = list ? blockIdx.x : 0; item < total; item += gridDim.x) {
     PagedItem it;
     decode(item, it);
     const int hk = it.hg / hblocks, hb = it.hg - hk * hblocks;
@@ -548,12 +582,28 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
     }
-    for (int tile = warp; tile * kTile < it.tokens; tile += kMmaWarps) {
-      cp_async_wait<S - 1>();
-      __syncwarp();
-      const uint32_t sk = my_ring + stage * L::kStage;
-      const uint32_t sv = sk + kTile * L::kRow, sq = sv + kTile * L::kRow;
+    for (int tile = warp; tile < it.tiles; tile += kMmaWarps) {
+      if (ok) ok = mbar_wait(&my_bars[stage], phase, abort_flag, p.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {  // a wait ran out: no more loads, zeros for what is left
+        bad = 1;
+        break;
+      }
+      const uint32_t sk = ring32 + stage * L::kStage, sv = sk + L::kKv, sq = sv + L::kKv;
       bad |= misc[warp * 8 + stage];
+      const int pos = it.z.base(it.t0 + tile);
+      const bool edge =
+          !(pos + kTile <= it.z.len && (pos >= it.z.start || pos + kTile <= it.z.sinks));
+      if (edge) {
+        // tokens out of sight have weight 0, but 0 * NaN is not 0
+        for (int r = 0; r < kTile; ++r)
+          if (!it.z.sees(pos + r))
+            for (int c = lane; c < vc * 8; c += 32)
+              *reinterpret_cast<uint4*>(my_ring + stage * L::kStage + L::kKv +
+                                        chunk(r, c, kTile)) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // the next load of this stage comes after these writes
+        __syncwarp();
+      }
       if (tile == warp) {
         // B operand: heads in rows of 8, four 8-dim chunks per ldmatrix
 #pragma unroll
@@ -562,7 +612,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
           for (int t = 0; t < DP / 16; t += 2) {
             uint32_t r[4];
             const int row = n * 8 + (lane & 7), ch = t * 2 + (lane >> 3);
-            ldsm_x4(sq + row * L::kRow + ((ch ^ (row & 7)) << 4), r);
+            ldsm_x4(sq + chunk(row, ch, HB), r);
             qf[t][n][0] = r[0];
             qf[t][n][1] = r[1];
             qf[t + 1][n][0] = r[2];
@@ -577,14 +627,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
         if (t < ksteps) {
           uint32_t a[4];
           const int row = lane & 15, ch = t * 2 + (lane >> 4);
-          ldsm_x4(sk + row * L::kRow + ((ch ^ (row & 7)) << 4), a);
+          ldsm_x4(sk + chunk(row, ch, kTile), a);
 #pragma unroll
           for (int n = 0; n < NH; ++n) mma16816<T>(s[n], a, qf[t][n][0], qf[t][n][1]);
         }
       }
       // rows of s: keys lane / 4 and lane / 4 + 8; columns: heads 2 (lane % 4) + {0, 1}
-      const int left = it.tokens - tile * kTile;
-      const bool on0 = (lane >> 2) < left, on1 = (lane >> 2) + 8 < left;
+      const bool on0 = !edge || it.z.sees(pos + (lane >> 2));
+      const bool on1 = !edge || it.z.sees(pos + (lane >> 2) + 8);
       uint32_t pf[NH][2];
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
@@ -597,10 +647,12 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
           top = fmaxf(top, m[n][e]);
-          f[e] = m[n][e] == -INFINITY ? 0.f : exp2f(m[n][e] - top);
+          // scores of -inf alone have no maximum to subtract: their weight is 0
+          const float ref = top == -INFINITY ? 0.f : top;
+          f[e] = pow2(m[n][e] - ref);
           m[n][e] = top;
-          s[n][e] = s0 == -INFINITY ? 0.f : exp2f(s0 - top);
-          s[n][2 + e] = s1 == -INFINITY ? 0.f : exp2f(s1 - top);
+          s[n][e] = pow2(s0 - ref);
+          s[n][2 + e] = pow2(s1 - ref);
         }
         float r00, r01, r10, r11;
         pf[n][0] = mov_trans(pack2<T>(s[n][0], s[n][1], r00, r01));
@@ -622,14 +674,18 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
         if (t < vsteps) {
           uint32_t a[4];
           const int i = lane >> 3, row = (lane & 7) + (i & 2) * 4, ch = t * 2 + (i & 1);
-          ldsm_x4_t(sv + row * L::kRow + ((ch ^ (row & 7)) << 4), a);
+          ldsm_x4_t(sv + chunk(row, ch, kTile), a);
 #pragma unroll
           for (int n = 0; n < NH; ++n) mma16816<T>(o[t][n], a, pf[n][0], pf[n][1]);
         }
       }
       __syncwarp();
       fetch(stage);
-      stage = stage + 1 == S ? 0 : stage + 1;
+      ++used;
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
     // ------------------------------------------------------- the item's result
 #pragma unroll
@@ -671,7 +727,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
         y.z = fmaf(a.z, w[x], y.z);
         y.w = fmaf(a.w, w[x], y.w);
       }
-      const int64_t bh = it.b * p.heads + h0 + h;
+      const int64_t bh = static_cast<int64_t>(it.b) * p.heads + h0 + h;
       if (it.pieces == 1) {
         const bool none = bad || sum == 0.f;
         T* out = static_cast<T*>(p.o) + it.b * p.o_sb + (h0 + h) * p.o_sh + e;
@@ -686,7 +742,9 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
     }
     __syncthreads();  // the partial results are free for the next item
   }
-  cp_async_wait<0>();
+  // after a wait that ran out, copies may still be in flight
+  for (; used < issued; ++used)
+    if (!mbar_wait_drain(&my_bars[used % S], (used / S) & 1)) raise_status(p.status, BIO_DEV_TIMEOUT);
 }
 
 // ---------------------------------------------------------------------------
@@ -701,9 +759,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads;
-  const Visible z = visible_of(p, b);
-  const int c = piece_tokens(z.n);
-  const int pieces = static_cast<int>((z.n + c - 1) / c);
+  const int pieces = pieces_of(visible_of(p, row_of(p, b)).tiles);
   if (pieces <= 1) return;
   const float2* ml = p.ml + bh * p.max_pieces;
   float top = -INFINITY;
@@ -758,14 +814,12 @@ namespace {
 
 constexpr int64_t kMaxGrid = 2147483647;
 
-// Most pieces that a row can have when it sees up to `most` tokens.
+// Most pieces that a row of up to `most` tiles can have.
 int64_t most_pieces(int64_t most) {
   int64_t pieces = 1;
-  for (int64_t top : {static_cast<int64_t>(1024), static_cast<int64_t>(8192),
-                      static_cast<int64_t>(32768), most}) {
-    const int64_t n = top < most ? top : most;
-    const int c = bio::piece_tokens(n);
-    const int64_t k = (n + c - 1) / c;
+  for (int64_t top : {static_cast<int64_t>(64), static_cast<int64_t>(512),
+                      static_cast<int64_t>(2048), most}) {
+    const int64_t k = bio::pieces_of(static_cast<int>(top < most ? top : most));
     if (k > pieces) pieces = k;
   }
   return pieces;
@@ -786,8 +840,10 @@ int split_of(const bio_paged_attn_args* a, Split* s) {
     return BIO_ERR_SHAPE;
   if (a->window < 0 || a->window > kMaxGrid || a->sinks < 0 || a->sinks > kMaxGrid)
     return BIO_ERR_ARG;
-  int64_t most = a->table_width * a->page_size;
-  if (a->window > 0 && a->window + a->sinks < most) most = a->window + a->sinks;
+  const int64_t T = bio::kTile;
+  int64_t most = (a->table_width * a->page_size + T - 1) / T;
+  if (a->window > 0)  // the window's tiles, one more where it starts inside one, the sinks'
+    most = std::min(most, (a->window + T - 1) / T + 1 + (a->sinks + T - 1) / T);
   s->pieces = most_pieces(most);
   s->dvp = (a->dv + 3) / 4 * 4;
   if (a->batch > kMaxGrid / a->heads || a->batch * a->heads > kMaxGrid / s->pieces)
@@ -816,6 +872,26 @@ int dispatch_simt(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   return wide ? launch_simt<T, 1, 16, VEC>(p, batch, s) : launch_simt<T, 1, 8, VEC>(p, batch, s);
 }
 
+// Tensor map {column, n1, n2, n3} of 16-bit elements with 128-byte swizzle; element strides.
+template <typename T>
+bool map_of(CUtensorMap* map, const void* ptr, int64_t cols, int64_t n1, int64_t n2, int64_t n3,
+            int64_t s1, int64_t s2, int64_t s3, int rows) {
+  bio_host::EncodeTiledFn enc = bio_host::encode_tiled_fn();
+  if (enc == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(n1),
+                              static_cast<cuuint64_t>(n2), static_cast<cuuint64_t>(n3)};
+  // the stride of a dimension of one element is never used, but has to be valid
+  auto bytes = [](int64_t n, int64_t s) { return static_cast<cuuint64_t>(n > 1 ? 2 * s : 16); };
+  const cuuint64_t strides[3] = {bytes(n1, s1), bytes(n2, s2), bytes(n3, s3)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, ones[4] = {1, 1, 1, 1};
+  return enc(map,
+             std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+             4, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP, int NH>
 int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   using L = bio::PagedSmem<DP, NH>;
@@ -829,6 +905,15 @@ int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
                                cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   });
   if (set != cudaSuccess) return BIO_ERR_LAUNCH;
+  CUtensorMap q, k, v;
+  // a pool without pages is never read: any aligned address will do for its maps
+  const int64_t pages = std::max<int64_t>(p.pages, 1);
+  if (!map_of<T>(&q, p.q, p.d, p.heads, batch, 1, p.q_sh, p.q_sb, 0, 8 * NH) ||
+      !map_of<T>(&k, p.pages > 0 ? p.k : p.q, p.d, p.page_size, p.kv_heads, pages, p.k_st, p.k_sh,
+                 p.k_sp, p.box_rows) ||
+      !map_of<T>(&v, p.pages > 0 ? p.v : p.q, p.dv, p.page_size, p.kv_heads, pages, p.v_st, p.v_sh,
+                 p.v_sp, p.box_rows))
+    return BIO_ERR_ALIGN;
   const int64_t slots = static_cast<int64_t>(bio_host::sm_count(device)) * L::kCtas;
   const int64_t items =
       batch * p.kv_heads * ((p.group + 8 * NH - 1) / (8 * NH)) * p.max_pieces;
@@ -839,7 +924,8 @@ int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   const int64_t grid = list ? slots : items;
   if (slots <= 0) return BIO_ERR_LAUNCH;
   bio::paged_mma_kernel<T, DP, NH>
-      <<<static_cast<unsigned>(grid), bio::kMmaWarps * 32, L::kBytes, s>>>(p, batch, list ? 1 : 0);
+      <<<static_cast<unsigned>(grid), bio::kMmaWarps * 32, L::kBytes, s>>>(q, k, v, p, batch,
+                                                                           list ? 1 : 0);
   return bio_host::launch_status(cudaGetLastError());
 }
 
@@ -868,7 +954,9 @@ int run(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
                           reinterpret_cast<uint64_t>(p.v) |
                           2 * static_cast<uint64_t>(p.q_sb | p.q_sh | p.k_sp | p.k_sh | p.k_st |
                                                     p.v_sp | p.v_sh | p.v_st | p.d | p.dv);
-    st = bits % 16 == 0 ? dispatch_mma<T>(p, batch, s) : dispatch_simt<T, false>(p, batch, s);
+    st = bits % 16 == 0 ? dispatch_mma<T>(p, batch, s) : BIO_ERR_ALIGN;
+    // rows off a 16-byte boundary, or strides that no tensor map takes
+    if (st == BIO_ERR_ALIGN) st = dispatch_simt<T, false>(p, batch, s);
   }
   if (st != BIO_OK || p.max_pieces == 1) return st;
   cudaLaunchConfig_t cfg = {};
@@ -920,8 +1008,11 @@ int bio_paged_attention(const bio_paged_attn_args* a, void* workspace, int64_t w
   p.page_size = static_cast<int>(a->page_size);
   p.d = a->d; p.dv = a->dv;
   p.table = a->page_table; p.lens = a->seq_lens; p.rows = a->rows;
-  p.window = a->window; p.sinks = a->sinks;
+  p.window = static_cast<int>(a->window);
+  p.sinks = static_cast<int>(a->sinks);
+  p.max_len = static_cast<int>(a->table_width * a->page_size);
   p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.box_rows = std::gcd(p.page_size, bio::kTile);
   p.max_pieces = s.pieces;
   p.dvp = s.dvp;
   p.acc = static_cast<float*>(workspace);
