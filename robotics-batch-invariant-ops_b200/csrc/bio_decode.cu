@@ -48,7 +48,7 @@ constexpr int kTile = 16;  // tokens of a tile
 // the SMs; long rows take longer ones, since every piece costs a write and a
 // read of its fp32 output.
 __host__ __device__ __forceinline__ int piece_tiles(int n) {
-  return n <= 64 ? 4 : n <= 512 ? 8 : n <= 2048 ? 16 : 32;
+  return n <= 64 ? 2 : n <= 512 ? 8 : n <= 2048 ? 16 : 32;
 }
 
 __host__ __device__ __forceinline__ int pieces_of(int tiles) {
@@ -268,12 +268,13 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 // ---------------------------------------------------------------------------
 // 16-bit kernel: TMA into swizzled shared memory, m16n8k16 products.
 //
-// Four warps share an item (one piece of one row for 8 * NH query heads of one
-// KV head); warp w takes the piece's tiles w, w + 4, ....  Every warp has its
-// own ring of S stages, each a tile's keys, values and the item's queries, and
-// refills a stage as soon as it has used it, across item borders, so the loads
-// never wait for the arithmetic.  A tile is fetched in boxes of 64 columns by
-// R tokens, R = gcd(page size, 16), so a box never leaves its page.  Per tile:
+// One warp owns one item: a piece of one row for 8 * NH query heads of one KV
+// head.  It walks the piece's tiles through its own ring of S stages, each a
+// tile's keys, values and the item's queries, and refills a stage as soon as
+// it has used it, across item borders, so that loads never wait for the
+// arithmetic and warps never wait for each other.  A tile is fetched in boxes
+// of 64 columns by R tokens, R = gcd(page size, 16), so a box never leaves its
+// page.  Per tile:
 //   S^T [16 keys x 8 heads] = K [16 x d] Q^T     A: ldmatrix, B: ldmatrix of Q
 //   p = 2^(s - m) in the accumulator layout, rounded to T; movmatrix turns its
 //   8 x 8 halves into the B operand of
@@ -283,9 +284,9 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 // holds that pair of O.  The cache is read once at a few flops per byte: what
 // bounds it is HBM, not the products (m16n8k16 covers 2048 products per
 // instruction; the tcgen05 tile of 128 rows would be 15/16 padding here).
-// Loads by TMA rather than per lane: copying a tile lane by lane took more
-// instructions than the arithmetic (1080 against about 350 per tile, and
-// 636 us against the time below on 128 rows of 1..8192 tokens).
+// Measured on 128 rows of 1..8192 tokens (32 heads on 8, d 128, 2.15 GB): lanes
+// copying the tiles by cp.async 636 us, TMA 614 us, both with four warps on an
+// item joining through shared memory.
 // ---------------------------------------------------------------------------
 constexpr int kMmaWarps = 4;
 constexpr int kListRows = 1024;   // rows whose piece counts fit in shared memory
@@ -296,17 +297,14 @@ struct PagedSmem {
   static constexpr int kKv = kTile * 128 * kBlocks;         // keys (or values) of a tile
   static constexpr int kQ = 8 * NH * 128 * kBlocks;
   static constexpr int kStage = 2 * kKv + kQ;
-  static constexpr int kPitch = DP + 4;                     // floats, spreads the banks
-  static constexpr int kPart = kMmaWarps * 8 * NH * kPitch * 4;
   static constexpr int kList = (3 * kListRows + 4) * 4;
-  static constexpr int kBars = kMmaWarps * 8 * 8;
-  static constexpr int kMisc = kBars + kMmaWarps * 8 * NH * 8 + 64 * 4 + kList;
+  static constexpr int kMisc = kMmaWarps * 8 * 8 + 64 * 4 + kList;
   // two CTAs per SM where two stages fit, else one with as many as fit
-  static constexpr int kTwo = (112 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
-  static constexpr int kOne = (225 * 1024 - kPart - kMisc) / (kMmaWarps * kStage);
+  static constexpr int kTwo = (112 * 1024 - kMisc) / (kMmaWarps * kStage);
+  static constexpr int kOne = (225 * 1024 - kMisc) / (kMmaWarps * kStage);
   static constexpr int kCtas = kTwo >= 2 ? 2 : 1;
   static constexpr int kStages = kTwo >= 2 ? (kTwo > 4 ? 4 : kTwo) : (kOne > 6 ? 6 : kOne);
-  static constexpr int kBytes = 1024 + kPart + kMisc + kMmaWarps * kStages * kStage;
+  static constexpr int kBytes = 1024 + kMisc + kMmaWarps * kStages * kStage;
   static_assert(kStages >= 2 && kStages <= 8, "a ring needs two stages");
   static_assert(kStage % 1024 == 0, "the swizzle counts from 1024-byte borders");
 };
@@ -385,18 +383,16 @@ struct PagedItem {
 template <typename T, int DP, int NH>
 __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
     paged_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const PagedParams p, int64_t batch,
-                     int list) {
+                     const __grid_constant__ CUtensorMap tmV, const PagedParams p, int items,
+                     int batch, int list) {
   using L = PagedSmem<DP, NH>;
   constexpr int S = L::kStages, HB = 8 * NH;
   extern __shared__ uint8_t smem[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* part = reinterpret_cast<float*>(ring + kMmaWarps * S * L::kStage);
-  float2* part_ml = reinterpret_cast<float2*>(part + L::kPart / 4);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(part_ml + kMmaWarps * HB);  // [warps][8]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kMmaWarps * S * L::kStage);  // [warps][8]
   int* misc = reinterpret_cast<int*>(bars + kMmaWarps * 8);  // [0..31] a stage's refused pages
-  int2* rows = reinterpret_cast<int2*>(misc + 64);  // table row and length of query b
+  int2* rows = reinterpret_cast<int2*>(misc + 64);  // list: table row and length of query b
   int* first = misc + 64 + 2 * kListRows;           // list: items before query b, [batch + 1]
   int* scan = misc + 40;                            // list: sums of the four warps
   volatile int* abort_flag = misc + 48;
@@ -415,7 +411,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
     tma_prefetch_desc(&tmV);
   }
   // an empty or refused row has one item, which writes zeros
-  int total = 1;
+  int total = items;
   if (list) {
     // items of every row, as a running sum in shared memory
     int carry = 0;
@@ -446,32 +442,32 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
     }
     if (threadIdx.x == 0) first[batch] = carry;
     total = carry;
-  } else if (threadIdx.x == 0) {
-    rows[0] = row_of(p, blockIdx.x / (static_cast<unsigned>(p.max_pieces) * hgs));
   }
   __syncthreads();
 
-  // item number -> what to do; without a list the block has one item
+  // item number -> what to do (without a list: nothing, for a piece that the row lacks)
   auto decode = [&](int item, PagedItem& it) {
     unsigned rest;
-    int slot = 0;
+    int2 row;
     if (list) {
-      int hi = static_cast<int>(batch);
-      while (hi - slot > 1) {
-        const int mid = (slot + hi) >> 1;
-        if (first[mid] <= item) slot = mid; else hi = mid;
+      int lo = 0, hi = batch;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= item) lo = mid; else hi = mid;
       }
-      it.b = slot;
-      rest = item - first[slot];
+      it.b = lo;
+      rest = item - first[lo];
       it.piece = rest / hgs;
       it.hg = rest - it.piece * hgs;
+      row = rows[lo];
     } else {
-      rest = blockIdx.x / static_cast<unsigned>(p.max_pieces);
-      it.piece = blockIdx.x - rest * static_cast<unsigned>(p.max_pieces);
+      rest = static_cast<unsigned>(item) / static_cast<unsigned>(p.max_pieces);
+      it.piece = item - rest * static_cast<unsigned>(p.max_pieces);
       it.b = rest / hgs;
       it.hg = rest - it.b * hgs;
+      row = row_of(p, it.b);
     }
-    it.z = visible_of(p, rows[slot]);
+    it.z = visible_of(p, row);
     const int c = piece_tiles(it.z.tiles);
     it.pieces = max(1, pieces_of(it.z.tiles));
     it.t0 = it.piece * c;
@@ -482,24 +478,21 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
   // the next tile to fetch: its item, its number, and its groups' pages
   uint8_t* my_ring = ring + warp * (S * L::kStage);
   uint64_t* my_bars = bars + warp * 8;
-  int in_item = list ? blockIdx.x : 0;
+  const int step = gridDim.x * kMmaWarps;
+  int in_item = blockIdx.x + gridDim.x * warp, in_tile = 0;
+  bool in_done = in_item >= total;
+  if (in_done) return;  // no barrier of the block follows
   PagedItem in;
   decode(in_item, in);
-  if (!list && in.piece >= in.pieces) return;
-  int in_tile = warp;
-  bool in_done = in_item >= total;
   const int groups = kTile / p.box_rows, group_mask = groups - 1;
   int in_page = 0, in_slot = 0;  // of group `lane` of the tile (lanes below groups)
   bool in_held = false;          // the group has a visible token
   auto look_up = [&]() {
     while (!in_done && in_tile >= in.tiles) {
-      in_item += gridDim.x;
-      if (!list || in_item >= total) {
-        in_done = true;
-      } else {
-        decode(in_item, in);
-        in_tile = warp;
-      }
+      in_item += step;
+      in_tile = 0;
+      in_done = in_item >= total;
+      if (!in_done) decode(in_item, in);
     }
     in_held = false;
     if (!in_done && lane < groups) {
@@ -525,7 +518,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
     const int boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
     const int hk = in.hg / hblocks;
     uint8_t* dst = my_ring + stage * L::kStage;
-    const bool query = in_tile == warp;  // the item's queries travel with its first tile
+    const bool query = in_tile == 0;  // the item's queries travel with its first tile
     if (lane == 0) {
       misc[warp * 8 + stage] = lost;
       mbar_arrive_expect_tx(&my_bars[stage], boxes * (kc + vc) * p.box_rows * 128 +
@@ -548,7 +541,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
                     key ? &tmK : &tmV, &my_bars[stage], cb * 64, slot, hk, pg);
       }
     }
-    in_tile += kMmaWarps;
+    ++in_tile;
     look_up();
   };
   look_up();
@@ -556,18 +549,21 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
   for (int s = 0; s < S; ++s) fetch(s);
 
   // ------------------------------------------------------------- consumer side
-  const int ksteps = (p.d + 15) / 16, vsteps = (p.dv + 15) / 16;
   const uint32_t ring32 = smem_u32(my_ring);
   int stage = 0, used = 0;
   uint32_t phase = 0;
   bool ok = true;
-  // byte offset of (row r, 16-byte chunk ch) in 64-column blocks of `rows` rows
-  auto chunk = [](int r, int ch, int rows) -> uint32_t {
-    return (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-  };
-  for (int item = list ? blockIdx.x : 0; item < total; item += gridDim.x) {
+  // A tile lies in 64-column blocks of 128-byte rows whose 16-byte chunks are
+  // xor-ed with the row: chunk 2 t + c of row r is at (r * 128 + ((c ^ r) * 16))
+  // ^ (t % 4 * 32) of block t / 4, so only an xor is left per k-step.
+  const int qrow = lane & 7, krow = lane & 15, vrow = (lane & 7) + ((lane >> 4) << 3);
+  const uint32_t qoff = qrow * 128 + (((lane >> 3) ^ qrow) << 4);
+  const uint32_t koff = krow * 128 + (((lane >> 4) ^ (krow & 7)) << 4);
+  const uint32_t voff = vrow * 128 + ((((lane >> 3) & 1) ^ (vrow & 7)) << 4);
+  for (int item = blockIdx.x + gridDim.x * warp; item < total; item += step) {
     PagedItem it;
     decode(item, it);
+    if (it.piece >= it.pieces) continue;
     const int hk = it.hg / hblocks, hb = it.hg - hk * hblocks;
     const int h0 = hk * p.group + hb * HB, nh = min(HB, p.group - hb * HB);
     int bad = it.z.row < 0;
@@ -582,7 +578,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
     }
-    for (int tile = warp; tile < it.tiles; tile += kMmaWarps) {
+    for (int tile = 0; tile < it.tiles; ++tile) {
       if (ok) ok = mbar_wait(&my_bars[stage], phase, abort_flag, p.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {  // a wait ran out: no more loads, zeros for what is left
@@ -596,23 +592,23 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
           !(pos + kTile <= it.z.len && (pos >= it.z.start || pos + kTile <= it.z.sinks));
       if (edge) {
         // tokens out of sight have weight 0, but 0 * NaN is not 0
+        uint8_t* v = my_ring + stage * L::kStage + L::kKv;
         for (int r = 0; r < kTile; ++r)
           if (!it.z.sees(pos + r))
             for (int c = lane; c < vc * 8; c += 32)
-              *reinterpret_cast<uint4*>(my_ring + stage * L::kStage + L::kKv +
-                                        chunk(r, c, kTile)) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + (c >> 3) * (kTile * 128) + r * 128 +
+                                        (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();  // the next load of this stage comes after these writes
         __syncwarp();
       }
-      if (tile == warp) {
+      if (tile == 0) {
         // B operand: heads in rows of 8, four 8-dim chunks per ldmatrix
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
           for (int t = 0; t < DP / 16; t += 2) {
             uint32_t r[4];
-            const int row = n * 8 + (lane & 7), ch = t * 2 + (lane >> 3);
-            ldsm_x4(sq + chunk(row, ch, HB), r);
+            ldsm_x4(((sq + n * 1024 + qoff) ^ ((t & 2) << 5)) + (t >> 2) * (HB * 128), r);
             qf[t][n][0] = r[0];
             qf[t][n][1] = r[1];
             qf[t + 1][n][0] = r[2];
@@ -624,26 +620,33 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
       for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
-        if (t < ksteps) {
+        if ((t >> 2) < kc) {
           uint32_t a[4];
-          const int row = lane & 15, ch = t * 2 + (lane >> 4);
-          ldsm_x4(sk + chunk(row, ch, kTile), a);
+          ldsm_x4(((sk + koff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128), a);
 #pragma unroll
           for (int n = 0; n < NH; ++n) mma16816<T>(s[n], a, qf[t][n][0], qf[t][n][1]);
         }
       }
       // rows of s: keys lane / 4 and lane / 4 + 8; columns: heads 2 (lane % 4) + {0, 1}
-      const bool on0 = !edge || it.z.sees(pos + (lane >> 2));
-      const bool on1 = !edge || it.z.sees(pos + (lane >> 2) + 8);
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
+      if (edge) {
+        const bool on0 = it.z.sees(pos + (lane >> 2)), on1 = it.z.sees(pos + (lane >> 2) + 8);
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(e < 2 ? on0 : on1)) s[n][e] = -INFINITY;
+      }
       uint32_t pf[NH][2];
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float s0 = on0 ? s[n][e] * p.scale_log2 : -INFINITY;
-          const float s1 = on1 ? s[n][2 + e] * p.scale_log2 : -INFINITY;
-          float top = fmaxf(s0, s1);
+          float top = fmaxf(s[n][e], s[n][2 + e]);
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
           top = fmaxf(top, m[n][e]);
@@ -651,8 +654,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
           const float ref = top == -INFINITY ? 0.f : top;
           f[e] = pow2(m[n][e] - ref);
           m[n][e] = top;
-          s[n][e] = pow2(s0 - ref);
-          s[n][2 + e] = pow2(s1 - ref);
+          s[n][e] = pow2(s[n][e] - ref);
+          s[n][2 + e] = pow2(s[n][2 + e] - ref);
         }
         float r00, r01, r10, r11;
         pf[n][0] = mov_trans(pack2<T>(s[n][0], s[n][1], r00, r01));
@@ -671,10 +674,9 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
       }
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
-        if (t < vsteps) {
+        if ((t >> 2) < vc) {
           uint32_t a[4];
-          const int i = lane >> 3, row = (lane & 7) + (i & 2) * 4, ch = t * 2 + (i & 1);
-          ldsm_x4_t(sv + chunk(row, ch, kTile), a);
+          ldsm_x4_t(((sv + voff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128), a);
 #pragma unroll
           for (int n = 0; n < NH; ++n) mma16816<T>(o[t][n], a, pf[n][0], pf[n][1]);
         }
@@ -688,6 +690,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
       }
     }
     // ------------------------------------------------------- the item's result
+    if (bad && lane == 0) raise_status(p.status, BIO_DEV_INDEX);
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
 #pragma unroll
@@ -695,52 +698,35 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
         const int h = n * 8 + 2 * (lane & 3) + e;
-        if (lane < 4) part_ml[warp * HB + h] = make_float2(m[n][e], l[n][e]);
-        float* row = part + (warp * HB + h) * L::kPitch + (lane >> 2);
+        if (h >= nh) continue;
+        if (it.pieces == 1) {
+          const bool none = bad || l[n][e] == 0.f;
+          const float inv = 1.f / l[n][e];
+          T* out = static_cast<T*>(p.o) + it.b * p.o_sb + (h0 + h) * p.o_sh;
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t) {
-          if (t < vsteps) {
-            row[t * 16] = o[t][n][e];
-            row[t * 16 + 8] = o[t][n][2 + e];
+          for (int t = 0; t < DP / 16; ++t) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int c = t * 16 + u * 8 + (lane >> 2);
+              if (c < p.dv) out[c] = from_f32<T>(none ? 0.f : o[t][n][2 * u + e] * inv);
+            }
           }
+        } else {
+          const int64_t at = (static_cast<int64_t>(it.b) * p.heads + h0 + h) * p.max_pieces +
+                             it.piece;
+          float* acc = p.acc + at * p.dvp;
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int c = t * 16 + u * 8 + (lane >> 2);
+              if (c < p.dv) acc[c] = o[t][n][2 * u + e];
+            }
+          }
+          if (lane < 4) p.ml[at] = make_float2(m[n][e], bad ? -1.f : l[n][e]);
         }
       }
     }
-    bad = __syncthreads_or(bad);
-    if (bad && threadIdx.x == 0) raise_status(p.status, BIO_DEV_INDEX);
-    const int quads = p.dv / 4;
-    for (int i = threadIdx.x; i < nh * quads; i += blockDim.x) {
-      const int h = i / quads, e = (i - h * quads) * 4;
-      float top = -INFINITY, w[kMmaWarps], sum = 0.f;
-#pragma unroll
-      for (int x = 0; x < kMmaWarps; ++x) top = fmaxf(top, part_ml[x * HB + h].x);
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int x = 0; x < kMmaWarps; ++x) {
-        const float2 ml = part_ml[x * HB + h];
-        w[x] = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-        sum = fmaf(ml.y, w[x], sum);
-        const float4 a =
-            *reinterpret_cast<const float4*>(part + (x * HB + h) * L::kPitch + e);
-        y.x = fmaf(a.x, w[x], y.x);
-        y.y = fmaf(a.y, w[x], y.y);
-        y.z = fmaf(a.z, w[x], y.z);
-        y.w = fmaf(a.w, w[x], y.w);
-      }
-      const int64_t bh = static_cast<int64_t>(it.b) * p.heads + h0 + h;
-      if (it.pieces == 1) {
-        const bool none = bad || sum == 0.f;
-        T* out = static_cast<T*>(p.o) + it.b * p.o_sb + (h0 + h) * p.o_sh + e;
-        out[0] = from_f32<T>(none ? 0.f : y.x / sum);
-        out[1] = from_f32<T>(none ? 0.f : y.y / sum);
-        out[2] = from_f32<T>(none ? 0.f : y.z / sum);
-        out[3] = from_f32<T>(none ? 0.f : y.w / sum);
-      } else {
-        *reinterpret_cast<float4*>(p.acc + (bh * p.max_pieces + it.piece) * p.dvp + e) = y;
-        if (e == 0) p.ml[bh * p.max_pieces + it.piece] = make_float2(top, bad ? -1.f : sum);
-      }
-    }
-    __syncthreads();  // the partial results are free for the next item
   }
   // after a wait that ran out, copies may still be in flight
   for (; used < issued; ++used)
@@ -917,15 +903,16 @@ int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   const int64_t slots = static_cast<int64_t>(bio_host::sm_count(device)) * L::kCtas;
   const int64_t items =
       batch * p.kv_heads * ((p.group + 8 * NH - 1) / (8 * NH)) * p.max_pieces;
-  // A block per possible item when they run in a few rounds: blocks of pieces
-  // that a row does not have end at once.  Beyond, every block builds the list
-  // of the items that exist and walks it.
-  const bool list = items > 4 * slots && batch <= bio::kListRows;
-  const int64_t grid = list ? slots : items;
   if (slots <= 0) return BIO_ERR_LAUNCH;
+  // A few possible items per warp are walked as they are (an item of a piece
+  // that the row does not have costs a look at its length).  Beyond, every
+  // block first builds the list of the items that exist.
+  const bool list = items > 2 * slots * bio::kMmaWarps && batch <= bio::kListRows;
+  // one block per item, until the SMs are full; then a block's warps take items too
+  const int64_t grid = std::min(items, slots);
   bio::paged_mma_kernel<T, DP, NH>
-      <<<static_cast<unsigned>(grid), bio::kMmaWarps * 32, L::kBytes, s>>>(q, k, v, p, batch,
-                                                                           list ? 1 : 0);
+      <<<static_cast<unsigned>(grid), bio::kMmaWarps * 32, L::kBytes, s>>>(
+          q, k, v, p, static_cast<int>(items), static_cast<int>(batch), list ? 1 : 0);
   return bio_host::launch_status(cudaGetLastError());
 }
 
