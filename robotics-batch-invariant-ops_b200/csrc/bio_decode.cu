@@ -2,7 +2,7 @@
 //
 // For query head h of row b, with the tokens V that its window leaves visible,
 //   o = sum_V e^(s_j - m) v_j / sum_V e^(s_j - m),  s_j = scale q.k_j,  m = max s_j.
-// A row's cache is a list of 16-token tiles (those with a visible token), cut
+// A row's cache is a list of 32-token tiles (those with a visible token), cut
 // into pieces of piece_tiles() tiles.  One block takes one piece of one row for
 // the query heads that share a KV head (each key and value is read once for
 // all of them) and leaves the piece's maximum, sum and unnormalised output in
@@ -42,13 +42,13 @@ struct PagedParams {
   int* status;
 };
 
-constexpr int kTile = 16;  // tokens of a tile
+constexpr int kTile = 32;  // tokens of a tile
 
 // Tiles of a piece of a row of n tiles.  Short pieces spread one sequence over
 // the SMs; long rows take longer ones, since every piece costs a write and a
 // read of its fp32 output.
 __host__ __device__ __forceinline__ int piece_tiles(int n) {
-  return n <= 64 ? 2 : n <= 512 ? 8 : n <= 2048 ? 16 : 32;
+  return n <= 32 ? 1 : n <= 256 ? 4 : n <= 1024 ? 8 : 16;
 }
 
 __host__ __device__ __forceinline__ int pieces_of(int tiles) {
@@ -273,11 +273,11 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 // tile's keys, values and the item's queries, and refills a stage as soon as
 // it has used it, across item borders, so that loads never wait for the
 // arithmetic and warps never wait for each other.  A tile is fetched in boxes
-// of 64 columns by R tokens, R = gcd(page size, 16), so a box never leaves its
-// page.  Per tile:
+// of 64 columns by R tokens, R = gcd(page size, 32), so a box never leaves its
+// page.  Per tile, in two halves of 16 tokens:
 //   S^T [16 keys x 8 heads] = K [16 x d] Q^T     A: ldmatrix, B: ldmatrix of Q
 //   p = 2^(s - m) in the accumulator layout, rounded to T; movmatrix turns its
-//   8 x 8 halves into the B operand of
+//   8 x 8 quarters into the B operand of
 //   O^T [d x 8 heads] += V^T [d x 16] P^T        A: ldmatrix.trans
 // Keys are the 16-row side, so a group of 8 heads fills the 8-column side
 // exactly and m, l and the rescale factors of a head pair sit in the lane that
@@ -285,11 +285,11 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 // bounds it is HBM, not the products (m16n8k16 covers 2048 products per
 // instruction; the tcgen05 tile of 128 rows would be 15/16 padding here).
 // Measured on 128 rows of 1..8192 tokens (32 heads on 8, d 128, 2.15 GB): lanes
-// copying the tiles by cp.async 636 us, TMA 614 us, both with four warps on an
-// item joining through shared memory.
+// copying 16-token tiles by cp.async 636 us, TMA 614 us, both with four warps
+// on an item joining through shared memory; a warp per item 450 us, then bound
+// by the serial chain of one warp's instructions, which 32-token tiles halve.
 // ---------------------------------------------------------------------------
-constexpr int kMmaWarps = 4;
-constexpr int kListRows = 1024;   // rows whose piece counts fit in shared memory
+constexpr int kListRows = 512;   // rows whose piece counts fit in shared memory
 
 template <int DP, int NH>
 struct PagedSmem {
@@ -297,15 +297,14 @@ struct PagedSmem {
   static constexpr int kKv = kTile * 128 * kBlocks;         // keys (or values) of a tile
   static constexpr int kQ = 8 * NH * 128 * kBlocks;
   static constexpr int kStage = 2 * kKv + kQ;
-  static constexpr int kList = (3 * kListRows + 4) * 4;
-  static constexpr int kMisc = kMmaWarps * 8 * 8 + 64 * 4 + kList;
-  // two CTAs per SM where two stages fit, else one with as many as fit
-  static constexpr int kTwo = (112 * 1024 - kMisc) / (kMmaWarps * kStage);
-  static constexpr int kOne = (225 * 1024 - kMisc) / (kMmaWarps * kStage);
-  static constexpr int kCtas = kTwo >= 2 ? 2 : 1;
-  static constexpr int kStages = kTwo >= 2 ? (kTwo > 4 ? 4 : kTwo) : (kOne > 6 ? 6 : kOne);
-  static constexpr int kBytes = 1024 + kMisc + kMmaWarps * kStages * kStage;
-  static_assert(kStages >= 2 && kStages <= 8, "a ring needs two stages");
+  static constexpr int kMaxWarps = 12;
+  static constexpr int kMisc = kMaxWarps * 8 * 2 + 72 * 4 + (3 * kListRows + 4) * 4;
+  // one CTA per SM, as many warps as find room with two stages each
+  static constexpr int kStages = 2;
+  static constexpr int kFit = (226 * 1024 - kMisc) / (kStages * kStage);
+  static constexpr int kWarps = kFit > kMaxWarps ? kMaxWarps : kFit;
+  static constexpr int kBytes = 1024 + kMisc + kWarps * kStages * kStage;
+  static_assert(kWarps >= 1 && kBytes <= 227 * 1024, "no room");
   static_assert(kStage % 1024 == 0, "the swizzle counts from 1024-byte borders");
 };
 
@@ -381,21 +380,21 @@ struct PagedItem {
 };
 
 template <typename T, int DP, int NH>
-__global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
+__global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
     paged_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const PagedParams p, int items,
                      int batch, int list) {
   using L = PagedSmem<DP, NH>;
-  constexpr int S = L::kStages, HB = 8 * NH;
+  constexpr int S = L::kStages, W = L::kWarps, HB = 8 * NH;
   extern __shared__ uint8_t smem[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kMmaWarps * S * L::kStage);  // [warps][8]
-  int* misc = reinterpret_cast<int*>(bars + kMmaWarps * 8);  // [0..31] a stage's refused pages
-  int2* rows = reinterpret_cast<int2*>(misc + 64);  // list: table row and length of query b
-  int* first = misc + 64 + 2 * kListRows;           // list: items before query b, [batch + 1]
-  int* scan = misc + 40;                            // list: sums of the four warps
-  volatile int* abort_flag = misc + 48;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + W * S * L::kStage);  // [W][S]
+  int* misc = reinterpret_cast<int*>(bars + W * S);  // [W][S]: a stage's refused pages
+  int* scan = misc + 48;                             // list: sums of the warps
+  volatile int* abort_flag = misc + 64;
+  int2* rows = reinterpret_cast<int2*>(misc + 72);   // list: table row and length of query b
+  int* first = misc + 72 + 2 * kListRows;            // list: items before query b, [batch + 1]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
   const int hgs = p.kv_heads * hblocks;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kMmaWarps * 8; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < W * S; ++i) mbar_init(&bars[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -432,7 +431,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
       __syncthreads();
       int base = carry, sum = 0;
 #pragma unroll
-      for (int w = 0; w < kMmaWarps; ++w) {
+      for (int w = 0; w < W; ++w) {
         if (w < warp) base += scan[w];
         sum += scan[w];
       }
@@ -477,8 +476,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
   // ------------------------------------------------------------- producer side
   // the next tile to fetch: its item, its number, and its groups' pages
   uint8_t* my_ring = ring + warp * (S * L::kStage);
-  uint64_t* my_bars = bars + warp * 8;
-  const int step = gridDim.x * kMmaWarps;
+  uint64_t* my_bars = bars + warp * S;
+  const int step = gridDim.x * W;
   int in_item = blockIdx.x + gridDim.x * warp, in_tile = 0;
   bool in_done = in_item >= total;
   if (in_done) return;  // no barrier of the block follows
@@ -520,7 +519,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
     uint8_t* dst = my_ring + stage * L::kStage;
     const bool query = in_tile == 0;  // the item's queries travel with its first tile
     if (lane == 0) {
-      misc[warp * 8 + stage] = lost;
+      misc[warp * S + stage] = lost;
       mbar_arrive_expect_tx(&my_bars[stage], boxes * (kc + vc) * p.box_rows * 128 +
                                                  (query ? kc * HB * 128 : 0));
       if (query) {
@@ -586,7 +585,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
         break;
       }
       const uint32_t sk = ring32 + stage * L::kStage, sv = sk + L::kKv, sq = sv + L::kKv;
-      bad |= misc[warp * 8 + stage];
+      bad |= misc[warp * S + stage];
       const int pos = it.z.base(it.t0 + tile);
       const bool edge =
           !(pos + kTile <= it.z.len && (pos >= it.z.start || pos + kTile <= it.z.sinks));
@@ -615,38 +614,47 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
             qf[t + 1][n][1] = r[3];
           }
       }
-      float s[NH][4];
-#pragma unroll
-      for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-      for (int t = 0; t < DP / 16; ++t) {
-        if ((t >> 2) < kc) {
-          uint32_t a[4];
-          ldsm_x4(((sk + koff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128), a);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) mma16816<T>(s[n], a, qf[t][n][0], qf[t][n][1]);
-        }
-      }
-      // rows of s: keys lane / 4 and lane / 4 + 8; columns: heads 2 (lane % 4) + {0, 1}
+      // s[half][n]: rows: keys lane / 4 and lane / 4 + 8; columns: heads 2 (lane % 4) + {0, 1}
+      float s[2][NH][4];
 #pragma unroll
       for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
-      if (edge) {
-        const bool on0 = it.z.sees(pos + (lane >> 2)), on1 = it.z.sees(pos + (lane >> 2) + 8);
+        for (int e = 0; e < 4; ++e) s[0][n][e] = s[1][n][e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) {
+        if ((t >> 2) < kc) {
+          const uint32_t at = ((sk + koff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t a[4];
+            ldsm_x4(at + x * 2048, a);
+#pragma unroll
+            for (int n = 0; n < NH; ++n) mma16816<T>(s[x][n], a, qf[t][n][0], qf[t][n][1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!(e < 2 ? on0 : on1)) s[n][e] = -INFINITY;
+          for (int e = 0; e < 4; ++e) s[x][n][e] *= p.scale_log2;
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (it.z.sees(pos + x * 8 + (lane >> 2))) continue;
+#pragma unroll
+          for (int n = 0; n < NH; ++n)
+            s[x >> 1][n][(x & 1) * 2] = s[x >> 1][n][(x & 1) * 2 + 1] = -INFINITY;
+        }
       }
-      uint32_t pf[NH][2];
+      uint32_t pf[2][NH][2];
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(s[n][e], s[n][2 + e]);
+          float top = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
           top = fmaxf(top, m[n][e]);
@@ -654,14 +662,23 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
           const float ref = top == -INFINITY ? 0.f : top;
           f[e] = pow2(m[n][e] - ref);
           m[n][e] = top;
-          s[n][e] = pow2(s[n][e] - ref);
-          s[n][2 + e] = pow2(s[n][2 + e] - ref);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            s[x][n][e] = pow2(s[x][n][e] - ref);
+            s[x][n][2 + e] = pow2(s[x][n][2 + e] - ref);
+          }
         }
-        float r00, r01, r10, r11;
-        pf[n][0] = mov_trans(pack2<T>(s[n][0], s[n][1], r00, r01));
-        pf[n][1] = mov_trans(pack2<T>(s[n][2], s[n][3], r10, r11));
-        l[n][0] = l[n][0] * f[0] + (r00 + r10);
-        l[n][1] = l[n][1] * f[1] + (r01 + r11);
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float r00, r01, r10, r11;
+          pf[x][n][0] = mov_trans(pack2<T>(s[x][n][0], s[x][n][1], r00, r01));
+          pf[x][n][1] = mov_trans(pack2<T>(s[x][n][2], s[x][n][3], r10, r11));
+          sum[0] += r00 + r10;
+          sum[1] += r01 + r11;
+        }
+        l[n][0] = l[n][0] * f[0] + sum[0];
+        l[n][1] = l[n][1] * f[1] + sum[1];
         if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
           for (int t = 0; t < DP / 16; ++t) {
@@ -675,10 +692,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, PagedSmem<DP, NH>::kCtas)
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
         if ((t >> 2) < vc) {
-          uint32_t a[4];
-          ldsm_x4_t(((sv + voff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128), a);
+          const uint32_t at = ((sv + voff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128);
 #pragma unroll
-          for (int n = 0; n < NH; ++n) mma16816<T>(o[t][n], a, pf[n][0], pf[n][1]);
+          for (int x = 0; x < 2; ++x) {
+            uint32_t a[4];
+            ldsm_x4_t(at + x * 2048, a);
+#pragma unroll
+            for (int n = 0; n < NH; ++n) mma16816<T>(o[t][n], a, pf[x][n][0], pf[x][n][1]);
+          }
         }
       }
       __syncwarp();
@@ -803,8 +824,8 @@ constexpr int64_t kMaxGrid = 2147483647;
 // Most pieces that a row of up to `most` tiles can have.
 int64_t most_pieces(int64_t most) {
   int64_t pieces = 1;
-  for (int64_t top : {static_cast<int64_t>(64), static_cast<int64_t>(512),
-                      static_cast<int64_t>(2048), most}) {
+  for (int64_t top : {static_cast<int64_t>(32), static_cast<int64_t>(256),
+                      static_cast<int64_t>(1024), most}) {
     const int64_t k = bio::pieces_of(static_cast<int>(top < most ? top : most));
     if (k > pieces) pieces = k;
   }
@@ -900,18 +921,18 @@ int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
       !map_of<T>(&v, p.pages > 0 ? p.v : p.q, p.dv, p.page_size, p.kv_heads, pages, p.v_st, p.v_sh,
                  p.v_sp, p.box_rows))
     return BIO_ERR_ALIGN;
-  const int64_t slots = static_cast<int64_t>(bio_host::sm_count(device)) * L::kCtas;
+  const int64_t sms = bio_host::sm_count(device);
   const int64_t items =
       batch * p.kv_heads * ((p.group + 8 * NH - 1) / (8 * NH)) * p.max_pieces;
-  if (slots <= 0) return BIO_ERR_LAUNCH;
+  if (sms <= 0) return BIO_ERR_LAUNCH;
   // A few possible items per warp are walked as they are (an item of a piece
   // that the row does not have costs a look at its length).  Beyond, every
   // block first builds the list of the items that exist.
-  const bool list = items > 2 * slots * bio::kMmaWarps && batch <= bio::kListRows;
+  const bool list = items > 2 * sms * L::kWarps && batch <= bio::kListRows;
   // one block per item, until the SMs are full; then a block's warps take items too
-  const int64_t grid = std::min(items, slots);
+  const int64_t grid = std::min(items, sms);
   bio::paged_mma_kernel<T, DP, NH>
-      <<<static_cast<unsigned>(grid), bio::kMmaWarps * 32, L::kBytes, s>>>(
+      <<<static_cast<unsigned>(grid), L::kWarps * 32, L::kBytes, s>>>(
           q, k, v, p, static_cast<int>(items), static_cast<int>(batch), list ? 1 : 0);
   return bio_host::launch_status(cudaGetLastError());
 }
