@@ -34,6 +34,8 @@ struct PagedParams {
   int window, sinks;   // window 0: everything is visible
   int max_len;         // tokens that a row of the table can hold
   int box_rows;        // tokens of a TMA box: gcd(page size, tile)
+  int group_shift;     // log2 of the boxes along a tile
+  unsigned page_mul, page_shift;  // position / page size = (mulhi(position, mul) + position) >> shift
   float scale_log2;
   int64_t max_pieces;  // most pieces that any row can have
   int dvp;             // floats between partial outputs
@@ -54,6 +56,11 @@ __host__ __device__ __forceinline__ int piece_tiles(int n) {
 __host__ __device__ __forceinline__ int pieces_of(int tiles) {
   const int c = piece_tiles(tiles);
   return (tiles + c - 1) / c;
+}
+
+__device__ __forceinline__ int page_of(const PagedParams& p, int pos) {
+  return static_cast<int>((__umulhi(static_cast<unsigned>(pos), p.page_mul) +
+                           static_cast<unsigned>(pos)) >> p.page_shift);
 }
 
 // What a row sees: token j with j < len and (j < sinks or j >= start).  Tile t
@@ -178,7 +185,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
   for (int x0 = warp * kKeys; x0 < left; x0 += kSimtWarps * kKeys) {
     const int x1 = x0 + sub;  // kKeys divides the tile: all of them lie in one
     const int pos = z.base(t0 + x1 / kTile) + x1 % kTile;
-    const int col = pos / p.page_size;
+    const int col = page_of(p, pos);
     bool on = z.sees(pos);
     const int page = on ? p.table[z.row * p.t_sr + col] : 0;
     if (page < 0 || page >= p.pages) {
@@ -374,7 +381,7 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b, float& ra, f
 struct PagedItem {
   Visible z;
   int b;           // query
-  int hg;          // KV head * blocks of heads + block
+  int hk, h0, nh;  // KV head, first query head, number of them
   int piece, pieces;
   int t0, tiles;   // of the piece
 };
@@ -446,7 +453,7 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
 
   // item number -> what to do (without a list: nothing, for a piece that the row lacks)
   auto decode = [&](int item, PagedItem& it) {
-    unsigned rest;
+    unsigned rest, hg;
     int2 row;
     if (list) {
       int lo = 0, hi = batch;
@@ -457,15 +464,19 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
       it.b = lo;
       rest = item - first[lo];
       it.piece = rest / hgs;
-      it.hg = rest - it.piece * hgs;
+      hg = rest - it.piece * hgs;
       row = rows[lo];
     } else {
       rest = static_cast<unsigned>(item) / static_cast<unsigned>(p.max_pieces);
       it.piece = item - rest * static_cast<unsigned>(p.max_pieces);
       it.b = rest / hgs;
-      it.hg = rest - it.b * hgs;
+      hg = rest - it.b * hgs;
       row = row_of(p, it.b);
     }
+    it.hk = hblocks == 1 ? hg : hg / hblocks;
+    const int before = (hg - it.hk * hblocks) * HB;  // heads of the group in earlier blocks
+    it.h0 = it.hk * p.group + before;
+    it.nh = min(HB, p.group - before);
     it.z = visible_of(p, row);
     const int c = piece_tiles(it.z.tiles);
     it.pieces = max(1, pieces_of(it.z.tiles));
@@ -483,7 +494,7 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
   if (in_done) return;  // no barrier of the block follows
   PagedItem in;
   decode(in_item, in);
-  const int groups = kTile / p.box_rows, group_mask = groups - 1;
+  const int groups = 1 << p.group_shift, group_mask = groups - 1;
   int in_page = 0, in_slot = 0;  // of group `lane` of the tile (lanes below groups)
   bool in_held = false;          // the group has a visible token
   auto look_up = [&]() {
@@ -499,7 +510,7 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
       // visible in [pos, pos + box_rows): before the sinks' end, or from start to the length
       in_held = pos < in.z.sinks || (pos < in.z.len && pos + p.box_rows > in.z.start);
       if (in_held) {
-        const int col = pos / p.page_size;
+        const int col = page_of(p, pos);
         in_slot = pos - col * p.page_size;
         // not looked at before the next fetch, so that nobody waits for it here
         in_page = p.table[in.z.row * p.t_sr + col];
@@ -515,7 +526,6 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
     const int lost = __any_sync(0xffffffffu, refused);
     const int page = in_held && !refused ? in_page : -1;
     const int boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
-    const int hk = in.hg / hblocks;
     uint8_t* dst = my_ring + stage * L::kStage;
     const bool query = in_tile == 0;  // the item's queries travel with its first tile
     if (lane == 0) {
@@ -523,21 +533,21 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
       mbar_arrive_expect_tx(&my_bars[stage], boxes * (kc + vc) * p.box_rows * 128 +
                                                  (query ? kc * HB * 128 : 0));
       if (query) {
-        const int h0 = hk * p.group + (in.hg - hk * hblocks) * HB;
         for (int c = 0; c < kc; ++c)
-          tma_load_4d(dst + 2 * L::kKv + c * HB * 128, &tmQ, &my_bars[stage], c * 64, h0, in.b, 0);
+          tma_load_4d(dst + 2 * L::kKv + c * HB * 128, &tmQ, &my_bars[stage], c * 64, in.h0, in.b,
+                      0);
       }
     }
     __syncwarp();
     for (int x0 = 0; x0 < groups * (kc + vc); x0 += 32) {
-      const int x = x0 + lane, g = x & group_mask, c = x / groups;
+      const int x = x0 + lane, g = x & group_mask, c = x >> p.group_shift;
       const int pg = __shfl_sync(0xffffffffu, page, g);
       const int slot = __shfl_sync(0xffffffffu, in_slot, g);
       if (pg >= 0 && c < kc + vc) {
         const bool key = c < kc;
         const int cb = key ? c : c - kc;
         tma_load_4d(dst + (key ? 0 : L::kKv) + cb * (kTile * 128) + g * p.box_rows * 128,
-                    key ? &tmK : &tmV, &my_bars[stage], cb * 64, slot, hk, pg);
+                    key ? &tmK : &tmV, &my_bars[stage], cb * 64, slot, in.hk, pg);
       }
     }
     ++in_tile;
@@ -563,8 +573,6 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
     PagedItem it;
     decode(item, it);
     if (it.piece >= it.pieces) continue;
-    const int hk = it.hg / hblocks, hb = it.hg - hk * hblocks;
-    const int h0 = hk * p.group + hb * HB, nh = min(HB, p.group - hb * HB);
     int bad = it.z.row < 0;
     float m[NH][2], l[NH][2], o[DP / 16][NH][4];
     uint32_t qf[DP / 16][NH][2];
@@ -614,12 +622,13 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
             qf[t + 1][n][1] = r[3];
           }
       }
-      // s[half][n]: rows: keys lane / 4 and lane / 4 + 8; columns: heads 2 (lane % 4) + {0, 1}
-      float s[2][NH][4];
+      // s[half][n]: rows: keys lane / 4 and lane / 4 + 8; columns: heads 2 (lane % 4) + {0, 1}.
+      // Even and odd k-steps have sums of their own: a product waits for the one before it.
+      float s[2][NH][4], s2[2][NH][4];
 #pragma unroll
       for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][n][e] = s[1][n][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[0][n][e] = s[1][n][e] = s2[0][n][e] = s2[1][n][e] = 0.f;
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
         if ((t >> 2) < kc) {
@@ -629,7 +638,8 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
             uint32_t a[4];
             ldsm_x4(at + x * 2048, a);
 #pragma unroll
-            for (int n = 0; n < NH; ++n) mma16816<T>(s[x][n], a, qf[t][n][0], qf[t][n][1]);
+            for (int n = 0; n < NH; ++n)
+              mma16816<T>(t & 1 ? s2[x][n] : s[x][n], a, qf[t][n][0], qf[t][n][1]);
           }
         }
       }
@@ -638,7 +648,7 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[x][n][e] *= p.scale_log2;
+          for (int e = 0; e < 4; ++e) s[x][n][e] = (s[x][n][e] + s2[x][n][e]) * p.scale_log2;
       if (edge) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -719,11 +729,11 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
         const int h = n * 8 + 2 * (lane & 3) + e;
-        if (h >= nh) continue;
+        if (h >= it.nh) continue;
         if (it.pieces == 1) {
           const bool none = bad || l[n][e] == 0.f;
           const float inv = 1.f / l[n][e];
-          T* out = static_cast<T*>(p.o) + it.b * p.o_sb + (h0 + h) * p.o_sh;
+          T* out = static_cast<T*>(p.o) + it.b * p.o_sb + (it.h0 + h) * p.o_sh;
 #pragma unroll
           for (int t = 0; t < DP / 16; ++t) {
 #pragma unroll
@@ -733,7 +743,7 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
             }
           }
         } else {
-          const int64_t at = (static_cast<int64_t>(it.b) * p.heads + h0 + h) * p.max_pieces +
+          const int64_t at = (static_cast<int64_t>(it.b) * p.heads + it.h0 + h) * p.max_pieces +
                              it.piece;
           float* acc = p.acc + at * p.dvp;
 #pragma unroll
@@ -1021,6 +1031,14 @@ int bio_paged_attention(const bio_paged_attn_args* a, void* workspace, int64_t w
   p.max_len = static_cast<int>(a->table_width * a->page_size);
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.box_rows = std::gcd(p.page_size, bio::kTile);
+  p.group_shift = 0;
+  while ((p.box_rows << p.group_shift) < bio::kTile) ++p.group_shift;
+  // Division of a position (below 2^31) by the page size n with 2^(s-1) < n <= 2^s:
+  // floor(2^32 (2^s - n) / n) + 1 is the 33-bit reciprocal's low word.
+  p.page_shift = 0;
+  while ((1u << p.page_shift) < static_cast<unsigned>(p.page_size)) ++p.page_shift;
+  p.page_mul = static_cast<unsigned>(((1ull << 32) * ((1ull << p.page_shift) - p.page_size)) /
+                                     p.page_size + 1);
   p.max_pieces = s.pieces;
   p.dvp = s.dvp;
   p.acc = static_cast<float*>(workspace);

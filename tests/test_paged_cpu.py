@@ -222,12 +222,12 @@ def attention_args(**change):
 
 def test_attention_workspace_is_a_function_of_the_sizes():
     need = _lib.load().bio_paged_attention_workspace
-    assert need(attention_args(width=4)) == 0  # 64 tokens: one piece, nothing to join
+    assert need(attention_args(width=1)) == 0  # 16 tokens: one piece, nothing to join
     assert need(attention_args()) > 0          # 128 tokens
     more = need(attention_args(width=1024))
     assert more >= need(attention_args(width=512))  # longer rows have longer pieces
     # a window bounds what a row sees, whatever the table could hold
-    assert need(attention_args(width=1024, window=40, sinks=4)) == 0
+    assert need(attention_args(width=1024, window=40, sinks=4)) < need(attention_args())
     assert need(attention_args(batch=8)) == 2 * need(attention_args())
 
 
