@@ -50,7 +50,7 @@ constexpr int kTile = 32;  // tokens of a tile
 // the SMs; long rows take longer ones, since every piece costs a write and a
 // read of its fp32 output.
 __host__ __device__ __forceinline__ int piece_tiles(int n) {
-  return n <= 32 ? 1 : n <= 256 ? 4 : n <= 1024 ? 8 : 16;
+  return n <= 32 ? 1 : n <= 64 ? 2 : n <= 256 ? 8 : 16;
 }
 
 __host__ __device__ __forceinline__ int pieces_of(int tiles) {
@@ -318,14 +318,12 @@ struct PagedSmem {
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ uint32_t mov_trans(uint32_t x) {
   uint32_t y;
@@ -386,6 +384,43 @@ struct PagedItem {
   int t0, tiles;   // of the piece
 };
 
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0,
+                                         int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+
+// Bounded wait (the contract of mbar_wait) whose polls park the warp: polling
+// warps take issue slots from the one or two that share their scheduler.
+__device__ __forceinline__ bool parked_wait(uint32_t a, uint32_t parity,
+                                            volatile int* abort_flag, int* status) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0; i < kWaitMaxIters; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity), "r"(100000u)
+        : "memory");
+    if (done) return true;
+    if (i == 0) t0 = global_timer_ns();
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > kWaitTimeoutNs) break;
+  }
+  *abort_flag = 1;
+  raise_status(status, BIO_DEV_TIMEOUT);
+  return false;
+}
+
 template <typename T, int DP, int NH>
 __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
     paged_mma_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -415,6 +450,14 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
+  }
+  // The products run over all DP columns.  The boxes fill up to the next 64
+  // with zeros; blocks that no box covers (d and dv differ) are zeroed here.
+  if (p.d <= DP - 64 || p.dv <= DP - 64) {
+    uint4* z = reinterpret_cast<uint4*>(ring);
+    for (int i = threadIdx.x; i < W * S * L::kStage / 16; i += blockDim.x)
+      z[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
   // an empty or refused row has one item, which writes zeros
   int total = items;
@@ -518,36 +561,38 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
     }
   };
   const int kc = (p.d + 63) / 64, vc = (p.dv + 63) / 64;  // 64-column boxes of a row
+  // box x of a tile: group x % groups, column block x / groups (the keys', then the values')
+  const int boxes = groups * (kc + vc), tile_bytes = (kc + vc) * p.box_rows * 128;
+  const uint32_t my_ring32 = smem_u32(my_ring), my_bars32 = smem_u32(my_bars);
   int issued = 0;  // tiles fetched so far
   auto fetch = [&](int stage) {
     if (in_done) return;
     ++issued;
     const bool refused = in_held && (in_page < 0 || in_page >= p.pages);
-    const int lost = __any_sync(0xffffffffu, refused);
     const int page = in_held && !refused ? in_page : -1;
-    const int boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
-    uint8_t* dst = my_ring + stage * L::kStage;
-    const bool query = in_tile == 0;  // the item's queries travel with its first tile
+    const int held = __popc(__ballot_sync(0xffffffffu, page >= 0));
+    const int lost = __any_sync(0xffffffffu, refused);
+    const uint32_t dst = my_ring32 + stage * L::kStage, bar = my_bars32 + stage * 8;
     if (lane == 0) {
+      const bool query = in_tile == 0;  // the item's queries travel with its first tile
       misc[warp * S + stage] = lost;
-      mbar_arrive_expect_tx(&my_bars[stage], boxes * (kc + vc) * p.box_rows * 128 +
-                                                 (query ? kc * HB * 128 : 0));
-      if (query) {
+      expect_bytes(bar, held * tile_bytes + (query ? kc * HB * 128 : 0));
+      if (query)
         for (int c = 0; c < kc; ++c)
-          tma_load_4d(dst + 2 * L::kKv + c * HB * 128, &tmQ, &my_bars[stage], c * 64, in.h0, in.b,
-                      0);
-      }
+          load_box(dst + 2 * L::kKv + c * HB * 128, &tmQ, bar, c * 64, in.h0, in.b, 0);
     }
     __syncwarp();
-    for (int x0 = 0; x0 < groups * (kc + vc); x0 += 32) {
+    for (int x0 = 0; x0 < boxes; x0 += 32) {
       const int x = x0 + lane, g = x & group_mask, c = x >> p.group_shift;
       const int pg = __shfl_sync(0xffffffffu, page, g);
       const int slot = __shfl_sync(0xffffffffu, in_slot, g);
-      if (pg >= 0 && c < kc + vc) {
-        const bool key = c < kc;
-        const int cb = key ? c : c - kc;
-        tma_load_4d(dst + (key ? 0 : L::kKv) + cb * (kTile * 128) + g * p.box_rows * 128,
-                    key ? &tmK : &tmV, &my_bars[stage], cb * 64, slot, in.hk, pg);
+      if (x < boxes && pg >= 0) {
+        const uint32_t to = dst + g * p.box_rows * 128;
+        if (c < kc)
+          load_box(to + c * (kTile * 128), &tmK, bar, c * 64, slot, in.hk, pg);
+        else
+          load_box(to + L::kKv + (c - kc) * (kTile * 128), &tmV, bar, (c - kc) * 64, slot, in.hk,
+                   pg);
       }
     }
     ++in_tile;
@@ -558,7 +603,6 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
   for (int s = 0; s < S; ++s) fetch(s);
 
   // ------------------------------------------------------------- consumer side
-  const uint32_t ring32 = smem_u32(my_ring);
   int stage = 0, used = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -586,13 +630,13 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
         for (int e = 0; e < 4; ++e) o[t][n][e] = 0.f;
     }
     for (int tile = 0; tile < it.tiles; ++tile) {
-      if (ok) ok = mbar_wait(&my_bars[stage], phase, abort_flag, p.status);
+      if (ok) ok = parked_wait(my_bars32 + stage * 8, phase, abort_flag, p.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {  // a wait ran out: no more loads, zeros for what is left
         bad = 1;
         break;
       }
-      const uint32_t sk = ring32 + stage * L::kStage, sv = sk + L::kKv, sq = sv + L::kKv;
+      const uint32_t sk = my_ring32 + stage * L::kStage, sv = sk + L::kKv, sq = sv + L::kKv;
       bad |= misc[warp * S + stage];
       const int pos = it.z.base(it.t0 + tile);
       const bool edge =
@@ -631,16 +675,14 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
         for (int e = 0; e < 4; ++e) s[0][n][e] = s[1][n][e] = s2[0][n][e] = s2[1][n][e] = 0.f;
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
-        if ((t >> 2) < kc) {
-          const uint32_t at = ((sk + koff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128);
+        const uint32_t at = ((sk + koff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            uint32_t a[4];
-            ldsm_x4(at + x * 2048, a);
+        for (int x = 0; x < 2; ++x) {
+          uint32_t a[4];
+          ldsm_x4(at + x * 2048, a);
 #pragma unroll
-            for (int n = 0; n < NH; ++n)
-              mma16816<T>(t & 1 ? s2[x][n] : s[x][n], a, qf[t][n][0], qf[t][n][1]);
-          }
+          for (int n = 0; n < NH; ++n)
+            mma16816<T>(t & 1 ? s2[x][n] : s[x][n], a, qf[t][n][0], qf[t][n][1]);
         }
       }
 #pragma unroll
@@ -701,15 +743,13 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
       }
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) {
-        if ((t >> 2) < vc) {
-          const uint32_t at = ((sv + voff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128);
+        const uint32_t at = ((sv + voff) ^ ((t & 3) << 5)) + (t >> 2) * (kTile * 128);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            uint32_t a[4];
-            ldsm_x4_t(at + x * 2048, a);
+        for (int x = 0; x < 2; ++x) {
+          uint32_t a[4];
+          ldsm_x4_t(at + x * 2048, a);
 #pragma unroll
-            for (int n = 0; n < NH; ++n) mma16816<T>(o[t][n], a, pf[x][n][0], pf[x][n][1]);
-          }
+          for (int n = 0; n < NH; ++n) mma16816<T>(o[t][n], a, pf[x][n][0], pf[x][n][1]);
         }
       }
       __syncwarp();
@@ -834,8 +874,8 @@ constexpr int64_t kMaxGrid = 2147483647;
 // Most pieces that a row of up to `most` tiles can have.
 int64_t most_pieces(int64_t most) {
   int64_t pieces = 1;
-  for (int64_t top : {static_cast<int64_t>(32), static_cast<int64_t>(256),
-                      static_cast<int64_t>(1024), most}) {
+  for (int64_t top : {static_cast<int64_t>(32), static_cast<int64_t>(64),
+                      static_cast<int64_t>(256), most}) {
     const int64_t k = bio::pieces_of(static_cast<int>(top < most ? top : most));
     if (k > pieces) pieces = k;
   }

@@ -227,7 +227,7 @@ def test_attention_workspace_is_a_function_of_the_sizes():
     more = need(attention_args(width=1024))
     assert more >= need(attention_args(width=512))  # longer rows have longer pieces
     # a window bounds what a row sees, whatever the table could hold
-    assert need(attention_args(width=1024, window=40, sinks=4)) < need(attention_args())
+    assert need(attention_args(width=1024, window=40, sinks=4)) < need(attention_args(width=16))
     assert need(attention_args(batch=8)) == 2 * need(attention_args())
 
 
