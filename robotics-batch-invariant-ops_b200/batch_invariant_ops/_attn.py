@@ -218,7 +218,7 @@ def varlen(q, k, v, cu_q, cu_k, *, is_causal, causal_name, scale):
     return out
 
 
-def _window_args(q, k, v, out, q_s, k_s, v_s, o_s, batch, heads, kv_heads, lq, lk, scale):
+def _window_args(q, k, v, out, q_s, k_s, v_s, o_s, batch, heads, kv_heads, lq, lk, d, dv, scale):
     a = _AttnArgs()
     a.dtype = _lib.DTYPE_CODE[q.dtype]
     a.device = q.device.index
@@ -228,8 +228,8 @@ def _window_args(q, k, v, out, q_s, k_s, v_s, o_s, batch, heads, kv_heads, lq, l
     a.v_sb, a.v_sh, a.v_st = v_s
     a.o_sb, a.o_sh, a.o_st = o_s
     a.batch, a.heads, a.kv_heads = batch, heads, kv_heads
-    a.lq, a.lk, a.d, a.dv = lq, lk, q.shape[-1], v.shape[-1]
-    a.scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    a.lq, a.lk, a.d, a.dv = lq, lk, d, dv
+    a.scale = scale if scale is not None else 1.0 / math.sqrt(d)
     return a
 
 
@@ -242,12 +242,14 @@ def window(q, k, v, window, sinks, scale):
     q4 = _dim_contiguous(q.reshape(nb, h, lq, d))
     k4 = _dim_contiguous(k.reshape(nb, hkv, lk, d))
     v4 = _dim_contiguous(v.reshape(nb, hkv, lk, dv))
+    if q.dtype != torch.float32:
+        q4, k4, v4 = _tma_ready(q4), _tma_ready(k4), _tma_ready(v4)
     # token-major like the output of sdpa
     out = torch.empty((nb, lq, h, dv), device=q.device, dtype=q.dtype).transpose(1, 2)
     if out.numel() == 0:
         return out.reshape(*lead, h, lq, dv)
     a = _window_args(q4, k4, v4, out, q4.stride()[:3], k4.stride()[:3], v4.stride()[:3],
-                     out.stride()[:3], nb, h, hkv, lq, lk, scale)
+                     out.stride()[:3], nb, h, hkv, lq, lk, d, dv, scale)
     seen = min(lk, window + sinks)
     with tracing.span("window_attention", f"bio_attention_window [B={nb}, H={h}/{hkv}, Lq={lq}, "
                       f"Lk={lk}, D={d}/{dv}, window={window}, sinks={sinks}]",
@@ -261,10 +263,14 @@ def window(q, k, v, window, sinks, scale):
 
 def window_varlen(q, k, v, cu_q, cu_k, window, sinks, scale):
     """Packed q [1, Tq, H, D], k/v [1, Tk, Hkv, D|Dv] -> [1, Tq, H, Dv]."""
-    _, tq, h, _ = q.shape
+    _, tq, h, d = q.shape
     _, tk, hkv, _ = k.shape
     dv = v.shape[3]
     q3, k3, v3 = _dim_contiguous(q[0]), _dim_contiguous(k[0]), _dim_contiguous(v[0])
+    if q.dtype != torch.float32:
+        # [T, H, D] -> [1, H, T, D] views for the TMA check, back to [T, H, D]
+        q3, k3, v3 = (_tma_ready(t.permute(1, 0, 2).unsqueeze(0))[0].permute(1, 0, 2)
+                      for t in (q3, k3, v3))
     out = torch.zeros((1, tq, h, dv), device=q.device, dtype=q.dtype)
     if out.numel() == 0 or cu_q.numel() == 1:
         return out
@@ -272,7 +278,7 @@ def window_varlen(q, k, v, cu_q, cu_k, window, sinks, scale):
     cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
     by_token = lambda t: (0, t.stride(1), t.stride(0))  # noqa: E731
     a = _window_args(q3, k3, v3, out, by_token(q3), by_token(k3), by_token(v3), by_token(out[0]),
-                     1, h, hkv, tq, tk, scale)
+                     1, h, hkv, tq, tk, d, dv, scale)
     a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
     a.cu_is64 = 1 if cu_q.dtype == torch.int64 else 0
     a.nseq = cu_q.numel() - 1

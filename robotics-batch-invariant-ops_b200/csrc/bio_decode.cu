@@ -16,7 +16,7 @@
 #include <mutex>
 #include <numeric>
 
-#include "bio_common.cuh"
+#include "bio_tile.cuh"
 
 namespace bio {
 
@@ -331,13 +331,6 @@ __device__ __forceinline__ uint32_t mov_trans(uint32_t x) {
   return y;
 }
 
-// 2^x on the special-function unit (PTX ex2.approx: 2 ulp, 2^-inf = 0).
-__device__ __forceinline__ float pow2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1);
@@ -383,43 +376,6 @@ struct PagedItem {
   int piece, pieces;
   int t0, tiles;   // of the piece
 };
-
-__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0,
-                                         int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
-      : "memory");
-}
-
-// Bounded wait (the contract of mbar_wait) whose polls park the warp: polling
-// warps take issue slots from the one or two that share their scheduler.
-__device__ __forceinline__ bool parked_wait(uint32_t a, uint32_t parity,
-                                            volatile int* abort_flag, int* status) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 0; i < kWaitMaxIters; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(a), "r"(parity), "r"(100000u)
-        : "memory");
-    if (done) return true;
-    if (i == 0) t0 = global_timer_ns();
-    if (*abort_flag) return false;
-    if (global_timer_ns() - t0 > kWaitTimeoutNs) break;
-  }
-  *abort_flag = 1;
-  raise_status(status, BIO_DEV_TIMEOUT);
-  return false;
-}
 
 template <typename T, int DP, int NH>
 __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
@@ -929,26 +885,6 @@ int dispatch_simt(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   return wide ? launch_simt<T, 1, 16, VEC>(p, batch, s) : launch_simt<T, 1, 8, VEC>(p, batch, s);
 }
 
-// Tensor map {column, n1, n2, n3} of 16-bit elements with 128-byte swizzle; element strides.
-template <typename T>
-bool map_of(CUtensorMap* map, const void* ptr, int64_t cols, int64_t n1, int64_t n2, int64_t n3,
-            int64_t s1, int64_t s2, int64_t s3, int rows) {
-  bio_host::EncodeTiledFn enc = bio_host::encode_tiled_fn();
-  if (enc == nullptr) return false;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(n1),
-                              static_cast<cuuint64_t>(n2), static_cast<cuuint64_t>(n3)};
-  // the stride of a dimension of one element is never used, but has to be valid
-  auto bytes = [](int64_t n, int64_t s) { return static_cast<cuuint64_t>(n > 1 ? 2 * s : 16); };
-  const cuuint64_t strides[3] = {bytes(n1, s1), bytes(n2, s2), bytes(n3, s3)};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, ones[4] = {1, 1, 1, 1};
-  return enc(map,
-             std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-             4, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int DP, int NH>
 int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   using L = bio::PagedSmem<DP, NH>;
@@ -965,10 +901,10 @@ int launch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   CUtensorMap q, k, v;
   // a pool without pages is never read: any aligned address will do for its maps
   const int64_t pages = std::max<int64_t>(p.pages, 1);
-  if (!map_of<T>(&q, p.q, p.d, p.heads, batch, 1, p.q_sh, p.q_sb, 0, 8 * NH) ||
-      !map_of<T>(&k, p.pages > 0 ? p.k : p.q, p.d, p.page_size, p.kv_heads, pages, p.k_st, p.k_sh,
+  if (!bio_host::map_of<T>(&q, p.q, p.d, p.heads, batch, 1, p.q_sh, p.q_sb, 0, 8 * NH) ||
+      !bio_host::map_of<T>(&k, p.pages > 0 ? p.k : p.q, p.d, p.page_size, p.kv_heads, pages, p.k_st, p.k_sh,
                  p.k_sp, p.box_rows) ||
-      !map_of<T>(&v, p.pages > 0 ? p.v : p.q, p.dv, p.page_size, p.kv_heads, pages, p.v_st, p.v_sh,
+      !bio_host::map_of<T>(&v, p.pages > 0 ? p.v : p.q, p.dv, p.page_size, p.kv_heads, pages, p.v_st, p.v_sh,
                  p.v_sp, p.box_rows))
     return BIO_ERR_ALIGN;
   const int64_t sms = bio_host::sm_count(device);

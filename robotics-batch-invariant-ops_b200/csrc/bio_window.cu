@@ -5,15 +5,15 @@
 //   o_i = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q_i.k_j.
 // A row that sees no key (p < 0) gives zeros.
 //
-// One warp owns one query row.  It walks the row's visible keys in order, 32
-// at a time: lane j computes the score of key j, the maximum and the sum of
-// exponentials use a fixed xor-shuffle tree, and lane t accumulates output
-// columns t, t + 32, ....  Keys that the row does not see are never read, and
-// nothing depends on the other rows of the launch.
+// 16-bit operands run on tcgen05 (window_tc_kernel), fp32 on the CUDA cores
+// (window_row_kernel).
 //
 // Not in the reference, whose SDPA (batch_invariant_ops.py:1148-1213) would
 // need the mask as a tensor and visits every key.
-#include "bio_common.cuh"
+#include <algorithm>
+#include <mutex>
+
+#include "bio_tile.cuh"
 
 namespace bio {
 
@@ -42,9 +42,66 @@ __device__ __forceinline__ int64_t win_off(const void* p, int is64, int64_t i) {
 constexpr int kWinWarps = 8;
 constexpr int kWinDims = 256;
 
+// One warp computes one row.  It walks the row's visible keys in order, 32 at a
+// time: lane j computes the score of key j, the maximum and the sum of
+// exponentials use a fixed xor-shuffle tree, and lane t accumulates output
+// columns t, t + 32, ....  Keys that the row does not see are never read.
+// `pos` is the query's position; kb and vb point at key 0 of its sequence.
+template <typename T>
+__device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb, T* out,
+                                        int64_t k_st, int64_t v_st, int d, int dv, float scale,
+                                        int64_t window, int64_t sinks, int64_t pos) {
+  const int lane = threadIdx.x & 31;
+  // visible keys u = 0..n-1: key u < few ? u : u + skip
+  const int64_t lo = max(static_cast<int64_t>(0), pos - window + 1);
+  const int64_t few = min(sinks, lo), skip = lo - few;
+  const int64_t n = max(static_cast<int64_t>(0), pos + 1 - skip);
+  float m = -INFINITY, l = 0.f, o[kWinDims / 32];
+#pragma unroll
+  for (int e = 0; e < kWinDims / 32; ++e) o[e] = 0.f;
+  for (int64_t u0 = 0; u0 < n; u0 += 32) {
+    const int64_t u = u0 + lane;
+    float s = -INFINITY;
+    if (u < n) {
+      const T* krow = kb + (u < few ? u : u + skip) * k_st;
+      float a = 0.f;
+      for (int c = 0; c < d; ++c) a = fmaf(to_f32(qrow[c]), to_f32(krow[c]), a);
+      s = a * scale;
+    }
+    float top = s;
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    top = fmaxf(top, m);
+    const float f = m == -INFINITY ? 0.f : expf(m - top);
+    const float w = s == -INFINITY ? 0.f : expf(s - top);
+    float sum = w;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    l = l * f + sum;
+    m = top;
+#pragma unroll
+    for (int e = 0; e < kWinDims / 32; ++e) o[e] *= f;
+    const int keys = static_cast<int>(min(static_cast<int64_t>(32), n - u0));
+    for (int j = 0; j < keys; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const int64_t uj = u0 + j;
+      const T* vrow = vb + (uj < few ? uj : uj + skip) * v_st;
+#pragma unroll
+      for (int e = 0; e < kWinDims / 32; ++e) {
+        const int c = lane + 32 * e;
+        if (c < dv) o[e] = fmaf(wj, to_f32(vrow[c]), o[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kWinDims / 32; ++e) {
+    const int c = lane + 32 * e;
+    if (c < dv) out[c] = from_f32<T>(l == 0.f ? 0.f : o[e] / l);
+  }
+}
+
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(kWinWarps * 32) window_row_kernel(const WindowParams p) {
-  __shared__ float qs[kWinWarps][kWinDims];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kWinWarps + warp;
   if (row >= (PACKED ? 1 : p.batch) * p.heads * p.lq) return;
@@ -69,59 +126,692 @@ __global__ void __launch_bounds__(kWinWarps * 32) window_row_kernel(const Window
     pos = (t - q0) + (k1 - k0) - (q1 - q0);
   }
   const int64_t bq = PACKED ? 0 : b;
-  T* out = static_cast<T*>(p.o) + bq * p.o_sb + h * p.o_sh + t * p.o_st;
-  const T* qrow = static_cast<const T*>(p.q) + bq * p.q_sb + h * p.q_sh + t * p.q_st;
-  const T* kb = static_cast<const T*>(p.k) + bq * p.k_sb + h / p.group * p.k_sh + k0 * p.k_st;
-  const T* vb = static_cast<const T*>(p.v) + bq * p.v_sb + h / p.group * p.v_sh + k0 * p.v_st;
-  for (int c = lane; c < p.d; c += 32) qs[warp][c] = to_f32(qrow[c]);
-  __syncwarp();
+  window_row<T>(static_cast<const T*>(p.q) + bq * p.q_sb + h * p.q_sh + t * p.q_st,
+                static_cast<const T*>(p.k) + bq * p.k_sb + h / p.group * p.k_sh + k0 * p.k_st,
+                static_cast<const T*>(p.v) + bq * p.v_sb + h / p.group * p.v_sh + k0 * p.v_st,
+                static_cast<T*>(p.o) + bq * p.o_sb + h * p.o_sh + t * p.o_st, p.k_st, p.v_st, p.d,
+                p.dv, p.scale, p.window, p.sinks, pos);
+}
 
-  // visible keys u = 0..n-1: key u < few ? u : u + skip
-  const int64_t lo = max(static_cast<int64_t>(0), pos - p.window + 1);
-  const int64_t few = min(p.sinks, lo), skip = lo - few;
-  const int64_t n = max(static_cast<int64_t>(0), pos + 1 - skip);
-  float m = -INFINITY, l = 0.f, o[kWinDims / 32];
+// ---------------------------------------------------------------------------
+// tcgen05 kernel.
+//
+// A block of CTAs' work is a job: NT tiles of 128 query rows that share a KV
+// head.  A tile packs `gh` query heads of the group with `tok` = 128 / gh
+// consecutive tokens each (row r: head r / tok, token r % tok), so the keys
+// that a tile visits are its window plus tok - 1, not plus 127, and a key block
+// is loaded once for the whole group.  Jobs are dealt out round robin to one
+// persistent CTA per SM:
+//   warp 0      TMA: Q tiles, then K and V blocks of BN keys through one ring.
+//   warp 1      MMA (one thread): S_t = Q_t K^T, O_t += P_t V, fp32 in TMEM; P
+//               (16 bits) lies over the S that it came from.
+//   warps 4..   softmax: one thread per query row; the 128 rows of tile t belong
+//               to warps 4 + 4 t .. 7 + 4 t, which take over registers of the
+//               first four warps (two of them idle).
+// The ring, S and O run on across jobs: a job's first products start while the
+// last rows of the one before are still being stored.  With two tiles
+// (D <= 128) the tensor cores work on one tile while the other is in its
+// softmax; with one tile (D <= 256) S has two buffers, and S of block j + 1 is
+// issued before P_j is waited for.
+//
+// Blocks are cut on the absolute grid of BN keys and trimmed, per tile, to the
+// 32-key columns that some row of the tile sees: a window costs about window +
+// tok + 32 columns per row, four sink tokens one 32-key column.  Masked scores
+// weigh exactly 0 and untrimmed columns add exactly 0, so a row's bits depend
+// on its own query, keys and position only.
+//
+// Scores stay in fp32 registers (128 a thread).  The reference m of the
+// exponentials moves only when a block's maximum exceeds it by more than 8
+// (log2), so O is rarely rescaled and P stays below 2^8; P is rounded to the
+// operand type, as the product needs, l sums it unrounded in fp32.
+//
+// A hidden key in a visited block has weight 0, but 0 * Inf or 0 * NaN in V
+// would still reach the row: a row whose output is not finite is computed once
+// more, by its warp, from its visible keys alone (window_row).  Keys of a
+// neighbouring packed sequence are zeroed in shared memory instead, so that
+// they cannot even change a row's bits.
+// ---------------------------------------------------------------------------
+struct WindowJobs {
+  int gh, tok, hblocks;  // heads and tokens of a tile, tiles across a group
+  int qblocks;           // dense: blocks of NT * tok tokens per sequence; packed: at most
+  int jobs;
+  int window, sinks;     // at most 2^30
+  float scale_log2;      // > 0
+  int negate;            // the scale was negative: scores change sign
+  int vec_out;           // output rows take 16-byte stores
+};
+
+template <int DP>
+struct WinSmem {
+  static constexpr int NT = DP == 256 ? 1 : 2;     // tiles of a job
+  static constexpr int BN = DP == 256 ? 64 : 128;  // keys of a block
+  static constexpr uint32_t kQ = 128 * DP * 2;
+  static constexpr uint32_t kSlot = BN * DP * 2;   // K or V of a block
+  static constexpr int kFit = (226 * 1024 - 1024 - 512 - NT * static_cast<int>(kQ)) /
+                              static_cast<int>(kSlot);
+  static constexpr int kSlots = kFit > 8 ? 8 : kFit;
+  static constexpr uint32_t kBytes = 1024 + NT * kQ + kSlots * kSlot + 512;
+  static constexpr int kThreads = 128 + 128 * NT;
+  static_assert(kSlots >= 4, "K and V of two blocks");
+};
+
+struct WinJob {
+  int b, hk, h0, nh;        // sequence of the batch, KV head, query heads
+  int q0, lq, lk;           // first query of the job, lengths of its sequence
+  int qt, kt;               // tokens of the operands at which the sequence starts
+};
+
+// Keys of a tile: [lo, hi) for the windows of its rows, [0, sx) sinks before it.
+struct WinTile {
+  int pf, n;   // position of its first token, number of tokens
+  int lo, hi, sx;
+};
+
+struct WinPlan {
+  int head, jump, blocks;  // block i of the job is block i < head ? i : i + jump of the keys
+};
+
+template <int NT, int BN>
+__device__ __forceinline__ WinPlan window_plan(const WindowJobs& w, const WinJob& j,
+                                               WinTile (&tile)[NT]) {
+  int head = 0, first = 0x7fffffff, last = -1;
 #pragma unroll
-  for (int e = 0; e < kWinDims / 32; ++e) o[e] = 0.f;
-  for (int64_t u0 = 0; u0 < n; u0 += 32) {
-    const int64_t u = u0 + lane;
-    float s = -INFINITY;
-    if (u < n) {
-      const T* krow = kb + (u < few ? u : u + skip) * p.k_st;
-      float a = 0.f;
-      for (int c = 0; c < p.d; ++c) a = fmaf(qs[warp][c], to_f32(krow[c]), a);
-      s = a * p.scale;
+  for (int t = 0; t < NT; ++t) {
+    WinTile& x = tile[t];
+    const int q = j.q0 + t * w.tok;
+    x.n = max(0, min(w.tok, j.lq - q));
+    x.pf = q + j.lk - j.lq;
+    x.hi = x.n > 0 ? max(0, x.pf + x.n) : 0;
+    x.lo = x.hi > 0 ? max(0, x.pf - w.window + 1) : 0;
+    x.sx = min(w.sinks, x.lo);
+    if (x.hi > 0) {
+      head = max(head, (x.sx + BN - 1) / BN);
+      first = min(first, x.lo / BN);
+      last = max(last, (x.hi - 1) / BN);
     }
-    float top = s;
+  }
+  WinPlan p;
+  p.head = head;
+  p.jump = last < 0 ? 0 : max(0, first - head);
+  p.blocks = last < 0 ? 0 : last + 1 - p.jump;
+  return p;
+}
+
+// Columns [x, y) of block b (keys b * BN ...) that some row of the tile sees, on
+// the 32-column grid; empty: x == y.
+template <int BN>
+__device__ __forceinline__ int2 window_span(const WinTile& t, int b) {
+  const int base = b * BN;
+  int x = max(t.lo - base, 0), y = min(t.hi - base, BN);
+  if (x >= y) x = y = 0;
+  const int s = min(t.sx - base, BN);
+  if (s > 0) {
+    x = 0;
+    y = max(y, s);
+  }
+  return make_int2(x & ~31, (y + 31) & ~31);
+}
+
+// Job number -> job.  All lanes of the warp call it; false: no such job.
+template <int NT>
+__device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJobs& w, int number,
+                                           WinJob& j) {
+  const int lane = threadIdx.x & 31;
+  const int tiles = static_cast<int>(p.heads / p.group) * w.hblocks;
+  int qb, hx;
+  if (p.cu_q == nullptr) {
+    const int rest = number / w.qblocks;
+    qb = number - rest * w.qblocks;
+    j.b = rest / tiles;
+    hx = rest - j.b * tiles;
+    j.lq = static_cast<int>(p.lq);
+    j.lk = static_cast<int>(p.lk);
+    j.qt = j.kt = 0;
+  } else {
+    qb = number / tiles;
+    hx = number - qb * tiles;
+    j.b = 0;
+    if (win_off(p.cu_q, p.cu_is64, 0) != 0 || win_off(p.cu_k, p.cu_is64, 0) != 0) {
+      raise_status(p.status, BIO_DEV_INDEX);
+      return false;
+    }
+    // 32 sequences at a time: the one whose blocks hold block qb
+    const int span = NT * w.tok;
+    bool found = false;
+    for (int64_t s0 = 0; s0 < p.nseq && !found; s0 += 32) {
+      const int64_t s = s0 + lane;
+      int64_t qa = 0, qz = 0, ka = 0, kz = 0;
+      int n = 0;
+      if (s < p.nseq) {
+        qa = win_off(p.cu_q, p.cu_is64, s);
+        qz = win_off(p.cu_q, p.cu_is64, s + 1);
+        ka = win_off(p.cu_k, p.cu_is64, s);
+        kz = win_off(p.cu_k, p.cu_is64, s + 1);
+        if (qa < 0 || qz < qa || qz > p.lq || ka < 0 || kz < ka || kz > p.lk)
+          raise_status(p.status, BIO_DEV_INDEX);
+        else
+          n = static_cast<int>((qz - qa + span - 1) / span);
+      }
+      int inc = n;
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    top = fmaxf(top, m);
-    const float f = m == -INFINITY ? 0.f : expf(m - top);
-    const float w = s == -INFINITY ? 0.f : expf(s - top);
-    float sum = w;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, inc > qb);
+      if (past == 0) {
+        qb -= __shfl_sync(0xffffffffu, inc, 31);
+        continue;
+      }
+      const int f = __ffs(past) - 1;
+      qb -= __shfl_sync(0xffffffffu, inc - n, f);
+      j.lq = __shfl_sync(0xffffffffu, static_cast<int>(qz - qa), f);
+      j.lk = __shfl_sync(0xffffffffu, static_cast<int>(kz - ka), f);
+      j.qt = __shfl_sync(0xffffffffu, static_cast<int>(qa), f);
+      j.kt = __shfl_sync(0xffffffffu, static_cast<int>(ka), f);
+      found = true;
+    }
+    if (!found) return false;
+  }
+  j.q0 = qb * NT * w.tok;
+  j.hk = hx / w.hblocks;
+  const int before = (hx - j.hk * w.hblocks) * w.gh;
+  j.h0 = j.hk * static_cast<int>(p.group) + before;
+  j.nh = min(w.gh, static_cast<int>(p.group) - before);
+  return true;
+}
+
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void commit_to(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void split_pair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_two(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack_two<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_two<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Bits [x, y) of a 32-bit word, x and y anywhere.
+__device__ __forceinline__ uint32_t bits_between(int x, int y) {
+  const int a = min(max(x, 0), 32), b = min(max(y, 0), 32);
+  const uint64_t below_b = (1ull << b) - 1, below_a = (1ull << a) - 1;
+  return static_cast<uint32_t>(below_b & ~below_a);
+}
+
+// Shared-space addresses of the barriers and the TMEM base slot.
+template <int DP>
+struct WinBars {
+  using L = WinSmem<DP>;
+  uint32_t base;
+  __device__ uint32_t full(int s) const { return base + s * 8; }
+  __device__ uint32_t empty(int s) const { return base + 64 + s * 8; }
+  __device__ uint32_t q_full(int t) const { return base + 128 + t * 8; }
+  __device__ uint32_t q_empty(int t) const { return base + 144 + t * 8; }
+  __device__ uint32_t s_full(int x) const { return base + 160 + x * 8; }
+  __device__ uint32_t p_ready(int x) const { return base + 176 + x * 8; }
+  __device__ uint32_t o_done(int t) const { return base + 192 + t * 8; }
+  __device__ uint32_t pv_done() const { return base + 208; }
+  __device__ uint32_t all_done() const { return base + 216; }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
+    window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const WindowParams p,
+                     const WindowJobs w) {
+  using L = WinSmem<DP>;
+  constexpr int NT = L::NT, BN = L::BN, NS = L::kSlots;
+  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = smem + NT * L::kQ;
+  uint8_t* tail = ring + NS * L::kSlot;
+  const uint32_t q32 = smem_u32(smem), ring32 = smem_u32(ring);
+  const WinBars<DP> bar{smem_u32(tail)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 256);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 260);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kc = (p.d + 63) / 64, vc = (p.dv + 63) / 64;
+
+  if (threadIdx.x == 0) {
+    uint64_t* b = reinterpret_cast<uint64_t*>(tail);
+    for (int i = 0; i < 28; ++i) mbar_init(b + i, i == 22 || i == 23 ? 4 : 1);  // p_ready: 4 warps
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // S at column 0 and 128, O_t at 256 + 128 t
+  auto wait = [&](uint32_t b, uint32_t parity) -> bool {
+    return parked_wait(b, parity & 1u, abort_flag, p.status);
+  };
+
+  // 384 threads start with 168 registers each, 128 of them go on with 56 and
+  // 256 with 216: 62464 of the 64512
+  constexpr bool kShift = NT == 2;
+  if (warp < 4) {
+    if (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    int pos = 0;                 // ring position: K and V of every block in turn
+    int q_used[2] = {0, 0};
+    bool ok = true;
+    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+      WinJob j;
+      if (!window_job<NT>(p, w, number, j)) continue;
+      WinTile tile[NT];
+      const WinPlan plan = window_plan<NT, BN>(w, j, tile);
+      for (int i = 0; ok && i < plan.blocks; ++i) {
+        const int b = i < plan.head ? i : i + plan.jump;
+        int x = BN, y = 0;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    l = l * f + sum;
-    m = top;
+        for (int t = 0; t < NT; ++t) {
+          const int2 s = window_span<BN>(tile[t], b);
+          if (s.x < s.y) {
+            x = min(x, s.x);
+            y = max(y, s.y);
+          }
+        }
+        const int rows = max(0, y - x);
+        for (int kv = 0; ok && kv < 2; ++kv, ++pos) {
+          const int slot = pos % NS;
+          ok = wait(bar.empty(slot), (pos / NS) ^ 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int chunks = kv == 0 ? kc : vc, boxes = chunks * (rows / 32);
+          if (lane == 0) expect_bytes(bar.full(slot), boxes * 32 * 128);
+          __syncwarp();
+          if (lane < boxes) {
+            const int c = lane % chunks, r = x + lane / chunks * 32;
+            load_box(ring32 + slot * L::kSlot + c * (BN * 128) + r * 128, kv == 0 ? &tmK : &tmV,
+                     bar.full(slot), c * 64, j.kt + b * BN + r, j.hk, j.b);
+          }
+          if (kv == 0 && i == 0) {  // the job's queries go out after its first keys
 #pragma unroll
-    for (int e = 0; e < kWinDims / 32; ++e) o[e] *= f;
-    const int keys = static_cast<int>(min(static_cast<int64_t>(32), n - u0));
-    for (int j = 0; j < keys; ++j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      const int64_t uj = u0 + j;
-      const T* vrow = vb + (uj < few ? uj : uj + skip) * p.v_st;
+            for (int t = 0; t < NT; ++t) {
+              if (tile[t].hi == 0 || !ok) continue;
+              ok = wait(bar.q_empty(t), q_used[t] ^ 1);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              if (lane == 0) {
+                expect_bytes(bar.q_full(t), kc * w.gh * w.tok * 128);
+                for (int c = 0; c < kc; ++c)
+                  load_box(q32 + t * L::kQ + c * 16384, &tmQ, bar.q_full(t), c * 64,
+                           j.qt + j.q0 + t * w.tok, j.h0, j.b);
+              }
+              ++q_used[t];
+            }
+          }
+        }
+      }
+    }
+    // every copy has to land before the block's shared memory goes
+    if (lane == 0) {
+      for (int i = max(0, pos - NS); i < pos; ++i)
+        if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + i % NS, (i / NS) & 1))
+          raise_status(p.status, BIO_DEV_TIMEOUT);
+      for (int t = 0; t < NT; ++t)
+        if (q_used[t] > 0 &&
+            !mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 16 + t, (q_used[t] - 1) & 1))
+          raise_status(p.status, BIO_DEV_TIMEOUT);
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------------------- MMA
+    int pos = 0;                       // ring position of the job's first K
+    int s_used[NT], q_used[NT];        // S products, jobs of tile t
 #pragma unroll
-      for (int e = 0; e < kWinDims / 32; ++e) {
-        const int c = lane + 32 * e;
-        if (c < p.dv) o[e] = fmaf(wj, to_f32(vrow[c]), o[e]);
+    for (int t = 0; t < NT; ++t) s_used[t] = q_used[t] = 0;
+    bool ok = true;
+    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+      WinJob j;
+      if (!window_job<NT>(p, w, number, j)) continue;
+      WinTile tile[NT];
+      const WinPlan plan = window_plan<NT, BN>(w, j, tile);
+      if (lane == 0) {
+        int2 held[NT];                 // columns of the P that waits for its PV
+        bool asked[NT], begun[NT];     // queries waited for; O holds something
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          held[t] = make_int2(0, 0);
+          asked[t] = begun[t] = false;
+        }
+        auto last_block = [&](int t) {  // index of the tile's last block
+          const int b = (tile[t].hi - 1) / BN;
+          return b < plan.head ? b : b - plan.jump;
+        };
+        auto issue_s = [&](int t, int i, int2 s) {
+          const int slot = (pos + 2 * i) % NS;
+          const int x = NT == 2 ? t : s_used[t] & 1;  // S buffer
+          if (!asked[t]) {
+            ok = wait(bar.q_full(t), q_used[t]);
+            if (!ok) return;
+            asked[t] = true;
+          }
+          tc_fence_after();
+          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
+          const uint32_t qa = q32 + t * L::kQ;
+          const uint32_t ka = ring32 + slot * L::kSlot + s.x * 128;
+          for (int k = 0; k < kc * 4; ++k)
+            umma_f16(tmem + x * 128 + s.x,
+                     smem_desc_sw128(qa + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
+                     smem_desc_sw128(ka + (k >> 2) * (BN * 128) + (k & 3) * 32, 16, 1024), idesc,
+                     k > 0 ? 1u : 0u);
+          commit_to(bar.s_full(x));
+          ++s_used[t];
+          if (i == last_block(t)) {
+            commit_to(bar.q_empty(t));
+            ++q_used[t];
+          }
+        };
+        // PV of block i, whose P came from the tile's S product number `of`
+        auto issue_pv = [&](int t, int i, int of) {
+          const int slot = (pos + 2 * i + 1) % NS;
+          const int x = NT == 2 ? t : of & 1;
+          ok = wait(bar.p_ready(x), NT == 2 ? of : of >> 1);
+          if (!ok) return;
+          ok = wait(bar.full(slot), (pos + 2 * i + 1) / NS);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
+          const uint32_t va = ring32 + slot * L::kSlot;
+          for (int k = held[t].x / 16; k < held[t].y / 16; ++k) {
+            umma_f16_ts(tmem + 256 + t * 128, tmem + x * 128 + k * 8,
+                        smem_desc_sw128(va + k * 2048, BN * 128, 1024), idesc, begun[t] ? 1u : 0u);
+            begun[t] = true;
+          }
+          held[t] = make_int2(0, 0);
+          if (NT == 1) commit_to(bar.pv_done());
+          if (i == last_block(t)) commit_to(bar.o_done(t));
+        };
+        for (int i = 0; ok && i <= plan.blocks; ++i) {
+          if (i < plan.blocks) ok = wait(bar.full((pos + 2 * i) % NS), (pos + 2 * i) / NS);
+          const int b = i < plan.head ? i : i + plan.jump;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            int2 s = make_int2(0, 0);
+            if (i < plan.blocks) s = window_span<BN>(tile[t], b);
+            const bool waiting = held[t].x < held[t].y;
+            if (NT == 2) {
+              if (ok && waiting) issue_pv(t, i - 1, s_used[t] - 1);
+              if (ok && s.x < s.y) issue_s(t, i, s);
+            } else {
+              if (ok && s.x < s.y) issue_s(t, i, s);
+              if (ok && waiting) issue_pv(t, i - 1, s_used[t] - (s.x < s.y ? 2 : 1));
+            }
+            if (s.x < s.y) held[t] = s;
+          }
+          // what the products issued so far have read is free once they are done
+          if (ok && i > 0) commit_to(bar.empty((pos + 2 * i - 1) % NS));
+          if (ok && i < plan.blocks) commit_to(bar.empty((pos + 2 * i) % NS));
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      pos += 2 * plan.blocks;
+    }
+    if (lane == 0) {
+      commit_to(bar.all_done());
+      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 27, 0))
+        raise_status(p.status, BIO_DEV_TIMEOUT);
+    }
+  }
+  } else {
+    if (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // ----------------------------------------------------------------- softmax
+    const int t = NT == 2 ? (warp - 4) >> 2 : 0;
+    const int r = (warp & 3) * 32 + lane;  // row of the tile: the warp's quarter of the lanes
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // (quarter * 32) << 16
+    const int rh = r / w.tok, rt = r - rh * w.tok;
+    const uint64_t scale2 = pair_of(w.scale_log2, w.scale_log2);
+    int pos = 0, s_used = 0, jobs_done = 0, pv_used = 0;
+    bool ok = true;
+    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+      WinJob j;
+      if (!window_job<NT>(p, w, number, j)) continue;
+      WinTile tiles[NT];
+      const WinPlan plan = window_plan<NT, BN>(w, j, tiles);
+      WinTile tile = tiles[0];
+      if (NT == 2 && t == 1) tile = tiles[NT - 1];
+      const bool valid = rh < j.nh && rt < tile.n;
+      const int at = tile.pf + rt;                     // position of the row
+      const int row_lo = at - w.window + 1, row_s = min(w.sinks, at + 1);
+      float m = -INFINITY, l = 0.f;
+      bool first = true;
+      for (int i = 0; i < plan.blocks; ++i) {
+        const int b = i < plan.head ? i : i + plan.jump;
+        const int2 s = window_span<BN>(tile, b);
+        if (s.x >= s.y) continue;
+        const int x = NT == 2 ? t : s_used & 1;
+        ok = wait(bar.s_full(x), NT == 2 ? s_used : s_used >> 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t s_at = tmem + lanes + x * 128;
+        const int j0 = b * BN;
+        uint32_t f[BN / 32][32];
+        float top = -INFINITY;
+        // every row of the tile sees every column of the block
+        const bool whole = s.x == 0 && s.y == BN && !w.negate && tile.n == w.tok &&
+                           j.nh == w.gh && j0 + BN <= tile.pf + 1 &&
+                           (j0 >= tile.pf + tile.n - w.window || j0 + BN <= w.sinks);
+        if (whole) {
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
+          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {
+            tmem_ld_wait_tied(f[c]);
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              a0 = max3(a0, __uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1]));
+              a1 = max3(a1, __uint_as_float(f[c][e + 2]), __uint_as_float(f[c][e + 3]));
+              a2 = max3(a2, __uint_as_float(f[c][e + 4]), __uint_as_float(f[c][e + 5]));
+              a3 = max3(a3, __uint_as_float(f[c][e + 6]), __uint_as_float(f[c][e + 7]));
+            }
+          }
+          top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
+        } else {
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {
+            if (c * 32 < s.x || c * 32 >= s.y) continue;
+            tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
+            tmem_ld_wait_tied(f[c]);
+            const int a = j0 + c * 32;
+            const uint32_t sees =
+                valid ? bits_between(row_lo - a, at + 1 - a) | bits_between(0, row_s - a) : 0u;
+            const uint32_t flip = w.negate ? 0x80000000u : 0u;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              f[c][e] = (sees >> e) & 1u ? f[c][e] ^ flip : 0xff800000u;  // -inf
+              top = fmaxf(top, __uint_as_float(f[c][e]));
+            }
+          }
+        }
+        const float scaled = top == -INFINITY ? top : top * w.scale_log2;
+        const bool move = scaled > m + 8.f;
+        const float alpha = move ? pow2(m - scaled) : 1.f;
+        if (move) m = scaled;
+        l *= alpha;
+        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // S of this block was issued after the PV before it (two tiles), or that
+          // one has to be waited for (one tile)
+          if (NT == 1) {
+            ok = wait(bar.pv_done(), pv_used - 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int c = 0; c < vc * 2; ++c) {
+            uint32_t v[32];
+            const uint32_t o_at = tmem + lanes + 256 + t * 128 + c * 32;
+            tmem_ld_32x32b_x32(o_at, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+            tmem_st_32x32b_x32(o_at, v);
+          }
+        }
+        first = false;
+        const float ref = m == -INFINITY ? 0.f : m;
+        const uint64_t ref2 = pair_of(-ref, -ref);
+        uint64_t sum2 = 0, sum3 = 0;
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          if (!whole && (c * 32 < s.x || c * 32 >= s.y)) continue;
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float a, bb;
+            split_pair(fma_pair(pair_of(__uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1])), scale2,
+                                ref2), a, bb);
+            a = pow2(a);
+            bb = pow2(bb);
+            packed[e / 2] = pack_two<T>(a, bb);
+            if (e & 2)
+              sum3 = add_pair(sum3, pair_of(a, bb));
+            else
+              sum2 = add_pair(sum2, pair_of(a, bb));
+          }
+          tmem_st_32x32b_x16(s_at + c * 16, packed);
+        }
+        float s0, s1;
+        split_pair(add_pair(sum2, sum3), s0, s1);
+        l += s0 + s1;
+        if (p.cu_q != nullptr && j0 + s.y > j.lk) {
+          // the block's last columns may be another sequence's tokens
+          const int slot = (pos + 2 * i + 1) % NS;
+          ok = wait(bar.full(slot), (pos + 2 * i + 1) / NS);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          uint8_t* v = ring + slot * L::kSlot;
+          for (int row = max(0, j.lk - j0); row < s.y; ++row)
+            for (int c = r; c < vc * 8; c += 128)
+              *reinterpret_cast<uint4*>(v + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(bar.p_ready(x));
+        ++s_used;
+        ++pv_used;
+      }
+      pos += 2 * plan.blocks;
+      if (!ok) break;
+      // ------------------------------------------------------------- the output
+      const int tok = j.qt + j.q0 + t * w.tok + rt;
+      T* out = valid ? static_cast<T*>(p.o) + j.b * p.o_sb + (j.h0 + rh) * p.o_sh + tok * p.o_st
+                     : nullptr;
+      if (tile.hi > 0) {
+        ok = wait(bar.o_done(t), jobs_done);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++jobs_done;
+        tc_fence_after();
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float odd = 0.f;  // becomes NaN with the first output that is not finite
+#pragma unroll 1
+      for (int c = 0; c < vc * 2; ++c) {
+        uint32_t v[32];
+        if (tile.hi > 0) {
+          tmem_ld_32x32b_x32(tmem + lanes + 256 + t * 128 + c * 32, v);
+          tmem_ld_wait();
+        }
+        if (l == 0.f || tile.hi == 0) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = 0;
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float y = __uint_as_float(v[e]) * inv;
+          odd = fmaf(y, 0.f, odd);
+          v[e] = __float_as_uint(y);
+        }
+        if (w.vec_out) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            if (c * 32 + e < p.dv)
+              *reinterpret_cast<uint4*>(out + c * 32 + e) = make_uint4(
+                  pack_two<T>(__uint_as_float(v[e]), __uint_as_float(v[e + 1])),
+                  pack_two<T>(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])),
+                  pack_two<T>(__uint_as_float(v[e + 4]), __uint_as_float(v[e + 5])),
+                  pack_two<T>(__uint_as_float(v[e + 6]), __uint_as_float(v[e + 7])));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c * 32 + e < p.dv) out[c * 32 + e] = from_f32<T>(__uint_as_float(v[e]));
+        }
+      }
+      tc_fence_before();  // the next job's PV overwrites O after this row's next P
+      unsigned again = __ballot_sync(0xffffffffu, valid && !(odd == 0.f));
+      while (again != 0) {
+        const int x = __ffs(again) - 1;
+        again &= again - 1;
+        const int xh = j.h0 + __shfl_sync(0xffffffffu, rh, x);
+        const int xt = __shfl_sync(0xffffffffu, rt, x);
+        const int64_t xtok = j.qt + j.q0 + t * w.tok + xt;
+        window_row<T>(
+            static_cast<const T*>(p.q) + j.b * p.q_sb + xh * p.q_sh + xtok * p.q_st,
+            static_cast<const T*>(p.k) + j.b * p.k_sb + j.hk * p.k_sh + j.kt * p.k_st,
+            static_cast<const T*>(p.v) + j.b * p.v_sb + j.hk * p.v_sh + j.kt * p.v_st,
+            static_cast<T*>(p.o) + j.b * p.o_sb + xh * p.o_sh + xtok * p.o_st, p.k_st, p.v_st, p.d,
+            p.dv, p.scale, p.window, p.sinks, tile.pf + xt);
       }
     }
   }
-#pragma unroll
-  for (int e = 0; e < kWinDims / 32; ++e) {
-    const int c = lane + 32 * e;
-    if (c < p.dv) out[c] = from_f32<T>(l == 0.f ? 0.f : o[e] / l);
-  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace bio
@@ -142,12 +832,72 @@ int launch_rows(const bio::WindowParams& p, bool packed, cudaStream_t s) {
   return bio_host::launch_status(cudaGetLastError());
 }
 
+template <typename T, int DP>
+int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, bool packed, cudaStream_t s) {
+  using L = bio::WinSmem<DP>;
+  static std::once_flag once[bio_host::kMaxDevices];
+  cudaError_t set = cudaSuccess;
+  std::call_once(once[a->device], [&] {
+    set = cudaFuncSetAttribute(bio::window_tc_kernel<T, DP>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  });
+  if (set != cudaSuccess) return BIO_ERR_LAUNCH;
+  const int sms = bio_host::sm_count(a->device);
+  if (sms <= 0) return BIO_ERR_LAUNCH;
+  bio::WindowJobs w;
+  const int64_t group = p.group;
+  w.hblocks = static_cast<int>((group + 15) / 16);  // up to 16 heads of a group in a tile
+  w.gh = static_cast<int>((group + w.hblocks - 1) / w.hblocks);
+  w.tok = 128 / w.gh;
+  const int64_t span = L::NT * w.tok, tiles = a->kv_heads * w.hblocks;
+  const int64_t qblocks = (p.lq + span - 1) / span + (packed ? p.nseq : 0);
+  const int64_t jobs = qblocks * tiles * (packed ? 1 : p.batch);
+  if (qblocks > kMaxGrid || jobs > kMaxGrid) return BIO_ERR_SHAPE;
+  w.qblocks = static_cast<int>(qblocks);
+  w.jobs = static_cast<int>(jobs);
+  w.window = static_cast<int>(std::min<int64_t>(p.window, 1 << 30));
+  w.sinks = static_cast<int>(std::min<int64_t>(p.sinks, 1 << 30));
+  w.negate = p.scale < 0.f;
+  // a scale of 0 weighs every visible key alike; hidden ones stay at -inf
+  const float scale = (w.negate ? -p.scale : p.scale) * 1.4426950408889634f;
+  w.scale_log2 = scale == 0.f ? 1.17549435e-38f : scale;
+  w.vec_out = reinterpret_cast<uintptr_t>(p.o) % 16 == 0 &&
+              (p.o_sb | p.o_sh | p.o_st | p.dv) % 8 == 0;
+  CUtensorMap q, k, v;
+  const int64_t batch = packed ? 1 : p.batch;
+  // without keys nothing is read through K and V: any operand will do for their maps
+  const bool none = p.lk == 0;
+  if (!bio_host::map_of<T>(&q, p.q, p.d, p.lq, p.heads, batch, p.q_st, p.q_sh, p.q_sb, w.tok,
+                           w.gh) ||
+      !bio_host::map_of<T>(&k, none ? p.q : p.k, p.d, none ? 1 : p.lk, a->kv_heads, batch, p.k_st,
+                           p.k_sh, p.k_sb, 32) ||
+      !bio_host::map_of<T>(&v, none ? p.q : p.v, p.dv, none ? 1 : p.lk, a->kv_heads, batch, p.v_st,
+                           p.v_sh, p.v_sb, 32))
+    return BIO_ERR_ALIGN;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(jobs, sms));
+  bio::window_tc_kernel<T, DP><<<grid, L::kThreads, L::kBytes, s>>>(q, k, v, p, w);
+  return bio_host::launch_status(cudaGetLastError());
+}
+
+template <typename T>
+int launch_half(const bio::WindowParams& p, const bio_attn_args* a, bool packed, cudaStream_t s) {
+  const uint64_t bits = reinterpret_cast<uint64_t>(p.q) | reinterpret_cast<uint64_t>(p.k) |
+                        reinterpret_cast<uint64_t>(p.v) |
+                        2 * static_cast<uint64_t>(p.q_sb | p.q_sh | p.q_st | p.k_sb | p.k_sh |
+                                                  p.k_st | p.v_sb | p.v_sh | p.v_st);
+  if (bits % 16 != 0) return BIO_ERR_ALIGN;
+  const int dim = std::max(p.d, p.dv);
+  return dim <= 64    ? launch_tc<T, 64>(p, a, packed, s)
+         : dim <= 128 ? launch_tc<T, 128>(p, a, packed, s)
+                      : launch_tc<T, 256>(p, a, packed, s);
+}
+
 int run_window(const bio_attn_args* a, int64_t window, int64_t sinks, bool packed, void* stream) {
   if (a == nullptr) return BIO_ERR_ARG;
   if (a->d < 1 || a->dv < 1 || a->d > bio::kWinDims || a->dv > bio::kWinDims)
     return BIO_ERR_SHAPE;
   if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->heads > 65536 ||
-      a->batch < 0 || a->lq < 0 || a->lk < 0 || a->lq > kMaxGrid || a->lk > kMaxGrid)
+      a->batch < 0 || a->lq < 0 || a->lk < 0 || a->lq > (1 << 30) || a->lk > (1 << 30))
     return BIO_ERR_SHAPE;
   if (window < 1 || window > kMaxGrid || sinks < 0 || sinks > kMaxGrid || a->causal != 0 ||
       a->mask_kind != BIO_MASK_NONE)
@@ -176,8 +926,8 @@ int run_window(const bio_attn_args* a, int64_t window, int64_t sinks, bool packe
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case BIO_F32: return launch_rows<float>(p, packed, s);
-    case BIO_F16: return launch_rows<__half>(p, packed, s);
-    case BIO_BF16: return launch_rows<__nv_bfloat16>(p, packed, s);
+    case BIO_F16: return launch_half<__half>(p, a, packed, s);
+    case BIO_BF16: return launch_half<__nv_bfloat16>(p, a, packed, s);
     default: return BIO_ERR_DTYPE;
   }
 }
