@@ -253,13 +253,13 @@ __device__ __forceinline__ int2 window_span(const WinTile& t, int b) {
 }
 
 // Job number -> job.  All lanes of the warp call it; false: no such job.
-template <int NT>
+template <int NT, bool PACKED>
 __device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJobs& w, int number,
                                            WinJob& j) {
   const int lane = threadIdx.x & 31;
   const int tiles = static_cast<int>(p.heads / p.group) * w.hblocks;
   int qb, hx;
-  if (p.cu_q == nullptr) {
+  if constexpr (!PACKED) {
     const int rest = number / w.qblocks;
     qb = number - rest * w.qblocks;
     j.b = rest / tiles;
@@ -325,9 +325,40 @@ __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void commit_to(uint32_t bar) {
+// tcgen05 instructions of a warp that runs in step: one thread (`leader`, the
+// same each time) issues them, and everything around stays uniform, so that the
+// descriptors can be made in uniform registers.  With the issuing loop inside
+// `if (lane == 0)` a product took about 140 cycles to issue and 90 to run.
+__device__ __forceinline__ uint32_t elect_leader() {
+  uint32_t is;
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is;
+}
+__device__ __forceinline__ void commit_to(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          bar),
+      "r"(leader)
+      : "memory");
+}
+// D (+)= A B with A from shared memory (K-major) or from TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
 
@@ -391,7 +422,7 @@ struct WinBars {
   __device__ uint32_t all_done() const { return base + 216; }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool PACKED>
 __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const WindowParams p,
@@ -444,7 +475,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     bool ok = true;
     for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
       WinJob j;
-      if (!window_job<NT>(p, w, number, j)) continue;
+      if (!window_job<NT, PACKED>(p, w, number, j)) continue;
       WinTile tile[NT];
       const WinPlan plan = window_plan<NT, BN>(w, j, tile);
       for (int i = 0; ok && i < plan.blocks; ++i) {
@@ -503,102 +534,115 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     }
   } else if (warp == 1) {
     // --------------------------------------------------------------------- MMA
-    int pos = 0;                       // ring position of the job's first K
+    const uint32_t leader = elect_leader();
+    int slot = 0;                      // ring position of the next K
+    uint32_t turn = 0;
     int s_used[NT], q_used[NT];        // S products, jobs of tile t
 #pragma unroll
     for (int t = 0; t < NT; ++t) s_used[t] = q_used[t] = 0;
     bool ok = true;
     for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
       WinJob j;
-      if (!window_job<NT>(p, w, number, j)) continue;
+      if (!window_job<NT, PACKED>(p, w, number, j)) continue;
       WinTile tile[NT];
       const WinPlan plan = window_plan<NT, BN>(w, j, tile);
-      if (lane == 0) {
-        int2 held[NT];                 // columns of the P that waits for its PV
-        bool asked[NT], begun[NT];     // queries waited for; O holds something
+      int2 held[NT];                   // columns of the P that waits for its PV
+      int last[NT];                    // the tile's last block
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        held[t] = make_int2(0, 0);
+        const int b = (tile[t].hi - 1) / BN;
+        last[t] = tile[t].hi == 0 ? -1 : b < plan.head ? b : b - plan.jump;
+      }
+      uint32_t asked = 0, begun = 0;   // bit t: queries waited for; O holds something
+      int v_slot = 0;                  // V of the block before
+      uint32_t v_turn = 0;
+      for (int i = 0; ok && i <= plan.blocks; ++i) {
+        const bool more = i < plan.blocks;
+        const int b = i < plan.head ? i : i + plan.jump;
+        if (more) ok = __all_sync(0xffffffffu, wait(bar.full(slot), turn));
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          held[t] = make_int2(0, 0);
-          asked[t] = begun[t] = false;
-        }
-        auto last_block = [&](int t) {  // index of the tile's last block
-          const int b = (tile[t].hi - 1) / BN;
-          return b < plan.head ? b : b - plan.jump;
-        };
-        auto issue_s = [&](int t, int i, int2 s) {
-          const int slot = (pos + 2 * i) % NS;
-          const int x = NT == 2 ? t : s_used[t] & 1;  // S buffer
-          if (!asked[t]) {
-            ok = wait(bar.q_full(t), q_used[t]);
-            if (!ok) return;
-            asked[t] = true;
-          }
-          tc_fence_after();
-          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
-          const uint32_t qa = q32 + t * L::kQ;
-          const uint32_t ka = ring32 + slot * L::kSlot + s.x * 128;
-          for (int k = 0; k < kc * 4; ++k)
-            umma_f16(tmem + x * 128 + s.x,
-                     smem_desc_sw128(qa + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
-                     smem_desc_sw128(ka + (k >> 2) * (BN * 128) + (k & 3) * 32, 16, 1024), idesc,
-                     k > 0 ? 1u : 0u);
-          commit_to(bar.s_full(x));
-          ++s_used[t];
-          if (i == last_block(t)) {
-            commit_to(bar.q_empty(t));
-            ++q_used[t];
-          }
-        };
-        // PV of block i, whose P came from the tile's S product number `of`
-        auto issue_pv = [&](int t, int i, int of) {
-          const int slot = (pos + 2 * i + 1) % NS;
-          const int x = NT == 2 ? t : of & 1;
-          ok = wait(bar.p_ready(x), NT == 2 ? of : of >> 1);
-          if (!ok) return;
-          ok = wait(bar.full(slot), (pos + 2 * i + 1) / NS);
-          if (!ok) return;
-          tc_fence_after();
-          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
-          const uint32_t va = ring32 + slot * L::kSlot;
-          for (int k = held[t].x / 16; k < held[t].y / 16; ++k) {
-            umma_f16_ts(tmem + 256 + t * 128, tmem + x * 128 + k * 8,
-                        smem_desc_sw128(va + k * 2048, BN * 128, 1024), idesc, begun[t] ? 1u : 0u);
-            begun[t] = true;
-          }
-          held[t] = make_int2(0, 0);
-          if (NT == 1) commit_to(bar.pv_done());
-          if (i == last_block(t)) commit_to(bar.o_done(t));
-        };
-        for (int i = 0; ok && i <= plan.blocks; ++i) {
-          if (i < plan.blocks) ok = wait(bar.full((pos + 2 * i) % NS), (pos + 2 * i) / NS);
-          const int b = i < plan.head ? i : i + plan.jump;
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            int2 s = make_int2(0, 0);
-            if (i < plan.blocks) s = window_span<BN>(tile[t], b);
-            const bool waiting = held[t].x < held[t].y;
-            if (NT == 2) {
-              if (ok && waiting) issue_pv(t, i - 1, s_used[t] - 1);
-              if (ok && s.x < s.y) issue_s(t, i, s);
-            } else {
-              if (ok && s.x < s.y) issue_s(t, i, s);
-              if (ok && waiting) issue_pv(t, i - 1, s_used[t] - (s.x < s.y ? 2 : 1));
+          int2 s = make_int2(0, 0);
+          if (more) s = window_span<BN>(tile[t], b);
+          auto products_s = [&]() {
+            const int x = NT == 2 ? t : s_used[t] & 1;  // S buffer
+            if (!((asked >> t) & 1u)) {
+              ok = __all_sync(0xffffffffu, wait(bar.q_full(t), q_used[t]));
+              asked |= 1u << t;
+              if (!ok) return;
             }
-            if (s.x < s.y) held[t] = s;
+            tc_fence_after();
+            const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
+            uint64_t qd = smem_desc_sw128(q32 + t * L::kQ, 16, 1024);
+            uint64_t kd = smem_desc_sw128(ring32 + slot * L::kSlot + s.x * 128, 16, 1024);
+            const uint32_t to = tmem + x * 128 + s.x;
+            // 16 columns are 32 bytes, 2 units of a descriptor; 64 columns a chunk
+#pragma unroll 1
+            for (int c = 0; c < kc; ++c) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_ss(to, qd + 2 * k, kd + 2 * k, idesc, k > 0 ? 1u : c, leader);
+              qd += 1024;
+              kd += BN * 8;
+            }
+            commit_to(bar.s_full(x), leader);
+            ++s_used[t];
+            if (i == last[t]) {
+              commit_to(bar.q_empty(t), leader);
+              ++q_used[t];
+            }
+          };
+          // PV of the block before, whose P came from the tile's S product number `of`
+          auto products_pv = [&](int of) {
+            const int x = NT == 2 ? t : of & 1;
+            ok = __all_sync(0xffffffffu, wait(bar.p_ready(x), NT == 2 ? of : of >> 1) &&
+                                             wait(bar.full(v_slot), v_turn));
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
+            // 16 keys are 2048 bytes of V and 8 columns of P
+            const int k0 = held[t].x / 16;
+            uint64_t vd = smem_desc_sw128(ring32 + v_slot * L::kSlot, BN * 128, 1024) + k0 * 128;
+            uint32_t pa = tmem + x * 128 + k0 * 8;
+            const uint32_t to = tmem + 256 + t * 128;
+            uint32_t on = (begun >> t) & 1u;
+#pragma unroll 1
+            for (int k = k0; k < held[t].y / 16; k += 2) {  // 32 columns at a time
+              mma_ts(to, pa, vd, idesc, on, leader);
+              mma_ts(to, pa + 8, vd + 128, idesc, 1u, leader);
+              on = 1u;
+              pa += 16;
+              vd += 256;
+            }
+            begun |= 1u << t;
+            if (NT == 1) commit_to(bar.pv_done(), leader);
+            if (i - 1 == last[t]) commit_to(bar.o_done(t), leader);
+          };
+          const bool now = s.x < s.y, waiting = held[t].x < held[t].y;
+          if (NT == 2) {
+            if (ok && waiting) products_pv(s_used[t] - 1);
+            if (ok && now) products_s();
+          } else {
+            if (ok && now) products_s();
+            if (ok && waiting) products_pv(s_used[t] - (now ? 2 : 1));
           }
-          // what the products issued so far have read is free once they are done
-          if (ok && i > 0) commit_to(bar.empty((pos + 2 * i - 1) % NS));
-          if (ok && i < plan.blocks) commit_to(bar.empty((pos + 2 * i) % NS));
+          held[t] = s;
+        }
+        // what the products issued so far have read is free once they are done
+        if (ok && i > 0) commit_to(bar.empty(v_slot), leader);
+        if (ok && more) {
+          commit_to(bar.empty(slot), leader);
+          v_turn = slot + 1 == NS ? turn ^ 1u : turn;
+          v_slot = slot + 1 == NS ? 0 : slot + 1;
+          turn = v_slot + 1 == NS ? v_turn ^ 1u : v_turn;
+          slot = v_slot + 1 == NS ? 0 : v_slot + 1;
         }
       }
-      ok = __all_sync(0xffffffffu, ok);
-      pos += 2 * plan.blocks;
     }
-    if (lane == 0) {
-      commit_to(bar.all_done());
-      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 27, 0))
-        raise_status(p.status, BIO_DEV_TIMEOUT);
-    }
+    commit_to(bar.all_done(), leader);
+    if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 27, 0))
+      raise_status(p.status, BIO_DEV_TIMEOUT);
   }
   } else {
     if (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -612,7 +656,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     bool ok = true;
     for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
       WinJob j;
-      if (!window_job<NT>(p, w, number, j)) continue;
+      if (!window_job<NT, PACKED>(p, w, number, j)) continue;
       WinTile tiles[NT];
       const WinPlan plan = window_plan<NT, BN>(w, j, tiles);
       WinTile tile = tiles[0];
@@ -723,7 +767,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         float s0, s1;
         split_pair(add_pair(sum2, sum3), s0, s1);
         l += s0 + s1;
-        if (p.cu_q != nullptr && j0 + s.y > j.lk) {
+        if (PACKED && j0 + s.y > j.lk) {
           // the block's last columns may be another sequence's tokens
           const int slot = (pos + 2 * i + 1) % NS;
           ok = wait(bar.full(slot), (pos + 2 * i + 1) / NS);
@@ -832,13 +876,14 @@ int launch_rows(const bio::WindowParams& p, bool packed, cudaStream_t s) {
   return bio_host::launch_status(cudaGetLastError());
 }
 
-template <typename T, int DP>
-int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, bool packed, cudaStream_t s) {
+template <typename T, int DP, bool PACKED>
+int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s) {
+  constexpr bool packed = PACKED;
   using L = bio::WinSmem<DP>;
   static std::once_flag once[bio_host::kMaxDevices];
   cudaError_t set = cudaSuccess;
   std::call_once(once[a->device], [&] {
-    set = cudaFuncSetAttribute(bio::window_tc_kernel<T, DP>,
+    set = cudaFuncSetAttribute(bio::window_tc_kernel<T, DP, PACKED>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   });
   if (set != cudaSuccess) return BIO_ERR_LAUNCH;
@@ -875,7 +920,7 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, bool packed, c
                            p.v_sh, p.v_sb, 32))
     return BIO_ERR_ALIGN;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(jobs, sms));
-  bio::window_tc_kernel<T, DP><<<grid, L::kThreads, L::kBytes, s>>>(q, k, v, p, w);
+  bio::window_tc_kernel<T, DP, PACKED><<<grid, L::kThreads, L::kBytes, s>>>(q, k, v, p, w);
   return bio_host::launch_status(cudaGetLastError());
 }
 
@@ -887,9 +932,13 @@ int launch_half(const bio::WindowParams& p, const bio_attn_args* a, bool packed,
                                                   p.k_st | p.v_sb | p.v_sh | p.v_st);
   if (bits % 16 != 0) return BIO_ERR_ALIGN;
   const int dim = std::max(p.d, p.dv);
-  return dim <= 64    ? launch_tc<T, 64>(p, a, packed, s)
-         : dim <= 128 ? launch_tc<T, 128>(p, a, packed, s)
-                      : launch_tc<T, 256>(p, a, packed, s);
+  if (packed)
+    return dim <= 64    ? launch_tc<T, 64, true>(p, a, s)
+           : dim <= 128 ? launch_tc<T, 128, true>(p, a, s)
+                        : launch_tc<T, 256, true>(p, a, s);
+  return dim <= 64    ? launch_tc<T, 64, false>(p, a, s)
+         : dim <= 128 ? launch_tc<T, 128, false>(p, a, s)
+                      : launch_tc<T, 256, false>(p, a, s);
 }
 
 int run_window(const bio_attn_args* a, int64_t window, int64_t sinks, bool packed, void* stream) {
