@@ -29,6 +29,30 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, u
       : "memory");
 }
 
+// Bounded wait that polls without giving the warp up.
+__device__ __forceinline__ bool spin_wait(uint32_t a, uint32_t parity, volatile int* abort_flag,
+                                          int* status) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0; i < kWaitMaxIters; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255u) != 255u) continue;
+    if (t0 == 0) t0 = global_timer_ns();
+    if (*abort_flag) return false;
+    if (global_timer_ns() - t0 > kWaitTimeoutNs) break;
+  }
+  *abort_flag = 1;
+  raise_status(status, BIO_DEV_TIMEOUT);
+  return false;
+}
+
 // Bounded wait (the contract of mbar_wait) whose polls park the warp: polling
 // warps take issue slots from the one or two that share their scheduler.
 __device__ __forceinline__ bool parked_wait(uint32_t a, uint32_t parity,

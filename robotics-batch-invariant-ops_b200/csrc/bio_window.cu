@@ -136,34 +136,41 @@ __global__ void __launch_bounds__(kWinWarps * 32) window_row_kernel(const Window
 // ---------------------------------------------------------------------------
 // tcgen05 kernel.
 //
-// A block of CTAs' work is a job: NT tiles of 128 query rows that share a KV
-// head.  A tile packs `gh` query heads of the group with `tok` = 128 / gh
-// consecutive tokens each (row r: head r / tok, token r % tok), so the keys
-// that a tile visits are its window plus tok - 1, not plus 127, and a key block
-// is loaded once for the whole group.  Jobs are dealt out round robin to one
-// persistent CTA per SM:
-//   warp 0      TMA: Q tiles, then K and V blocks of BN keys through one ring.
-//   warp 1      MMA (one thread): S_t = Q_t K^T, O_t += P_t V, fp32 in TMEM; P
-//               (16 bits) lies over the S that it came from.
-//   warps 4..   softmax: one thread per query row; the 128 rows of tile t belong
-//               to warps 4 + 4 t .. 7 + 4 t, which take over registers of the
-//               first four warps (two of them idle).
-// The ring, S and O run on across jobs: a job's first products start while the
-// last rows of the one before are still being stored.  With two tiles
-// (D <= 128) the tensor cores work on one tile while the other is in its
-// softmax; with one tile (D <= 256) S has two buffers, and S of block j + 1 is
-// issued before P_j is waited for.
+// A job is a tile of 128 query rows that share a KV head: `gh` query heads of
+// the group with `tok` = 128 / gh consecutive tokens each (row r: head r / tok,
+// token r % tok), so the keys that a tile visits are its window plus tok - 1, not
+// plus 127, and a key block is loaded once for all those heads.  Jobs are dealt
+// out round robin to one persistent CTA per SM:
+//   warp 0      TMA: Q, then K and V blocks of BN keys through one ring.
+//   warp 1      MMA: S = Q K^T into one of three buffers, O += P V, fp32 in TMEM;
+//               P (16 bits) lies over the S that it came from.
+//   warps 4-11  softmax: two groups of 128 threads, a thread per query row, take
+//               the blocks in turn.
+// S of block i + 2 is issued before PV of block i, so each group finds its next
+// scores ready while the other one and the tensor cores are at work, and nobody
+// waits for one chain.  The groups hand the rows' running reference m to each
+// other right after a block's maximum; each keeps its own sum l.  The ring, S and
+// O run on across jobs: a job's first blocks start while the last rows of the
+// one before are still being stored.
 //
-// Blocks are cut on the absolute grid of BN keys and trimmed, per tile, to the
-// 32-key columns that some row of the tile sees: a window costs about window +
-// tok + 32 columns per row, four sink tokens one 32-key column.  Masked scores
-// weigh exactly 0 and untrimmed columns add exactly 0, so a row's bits depend
-// on its own query, keys and position only.
+// What was measured on the way (32768 tokens, 32 heads on 8, d 128, window 1024):
+// two tiles with one S buffer each 842 us, bound by the chain softmax -> PV -> S of
+// a tile (4900 clocks a round, 3200 of them products: an M = 128, K = 16 product
+// takes about 100 clocks at N = 64 as at N = 128); two threads per row 838 us (the
+// two tiles' exponentials then run at the same time, and the special-function
+// unit is what both want); 64-key blocks with two buffers per tile 977 us (twice
+// the products).
 //
-// Scores stay in fp32 registers (128 a thread).  The reference m of the
+// Blocks are cut on the absolute grid of BN keys and trimmed to the 32-key
+// columns that some row of the tile sees: a window costs about window + tok + 32
+// columns per row, four sink tokens one 32-key column.  Masked scores weigh
+// exactly 0 and untrimmed columns add exactly 0, so a row's bits depend on its
+// own query, keys and position only.
+//
+// Scores, maxima and sums are fp32 in registers.  The reference m of the
 // exponentials moves only when a block's maximum exceeds it by more than 8
 // (log2), so O is rarely rescaled and P stays below 2^8; P is rounded to the
-// operand type, as the product needs, l sums it unrounded in fp32.
+// operand type, as the product needs, l sums it unrounded.
 //
 // A hidden key in a visited block has weight 0, but 0 * Inf or 0 * NaN in V
 // would still reach the row: a row whose output is not finite is computed once
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(kWinWarps * 32) window_row_kernel(const Window
 // ---------------------------------------------------------------------------
 struct WindowJobs {
   int gh, tok, hblocks;  // heads and tokens of a tile, tiles across a group
-  int qblocks;           // dense: blocks of NT * tok tokens per sequence; packed: at most
+  int qblocks;           // dense: blocks of tok tokens per sequence; packed: at most
   int jobs;
   int window, sinks;     // at most 2^30
   float scale_log2;      // > 0
@@ -183,68 +190,47 @@ struct WindowJobs {
 
 template <int DP>
 struct WinSmem {
-  static constexpr int NT = DP == 256 ? 1 : 2;     // tiles of a job
   static constexpr int BN = DP == 256 ? 64 : 128;  // keys of a block
   static constexpr uint32_t kQ = 128 * DP * 2;
   static constexpr uint32_t kSlot = BN * DP * 2;   // K or V of a block
-  static constexpr int kFit = (226 * 1024 - 1024 - 512 - NT * static_cast<int>(kQ)) /
+  static constexpr uint32_t kSwap = 4 * 128 * 4;   // m of two groups, l of two jobs
+  static constexpr int kFit = (227 * 1024 - 1024 - 512 - static_cast<int>(kSwap + kQ)) /
                               static_cast<int>(kSlot);
-  static constexpr int kSlots = kFit > 8 ? 8 : kFit;
-  static constexpr uint32_t kBytes = 1024 + NT * kQ + kSlots * kSlot + 512;
-  static constexpr int kThreads = 128 + 128 * NT;
-  static_assert(kSlots >= 4, "K and V of two blocks");
+  static constexpr int kSlots = kFit > 12 ? 12 : kFit;
+  static constexpr uint32_t kBytes = 1024 + kQ + kSlots * kSlot + 512 + kSwap;
+  static constexpr int kThreads = 384;
+  static constexpr uint32_t kO = DP == 256 ? 256 : 384;  // TMEM columns of O; S buffers x at x * BN
+  static_assert(kSlots >= 4, "K of three blocks and a V");
 };
 
 struct WinJob {
   int b, hk, h0, nh;        // sequence of the batch, KV head, query heads
-  int q0, lq, lk;           // first query of the job, lengths of its sequence
+  int q0, lq, lk;           // first query of the tile, lengths of its sequence
   int qt, kt;               // tokens of the operands at which the sequence starts
+  int pf, n;                // position of the tile's first token, number of tokens
+  int lo, hi, sx;           // keys: [lo, hi) for the windows of its rows, [0, sx) sinks before
+  int head, jump, blocks;   // block i of the job is block i < head ? i : i + jump of the keys
 };
 
-// Keys of a tile: [lo, hi) for the windows of its rows, [0, sx) sinks before it.
-struct WinTile {
-  int pf, n;   // position of its first token, number of tokens
-  int lo, hi, sx;
-};
-
-struct WinPlan {
-  int head, jump, blocks;  // block i of the job is block i < head ? i : i + jump of the keys
-};
-
-template <int NT, int BN>
-__device__ __forceinline__ WinPlan window_plan(const WindowJobs& w, const WinJob& j,
-                                               WinTile (&tile)[NT]) {
-  int head = 0, first = 0x7fffffff, last = -1;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    WinTile& x = tile[t];
-    const int q = j.q0 + t * w.tok;
-    x.n = max(0, min(w.tok, j.lq - q));
-    x.pf = q + j.lk - j.lq;
-    x.hi = x.n > 0 ? max(0, x.pf + x.n) : 0;
-    x.lo = x.hi > 0 ? max(0, x.pf - w.window + 1) : 0;
-    x.sx = min(w.sinks, x.lo);
-    if (x.hi > 0) {
-      head = max(head, (x.sx + BN - 1) / BN);
-      first = min(first, x.lo / BN);
-      last = max(last, (x.hi - 1) / BN);
-    }
-  }
-  WinPlan p;
-  p.head = head;
-  p.jump = last < 0 ? 0 : max(0, first - head);
-  p.blocks = last < 0 ? 0 : last + 1 - p.jump;
-  return p;
+template <int BN>
+__device__ __forceinline__ void window_plan(const WindowJobs& w, WinJob& j) {
+  j.n = max(0, min(w.tok, j.lq - j.q0));
+  j.pf = j.q0 + j.lk - j.lq;
+  j.hi = j.n > 0 ? max(0, j.pf + j.n) : 0;
+  j.lo = j.hi > 0 ? max(0, j.pf - w.window + 1) : 0;
+  j.sx = min(w.sinks, j.lo);
+  j.head = (j.sx + BN - 1) / BN;
+  j.jump = max(0, j.lo / BN - j.head);
+  j.blocks = j.hi == 0 ? 0 : (j.hi - 1) / BN + 1 - j.jump;
 }
 
-// Columns [x, y) of block b (keys b * BN ...) that some row of the tile sees, on
-// the 32-column grid; empty: x == y.
+// Columns [x, y) of the job's block i that some row sees, on the 32-column grid.
 template <int BN>
-__device__ __forceinline__ int2 window_span(const WinTile& t, int b) {
-  const int base = b * BN;
-  int x = max(t.lo - base, 0), y = min(t.hi - base, BN);
+__device__ __forceinline__ int2 window_span(const WinJob& j, int i) {
+  const int base = (i < j.head ? i : i + j.jump) * BN;
+  int x = max(j.lo - base, 0), y = min(j.hi - base, BN);
   if (x >= y) x = y = 0;
-  const int s = min(t.sx - base, BN);
+  const int s = min(j.sx - base, BN);
   if (s > 0) {
     x = 0;
     y = max(y, s);
@@ -252,8 +238,19 @@ __device__ __forceinline__ int2 window_span(const WinTile& t, int b) {
   return make_int2(x & ~31, (y + 31) & ~31);
 }
 
+// Blocks x <= i < y of the job: every row sees every key by its window, and all
+// 128 rows exist (or are padding of the tile's shape).
+template <int BN>
+__device__ __forceinline__ int2 window_whole(const WindowJobs& w, const WinJob& j) {
+  if (w.negate || j.n < w.tok || j.nh < w.gh || j.pf < 0) return make_int2(0, 0);
+  const int x = (max(0, j.pf + j.n - w.window) + BN - 1) / BN;  // first inside the last window
+  const int y = (j.pf + 1) / BN;                                // first past the first row
+  // only what lies behind the sinks' blocks keeps its distance
+  return make_int2(max(x, j.head + j.jump) - j.jump, y - j.jump);
+}
+
 // Job number -> job.  All lanes of the warp call it; false: no such job.
-template <int NT, bool PACKED>
+template <int BN, bool PACKED>
 __device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJobs& w, int number,
                                            WinJob& j) {
   const int lane = threadIdx.x & 31;
@@ -276,7 +273,7 @@ __device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJo
       return false;
     }
     // 32 sequences at a time: the one whose blocks hold block qb
-    const int span = NT * w.tok;
+    const int span = w.tok;
     bool found = false;
     for (int64_t s0 = 0; s0 < p.nseq && !found; s0 += 32) {
       const int64_t s = s0 + lane;
@@ -313,11 +310,12 @@ __device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJo
     }
     if (!found) return false;
   }
-  j.q0 = qb * NT * w.tok;
+  j.q0 = qb * w.tok;
   j.hk = hx / w.hblocks;
   const int before = (hx - j.hk * w.hblocks) * w.gh;
   j.h0 = j.hk * static_cast<int>(p.group) + before;
   j.nh = min(w.gh, static_cast<int>(p.group) - before);
+  window_plan<BN>(w, j);
   return true;
 }
 
@@ -325,40 +323,18 @@ __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// tcgen05 instructions of a warp that runs in step: one thread (`leader`, the
-// same each time) issues them, and everything around stays uniform, so that the
-// descriptors can be made in uniform registers.  With the issuing loop inside
-// `if (lane == 0)` a product took about 140 cycles to issue and 90 to run.
-__device__ __forceinline__ uint32_t elect_leader() {
+// The MMA warp runs in step and one elected thread issues the tcgen05
+// instructions, so that waits, spans and descriptors stay uniform.
+__device__ __forceinline__ bool elect_leader() {
   uint32_t is;
   asm volatile(
       "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(is));
-  return is;
+  return is != 0;
 }
-__device__ __forceinline__ void commit_to(uint32_t bar, uint32_t leader) {
+__device__ __forceinline__ void commit_to(uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
-          bar),
-      "r"(leader)
-      : "memory");
-}
-// D (+)= A B with A from shared memory (K-major) or from TMEM.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate, uint32_t leader) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate, uint32_t leader) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
       : "memory");
 }
 
@@ -406,21 +382,45 @@ __device__ __forceinline__ uint32_t bits_between(int x, int y) {
   return static_cast<uint32_t>(below_b & ~below_a);
 }
 
-// Shared-space addresses of the barriers and the TMEM base slot.
-template <int DP>
+// 32 lanes x 8 columns of TMEM, the load waited for.
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
+// Shared-space addresses of the barriers (8 bytes each).
 struct WinBars {
-  using L = WinSmem<DP>;
   uint32_t base;
   __device__ uint32_t full(int s) const { return base + s * 8; }
-  __device__ uint32_t empty(int s) const { return base + 64 + s * 8; }
-  __device__ uint32_t q_full(int t) const { return base + 128 + t * 8; }
-  __device__ uint32_t q_empty(int t) const { return base + 144 + t * 8; }
-  __device__ uint32_t s_full(int x) const { return base + 160 + x * 8; }
-  __device__ uint32_t p_ready(int x) const { return base + 176 + x * 8; }
-  __device__ uint32_t o_done(int t) const { return base + 192 + t * 8; }
-  __device__ uint32_t pv_done() const { return base + 208; }
-  __device__ uint32_t all_done() const { return base + 216; }
+  __device__ uint32_t empty(int s) const { return base + 96 + s * 8; }
+  __device__ uint32_t s_full(int x) const { return base + 192 + x * 8; }
+  __device__ uint32_t p_ready(int x) const { return base + 216 + x * 8; }
+  __device__ uint32_t pv_done(int x) const { return base + 240 + x * 8; }
+  __device__ uint32_t l_ready(int x) const { return base + 256 + x * 8; }
+  __device__ uint32_t q_full() const { return base + 272; }
+  __device__ uint32_t q_empty() const { return base + 280; }
+  __device__ uint32_t o_done() const { return base + 288; }
+  __device__ uint32_t o_free() const { return base + 296; }
+  __device__ uint32_t all_done() const { return base + 304; }
+  __device__ uint32_t m_ready(int group, int quarter) const {
+    return base + 312 + group * 32 + quarter * 8;
+  }
 };
+
+// The ring of a job of n blocks carries K0 K1 K2 V0 K3 V1 ..., the order in which
+// the products need them: the place of V of block i.
+__device__ __forceinline__ int ring_of_v(int i, int n) { return min(i + 3, n) + i; }
 
 template <typename T, int DP, bool PACKED>
 __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
@@ -428,23 +428,25 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
                      const __grid_constant__ CUtensorMap tmV, const WindowParams p,
                      const WindowJobs w) {
   using L = WinSmem<DP>;
-  constexpr int NT = L::NT, BN = L::BN, NS = L::kSlots;
+  constexpr int BN = L::BN, NS = L::kSlots, NC = BN / 32;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* ring = smem + NT * L::kQ;
+  uint8_t* ring = smem + L::kQ;
   uint8_t* tail = ring + NS * L::kSlot;
   const uint32_t q32 = smem_u32(smem), ring32 = smem_u32(ring);
-  const WinBars<DP> bar{smem_u32(tail)};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 256);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 260);
+  const WinBars bar{smem_u32(tail)};
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 384);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 388);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kc = (p.d + 63) / 64, vc = (p.dv + 63) / 64;
 
   if (threadIdx.x == 0) {
     uint64_t* b = reinterpret_cast<uint64_t*>(tail);
-    for (int i = 0; i < 28; ++i) mbar_init(b + i, i == 22 || i == 23 ? 4 : 1);  // p_ready: 4 warps
+    // p_ready, l_ready and o_free: four warps arrive
+    for (int i = 0; i < 47; ++i)
+      mbar_init(b + i, (i >= 27 && i < 30) || i == 32 || i == 33 || i == 37 ? 4 : 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -458,238 +460,236 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // S at column 0 and 128, O_t at 256 + 128 t
+  // All 512 columns of TMEM start at address 0, which as a constant costs the MMA
+  // warp no move to a uniform register.
+  constexpr uint32_t tmem = 0;
+  if (*tmem_slot != tmem) {  // the same for every thread
+    if (threadIdx.x == 0) raise_status(p.status, BIO_DEV_TIMEOUT);
+    if (warp == 1) tmem_dealloc(*tmem_slot, 512);
+    return;
+  }
   auto wait = [&](uint32_t b, uint32_t parity) -> bool {
-    return parked_wait(b, parity & 1u, abort_flag, p.status);
+    return __all_sync(0xffffffffu, parked_wait(b, parity & 1u, abort_flag, p.status));
   };
 
   // 384 threads start with 168 registers each, 128 of them go on with 56 and
   // 256 with 216: 62464 of the 64512
-  constexpr bool kShift = NT == 2;
   if (warp < 4) {
-    if (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == 0) {
-    // ---------------------------------------------------------------- producer
-    int pos = 0;                 // ring position: K and V of every block in turn
-    int q_used[2] = {0, 0};
-    bool ok = true;
-    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
-      WinJob j;
-      if (!window_job<NT, PACKED>(p, w, number, j)) continue;
-      WinTile tile[NT];
-      const WinPlan plan = window_plan<NT, BN>(w, j, tile);
-      for (int i = 0; ok && i < plan.blocks; ++i) {
-        const int b = i < plan.head ? i : i + plan.jump;
-        int x = BN, y = 0;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int2 s = window_span<BN>(tile[t], b);
-          if (s.x < s.y) {
-            x = min(x, s.x);
-            y = max(y, s.y);
-          }
-        }
-        const int rows = max(0, y - x);
-        for (int kv = 0; ok && kv < 2; ++kv, ++pos) {
-          const int slot = pos % NS;
-          ok = wait(bar.empty(slot), (pos / NS) ^ 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int chunks = kv == 0 ? kc : vc, boxes = chunks * (rows / 32);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // -------------------------------------------------------------- producer
+      int slot = 0, count = 0, q_used = 0;  // ring position; blocks, queries loaded so far
+      uint32_t turn = 0;
+      bool ok = true;
+      for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+        WinJob j;
+        if (!window_job<BN, PACKED>(p, w, number, j)) continue;
+        auto load = [&](bool key, int i) {
+          const int2 s = window_span<BN>(j, i);
+          const int chunks = key ? kc : vc, boxes = chunks * ((s.y - s.x) / 32);
+          ok = wait(bar.empty(slot), turn ^ 1u);
+          if (!ok) return;
           if (lane == 0) expect_bytes(bar.full(slot), boxes * 32 * 128);
           __syncwarp();
           if (lane < boxes) {
-            const int c = lane % chunks, r = x + lane / chunks * 32;
-            load_box(ring32 + slot * L::kSlot + c * (BN * 128) + r * 128, kv == 0 ? &tmK : &tmV,
-                     bar.full(slot), c * 64, j.kt + b * BN + r, j.hk, j.b);
+            const int c = lane % chunks, r = s.x + lane / chunks * 32;
+            load_box(ring32 + slot * L::kSlot + c * (BN * 128) + r * 128, key ? &tmK : &tmV,
+                     bar.full(slot), c * 64, j.kt + (i < j.head ? i : i + j.jump) * BN + r, j.hk,
+                     j.b);
           }
-          if (kv == 0 && i == 0) {  // the job's queries go out after its first keys
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              if (tile[t].hi == 0 || !ok) continue;
-              ok = wait(bar.q_empty(t), q_used[t] ^ 1);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              if (lane == 0) {
-                expect_bytes(bar.q_full(t), kc * w.gh * w.tok * 128);
-                for (int c = 0; c < kc; ++c)
-                  load_box(q32 + t * L::kQ + c * 16384, &tmQ, bar.q_full(t), c * 64,
-                           j.qt + j.q0 + t * w.tok, j.h0, j.b);
-              }
-              ++q_used[t];
-            }
+          ++count;
+          if (++slot == NS) {
+            slot = 0;
+            turn ^= 1u;
           }
+        };
+        const int n = j.blocks;
+        if (n == 0) continue;
+        load(true, 0);
+        if (ok) ok = wait(bar.q_empty(), q_used ^ 1);
+        if (!ok) break;
+        if (lane == 0) {
+          expect_bytes(bar.q_full(), kc * w.gh * w.tok * 128);
+          for (int c = 0; c < kc; ++c)
+            load_box(q32 + c * 16384, &tmQ, bar.q_full(), c * 64, j.qt + j.q0, j.h0, j.b);
+        }
+        ++q_used;
+        if (n > 1) load(true, 1);
+        for (int i = 0; ok && i < n; ++i) {
+          if (i + 2 < n) load(true, i + 2);
+          if (ok) load(false, i);
         }
       }
-    }
-    // every copy has to land before the block's shared memory goes
-    if (lane == 0) {
-      for (int i = max(0, pos - NS); i < pos; ++i)
-        if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + i % NS, (i / NS) & 1))
+      // every copy has to land before the block's shared memory goes
+      if (lane == 0) {
+        for (int i = max(0, count - NS); i < count; ++i)
+          if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + i % NS, (i / NS) & 1))
+            raise_status(p.status, BIO_DEV_TIMEOUT);
+        if (q_used > 0 &&
+            !mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 34, (q_used - 1) & 1))
           raise_status(p.status, BIO_DEV_TIMEOUT);
-      for (int t = 0; t < NT; ++t)
-        if (q_used[t] > 0 &&
-            !mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 16 + t, (q_used[t] - 1) & 1))
-          raise_status(p.status, BIO_DEV_TIMEOUT);
-    }
-  } else if (warp == 1) {
-    // --------------------------------------------------------------------- MMA
-    const uint32_t leader = elect_leader();
-    int slot = 0;                      // ring position of the next K
-    uint32_t turn = 0;
-    int s_used[NT], q_used[NT];        // S products, jobs of tile t
-#pragma unroll
-    for (int t = 0; t < NT; ++t) s_used[t] = q_used[t] = 0;
-    bool ok = true;
-    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
-      WinJob j;
-      if (!window_job<NT, PACKED>(p, w, number, j)) continue;
-      WinTile tile[NT];
-      const WinPlan plan = window_plan<NT, BN>(w, j, tile);
-      int2 held[NT];                   // columns of the P that waits for its PV
-      int last[NT];                    // the tile's last block
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        held[t] = make_int2(0, 0);
-        const int b = (tile[t].hi - 1) / BN;
-        last[t] = tile[t].hi == 0 ? -1 : b < plan.head ? b : b - plan.jump;
       }
-      uint32_t asked = 0, begun = 0;   // bit t: queries waited for; O holds something
-      int v_slot = 0;                  // V of the block before
-      uint32_t v_turn = 0;
-      for (int i = 0; ok && i <= plan.blocks; ++i) {
-        const bool more = i < plan.blocks;
-        const int b = i < plan.head ? i : i + plan.jump;
-        if (more) ok = __all_sync(0xffffffffu, wait(bar.full(slot), turn));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          int2 s = make_int2(0, 0);
-          if (more) s = window_span<BN>(tile[t], b);
-          auto products_s = [&]() {
-            const int x = NT == 2 ? t : s_used[t] & 1;  // S buffer
-            if (!((asked >> t) & 1u)) {
-              ok = __all_sync(0xffffffffu, wait(bar.q_full(t), q_used[t]));
-              asked |= 1u << t;
-              if (!ok) return;
-            }
-            tc_fence_after();
-            const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
-            uint64_t qd = smem_desc_sw128(q32 + t * L::kQ, 16, 1024);
-            uint64_t kd = smem_desc_sw128(ring32 + slot * L::kSlot + s.x * 128, 16, 1024);
-            const uint32_t to = tmem + x * 128 + s.x;
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------- MMA
+      int slot = 0;                         // ring position of what comes next
+      uint32_t turn = 0;
+      int s_buf = 0, p_buf = 0;             // buffers of the next S and the next P
+      uint32_t p_turn = 0;
+      int pvs = 0, jobs_done = 0;           // PV products and jobs so far
+      bool ok = true;
+      for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+        WinJob j;
+        if (!window_job<BN, PACKED>(p, w, number, j)) continue;
+        const int n = j.blocks;
+        if (n == 0) continue;
+        const int2 open = window_whole<BN>(w, j);
+        auto span = [&](int i) -> int2 {
+          return i >= open.x && i < open.y ? make_int2(0, BN) : window_span<BN>(j, i);
+        };
+        auto next = [&]() {
+          if (++slot == NS) {
+            slot = 0;
+            turn ^= 1u;
+          }
+        };
+        auto products_s = [&](int i) {
+          const int2 s = span(i);
+          if (ok) ok = wait(bar.full(slot), turn);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
+          uint64_t qd = smem_desc_sw128(q32, 16, 1024);
+          uint64_t kd = smem_desc_sw128(ring32 + slot * L::kSlot + s.x * 128, 16, 1024);
+          const uint32_t to = tmem + s_buf * BN + s.x;
+          if (elect_leader()) {
             // 16 columns are 32 bytes, 2 units of a descriptor; 64 columns a chunk
-#pragma unroll 1
             for (int c = 0; c < kc; ++c) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                mma_ss(to, qd + 2 * k, kd + 2 * k, idesc, k > 0 ? 1u : c, leader);
+                umma_f16(to, qd + 2 * k, kd + 2 * k, idesc, k > 0 ? 1u : c);
               qd += 1024;
               kd += BN * 8;
             }
-            commit_to(bar.s_full(x), leader);
-            ++s_used[t];
-            if (i == last[t]) {
-              commit_to(bar.q_empty(t), leader);
-              ++q_used[t];
-            }
-          };
-          // PV of the block before, whose P came from the tile's S product number `of`
-          auto products_pv = [&](int of) {
-            const int x = NT == 2 ? t : of & 1;
-            ok = __all_sync(0xffffffffu, wait(bar.p_ready(x), NT == 2 ? of : of >> 1) &&
-                                             wait(bar.full(v_slot), v_turn));
-            if (!ok) return;
-            tc_fence_after();
-            const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
-            // 16 keys are 2048 bytes of V and 8 columns of P
-            const int k0 = held[t].x / 16;
-            uint64_t vd = smem_desc_sw128(ring32 + v_slot * L::kSlot, BN * 128, 1024) + k0 * 128;
-            uint32_t pa = tmem + x * 128 + k0 * 8;
-            const uint32_t to = tmem + 256 + t * 128;
-            uint32_t on = (begun >> t) & 1u;
-#pragma unroll 1
-            for (int k = k0; k < held[t].y / 16; k += 2) {  // 32 columns at a time
-              mma_ts(to, pa, vd, idesc, on, leader);
-              mma_ts(to, pa + 8, vd + 128, idesc, 1u, leader);
-              on = 1u;
+            commit_to(bar.s_full(s_buf));
+            commit_to(bar.empty(slot));  // the keys are free once the products are done
+            if (i == n - 1) commit_to(bar.q_empty());
+          }
+          s_buf = s_buf == 2 ? 0 : s_buf + 1;
+          next();
+        };
+        ok = wait(bar.q_full(), jobs_done);
+        products_s(0);
+        if (n > 1) products_s(1);
+        for (int i = 0; ok && i < n; ++i) {
+          if (i + 2 < n) products_s(i + 2);
+          const int2 s = span(i);
+          // 16 keys are 2048 bytes of V and 8 columns of P
+          const int k0 = s.x / 16;
+          uint64_t vd = smem_desc_sw128(ring32 + slot * L::kSlot, BN * 128, 1024) + k0 * 128;
+          uint32_t pa = tmem + p_buf * BN + k0 * 8;
+          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
+          if (ok) ok = wait(bar.full(slot), turn);
+          // the rows of the job before have left O
+          if (ok && i == 0 && jobs_done > 0) ok = wait(bar.o_free(), jobs_done - 1);
+          if (ok) ok = wait(bar.p_ready(p_buf), p_turn);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_leader()) {
+            for (int k = k0; k < s.y / 16; k += 2) {  // 32 columns at a time
+              umma_f16_ts(tmem + L::kO, pa, vd, idesc, i > 0 || k > k0 ? 1u : 0u);
+              umma_f16_ts(tmem + L::kO, pa + 8, vd + 128, idesc, 1u);
               pa += 16;
               vd += 256;
             }
-            begun |= 1u << t;
-            if (NT == 1) commit_to(bar.pv_done(), leader);
-            if (i - 1 == last[t]) commit_to(bar.o_done(t), leader);
-          };
-          const bool now = s.x < s.y, waiting = held[t].x < held[t].y;
-          if (NT == 2) {
-            if (ok && waiting) products_pv(s_used[t] - 1);
-            if (ok && now) products_s();
-          } else {
-            if (ok && now) products_s();
-            if (ok && waiting) products_pv(s_used[t] - (now ? 2 : 1));
+            commit_to(bar.pv_done(pvs & 1));
+            commit_to(bar.empty(slot));
+            if (i == n - 1) commit_to(bar.o_done());
           }
-          held[t] = s;
+          ++pvs;
+          if (++p_buf == 3) {
+            p_buf = 0;
+            p_turn ^= 1u;
+          }
+          next();
         }
-        // what the products issued so far have read is free once they are done
-        if (ok && i > 0) commit_to(bar.empty(v_slot), leader);
-        if (ok && more) {
-          commit_to(bar.empty(slot), leader);
-          v_turn = slot + 1 == NS ? turn ^ 1u : turn;
-          v_slot = slot + 1 == NS ? 0 : slot + 1;
-          turn = v_slot + 1 == NS ? v_turn ^ 1u : v_turn;
-          slot = v_slot + 1 == NS ? 0 : v_slot + 1;
-        }
+        ++jobs_done;
       }
+      if (elect_leader()) commit_to(bar.all_done());
+      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 38, 0))
+        raise_status(p.status, BIO_DEV_TIMEOUT);
     }
-    commit_to(bar.all_done(), leader);
-    if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 27, 0))
-      raise_status(p.status, BIO_DEV_TIMEOUT);
-  }
   } else {
-    if (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ----------------------------------------------------------------- softmax
-    const int t = NT == 2 ? (warp - 4) >> 2 : 0;
+    const int group = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile: the warp's quarter of the lanes
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // (quarter * 32) << 16
+    const uint32_t o_at = tmem + lanes + L::kO;
     const int rh = r / w.tok, rt = r - rh * w.tok;
     const uint64_t scale2 = pair_of(w.scale_log2, w.scale_log2);
-    int pos = 0, s_used = 0, jobs_done = 0, pv_used = 0;
+    float* m_of = reinterpret_cast<float*>(tail + 512);  // [group][row]
+    float* l_of = m_of + 256;                            // [job & 1][row]
+    // m goes from warp to warp: of a quarter of the rows, from group to group
+    const uint32_t give = bar.m_ready(group, warp & 3), take = bar.m_ready(group ^ 1, warp & 3);
+    uint32_t taken = 0;                        // times that this warp took m
+    int blocks_before = 0, jobs_done = 0, sums_left = 0;
+    // After a wait that ran out the rest goes through without waiting for anything.
     bool ok = true;
-    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+    auto hold = [&](uint32_t b, uint32_t parity) {
+      if (ok) ok = wait(b, parity);
+    };
+    for (int number = blockIdx.x; number < w.jobs; number += gridDim.x) {
       WinJob j;
-      if (!window_job<NT, PACKED>(p, w, number, j)) continue;
-      WinTile tiles[NT];
-      const WinPlan plan = window_plan<NT, BN>(w, j, tiles);
-      WinTile tile = tiles[0];
-      if (NT == 2 && t == 1) tile = tiles[NT - 1];
-      const bool valid = rh < j.nh && rt < tile.n;
-      const int at = tile.pf + rt;                     // position of the row
-      const int row_lo = at - w.window + 1, row_s = min(w.sinks, at + 1);
-      float m = -INFINITY, l = 0.f;
-      bool first = true;
-      for (int i = 0; i < plan.blocks; ++i) {
-        const int b = i < plan.head ? i : i + plan.jump;
-        const int2 s = window_span<BN>(tile, b);
-        if (s.x >= s.y) continue;
-        const int x = NT == 2 ? t : s_used & 1;
-        ok = wait(bar.s_full(x), NT == 2 ? s_used : s_used >> 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      if (!window_job<BN, PACKED>(p, w, number, j)) continue;
+      const bool valid = rh < j.nh && rt < j.n;
+      const int at = j.pf + rt;                     // position of the row
+      const int2 open = window_whole<BN>(w, j);
+      float m = -INFINITY, l = 0.f, m_before = -INFINITY;
+      // global block number g = blocks_before + i: group g & 1, buffer g % 3
+      for (int i = (blocks_before & 1) ^ group; i < j.blocks; i += 2) {
+        const int g = blocks_before + i, x = g % 3;
+        const bool whole = i >= open.x && i < open.y;
+        int2 s = make_int2(0, BN);
+        if (!whole) s = window_span<BN>(j, i);
+        hold(bar.s_full(x), g / 3);
         tc_fence_after();
-        const uint32_t s_at = tmem + lanes + x * 128;
-        const int j0 = b * BN;
-        uint32_t f[BN / 32][32];
-        float top = -INFINITY;
-        // every row of the tile sees every column of the block
-        const bool whole = s.x == 0 && s.y == BN && !w.negate && tile.n == w.tok &&
-                           j.nh == w.gh && j0 + BN <= tile.pf + 1 &&
-                           (j0 >= tile.pf + tile.n - w.window || j0 + BN <= w.sinks);
+        const uint32_t s_at = tmem + lanes + x * BN;
+        uint32_t f[NC][32];
+        float top;
         if (whole) {
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
+          for (int c = 0; c < NC; ++c) tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) tmem_ld_wait_tied(f[c]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            if (c * 32 < s.x || c * 32 >= s.y) {  // trimmed: as if hidden
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[c][e] = 0xff800000u;
+              continue;
+            }
+            tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
+            tmem_ld_wait_tied(f[c]);
+            if (w.negate) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[c][e] ^= 0x80000000u;
+            }
+            const int a = (i < j.head ? i : i + j.jump) * BN + c * 32;
+            const uint32_t sees = valid ? bits_between(at - w.window + 1 - a, at + 1 - a) |
+                                              bits_between(0, min(w.sinks, at + 1) - a)
+                                        : 0u;
+            if (!__all_sync(0xffffffffu, sees == 0xffffffffu)) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(sees & (1u << e))) f[c][e] = 0xff800000u;  // -inf
+            }
+          }
+        }
+        {
           float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {
-            tmem_ld_wait_tied(f[c]);
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               a0 = max3(a0, __uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1]));
@@ -697,67 +697,55 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
               a2 = max3(a2, __uint_as_float(f[c][e + 4]), __uint_as_float(f[c][e + 5]));
               a3 = max3(a3, __uint_as_float(f[c][e + 6]), __uint_as_float(f[c][e + 7]));
             }
-          }
           top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
-        } else {
-#pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {
-            if (c * 32 < s.x || c * 32 >= s.y) continue;
-            tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
-            tmem_ld_wait_tied(f[c]);
-            const int a = j0 + c * 32;
-            const uint32_t sees =
-                valid ? bits_between(row_lo - a, at + 1 - a) | bits_between(0, row_s - a) : 0u;
-            const uint32_t flip = w.negate ? 0x80000000u : 0u;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              f[c][e] = (sees >> e) & 1u ? f[c][e] ^ flip : 0xff800000u;  // -inf
-              top = fmaxf(top, __uint_as_float(f[c][e]));
-            }
-          }
         }
         const float scaled = top == -INFINITY ? top : top * w.scale_log2;
-        const bool move = scaled > m + 8.f;
-        const float alpha = move ? pow2(m - scaled) : 1.f;
-        if (move) m = scaled;
-        l *= alpha;
-        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // S of this block was issued after the PV before it (two tiles), or that
-          // one has to be waited for (one tile)
-          if (NT == 1) {
-            ok = wait(bar.pv_done(), pv_used - 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-          }
+        // the reference as the block before left it
+        if (i > 0) {
+          hold(take, taken++);
+          m_before = m_of[(group ^ 1) * 128 + r];
+        }
+        const float was = m;  // the reference of this group's l
+        m = scaled > m_before + 8.f ? scaled : m_before;
+        if (i + 1 < j.blocks) {
+          m_of[group * 128 + r] = m;
+          __syncwarp();
+          if (lane == 0) arrive(give);
+        }
+        l *= was == m ? 1.f : pow2(was - m);
+        const bool moved = m != m_before;
+        if (i > 0 && __any_sync(0xffffffffu, moved)) {
+          // O holds the blocks before this one, by the old reference
+          hold(bar.pv_done((g - 1) & 1), (g - 1) >> 1);
+          tc_fence_after();
+          const float alpha = moved ? pow2(m_before - m) : 1.f;
 #pragma unroll 1
-          for (int c = 0; c < vc * 2; ++c) {
-            uint32_t v[32];
-            const uint32_t o_at = tmem + lanes + 256 + t * 128 + c * 32;
-            tmem_ld_32x32b_x32(o_at, v);
-            tmem_ld_wait();
+          for (int c = 0; c < vc * 8; ++c) {  // 8 columns at a time: few registers
+            uint32_t v[8];
+            tmem_ld_x8(o_at + c * 8, v);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-            tmem_st_32x32b_x32(o_at, v);
+            for (int e = 0; e < 8; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+            tmem_st_x8(o_at + c * 8, v);
           }
         }
-        first = false;
         const float ref = m == -INFINITY ? 0.f : m;
         const uint64_t ref2 = pair_of(-ref, -ref);
         uint64_t sum2 = 0, sum3 = 0;
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
+        for (int c = 0; c < NC; ++c) {
           if (!whole && (c * 32 < s.x || c * 32 >= s.y)) continue;
           uint32_t packed[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
+          for (int e = 0; e < 16; ++e) {
             float a, bb;
-            split_pair(fma_pair(pair_of(__uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1])), scale2,
-                                ref2), a, bb);
+            split_pair(fma_pair(pair_of(__uint_as_float(f[c][2 * e]),
+                                        __uint_as_float(f[c][2 * e + 1])),
+                                scale2, ref2),
+                       a, bb);
             a = pow2(a);
             bb = pow2(bb);
-            packed[e / 2] = pack_two<T>(a, bb);
-            if (e & 2)
+            packed[e] = pack_two<T>(a, bb);
+            if (e & 1)
               sum3 = add_pair(sum3, pair_of(a, bb));
             else
               sum2 = add_pair(sum2, pair_of(a, bb));
@@ -767,37 +755,52 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         float s0, s1;
         split_pair(add_pair(sum2, sum3), s0, s1);
         l += s0 + s1;
-        if (PACKED && j0 + s.y > j.lk) {
-          // the block's last columns may be another sequence's tokens
-          const int slot = (pos + 2 * i + 1) % NS;
-          ok = wait(bar.full(slot), (pos + 2 * i + 1) / NS);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          uint8_t* v = ring + slot * L::kSlot;
-          for (int row = max(0, j.lk - j0); row < s.y; ++row)
-            for (int c = r; c < vc * 8; c += 128)
-              *reinterpret_cast<uint4*>(v + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
+        if (PACKED) {
+          const int first = (i < j.head ? i : i + j.jump) * BN;
+          if (first + s.y > j.lk) {
+            // the block's last columns may be another sequence's tokens
+            // (the ring took two places for each of the blocks before)
+            const int pos = 2 * blocks_before + ring_of_v(i, j.blocks);
+            hold(bar.full(pos % NS), pos / NS);
+            uint8_t* v = ring + pos % NS * L::kSlot;
+            for (int row = max(0, j.lk - first); row < s.y; ++row)
+              for (int c = r; c < vc * 8; c += 128)
+                *reinterpret_cast<uint4*>(v + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive(bar.p_ready(x));
-        ++s_used;
-        ++pv_used;
       }
-      pos += 2 * plan.blocks;
-      if (!ok) break;
+      // The group of the last block stores the rows; the other one leaves its sum.
+      const bool store = ((blocks_before + j.blocks - 1) & 1) == group;
+      blocks_before += j.blocks;
+      const int left = sums_left & 1, left_turn = sums_left >> 1;
+      if (j.blocks > 1) ++sums_left;
+      if (j.blocks > 0) ++jobs_done;
+      if (!store) {
+        if (j.blocks > 1) {
+          l_of[left * 128 + r] = l;
+          __syncwarp();
+          if (lane == 0) arrive(bar.l_ready(left));
+        }
+        continue;
+      }
       // ------------------------------------------------------------- the output
-      const int tok = j.qt + j.q0 + t * w.tok + rt;
+      if (j.blocks > 1) {
+        hold(bar.l_ready(left), left_turn);
+        // the other group's sum goes by the reference of the block before the last
+        const float theirs = l_of[left * 128 + r];
+        l += m_before == m ? theirs : theirs * pow2(m_before - m);
+      }
+      const int tok = j.qt + j.q0 + rt;
       T* out = valid ? static_cast<T*>(p.o) + j.b * p.o_sb + (j.h0 + rh) * p.o_sh + tok * p.o_st
                      : nullptr;
-      if (tile.hi > 0) {
-        ok = wait(bar.o_done(t), jobs_done);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        ++jobs_done;
+      if (j.blocks > 0) {
+        hold(bar.o_done(), jobs_done - 1);
         tc_fence_after();
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -805,11 +808,16 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < vc * 2; ++c) {
         uint32_t v[32];
-        if (tile.hi > 0) {
-          tmem_ld_32x32b_x32(tmem + lanes + 256 + t * 128 + c * 32, v);
-          tmem_ld_wait();
+        if (j.blocks > 0) {
+          tmem_ld_32x32b_x32(o_at + c * 32, v);
+          tmem_ld_wait_tied(v);
+          if (c == vc * 2 - 1) {  // O is free for the next job
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(bar.o_free());
+          }
         }
-        if (l == 0.f || tile.hi == 0) {
+        if (l == 0.f || j.blocks == 0) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0;
         }
@@ -835,20 +843,20 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
             if (c * 32 + e < p.dv) out[c * 32 + e] = from_f32<T>(__uint_as_float(v[e]));
         }
       }
-      tc_fence_before();  // the next job's PV overwrites O after this row's next P
+      __syncwarp();
       unsigned again = __ballot_sync(0xffffffffu, valid && !(odd == 0.f));
       while (again != 0) {
         const int x = __ffs(again) - 1;
         again &= again - 1;
         const int xh = j.h0 + __shfl_sync(0xffffffffu, rh, x);
         const int xt = __shfl_sync(0xffffffffu, rt, x);
-        const int64_t xtok = j.qt + j.q0 + t * w.tok + xt;
+        const int64_t xtok = j.qt + j.q0 + xt;
         window_row<T>(
             static_cast<const T*>(p.q) + j.b * p.q_sb + xh * p.q_sh + xtok * p.q_st,
             static_cast<const T*>(p.k) + j.b * p.k_sb + j.hk * p.k_sh + j.kt * p.k_st,
             static_cast<const T*>(p.v) + j.b * p.v_sb + j.hk * p.v_sh + j.kt * p.v_st,
             static_cast<T*>(p.o) + j.b * p.o_sb + xh * p.o_sh + xtok * p.o_st, p.k_st, p.v_st, p.d,
-            p.dv, p.scale, p.window, p.sinks, tile.pf + xt);
+            p.dv, p.scale, p.window, p.sinks, j.pf + xt);
       }
     }
   }
@@ -894,7 +902,7 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
   w.hblocks = static_cast<int>((group + 15) / 16);  // up to 16 heads of a group in a tile
   w.gh = static_cast<int>((group + w.hblocks - 1) / w.hblocks);
   w.tok = 128 / w.gh;
-  const int64_t span = L::NT * w.tok, tiles = a->kv_heads * w.hblocks;
+  const int64_t span = w.tok, tiles = a->kv_heads * w.hblocks;
   const int64_t qblocks = (p.lq + span - 1) / span + (packed ? p.nseq : 0);
   const int64_t jobs = qblocks * tiles * (packed ? 1 : p.batch);
   if (qblocks > kMaxGrid || jobs > kMaxGrid) return BIO_ERR_SHAPE;
