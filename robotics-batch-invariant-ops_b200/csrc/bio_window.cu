@@ -406,20 +406,21 @@ struct WinBars {
   __device__ uint32_t empty(int s) const { return base + 96 + s * 8; }
   __device__ uint32_t s_full(int x) const { return base + 192 + x * 8; }
   __device__ uint32_t p_ready(int x) const { return base + 216 + x * 8; }
-  __device__ uint32_t pv_done(int x) const { return base + 240 + x * 8; }
+  __device__ uint32_t pv_done(int x) const { return base + 400 + x * 8; }
   __device__ uint32_t l_ready(int x) const { return base + 256 + x * 8; }
   __device__ uint32_t q_full() const { return base + 272; }
   __device__ uint32_t q_empty() const { return base + 280; }
   __device__ uint32_t o_done() const { return base + 288; }
   __device__ uint32_t o_free() const { return base + 296; }
-  __device__ uint32_t all_done() const { return base + 304; }
+  __device__ uint32_t all_done(int x) const { return base + 304 + x * 8; }
   __device__ uint32_t m_ready(int group, int quarter) const {
-    return base + 312 + group * 32 + quarter * 8;
+    return base + 320 + group * 32 + quarter * 8;
   }
 };
 
 // The ring of a job of n blocks carries K0 K1 K2 V0 K3 V1 ..., the order in which
-// the products need them: the place of V of block i.
+// the products need them: the places of K and V of block i.
+__device__ __forceinline__ int ring_of_k(int i) { return i < 3 ? i : 2 * i - 2; }
 __device__ __forceinline__ int ring_of_v(int i, int n) { return min(i + 3, n) + i; }
 
 template <typename T, int DP, bool PACKED>
@@ -445,8 +446,10 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
   if (threadIdx.x == 0) {
     uint64_t* b = reinterpret_cast<uint64_t*>(tail);
     // p_ready, l_ready and o_free: four warps arrive
-    for (int i = 0; i < 47; ++i)
+    for (int i = 0; i < 53; ++i) {
+      if (i == 48 || i == 49) continue;  // the TMEM address and the abort flag
       mbar_init(b + i, (i >= 27 && i < 30) || i == 32 || i == 33 || i == 37 ? 4 : 1);
+    }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -530,12 +533,8 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
           raise_status(p.status, BIO_DEV_TIMEOUT);
       }
     } else if (warp == 1) {
-      // ------------------------------------------------------------------- MMA
-      int slot = 0;                         // ring position of what comes next
-      uint32_t turn = 0;
-      int s_buf = 0, p_buf = 0;             // buffers of the next S and the next P
-      uint32_t p_turn = 0;
-      int pvs = 0, jobs_done = 0;           // PV products and jobs so far
+      // ------------------------------------------------------------- S products
+      int before = 0, jobs_done = 0;        // blocks and jobs so far
       bool ok = true;
       for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
         WinJob j;
@@ -543,79 +542,78 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         const int n = j.blocks;
         if (n == 0) continue;
         const int2 open = window_whole<BN>(w, j);
-        auto span = [&](int i) -> int2 {
-          return i >= open.x && i < open.y ? make_int2(0, BN) : window_span<BN>(j, i);
-        };
-        auto next = [&]() {
-          if (++slot == NS) {
-            slot = 0;
-            turn ^= 1u;
-          }
-        };
-        auto products_s = [&](int i) {
-          const int2 s = span(i);
-          if (ok) ok = wait(bar.full(slot), turn);
-          if (!ok) return;
-          tc_fence_after();
-          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
-          uint64_t qd = smem_desc_sw128(q32, 16, 1024);
-          uint64_t kd = smem_desc_sw128(ring32 + slot * L::kSlot + s.x * 128, 16, 1024);
-          const uint32_t to = tmem + s_buf * BN + s.x;
-          if (elect_leader()) {
-            // 16 columns are 32 bytes, 2 units of a descriptor; 64 columns a chunk
-            for (int c = 0; c < kc; ++c) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16(to, qd + 2 * k, kd + 2 * k, idesc, k > 0 ? 1u : c);
-              qd += 1024;
-              kd += BN * 8;
-            }
-            commit_to(bar.s_full(s_buf));
-            commit_to(bar.empty(slot));  // the keys are free once the products are done
-            if (i == n - 1) commit_to(bar.q_empty());
-          }
-          s_buf = s_buf == 2 ? 0 : s_buf + 1;
-          next();
-        };
         ok = wait(bar.q_full(), jobs_done);
-        products_s(0);
-        if (n > 1) products_s(1);
         for (int i = 0; ok && i < n; ++i) {
-          if (i + 2 < n) products_s(i + 2);
-          const int2 s = span(i);
-          // 16 keys are 2048 bytes of V and 8 columns of P
-          const int k0 = s.x / 16;
-          uint64_t vd = smem_desc_sw128(ring32 + slot * L::kSlot, BN * 128, 1024) + k0 * 128;
-          uint32_t pa = tmem + p_buf * BN + k0 * 8;
-          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
-          if (ok) ok = wait(bar.full(slot), turn);
-          // the rows of the job before have left O
-          if (ok && i == 0 && jobs_done > 0) ok = wait(bar.o_free(), jobs_done - 1);
-          if (ok) ok = wait(bar.p_ready(p_buf), p_turn);
+          const int g = before + i, x = g % 3, pos = 2 * before + ring_of_k(i), slot = pos % NS;
+          const int2 s = i >= open.x && i < open.y ? make_int2(0, BN) : window_span<BN>(j, i);
+          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
+          const uint64_t qd = smem_desc_sw128(q32, 16, 1024);
+          const uint64_t kd = smem_desc_sw128(ring32 + slot * L::kSlot + s.x * 128, 16, 1024);
+          const uint32_t to = tmem + x * BN + s.x;
+          ok = wait(bar.full(slot), pos / NS);
+          // the P before in this buffer has been used
+          if (ok && g >= 3) ok = wait(bar.pv_done(x), g / 3 - 1);
           if (!ok) break;
           tc_fence_after();
           if (elect_leader()) {
-            for (int k = k0; k < s.y / 16; k += 2) {  // 32 columns at a time
-              umma_f16_ts(tmem + L::kO, pa, vd, idesc, i > 0 || k > k0 ? 1u : 0u);
-              umma_f16_ts(tmem + L::kO, pa + 8, vd + 128, idesc, 1u);
-              pa += 16;
-              vd += 256;
-            }
-            commit_to(bar.pv_done(pvs & 1));
+            // 16 columns are 32 bytes, 2 units of a descriptor; 64 columns a chunk
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+              if (DP == 64 || (k >> 2) < kc)
+                umma_f16(to, qd + (k >> 2) * 1024 + (k & 3) * 2,
+                         kd + (k >> 2) * (BN * 8) + (k & 3) * 2, idesc, k > 0 ? 1u : 0u);
+            commit_to(bar.s_full(x));
+            commit_to(bar.empty(slot));  // the keys are free once the products are done
+            if (i == n - 1) commit_to(bar.q_empty());
+          }
+          __syncwarp();
+        }
+        before += n;
+        ++jobs_done;
+      }
+      if (elect_leader()) commit_to(bar.all_done(0));
+      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 38, 0))
+        raise_status(p.status, BIO_DEV_TIMEOUT);
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ PV products
+      int before = 0, jobs_done = 0;
+      bool ok = true;
+      for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+        WinJob j;
+        if (!window_job<BN, PACKED>(p, w, number, j)) continue;
+        const int n = j.blocks;
+        if (n == 0) continue;
+        const int2 open = window_whole<BN>(w, j);
+        for (int i = 0; ok && i < n; ++i) {
+          const int g = before + i, x = g % 3, pos = 2 * before + ring_of_v(i, n), slot = pos % NS;
+          const int2 s = i >= open.x && i < open.y ? make_int2(0, BN) : window_span<BN>(j, i);
+          // 16 keys are 2048 bytes of V and 8 columns of P
+          const uint64_t vd = smem_desc_sw128(ring32 + slot * L::kSlot, BN * 128, 1024);
+          const uint32_t pa = tmem + x * BN;
+          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
+          ok = wait(bar.full(slot), pos / NS);
+          // the rows of the job before have left O
+          if (ok && i == 0 && jobs_done > 0) ok = wait(bar.o_free(), jobs_done - 1);
+          if (ok) ok = wait(bar.p_ready(x), g / 3);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_leader()) {
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              if (k * 16 >= s.x && k * 16 < s.y)
+                umma_f16_ts(tmem + L::kO, pa + k * 8, vd + k * 128, idesc,
+                            i > 0 || k * 16 > s.x ? 1u : 0u);
+            commit_to(bar.pv_done(x));
             commit_to(bar.empty(slot));
             if (i == n - 1) commit_to(bar.o_done());
           }
-          ++pvs;
-          if (++p_buf == 3) {
-            p_buf = 0;
-            p_turn ^= 1u;
-          }
-          next();
+          __syncwarp();
         }
+        before += n;
         ++jobs_done;
       }
-      if (elect_leader()) commit_to(bar.all_done());
-      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 38, 0))
+      if (elect_leader()) commit_to(bar.all_done(1));
+      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 39, 0))
         raise_status(p.status, BIO_DEV_TIMEOUT);
     }
   } else {
@@ -700,23 +698,23 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
           top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
         }
         const float scaled = top == -INFINITY ? top : top * w.scale_log2;
-        // the reference as the block before left it
+        // The reference as the block before left it.  Taking it in every block, a
+        // job's first one too, is also what keeps a group from leaving the next one
+        // over a value that the other has not read yet.
+        if (g > 0) hold(take, taken++);
         if (i > 0) {
-          hold(take, taken++);
           m_before = m_of[(group ^ 1) * 128 + r];
         }
         const float was = m;  // the reference of this group's l
         m = scaled > m_before + 8.f ? scaled : m_before;
-        if (i + 1 < j.blocks) {
-          m_of[group * 128 + r] = m;
-          __syncwarp();
-          if (lane == 0) arrive(give);
-        }
+        m_of[group * 128 + r] = m;
+        __syncwarp();
+        if (lane == 0) arrive(give);
         l *= was == m ? 1.f : pow2(was - m);
         const bool moved = m != m_before;
         if (i > 0 && __any_sync(0xffffffffu, moved)) {
           // O holds the blocks before this one, by the old reference
-          hold(bar.pv_done((g - 1) & 1), (g - 1) >> 1);
+          hold(bar.pv_done((g - 1) % 3), (g - 1) / 3);
           tc_fence_after();
           const float alpha = moved ? pow2(m_before - m) : 1.f;
 #pragma unroll 1
