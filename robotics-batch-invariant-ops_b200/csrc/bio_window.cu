@@ -136,41 +136,38 @@ __global__ void __launch_bounds__(kWinWarps * 32) window_row_kernel(const Window
 // ---------------------------------------------------------------------------
 // tcgen05 kernel.
 //
-// A job is a tile of 128 query rows that share a KV head: `gh` query heads of
-// the group with `tok` = 128 / gh consecutive tokens each (row r: head r / tok,
-// token r % tok), so the keys that a tile visits are its window plus tok - 1, not
-// plus 127, and a key block is loaded once for all those heads.  Jobs are dealt
-// out round robin to one persistent CTA per SM:
-//   warp 0      TMA: Q, then K and V blocks of BN keys through one ring.
-//   warp 1      MMA: S = Q K^T into one of three buffers, O += P V, fp32 in TMEM;
-//               P (16 bits) lies over the S that it came from.
-//   warps 4-11  softmax: two groups of 128 threads, a thread per query row, take
-//               the blocks in turn.
-// S of block i + 2 is issued before PV of block i, so each group finds its next
-// scores ready while the other one and the tensor cores are at work, and nobody
-// waits for one chain.  The groups hand the rows' running reference m to each
-// other right after a block's maximum; each keeps its own sum l.  The ring, S and
-// O run on across jobs: a job's first blocks start while the last rows of the
-// one before are still being stored.
+// A job is NT tiles of 128 query rows that share a KV head.  A tile packs `gh`
+// query heads of the group with `tok` = 128 / gh consecutive tokens each (row r:
+// head r / tok, token r % tok), so the keys that a tile visits are its window
+// plus tok - 1, not plus 127, and a key block is loaded once for the whole
+// group.  Jobs are dealt out round robin to one persistent CTA per SM:
+//   warp 0      TMA: Q tiles, then K and V blocks of BN keys through one ring.
+//   warp 1      MMA: S_t = Q_t K^T, O_t += P_t V, fp32 in TMEM; P (16 bits) lies
+//               over the S that it came from.
+//   warps 4..   softmax: one thread per query row; the 128 rows of tile t belong
+//               to warps 4 + 4 t .. 7 + 4 t, which take over registers of the
+//               first four warps.
+// The ring, S and O run on across jobs: a job's first products start while the
+// last rows of the one before are still being stored.  With two tiles (D <= 128)
+// the tensor cores work on one tile while the other is in its softmax; with one
+// (D <= 256) S has two buffers, and S of block i is issued before P of block
+// i - 1 is waited for.
 //
-// What was measured on the way (32768 tokens, 32 heads on 8, d 128, window 1024):
-// two tiles with one S buffer each 842 us, bound by the chain softmax -> PV -> S of
-// a tile (4900 clocks a round, 3200 of them products: an M = 128, K = 16 product
-// takes about 100 clocks at N = 64 as at N = 128); two threads per row 838 us (the
-// two tiles' exponentials then run at the same time, and the special-function
-// unit is what both want); 64-key blocks with two buffers per tile 977 us (twice
-// the products).
+// What bounds it is the chain softmax -> PV -> S of a tile and the instructions of
+// the single warps along it, not the products (an M = 128, N = 128, K = 16 product
+// runs for 64 clocks): a look at a barrier costs 125 clocks and more even when
+// nobody has to wait, so barriers that are due together are looked at together
+// (one per lane), and a TMA box about 50, so blocks are loaded whole.
 //
-// Blocks are cut on the absolute grid of BN keys and trimmed to the 32-key
-// columns that some row of the tile sees: a window costs about window + tok + 32
-// columns per row, four sink tokens one 32-key column.  Masked scores weigh
+// Blocks are cut on the absolute grid of BN keys; products are trimmed, per tile,
+// to the 32-key columns that some row of the tile sees.  Masked scores weigh
 // exactly 0 and untrimmed columns add exactly 0, so a row's bits depend on its
 // own query, keys and position only.
 //
-// Scores, maxima and sums are fp32 in registers.  The reference m of the
-// exponentials moves only when a block's maximum exceeds it by more than 8
-// (log2), so O is rarely rescaled and P stays below 2^8; P is rounded to the
-// operand type, as the product needs, l sums it unrounded.
+// Scores, maxima and sums are fp32 in registers (128 scores a thread).  The
+// reference m of the exponentials moves only when a block's maximum exceeds it
+// by more than 8 (log2), so O is rarely rescaled and P stays below 2^8; P is
+// rounded to the operand type, as the product needs, l sums it unrounded.
 //
 // A hidden key in a visited block has weight 0, but 0 * Inf or 0 * NaN in V
 // would still reach the row: a row whose output is not finite is computed once
@@ -178,59 +175,92 @@ __global__ void __launch_bounds__(kWinWarps * 32) window_row_kernel(const Window
 // neighbouring packed sequence are zeroed in shared memory instead, so that
 // they cannot even change a row's bits.
 // ---------------------------------------------------------------------------
+// Division of 0 <= x < 2^31 by a fixed n: (mulhi(x, mul) + x) >> shift with
+// 2^(shift-1) < n <= 2^shift and mul = floor(2^32 (2^shift - n) / n) + 1.
+struct FixedDiv {
+  unsigned mul, shift, n;
+  __device__ __forceinline__ int quotient(int x) const {
+    return static_cast<int>((__umulhi(static_cast<unsigned>(x), mul) + static_cast<unsigned>(x)) >>
+                            shift);
+  }
+};
+
 struct WindowJobs {
   int gh, tok, hblocks;  // heads and tokens of a tile, tiles across a group
-  int qblocks;           // dense: blocks of tok tokens per sequence; packed: at most
+  int qblocks;           // dense: blocks of NT * tok tokens per sequence; packed: at most
   int jobs;
   int window, sinks;     // at most 2^30
   float scale_log2;      // > 0
   int negate;            // the scale was negative: scores change sign
   int vec_out;           // output rows take 16-byte stores
+  FixedDiv by_qblocks, by_tiles, by_hblocks;
 };
 
 template <int DP>
 struct WinSmem {
+  static constexpr int NT = DP == 256 ? 1 : 2;     // tiles of a job
   static constexpr int BN = DP == 256 ? 64 : 128;  // keys of a block
   static constexpr uint32_t kQ = 128 * DP * 2;
   static constexpr uint32_t kSlot = BN * DP * 2;   // K or V of a block
-  static constexpr uint32_t kSwap = 4 * 128 * 4;   // m of two groups, l of two jobs
-  static constexpr int kFit = (227 * 1024 - 1024 - 512 - static_cast<int>(kSwap + kQ)) /
+  static constexpr int kFit = (227 * 1024 - 1024 - 512 - NT * static_cast<int>(kQ)) /
                               static_cast<int>(kSlot);
-  static constexpr int kSlots = kFit > 12 ? 12 : kFit;
-  static constexpr uint32_t kBytes = 1024 + kQ + kSlots * kSlot + 512 + kSwap;
-  static constexpr int kThreads = 384;
-  static constexpr uint32_t kO = DP == 256 ? 256 : 384;  // TMEM columns of O; S buffers x at x * BN
-  static_assert(kSlots >= 4, "K of three blocks and a V");
+  static constexpr int kSlots = kFit > 8 ? 8 : kFit;
+  static constexpr uint32_t kBytes = 1024 + NT * kQ + kSlots * kSlot + 512;
+  static constexpr int kThreads = 128 + 128 * NT;
+  static_assert(kSlots >= 4, "K and V of two blocks");
+};
+
+// Keys of a tile: [lo, hi) for the windows of its rows, [0, sx) sinks before it.
+struct WinTile {
+  int pf, n;   // position of its first token, number of tokens
+  int lo, hi, sx;
+  int last;    // the tile's last block of the job, -1: it sees no key
 };
 
 struct WinJob {
   int b, hk, h0, nh;        // sequence of the batch, KV head, query heads
-  int q0, lq, lk;           // first query of the tile, lengths of its sequence
+  int q0, lq, lk;           // first query of the job, lengths of its sequence
   int qt, kt;               // tokens of the operands at which the sequence starts
-  int pf, n;                // position of the tile's first token, number of tokens
-  int lo, hi, sx;           // keys: [lo, hi) for the windows of its rows, [0, sx) sinks before
   int head, jump, blocks;   // block i of the job is block i < head ? i : i + jump of the keys
+  WinTile tile[2];
 };
 
-template <int BN>
+template <int NT, int BN>
 __device__ __forceinline__ void window_plan(const WindowJobs& w, WinJob& j) {
-  j.n = max(0, min(w.tok, j.lq - j.q0));
-  j.pf = j.q0 + j.lk - j.lq;
-  j.hi = j.n > 0 ? max(0, j.pf + j.n) : 0;
-  j.lo = j.hi > 0 ? max(0, j.pf - w.window + 1) : 0;
-  j.sx = min(w.sinks, j.lo);
-  j.head = (j.sx + BN - 1) / BN;
-  j.jump = max(0, j.lo / BN - j.head);
-  j.blocks = j.hi == 0 ? 0 : (j.hi - 1) / BN + 1 - j.jump;
+  int first = 0x7fffffff, last = -1;
+  j.head = 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    WinTile& x = j.tile[t];
+    const int q = j.q0 + t * w.tok;
+    x.n = max(0, min(w.tok, j.lq - q));
+    x.pf = q + j.lk - j.lq;
+    x.hi = x.n > 0 ? max(0, x.pf + x.n) : 0;
+    x.lo = x.hi > 0 ? max(0, x.pf - w.window + 1) : 0;
+    x.sx = min(w.sinks, x.lo);
+    if (x.hi > 0) {
+      j.head = max(j.head, (x.sx + BN - 1) / BN);
+      first = min(first, x.lo / BN);
+      last = max(last, (x.hi - 1) / BN);
+    }
+  }
+  j.jump = last < 0 ? 0 : max(0, first - j.head);
+  j.blocks = last < 0 ? 0 : last + 1 - j.jump;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int b = (j.tile[t].hi - 1) / BN;
+    j.tile[t].last = j.tile[t].hi == 0 ? -1 : b < j.head ? b : b - j.jump;
+  }
 }
 
-// Columns [x, y) of the job's block i that some row sees, on the 32-column grid.
+// Columns [x, y) of the job's block i that some row of the tile sees, on the
+// 32-column grid; empty: x == y.
 template <int BN>
-__device__ __forceinline__ int2 window_span(const WinJob& j, int i) {
+__device__ __forceinline__ int2 window_span(const WinJob& j, const WinTile& t, int i) {
   const int base = (i < j.head ? i : i + j.jump) * BN;
-  int x = max(j.lo - base, 0), y = min(j.hi - base, BN);
+  int x = max(t.lo - base, 0), y = min(t.hi - base, BN);
   if (x >= y) x = y = 0;
-  const int s = min(j.sx - base, BN);
+  const int s = min(t.sx - base, BN);
   if (s > 0) {
     x = 0;
     y = max(y, s);
@@ -238,34 +268,35 @@ __device__ __forceinline__ int2 window_span(const WinJob& j, int i) {
   return make_int2(x & ~31, (y + 31) & ~31);
 }
 
-// Blocks x <= i < y of the job: every row sees every key by its window, and all
-// 128 rows exist (or are padding of the tile's shape).
+// Blocks x <= i < y of the job: every row of the tile sees every key by its
+// window, and all 128 rows exist (or are padding of the tile's shape).
 template <int BN>
-__device__ __forceinline__ int2 window_whole(const WindowJobs& w, const WinJob& j) {
-  if (w.negate || j.n < w.tok || j.nh < w.gh || j.pf < 0) return make_int2(0, 0);
-  const int x = (max(0, j.pf + j.n - w.window) + BN - 1) / BN;  // first inside the last window
-  const int y = (j.pf + 1) / BN;                                // first past the first row
+__device__ __forceinline__ int2 window_whole(const WindowJobs& w, const WinJob& j,
+                                             const WinTile& t) {
+  if (w.negate || t.n < w.tok || j.nh < w.gh || t.pf < 0) return make_int2(0, 0);
+  const int x = (max(0, t.pf + t.n - w.window) + BN - 1) / BN;  // first inside the last window
+  const int y = (t.pf + 1) / BN;                                // first past the first row
   // only what lies behind the sinks' blocks keeps its distance
   return make_int2(max(x, j.head + j.jump) - j.jump, y - j.jump);
 }
 
 // Job number -> job.  All lanes of the warp call it; false: no such job.
-template <int BN, bool PACKED>
+template <int NT, int BN, bool PACKED>
 __device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJobs& w, int number,
                                            WinJob& j) {
   const int lane = threadIdx.x & 31;
-  const int tiles = static_cast<int>(p.heads / p.group) * w.hblocks;
+  const int tiles = static_cast<int>(w.by_tiles.n);
   int qb, hx;
   if constexpr (!PACKED) {
-    const int rest = number / w.qblocks;
+    const int rest = w.by_qblocks.quotient(number);
     qb = number - rest * w.qblocks;
-    j.b = rest / tiles;
+    j.b = w.by_tiles.quotient(rest);
     hx = rest - j.b * tiles;
     j.lq = static_cast<int>(p.lq);
     j.lk = static_cast<int>(p.lk);
     j.qt = j.kt = 0;
   } else {
-    qb = number / tiles;
+    qb = w.by_tiles.quotient(number);
     hx = number - qb * tiles;
     j.b = 0;
     if (win_off(p.cu_q, p.cu_is64, 0) != 0 || win_off(p.cu_k, p.cu_is64, 0) != 0) {
@@ -273,7 +304,7 @@ __device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJo
       return false;
     }
     // 32 sequences at a time: the one whose blocks hold block qb
-    const int span = w.tok;
+    const int span = NT * w.tok;
     bool found = false;
     for (int64_t s0 = 0; s0 < p.nseq && !found; s0 += 32) {
       const int64_t s = s0 + lane;
@@ -310,13 +341,21 @@ __device__ __forceinline__ bool window_job(const WindowParams& p, const WindowJo
     }
     if (!found) return false;
   }
-  j.q0 = qb * w.tok;
-  j.hk = hx / w.hblocks;
+  j.q0 = qb * NT * w.tok;
+  j.hk = w.by_hblocks.quotient(hx);
   const int before = (hx - j.hk * w.hblocks) * w.gh;
   j.h0 = j.hk * static_cast<int>(p.group) + before;
   j.nh = min(w.gh, static_cast<int>(p.group) - before);
-  window_plan<BN>(w, j);
+  window_plan<NT, BN>(w, j);
   return true;
+}
+
+__device__ __forceinline__ void prefetch_box(const CUtensorMap* map, int c0, int c1, int c2,
+                                             int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
 }
 
 __device__ __forceinline__ void arrive(uint32_t bar) {
@@ -375,11 +414,9 @@ __device__ __forceinline__ uint32_t pack_two<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Bits [x, y) of a 32-bit word, x and y anywhere.
-__device__ __forceinline__ uint32_t bits_between(int x, int y) {
-  const int a = min(max(x, 0), 32), b = min(max(y, 0), 32);
-  const uint64_t below_b = (1ull << b) - 1, below_a = (1ull << a) - 1;
-  return static_cast<uint32_t>(below_b & ~below_a);
+// The lowest x bits of a word, x anywhere.
+__device__ __forceinline__ uint32_t low_bits(int x) {
+  return __funnelshift_lc(0xffffffffu, 0u, max(x, 0));
 }
 
 // 32 lanes x 8 columns of TMEM, the load waited for.
@@ -403,25 +440,19 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8
 struct WinBars {
   uint32_t base;
   __device__ uint32_t full(int s) const { return base + s * 8; }
-  __device__ uint32_t empty(int s) const { return base + 96 + s * 8; }
-  __device__ uint32_t s_full(int x) const { return base + 192 + x * 8; }
-  __device__ uint32_t p_ready(int x) const { return base + 216 + x * 8; }
-  __device__ uint32_t pv_done(int x) const { return base + 400 + x * 8; }
-  __device__ uint32_t l_ready(int x) const { return base + 256 + x * 8; }
-  __device__ uint32_t q_full() const { return base + 272; }
-  __device__ uint32_t q_empty() const { return base + 280; }
-  __device__ uint32_t o_done() const { return base + 288; }
-  __device__ uint32_t o_free() const { return base + 296; }
-  __device__ uint32_t all_done(int x) const { return base + 304 + x * 8; }
-  __device__ uint32_t m_ready(int group, int quarter) const {
-    return base + 320 + group * 32 + quarter * 8;
-  }
+  __device__ uint32_t empty(int s) const { return base + 64 + s * 8; }
+  __device__ uint32_t q_full(int t) const { return base + 128 + t * 8; }
+  __device__ uint32_t q_empty(int t) const { return base + 144 + t * 8; }
+  __device__ uint32_t s_full(int x) const { return base + 160 + x * 8; }
+  __device__ uint32_t p_ready(int x) const { return base + 176 + x * 8; }
+  __device__ uint32_t o_done(int t) const { return base + 192 + t * 8; }
+  __device__ uint32_t pv_done() const { return base + 208; }
+  __device__ uint32_t all_done() const { return base + 216; }
 };
 
-// The ring of a job of n blocks carries K0 K1 K2 V0 K3 V1 ..., the order in which
-// the products need them: the places of K and V of block i.
-__device__ __forceinline__ int ring_of_k(int i) { return i < 3 ? i : 2 * i - 2; }
-__device__ __forceinline__ int ring_of_v(int i, int n) { return min(i + 3, n) + i; }
+// The ring of a job of n blocks carries K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1): the
+// place of V of block i.
+__device__ __forceinline__ int ring_of_v(int i, int n) { return i < n - 1 ? 2 * i + 2 : 2 * n - 1; }
 
 template <typename T, int DP, bool PACKED>
 __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
@@ -429,27 +460,23 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
                      const __grid_constant__ CUtensorMap tmV, const WindowParams p,
                      const WindowJobs w) {
   using L = WinSmem<DP>;
-  constexpr int BN = L::BN, NS = L::kSlots, NC = BN / 32;
+  constexpr int NT = L::NT, BN = L::BN, NS = L::kSlots, NC = BN / 32;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* ring = smem + L::kQ;
+  uint8_t* ring = smem + NT * L::kQ;
   uint8_t* tail = ring + NS * L::kSlot;
   const uint32_t q32 = smem_u32(smem), ring32 = smem_u32(ring);
   const WinBars bar{smem_u32(tail)};
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 384);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 388);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 256);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 260);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kc = (p.d + 63) / 64, vc = (p.dv + 63) / 64;
 
   if (threadIdx.x == 0) {
     uint64_t* b = reinterpret_cast<uint64_t*>(tail);
-    // p_ready, l_ready and o_free: four warps arrive
-    for (int i = 0; i < 53; ++i) {
-      if (i == 48 || i == 49) continue;  // the TMEM address and the abort flag
-      mbar_init(b + i, (i >= 27 && i < 30) || i == 32 || i == 33 || i == 37 ? 4 : 1);
-    }
+    for (int i = 0; i < 28; ++i) mbar_init(b + i, i == 22 || i == 23 ? 4 : 1);  // p_ready: 4 warps
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -464,7 +491,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   // All 512 columns of TMEM start at address 0, which as a constant costs the MMA
-  // warp no move to a uniform register.
+  // warp no move to a uniform register.  S at column 0 and 128, O_t at 256 + 128 t.
   constexpr uint32_t tmem = 0;
   if (*tmem_slot != tmem) {  // the same for every thread
     if (threadIdx.x == 0) raise_status(p.status, BIO_DEV_TIMEOUT);
@@ -474,31 +501,37 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
   auto wait = [&](uint32_t b, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, parked_wait(b, parity & 1u, abort_flag, p.status));
   };
+  // Three barriers at once, one per lane.
+  auto wait_all = [&](uint32_t a, uint32_t pa, uint32_t b, uint32_t pb, uint32_t c,
+                      uint32_t pc) -> bool {
+    const uint32_t at = lane == 0 ? a : lane == 1 ? b : c;
+    const uint32_t parity = lane == 0 ? pa : lane == 1 ? pb : pc;
+    return __all_sync(0xffffffffu, parked_wait(at, parity & 1u, abort_flag, p.status));
+  };
 
   // 384 threads start with 168 registers each, 128 of them go on with 56 and
   // 256 with 216: 62464 of the 64512
+  constexpr bool kShift = NT == 2;
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0) {
       // -------------------------------------------------------------- producer
-      int slot = 0, count = 0, q_used = 0;  // ring position; blocks, queries loaded so far
+      int slot = 0, count = 0;              // ring position, blocks loaded so far
       uint32_t turn = 0;
+      int q_used[2] = {0, 0};
       bool ok = true;
       for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
         WinJob j;
-        if (!window_job<BN, PACKED>(p, w, number, j)) continue;
-        auto load = [&](bool key, int i) {
-          const int2 s = window_span<BN>(j, i);
-          const int chunks = key ? kc : vc, boxes = chunks * ((s.y - s.x) / 32);
-          ok = wait(bar.empty(slot), turn ^ 1u);
-          if (!ok) return;
-          if (lane == 0) expect_bytes(bar.full(slot), boxes * 32 * 128);
-          __syncwarp();
-          if (lane < boxes) {
-            const int c = lane % chunks, r = s.x + lane / chunks * 32;
-            load_box(ring32 + slot * L::kSlot + c * (BN * 128) + r * 128, key ? &tmK : &tmV,
-                     bar.full(slot), c * 64, j.kt + (i < j.head ? i : i + j.jump) * BN + r, j.hk,
-                     j.b);
+        if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
+        const int n = j.blocks;
+        if (n == 0) continue;
+        auto load = [&](const CUtensorMap* map, int chunks, int i) {
+          if (lane == 0) {
+            const int row = j.kt + (i < j.head ? i : i + j.jump) * BN;
+            expect_bytes(bar.full(slot), chunks * (BN * 128));
+            for (int c = 0; c < chunks; ++c)
+              load_box(ring32 + slot * L::kSlot + c * (BN * 128), map, bar.full(slot), c * 64, row,
+                       j.hk, j.b);
           }
           ++count;
           if (++slot == NS) {
@@ -506,21 +539,40 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
             turn ^= 1u;
           }
         };
-        const int n = j.blocks;
-        if (n == 0) continue;
-        load(true, 0);
-        if (ok) ok = wait(bar.q_empty(), q_used ^ 1);
+        ok = wait(bar.empty(slot), turn ^ 1u);
         if (!ok) break;
-        if (lane == 0) {
-          expect_bytes(bar.q_full(), kc * w.gh * w.tok * 128);
-          for (int c = 0; c < kc; ++c)
-            load_box(q32 + c * 16384, &tmQ, bar.q_full(), c * 64, j.qt + j.q0, j.h0, j.b);
+        load(&tmK, kc, 0);
+        {  // the next job's queries on their way into L2, behind this job's first keys
+          WinJob then;
+          const int at = number + static_cast<int>(gridDim.x);
+          if (at < w.jobs && window_job<NT, BN, PACKED>(p, w, at, then) && lane < NT * kc) {
+            const int t = lane / kc;
+            prefetch_box(&tmQ, (lane - t * kc) * 64, then.qt + then.q0 + t * w.tok, then.h0,
+                         then.b);
+          }
         }
-        ++q_used;
-        if (n > 1) load(true, 1);
-        for (int i = 0; ok && i < n; ++i) {
-          if (i + 2 < n) load(true, i + 2);
-          if (ok) load(false, i);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (j.tile[t].last < 0 || !ok) continue;
+          ok = wait(bar.q_empty(t), q_used[t] ^ 1);
+          if (!ok) break;
+          if (lane == 0) {
+            expect_bytes(bar.q_full(t), kc * w.gh * w.tok * 128);
+            for (int c = 0; c < kc; ++c)
+              load_box(q32 + t * L::kQ + c * 16384, &tmQ, bar.q_full(t), c * 64,
+                       j.qt + j.q0 + t * w.tok, j.h0, j.b);
+          }
+          ++q_used[t];
+        }
+        for (int i = 1; ok && i <= n; ++i) {
+          const bool key = i < n;           // K of block i, then V of block i - 1
+          const int slot2 = slot + 1 == NS ? 0 : slot + 1;
+          const uint32_t turn2 = slot + 1 == NS ? turn ^ 1u : turn;
+          const uint32_t e1 = bar.empty(slot), e2 = key ? bar.empty(slot2) : e1;
+          ok = wait_all(e1, turn ^ 1u, e2, (key ? turn2 : turn) ^ 1u, e1, turn ^ 1u);
+          if (!ok) break;
+          if (key) load(&tmK, kc, i);
+          load(&tmV, vc, i - 1);
         }
       }
       // every copy has to land before the block's shared memory goes
@@ -528,33 +580,45 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         for (int i = max(0, count - NS); i < count; ++i)
           if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + i % NS, (i / NS) & 1))
             raise_status(p.status, BIO_DEV_TIMEOUT);
-        if (q_used > 0 &&
-            !mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 34, (q_used - 1) & 1))
-          raise_status(p.status, BIO_DEV_TIMEOUT);
+        for (int t = 0; t < NT; ++t)
+          if (q_used[t] > 0 &&
+              !mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 16 + t, (q_used[t] - 1) & 1))
+            raise_status(p.status, BIO_DEV_TIMEOUT);
       }
     } else if (warp == 1) {
-      // ------------------------------------------------------------- S products
-      int before = 0, jobs_done = 0;        // blocks and jobs so far
+      // ------------------------------------------------------------------- MMA
+      int slot = 0;                         // ring position of what comes next
+      uint32_t turn = 0;
+      int s_used[NT], p_used[NT], q_used[NT];  // S, PV and jobs of tile t
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s_used[t] = p_used[t] = q_used[t] = 0;
       bool ok = true;
+      auto next = [&]() {
+        if (++slot == NS) {
+          slot = 0;
+          turn ^= 1u;
+        }
+      };
       for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
         WinJob j;
-        if (!window_job<BN, PACKED>(p, w, number, j)) continue;
+        if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
         const int n = j.blocks;
         if (n == 0) continue;
-        const int2 open = window_whole<BN>(w, j);
-        ok = wait(bar.q_full(), jobs_done);
-        for (int i = 0; ok && i < n; ++i) {
-          const int g = before + i, x = g % 3, pos = 2 * before + ring_of_k(i), slot = pos % NS;
-          const int2 s = i >= open.x && i < open.y ? make_int2(0, BN) : window_span<BN>(j, i);
-          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
-          const uint64_t qd = smem_desc_sw128(q32, 16, 1024);
-          const uint64_t kd = smem_desc_sw128(ring32 + slot * L::kSlot + s.x * 128, 16, 1024);
-          const uint32_t to = tmem + x * BN + s.x;
-          ok = wait(bar.full(slot), pos / NS);
-          // the P before in this buffer has been used
-          if (ok && g >= 3) ok = wait(bar.pv_done(x), g / 3 - 1);
-          if (!ok) break;
+        int2 open[NT], held[NT];            // whole blocks; columns of the P that waits
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          open[t] = window_whole<BN>(w, j, j.tile[t]);
+          held[t] = make_int2(0, 0);
+        }
+        uint32_t begun = 0;                 // bit t: O_t holds something
+        // S of block i, whose keys are at ring position `at`
+        auto products_s = [&](int t, int i, int at, int2 s) {
           tc_fence_after();
+          const int x = NT == 2 ? t : s_used[t] & 1;
+          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
+          const uint64_t qd = smem_desc_sw128(q32 + t * L::kQ, 16, 1024);
+          const uint64_t kd = smem_desc_sw128(ring32 + at * L::kSlot + s.x * 128, 16, 1024);
+          const uint32_t to = tmem + x * 128 + s.x;
           if (elect_leader()) {
             // 16 columns are 32 bytes, 2 units of a descriptor; 64 columns a chunk
 #pragma unroll
@@ -563,160 +627,168 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
                 umma_f16(to, qd + (k >> 2) * 1024 + (k & 3) * 2,
                          kd + (k >> 2) * (BN * 8) + (k & 3) * 2, idesc, k > 0 ? 1u : 0u);
             commit_to(bar.s_full(x));
-            commit_to(bar.empty(slot));  // the keys are free once the products are done
-            if (i == n - 1) commit_to(bar.q_empty());
+            if (i == j.tile[t].last) commit_to(bar.q_empty(t));
           }
           __syncwarp();
-        }
-        before += n;
-        ++jobs_done;
-      }
-      if (elect_leader()) commit_to(bar.all_done(0));
-      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 38, 0))
-        raise_status(p.status, BIO_DEV_TIMEOUT);
-    } else if (warp == 2) {
-      // ------------------------------------------------------------ PV products
-      int before = 0, jobs_done = 0;
-      bool ok = true;
-      for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
-        WinJob j;
-        if (!window_job<BN, PACKED>(p, w, number, j)) continue;
-        const int n = j.blocks;
-        if (n == 0) continue;
-        const int2 open = window_whole<BN>(w, j);
-        for (int i = 0; ok && i < n; ++i) {
-          const int g = before + i, x = g % 3, pos = 2 * before + ring_of_v(i, n), slot = pos % NS;
-          const int2 s = i >= open.x && i < open.y ? make_int2(0, BN) : window_span<BN>(j, i);
-          // 16 keys are 2048 bytes of V and 8 columns of P
-          const uint64_t vd = smem_desc_sw128(ring32 + slot * L::kSlot, BN * 128, 1024);
-          const uint32_t pa = tmem + x * BN;
-          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
-          ok = wait(bar.full(slot), pos / NS);
-          // the rows of the job before have left O
-          if (ok && i == 0 && jobs_done > 0) ok = wait(bar.o_free(), jobs_done - 1);
-          if (ok) ok = wait(bar.p_ready(x), g / 3);
-          if (!ok) break;
+          ++s_used[t];
+          if (i == j.tile[t].last) ++q_used[t];
+        };
+        // PV of block i, whose values are at ring position `at`
+        auto products_pv = [&](int t, int i, int at) {
           tc_fence_after();
+          const int x = NT == 2 ? t : p_used[t] & 1;
+          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
+          // 16 keys are 2048 bytes of V and 8 columns of P
+          const uint64_t vd = smem_desc_sw128(ring32 + at * L::kSlot, BN * 128, 1024);
+          const uint32_t pa = tmem + x * 128, to = tmem + 256 + t * 128;
+          const bool on = (begun >> t) & 1u;
           if (elect_leader()) {
 #pragma unroll
             for (int k = 0; k < BN / 16; ++k)
-              if (k * 16 >= s.x && k * 16 < s.y)
-                umma_f16_ts(tmem + L::kO, pa + k * 8, vd + k * 128, idesc,
-                            i > 0 || k * 16 > s.x ? 1u : 0u);
-            commit_to(bar.pv_done(x));
-            commit_to(bar.empty(slot));
-            if (i == n - 1) commit_to(bar.o_done());
+              if (k * 16 >= held[t].x && k * 16 < held[t].y)
+                umma_f16_ts(to, pa + k * 8, vd + k * 128, idesc,
+                            on || k * 16 > held[t].x ? 1u : 0u);
+            if (NT == 1) commit_to(bar.pv_done());
+            if (i == j.tile[t].last) commit_to(bar.o_done(t));
+          }
+          __syncwarp();
+          begun |= 1u << t;
+          ++p_used[t];
+        };
+        auto p_bar = [&](int t) { return bar.p_ready(NT == 2 ? t : p_used[t] & 1); };
+        auto p_turn = [&](int t) {
+          return static_cast<uint32_t>(NT == 2 ? p_used[t] : p_used[t] >> 1);
+        };
+        for (int i = 0; ok && i <= n; ++i) {
+          const bool key = i < n, value = i > 0;
+          const int k_at = slot;
+          const uint32_t k_turn = turn;
+          if (key) next();
+          const int v_at = slot;
+          const uint32_t v_turn = turn;
+          if (value) next();
+          int2 now[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            now[t] = make_int2(0, 0);
+            if (key)
+              now[t] = i >= open[t].x && i < open[t].y ? make_int2(0, BN)
+                                                       : window_span<BN>(j, j.tile[t], i);
+          }
+          const bool p0 = held[0].x < held[0].y;
+          // the block's keys, the values of the one before, and with two tiles the
+          // first tile's P; queries with a job's first keys
+          const uint32_t b0 = key ? bar.full(k_at) : bar.full(v_at), t0 = key ? k_turn : v_turn;
+          uint32_t b2 = b0, t2 = t0;
+          if (NT == 2 && p0) {
+            b2 = p_bar(0);
+            t2 = p_turn(0);
+          }
+          ok = wait_all(b0, t0, value ? bar.full(v_at) : b0, value ? v_turn : t0, b2, t2);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            if (ok && i == 0 && j.tile[t].last >= 0) ok = wait(bar.q_full(t), q_used[t]);
+          if (!ok) break;
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const bool s_on = now[t].x < now[t].y, p_on = held[t].x < held[t].y;
+            if (NT == 1 && s_on) products_s(t, i, k_at, now[t]);
+            if (p_on && ok) {
+              if (NT == 1 || t > 0) ok = wait(p_bar(t), p_turn(t));
+              if (ok) products_pv(t, i - 1, v_at);
+            }
+            if (NT == 2 && s_on && ok) products_s(t, i, k_at, now[t]);
+            held[t] = now[t];
+          }
+          // what the products issued so far have read is free once they are done
+          if (ok && elect_leader()) {
+            if (key) commit_to(bar.empty(k_at));
+            if (value) commit_to(bar.empty(v_at));
           }
           __syncwarp();
         }
-        before += n;
-        ++jobs_done;
       }
-      if (elect_leader()) commit_to(bar.all_done(1));
-      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 39, 0))
+      if (elect_leader()) commit_to(bar.all_done());
+      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 27, 0))
         raise_status(p.status, BIO_DEV_TIMEOUT);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ----------------------------------------------------------------- softmax
-    const int group = (warp - 4) >> 2;
+    const int t = NT == 2 ? (warp - 4) >> 2 : 0;
     const int r = (warp & 3) * 32 + lane;  // row of the tile: the warp's quarter of the lanes
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // (quarter * 32) << 16
-    const uint32_t o_at = tmem + lanes + L::kO;
+    const uint32_t o_at = tmem + lanes + 256 + t * 128;
     const int rh = r / w.tok, rt = r - rh * w.tok;
     const uint64_t scale2 = pair_of(w.scale_log2, w.scale_log2);
-    float* m_of = reinterpret_cast<float*>(tail + 512);  // [group][row]
-    float* l_of = m_of + 256;                            // [job & 1][row]
-    // m goes from warp to warp: of a quarter of the rows, from group to group
-    const uint32_t give = bar.m_ready(group, warp & 3), take = bar.m_ready(group ^ 1, warp & 3);
-    uint32_t taken = 0;                        // times that this warp took m
-    int blocks_before = 0, jobs_done = 0, sums_left = 0;
-    // After a wait that ran out the rest goes through without waiting for anything.
+    int base = 0, s_used = 0, jobs_done = 0;  // ring position of the job's first K
     bool ok = true;
-    auto hold = [&](uint32_t b, uint32_t parity) {
-      if (ok) ok = wait(b, parity);
-    };
-    for (int number = blockIdx.x; number < w.jobs; number += gridDim.x) {
+    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
       WinJob j;
-      if (!window_job<BN, PACKED>(p, w, number, j)) continue;
-      const bool valid = rh < j.nh && rt < j.n;
-      const int at = j.pf + rt;                     // position of the row
-      const int2 open = window_whole<BN>(w, j);
-      float m = -INFINITY, l = 0.f, m_before = -INFINITY;
-      // global block number g = blocks_before + i: group g & 1, buffer g % 3
-      for (int i = (blocks_before & 1) ^ group; i < j.blocks; i += 2) {
-        const int g = blocks_before + i, x = g % 3;
+      if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
+      WinTile tile = j.tile[0];
+      if (NT == 2 && t == 1) tile = j.tile[NT - 1];
+      const bool valid = rh < j.nh && rt < tile.n;
+      const int at = tile.pf + rt;                     // position of the row
+      const int2 open = window_whole<BN>(w, j, tile);
+      float m = -INFINITY, l = 0.f;
+      bool first = true;
+      for (int i = 0; i <= tile.last; ++i) {
         const bool whole = i >= open.x && i < open.y;
         int2 s = make_int2(0, BN);
-        if (!whole) s = window_span<BN>(j, i);
-        hold(bar.s_full(x), g / 3);
+        if (!whole) s = window_span<BN>(j, tile, i);
+        if (s.x >= s.y) continue;
+        const int x = NT == 2 ? t : s_used & 1;
+        ok = wait(bar.s_full(x), NT == 2 ? s_used : s_used >> 1);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t s_at = tmem + lanes + x * BN;
+        const uint32_t s_at = tmem + lanes + x * 128;
         uint32_t f[NC][32];
-        float top;
-        if (whole) {
 #pragma unroll
-          for (int c = 0; c < NC; ++c) tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
+        for (int c = 0; c < NC; ++c) tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) tmem_ld_wait_tied(f[c]);
-        } else {
+        for (int c = 0; c < NC; ++c) tmem_ld_wait_tied(f[c]);
+        if (!whole) {
+          const uint32_t flip = w.negate ? 0x80000000u : 0u;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            if (c * 32 < s.x || c * 32 >= s.y) {  // trimmed: as if hidden
-#pragma unroll
-              for (int e = 0; e < 32; ++e) f[c][e] = 0xff800000u;
-              continue;
-            }
-            tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
-            tmem_ld_wait_tied(f[c]);
-            if (w.negate) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) f[c][e] ^= 0x80000000u;
-            }
+            // keys a + e: inside the window, or one of the sinks; trimmed columns hold
+            // what was there before
             const int a = (i < j.head ? i : i + j.jump) * BN + c * 32;
-            const uint32_t sees = valid ? bits_between(at - w.window + 1 - a, at + 1 - a) |
-                                              bits_between(0, min(w.sinks, at + 1) - a)
-                                        : 0u;
-            if (!__all_sync(0xffffffffu, sees == 0xffffffffu)) {
+            uint32_t sees = (low_bits(at + 1 - a) & ~low_bits(at - w.window + 1 - a)) |
+                            low_bits(min(w.sinks, at + 1) - a);
+            if (!valid || c * 32 < s.x || c * 32 >= s.y) sees = 0u;
+            if (flip != 0u || !__all_sync(0xffffffffu, sees == 0xffffffffu)) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (!(sees & (1u << e))) f[c][e] = 0xff800000u;  // -inf
+                f[c][e] = sees & (1u << e) ? f[c][e] ^ flip : 0xff800000u;  // -inf
             }
           }
         }
-        {
-          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+        float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              a0 = max3(a0, __uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1]));
-              a1 = max3(a1, __uint_as_float(f[c][e + 2]), __uint_as_float(f[c][e + 3]));
-              a2 = max3(a2, __uint_as_float(f[c][e + 4]), __uint_as_float(f[c][e + 5]));
-              a3 = max3(a3, __uint_as_float(f[c][e + 6]), __uint_as_float(f[c][e + 7]));
-            }
-          top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
-        }
+          for (int e = 0; e < 32; e += 8) {
+            a0 = max3(a0, __uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1]));
+            a1 = max3(a1, __uint_as_float(f[c][e + 2]), __uint_as_float(f[c][e + 3]));
+            a2 = max3(a2, __uint_as_float(f[c][e + 4]), __uint_as_float(f[c][e + 5]));
+            a3 = max3(a3, __uint_as_float(f[c][e + 6]), __uint_as_float(f[c][e + 7]));
+          }
+        const float top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
         const float scaled = top == -INFINITY ? top : top * w.scale_log2;
-        // The reference as the block before left it.  Taking it in every block, a
-        // job's first one too, is also what keeps a group from leaving the next one
-        // over a value that the other has not read yet.
-        if (g > 0) hold(take, taken++);
-        if (i > 0) {
-          m_before = m_of[(group ^ 1) * 128 + r];
-        }
-        const float was = m;  // the reference of this group's l
-        m = scaled > m_before + 8.f ? scaled : m_before;
-        m_of[group * 128 + r] = m;
-        __syncwarp();
-        if (lane == 0) arrive(give);
-        l *= was == m ? 1.f : pow2(was - m);
-        const bool moved = m != m_before;
-        if (i > 0 && __any_sync(0xffffffffu, moved)) {
-          // O holds the blocks before this one, by the old reference
-          hold(bar.pv_done((g - 1) % 3), (g - 1) / 3);
-          tc_fence_after();
-          const float alpha = moved ? pow2(m_before - m) : 1.f;
+        const bool move = scaled > m + 8.f;
+        const float alpha = move ? pow2(m - scaled) : 1.f;
+        if (move) m = scaled;
+        l *= alpha;
+        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // S of this block was issued after the PV before it (two tiles), or that
+          // one has to be waited for (one tile)
+          if (NT == 1) {
+            ok = wait(bar.pv_done(), s_used - 1);
+            if (!ok) break;
+            tc_fence_after();
+          }
 #pragma unroll 1
           for (int c = 0; c < vc * 8; ++c) {  // 8 columns at a time: few registers
             uint32_t v[8];
@@ -726,6 +798,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
             tmem_st_x8(o_at + c * 8, v);
           }
         }
+        first = false;
         const float ref = m == -INFINITY ? 0.f : m;
         const uint64_t ref2 = pair_of(-ref, -ref);
         uint64_t sum2 = 0, sum3 = 0;
@@ -754,14 +827,14 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         split_pair(add_pair(sum2, sum3), s0, s1);
         l += s0 + s1;
         if (PACKED) {
-          const int first = (i < j.head ? i : i + j.jump) * BN;
-          if (first + s.y > j.lk) {
+          const int from = (i < j.head ? i : i + j.jump) * BN;
+          if (from + s.y > j.lk) {
             // the block's last columns may be another sequence's tokens
-            // (the ring took two places for each of the blocks before)
-            const int pos = 2 * blocks_before + ring_of_v(i, j.blocks);
-            hold(bar.full(pos % NS), pos / NS);
+            const int pos = base + ring_of_v(i, j.blocks);
+            ok = wait(bar.full(pos % NS), pos / NS);
+            if (!ok) break;
             uint8_t* v = ring + pos % NS * L::kSlot;
-            for (int row = max(0, j.lk - first); row < s.y; ++row)
+            for (int row = max(0, j.lk - from); row < s.y; ++row)
               for (int c = r; c < vc * 8; c += 128)
                 *reinterpret_cast<uint4*>(v + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
                     make_uint4(0, 0, 0, 0);
@@ -772,89 +845,77 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive(bar.p_ready(x));
+        ++s_used;
       }
-      // The group of the last block stores the rows; the other one leaves its sum.
-      const bool store = ((blocks_before + j.blocks - 1) & 1) == group;
-      blocks_before += j.blocks;
-      const int left = sums_left & 1, left_turn = sums_left >> 1;
-      if (j.blocks > 1) ++sums_left;
-      if (j.blocks > 0) ++jobs_done;
-      if (!store) {
-        if (j.blocks > 1) {
-          l_of[left * 128 + r] = l;
-          __syncwarp();
-          if (lane == 0) arrive(bar.l_ready(left));
-        }
-        continue;
-      }
+      base += 2 * j.blocks;
+      if (!ok) break;
       // ------------------------------------------------------------- the output
-      if (j.blocks > 1) {
-        hold(bar.l_ready(left), left_turn);
-        // the other group's sum goes by the reference of the block before the last
-        const float theirs = l_of[left * 128 + r];
-        l += m_before == m ? theirs : theirs * pow2(m_before - m);
-      }
-      const int tok = j.qt + j.q0 + rt;
+      const int tok = j.qt + j.q0 + t * w.tok + rt;
       T* out = valid ? static_cast<T*>(p.o) + j.b * p.o_sb + (j.h0 + rh) * p.o_sh + tok * p.o_st
                      : nullptr;
-      if (j.blocks > 0) {
-        hold(bar.o_done(), jobs_done - 1);
+      if (tile.last >= 0) {
+        ok = wait(bar.o_done(t), jobs_done);
+        if (!ok) break;
+        ++jobs_done;
         tc_fence_after();
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      float odd = 0.f;  // becomes NaN with the first output that is not finite
+      const uint64_t inv2 = pair_of(inv, inv);
+      uint64_t odd2 = 0;  // becomes NaN with the first output that is not finite
 #pragma unroll 1
       for (int c = 0; c < vc * 2; ++c) {
         uint32_t v[32];
-        if (j.blocks > 0) {
+        if (tile.last >= 0) {
           tmem_ld_32x32b_x32(o_at + c * 32, v);
           tmem_ld_wait_tied(v);
-          if (c == vc * 2 - 1) {  // O is free for the next job
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive(bar.o_free());
-          }
         }
-        if (l == 0.f || j.blocks == 0) {
+        if (l == 0.f || tile.last < 0) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0;
         }
         if (!valid) continue;
+        uint32_t y[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float y = __uint_as_float(v[e]) * inv;
-          odd = fmaf(y, 0.f, odd);
-          v[e] = __float_as_uint(y);
+        for (int e = 0; e < 16; ++e) {
+          const uint64_t o2 = fma_pair(
+              pair_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), inv2, 0);
+          odd2 = fma_pair(o2, 0, odd2);
+          float lo, hi;
+          split_pair(o2, lo, hi);
+          y[e] = pack_two<T>(lo, hi);
         }
         if (w.vec_out) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            if (c * 32 + e < p.dv)
-              *reinterpret_cast<uint4*>(out + c * 32 + e) = make_uint4(
-                  pack_two<T>(__uint_as_float(v[e]), __uint_as_float(v[e + 1])),
-                  pack_two<T>(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])),
-                  pack_two<T>(__uint_as_float(v[e + 4]), __uint_as_float(v[e + 5])),
-                  pack_two<T>(__uint_as_float(v[e + 6]), __uint_as_float(v[e + 7])));
+          for (int e = 0; e < 16; e += 4)
+            if (c * 32 + 2 * e < p.dv)
+              *reinterpret_cast<uint4*>(out + c * 32 + 2 * e) =
+                  make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (c * 32 + e < p.dv) out[c * 32 + e] = from_f32<T>(__uint_as_float(v[e]));
+            if (c * 32 + e < p.dv)
+              reinterpret_cast<uint16_t*>(out)[c * 32 + e] =
+                  static_cast<uint16_t>(y[e >> 1] >> (16 * (e & 1)));
         }
       }
+      tc_fence_before();  // the next job's PV overwrites O after this row's next P
+      float odd, odd_hi;
+      split_pair(odd2, odd, odd_hi);
+      odd += odd_hi;
       __syncwarp();
       unsigned again = __ballot_sync(0xffffffffu, valid && !(odd == 0.f));
       while (again != 0) {
-        const int x = __ffs(again) - 1;
+        const int y = __ffs(again) - 1;
         again &= again - 1;
-        const int xh = j.h0 + __shfl_sync(0xffffffffu, rh, x);
-        const int xt = __shfl_sync(0xffffffffu, rt, x);
-        const int64_t xtok = j.qt + j.q0 + xt;
+        const int xh = j.h0 + __shfl_sync(0xffffffffu, rh, y);
+        const int xt = __shfl_sync(0xffffffffu, rt, y);
+        const int64_t xtok = j.qt + j.q0 + t * w.tok + xt;
         window_row<T>(
             static_cast<const T*>(p.q) + j.b * p.q_sb + xh * p.q_sh + xtok * p.q_st,
             static_cast<const T*>(p.k) + j.b * p.k_sb + j.hk * p.k_sh + j.kt * p.k_st,
             static_cast<const T*>(p.v) + j.b * p.v_sb + j.hk * p.v_sh + j.kt * p.v_st,
             static_cast<T*>(p.o) + j.b * p.o_sb + xh * p.o_sh + xtok * p.o_st, p.k_st, p.v_st, p.d,
-            p.dv, p.scale, p.window, p.sinks, j.pf + xt);
+            p.dv, p.scale, p.window, p.sinks, tile.pf + xt);
       }
     }
   }
@@ -882,6 +943,15 @@ int launch_rows(const bio::WindowParams& p, bool packed, cudaStream_t s) {
   return bio_host::launch_status(cudaGetLastError());
 }
 
+bio::FixedDiv fixed_div(int64_t n) {
+  bio::FixedDiv d;
+  d.n = static_cast<unsigned>(n);
+  d.shift = 0;
+  while ((1ull << d.shift) < static_cast<uint64_t>(n)) ++d.shift;
+  d.mul = static_cast<unsigned>(((1ull << 32) * ((1ull << d.shift) - d.n)) / d.n + 1);
+  return d;
+}
+
 template <typename T, int DP, bool PACKED>
 int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s) {
   constexpr bool packed = PACKED;
@@ -900,12 +970,15 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
   w.hblocks = static_cast<int>((group + 15) / 16);  // up to 16 heads of a group in a tile
   w.gh = static_cast<int>((group + w.hblocks - 1) / w.hblocks);
   w.tok = 128 / w.gh;
-  const int64_t span = w.tok, tiles = a->kv_heads * w.hblocks;
+  const int64_t span = L::NT * w.tok, tiles = a->kv_heads * w.hblocks;
   const int64_t qblocks = (p.lq + span - 1) / span + (packed ? p.nseq : 0);
   const int64_t jobs = qblocks * tiles * (packed ? 1 : p.batch);
-  if (qblocks > kMaxGrid || jobs > kMaxGrid) return BIO_ERR_SHAPE;
+  if (qblocks > kMaxGrid || jobs > (1 << 30)) return BIO_ERR_SHAPE;
   w.qblocks = static_cast<int>(qblocks);
   w.jobs = static_cast<int>(jobs);
+  w.by_qblocks = fixed_div(qblocks);
+  w.by_tiles = fixed_div(tiles);
+  w.by_hblocks = fixed_div(w.hblocks);
   w.window = static_cast<int>(std::min<int64_t>(p.window, 1 << 30));
   w.sinks = static_cast<int>(std::min<int64_t>(p.sinks, 1 << 30));
   w.negate = p.scale < 0.f;
@@ -921,9 +994,9 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
   if (!bio_host::map_of<T>(&q, p.q, p.d, p.lq, p.heads, batch, p.q_st, p.q_sh, p.q_sb, w.tok,
                            w.gh) ||
       !bio_host::map_of<T>(&k, none ? p.q : p.k, p.d, none ? 1 : p.lk, a->kv_heads, batch, p.k_st,
-                           p.k_sh, p.k_sb, 32) ||
+                           p.k_sh, p.k_sb, L::BN) ||
       !bio_host::map_of<T>(&v, none ? p.q : p.v, p.dv, none ? 1 : p.lk, a->kv_heads, batch, p.v_st,
-                           p.v_sh, p.v_sb, 32))
+                           p.v_sh, p.v_sb, L::BN))
     return BIO_ERR_ALIGN;
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(jobs, sms));
   bio::window_tc_kernel<T, DP, PACKED><<<grid, L::kThreads, L::kBytes, s>>>(q, k, v, p, w);

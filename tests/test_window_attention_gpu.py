@@ -138,6 +138,30 @@ def test_a_row_does_not_depend_on_the_batch(d, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,hk,lq,lk,d,window,sinks", [
+    (400, 2, 2, 3, 3, 64, 2, 0),         # one block each
+    (260, 4, 2, 20, 150, 128, 130, 2),   # two
+    (150, 8, 2, 70, 400, 64, 300, 40),   # three and four
+    (40, 4, 1, 500, 500, 128, 200, 4),
+    (160, 4, 2, 90, 200, 256, 100, 3),
+    (3, 5, 1, 2500, 2500, 96, 700, 9),
+])
+def test_many_more_tiles_than_sms(b, h, hk, lq, lk, d, window, sinks, dtype):
+    """Blocks that work through several tiles in a row: every sample has the bits
+    that it has alone, and some are checked against the oracle."""
+    q, k, v = make(b, h, hk, lq, lk, d, dtype=dtype, seed=b)
+    full = bio.sliding_window_attention_batch_invariant(q, k, v, window, sinks)
+    for i in sorted({0, 1, b // 2, b - 1}):
+        alone = bio.sliding_window_attention_batch_invariant(
+            q[i:i + 1], k[i:i + 1], v[i:i + 1], window, sinks)
+        assert torch.equal(alone, full[i:i + 1])
+    some = slice(b // 2, b // 2 + 1)
+    rows = slice(max(0, lq - 300), lq)
+    check(full[some][:, :, rows], q[some][:, :, rows], k[some], v[some], window, sinks)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_leading_dims_strides_and_odd_offsets(dtype):
     q, k, v = make(6, 4, 2, 100, 100, 64, dtype=dtype)
     out = bio.sliding_window_attention_batch_invariant(q, k, v, 40, 4)
