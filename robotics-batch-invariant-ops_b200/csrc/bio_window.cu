@@ -499,14 +499,14 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     return;
   }
   auto wait = [&](uint32_t b, uint32_t parity) -> bool {
-    return __all_sync(0xffffffffu, parked_wait(b, parity & 1u, abort_flag, p.status));
+    return __all_sync(0xffffffffu, spin_wait(b, parity & 1u, abort_flag, p.status));
   };
   // Three barriers at once, one per lane.
   auto wait_all = [&](uint32_t a, uint32_t pa, uint32_t b, uint32_t pb, uint32_t c,
                       uint32_t pc) -> bool {
     const uint32_t at = lane == 0 ? a : lane == 1 ? b : c;
     const uint32_t parity = lane == 0 ? pa : lane == 1 ? pb : pc;
-    return __all_sync(0xffffffffu, parked_wait(at, parity & 1u, abort_flag, p.status));
+    return __all_sync(0xffffffffu, spin_wait(at, parity & 1u, abort_flag, p.status));
   };
 
   // 384 threads start with 168 registers each, 128 of them go on with 56 and
@@ -884,7 +884,16 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
           split_pair(o2, lo, hi);
           y[e] = pack_two<T>(lo, hi);
         }
-        if (w.vec_out) {
+        if (w.vec_out == 2) {  // whole 32-byte sectors
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            if (c * 32 + 2 * e < p.dv)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                               out + c * 32 + 2 * e),
+                           "r"(y[e]), "r"(y[e + 1]), "r"(y[e + 2]), "r"(y[e + 3]), "r"(y[e + 4]),
+                           "r"(y[e + 5]), "r"(y[e + 6]), "r"(y[e + 7])
+                           : "memory");
+        } else if (w.vec_out == 1) {
 #pragma unroll
           for (int e = 0; e < 16; e += 4)
             if (c * 32 + 2 * e < p.dv)
@@ -985,8 +994,9 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
   // a scale of 0 weighs every visible key alike; hidden ones stay at -inf
   const float scale = (w.negate ? -p.scale : p.scale) * 1.4426950408889634f;
   w.scale_log2 = scale == 0.f ? 1.17549435e-38f : scale;
-  w.vec_out = reinterpret_cast<uintptr_t>(p.o) % 16 == 0 &&
-              (p.o_sb | p.o_sh | p.o_st | p.dv) % 8 == 0;
+  const uint64_t out_bits = reinterpret_cast<uint64_t>(p.o) |
+                            2 * static_cast<uint64_t>(p.o_sb | p.o_sh | p.o_st | p.dv);
+  w.vec_out = out_bits % 32 == 0 ? 2 : out_bits % 16 == 0 ? 1 : 0;
   CUtensorMap q, k, v;
   const int64_t batch = packed ? 1 : p.batch;
   // without keys nothing is read through K and V: any operand will do for their maps
