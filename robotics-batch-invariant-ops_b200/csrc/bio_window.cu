@@ -6,7 +6,7 @@
 // A row that sees no key (p < 0) gives zeros.
 //
 // 16-bit operands run on tcgen05 (window_tc_kernel), fp32 on the CUDA cores
-// (window_row_kernel).
+// (window_f32_kernel).
 //
 // Not in the reference, whose SDPA (batch_invariant_ops.py:1148-1213) would
 // need the mask as a tensor and visits every key.
@@ -39,7 +39,6 @@ __device__ __forceinline__ int64_t win_off(const void* p, int is64, int64_t i) {
               : static_cast<int64_t>(static_cast<const int*>(p)[i]);
 }
 
-constexpr int kWinWarps = 8;
 constexpr int kWinDims = 256;
 
 // One warp computes one row.  It walks the row's visible keys in order, 32 at a
@@ -98,39 +97,6 @@ __device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb,
     const int c = lane + 32 * e;
     if (c < dv) out[c] = from_f32<T>(l == 0.f ? 0.f : o[e] / l);
   }
-}
-
-template <typename T, bool PACKED>
-__global__ void __launch_bounds__(kWinWarps * 32) window_row_kernel(const WindowParams p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWinWarps + warp;
-  if (row >= (PACKED ? 1 : p.batch) * p.heads * p.lq) return;
-  const int64_t t = row % p.lq, bh = row / p.lq, h = bh % p.heads, b = bh / p.heads;
-  int64_t pos = t + p.lk - p.lq, k0 = 0;  // position of the query, first key token
-  if constexpr (PACKED) {
-    int64_t lo = 0, hi = p.nseq;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (win_off(p.cu_q, p.cu_is64, mid) <= t) lo = mid; else hi = mid;
-    }
-    if (p.nseq < 1) return;
-    const int64_t q0 = win_off(p.cu_q, p.cu_is64, lo), q1 = win_off(p.cu_q, p.cu_is64, lo + 1);
-    k0 = win_off(p.cu_k, p.cu_is64, lo);
-    const int64_t k1 = win_off(p.cu_k, p.cu_is64, lo + 1);
-    if (t >= win_off(p.cu_q, p.cu_is64, p.nseq)) return;  // outside every sequence
-    if (q0 > t || q1 <= t || q1 > p.lq || k0 < 0 || k1 < k0 || k1 > p.lk ||
-        win_off(p.cu_q, p.cu_is64, 0) != 0 || win_off(p.cu_k, p.cu_is64, 0) != 0) {
-      if (lane == 0) raise_status(p.status, BIO_DEV_INDEX);
-      return;
-    }
-    pos = (t - q0) + (k1 - k0) - (q1 - q0);
-  }
-  const int64_t bq = PACKED ? 0 : b;
-  window_row<T>(static_cast<const T*>(p.q) + bq * p.q_sb + h * p.q_sh + t * p.q_st,
-                static_cast<const T*>(p.k) + bq * p.k_sb + h / p.group * p.k_sh + k0 * p.k_st,
-                static_cast<const T*>(p.v) + bq * p.v_sb + h / p.group * p.v_sh + k0 * p.v_st,
-                static_cast<T*>(p.o) + bq * p.o_sb + h * p.o_sh + t * p.o_st, p.k_st, p.v_st, p.d,
-                p.dv, p.scale, p.window, p.sinks, pos);
 }
 
 // ---------------------------------------------------------------------------
@@ -934,23 +900,224 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
+// ---------------------------------------------------------------------------
+// fp32 kernel: one CTA per tile of 64 query rows (packed like the tiles above,
+// tok = 64 / gh tokens of gh heads), key blocks of BN keys in shared memory.
+// Thread (ty, tx) computes scores of rows 4 ty .. 4 ty + 3 and keys tx + 16 c,
+// the 16 threads of a row share its maximum and sum by shuffles, the weights go
+// through shared memory, and it accumulates 4 rows x 4 columns per 64 columns of
+// O.  V of a block and K of the next one are copied (cp.async) while the
+// products before them run.  FFMA bounds it: 64 products per 8 shared loads of
+// 16 bytes in S, 128 per 12 in PV.  Rows that come out not finite are computed
+// once more from their visible keys alone, as above.
+// ---------------------------------------------------------------------------
+template <int DP>
+struct WinF32 {
+  static constexpr int BN = DP == 256 ? 32 : 64;
+  static constexpr int kPitch = DP + 4;  // floats: 16-byte loads of 8 rows hit all banks
+  static constexpr int kP = BN + 4;
+  static constexpr int kBytes = 4 * (64 * kPitch + 2 * BN * kPitch + 64 * kP) + 64;
+};
+
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes, bool on) {
+  // bytes 16 or 4; nothing but zeros arrives for `on` false
+  if (bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(on ? 16 : 0)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+                 "r"(on ? 4 : 0)
+                 : "memory");
+}
+
+// rows x cols floats of `src` (row stride in elements) into dst [rows][pitch]; rows
+// from `have` on and columns from cols to DP are zeros.
+template <int DP>
+__device__ __forceinline__ void copy_tile(float* dst, int pitch, int rows, const float* src,
+                                          int64_t stride, int have, int cols, bool vec) {
+  const uint32_t d = smem_u32(dst);
+  if (vec) {
+    for (int x = threadIdx.x; x < rows * (DP / 4); x += 256) {
+      const int r = x / (DP / 4), c = x % (DP / 4) * 4;
+      const bool on = r < have && c < cols;
+      copy_async(d + (r * pitch + c) * 4, on ? src + r * stride + c : src, 16, on);
+    }
+  } else {
+    for (int x = threadIdx.x; x < rows * DP; x += 256) {
+      const int r = x / DP, c = x % DP;
+      const bool on = r < have && c < cols;
+      copy_async(d + (r * pitch + c) * 4, on ? src + r * stride + c : src, 4, on);
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+template <int DP, bool PACKED>
+__global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, const WindowJobs w,
+                                                         int vec) {
+  using L = WinF32<DP>;
+  constexpr int BN = L::BN, NC = BN / 16, NO = DP / 64;
+  extern __shared__ float4 smem_f4[];
+  float* sq = reinterpret_cast<float*>(smem_f4);
+  float* sk = sq + 64 * L::kPitch;
+  float* sv = sk + BN * L::kPitch;
+  float* sp = sv + BN * L::kPitch;
+  uint32_t* redo = reinterpret_cast<uint32_t*>(sp + 64 * L::kP);  // [2] rows to compute again
+  WinJob j;
+  if (!window_job<1, BN, PACKED>(p, w, blockIdx.x, j)) return;  // the same for every warp
+  const WinTile tile = j.tile[0];
+  const float* q = static_cast<const float*>(p.q) + j.b * p.q_sb + j.h0 * p.q_sh +
+                   static_cast<int64_t>(j.qt + j.q0) * p.q_st;
+  const float* k = static_cast<const float*>(p.k) + j.b * p.k_sb + j.hk * p.k_sh + j.kt * p.k_st;
+  const float* v = static_cast<const float*>(p.v) + j.b * p.v_sb + j.hk * p.v_sh + j.kt * p.v_st;
+  float* o = static_cast<float*>(p.o) + j.b * p.o_sb + j.h0 * p.o_sh +
+             static_cast<int64_t>(j.qt + j.q0) * p.o_st;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  if (threadIdx.x < 2) redo[threadIdx.x] = 0;
+
+  // queries: row r is head r / tok, token r % tok
+  for (int x = threadIdx.x; x < 64 * DP; x += 256) {
+    const int r = x / DP, c = x % DP, h = r / w.tok, t = r - h * w.tok;
+    sq[r * L::kPitch + c] =
+        h < j.nh && t < tile.n && c < p.d ? q[h * p.q_sh + t * p.q_st + c] : 0.f;
+  }
+  auto first_of = [&](int i) { return (i < j.head ? i : i + j.jump) * BN; };
+  auto load = [&](float* dst, const float* src, int64_t stride, int i, int cols) {
+    const int at = first_of(i);
+    copy_tile<DP>(dst, L::kPitch, BN, src + at * stride, stride, min(BN, j.lk - at), cols, vec);
+  };
+  float m[4], l[4], acc[4][NO][4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    m[a] = -INFINITY;
+    l[a] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NO; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[a][c][e] = 0.f;
+  }
+  if (j.blocks > 0) load(sk, k, p.k_st, 0, p.d);
+  for (int i = 0; i < j.blocks; ++i) {
+    load(sv, v, p.v_st, i, p.dv);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys
+    __syncthreads();
+    float s[4][NC];
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[a][c] = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+      float4 x[4], y[NC];
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        x[a] = *reinterpret_cast<const float4*>(sq + (ty * 4 + a) * L::kPitch + d);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        y[c] = *reinterpret_cast<const float4*>(sk + (tx + 16 * c) * L::kPitch + d);
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s[a][c] = fmaf(x[a].x, y[c].x, s[a][c]);
+          s[a][c] = fmaf(x[a].y, y[c].y, s[a][c]);
+          s[a][c] = fmaf(x[a].z, y[c].z, s[a][c]);
+          s[a][c] = fmaf(x[a].w, y[c].w, s[a][c]);
+        }
+    }
+    const int key0 = first_of(i);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const int r = ty * 4 + a, h = r / w.tok, t = r - h * w.tok, at = tile.pf + t;
+      const bool valid = h < j.nh && t < tile.n;
+      float top = m[a];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int key = key0 + tx + 16 * c;
+        const bool sees = valid && key <= at && (key > at - w.window || key < w.sinks);
+        s[a][c] = sees ? s[a][c] * p.scale : -INFINITY;
+        top = fmaxf(top, s[a][c]);
+      }
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float f = expf(m[a] - ref);
+      m[a] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float e = expf(s[a][c] - ref);
+        sum += e;
+        sp[r * L::kP + tx + 16 * c] = e;
+      }
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      l[a] = l[a] * f + sum;
+#pragma unroll
+      for (int c = 0; c < NO; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[a][c][e] *= f;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");  // the values
+    __syncthreads();                                       // and nobody needs the keys any more
+    if (i + 1 < j.blocks) load(sk, k, p.k_st, i + 1, p.d);
+#pragma unroll 2
+    for (int n = 0; n < BN; n += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        x[a] = *reinterpret_cast<const float4*>(sp + (ty * 4 + a) * L::kP + n);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int c = 0; c < NO; ++c) {
+          const float4 y =
+              *reinterpret_cast<const float4*>(sv + (n + u) * L::kPitch + c * 64 + tx * 4);
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const float e = u == 0 ? x[a].x : u == 1 ? x[a].y : u == 2 ? x[a].z : x[a].w;
+            acc[a][c][0] = fmaf(e, y.x, acc[a][c][0]);
+            acc[a][c][1] = fmaf(e, y.y, acc[a][c][1]);
+            acc[a][c][2] = fmaf(e, y.z, acc[a][c][2]);
+            acc[a][c][3] = fmaf(e, y.w, acc[a][c][3]);
+          }
+        }
+      }
+    }
+    __syncthreads();  // the values and the weights may be overwritten
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const int r = ty * 4 + a, h = r / w.tok, t = r - h * w.tok;
+    if (h >= j.nh || t >= tile.n) continue;
+    float odd = 0.f;
+#pragma unroll
+    for (int c = 0; c < NO; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = c * 64 + tx * 4 + e;
+        const float y = l[a] == 0.f ? 0.f : acc[a][c][e] / l[a];
+        odd = fmaf(y, 0.f, odd);
+        if (col < p.dv) o[h * p.o_sh + t * p.o_st + col] = y;
+      }
+    if (!(odd == 0.f)) atomicOr(&redo[r >> 5], 1u << (r & 31));
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < 64; r += 8) {
+    if (!((redo[r >> 5] >> (r & 31)) & 1u)) continue;
+    const int h = r / w.tok, t = r - h * w.tok;
+    window_row<float>(q + h * p.q_sh + t * p.q_st, k, v, o + h * p.o_sh + t * p.o_st, p.k_st,
+                      p.v_st, p.d, p.dv, p.scale, p.window, p.sinks, tile.pf + t);
+  }
+}
+
 }  // namespace bio
 
 namespace {
 
 constexpr int64_t kMaxGrid = 2147483647;
-
-template <typename T>
-int launch_rows(const bio::WindowParams& p, bool packed, cudaStream_t s) {
-  const int64_t rows = (packed ? 1 : p.batch) * p.heads * p.lq;
-  const int64_t blocks = (rows + bio::kWinWarps - 1) / bio::kWinWarps;
-  if (blocks > kMaxGrid) return BIO_ERR_SHAPE;
-  if (packed)
-    bio::window_row_kernel<T, true><<<static_cast<unsigned>(blocks), bio::kWinWarps * 32, 0, s>>>(p);
-  else
-    bio::window_row_kernel<T, false><<<static_cast<unsigned>(blocks), bio::kWinWarps * 32, 0, s>>>(p);
-  return bio_host::launch_status(cudaGetLastError());
-}
 
 bio::FixedDiv fixed_div(int64_t n) {
   bio::FixedDiv d;
@@ -959,6 +1126,65 @@ bio::FixedDiv fixed_div(int64_t n) {
   while ((1ull << d.shift) < static_cast<uint64_t>(n)) ++d.shift;
   d.mul = static_cast<unsigned>(((1ull << 32) * ((1ull << d.shift) - d.n)) / d.n + 1);
   return d;
+}
+
+// Tiles of `rows` query rows, `tiles_per_job` of them in a job.
+int plan_jobs(const bio::WindowParams& p, const bio_attn_args* a, bool packed, int rows,
+              int tiles_per_job, bio::WindowJobs* w) {
+  const int64_t group = p.group;
+  w->hblocks = static_cast<int>((group + 15) / 16);  // up to 16 heads of a group in a tile
+  w->gh = static_cast<int>((group + w->hblocks - 1) / w->hblocks);
+  w->tok = rows / w->gh;
+  const int64_t span = static_cast<int64_t>(tiles_per_job) * w->tok;
+  const int64_t tiles = a->kv_heads * w->hblocks;
+  const int64_t qblocks = (p.lq + span - 1) / span + (packed ? p.nseq : 0);
+  const int64_t jobs = qblocks * tiles * (packed ? 1 : p.batch);
+  if (qblocks > kMaxGrid || jobs > (1 << 30)) return BIO_ERR_SHAPE;
+  w->qblocks = static_cast<int>(qblocks);
+  w->jobs = static_cast<int>(jobs);
+  w->by_qblocks = fixed_div(qblocks);
+  w->by_tiles = fixed_div(tiles);
+  w->by_hblocks = fixed_div(w->hblocks);
+  w->window = static_cast<int>(std::min<int64_t>(p.window, 1 << 30));
+  w->sinks = static_cast<int>(std::min<int64_t>(p.sinks, 1 << 30));
+  w->negate = p.scale < 0.f;
+  // a scale of 0 weighs every visible key alike; hidden ones stay at -inf
+  const float scale = (w->negate ? -p.scale : p.scale) * 1.4426950408889634f;
+  w->scale_log2 = scale == 0.f ? 1.17549435e-38f : scale;
+  w->vec_out = 0;
+  return BIO_OK;
+}
+
+template <int DP, bool PACKED>
+int launch_f32(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s) {
+  using L = bio::WinF32<DP>;
+  static std::once_flag once[bio_host::kMaxDevices];
+  cudaError_t set = cudaSuccess;
+  std::call_once(once[a->device], [&] {
+    set = cudaFuncSetAttribute(bio::window_f32_kernel<DP, PACKED>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  });
+  if (set != cudaSuccess) return BIO_ERR_LAUNCH;
+  bio::WindowJobs w;
+  const int st = plan_jobs(p, a, PACKED, 64, 1, &w);
+  if (st != BIO_OK) return st;
+  const uint64_t bits = reinterpret_cast<uint64_t>(p.k) | reinterpret_cast<uint64_t>(p.v) |
+                        4 * static_cast<uint64_t>(p.k_sb | p.k_sh | p.k_st | p.v_sb | p.v_sh |
+                                                  p.v_st | p.d | p.dv);
+  bio::window_f32_kernel<DP, PACKED><<<static_cast<unsigned>(w.jobs), 256, L::kBytes, s>>>(
+      p, w, bits % 16 == 0 ? 1 : 0);
+  return bio_host::launch_status(cudaGetLastError());
+}
+
+int launch_float(const bio::WindowParams& p, const bio_attn_args* a, bool packed, cudaStream_t s) {
+  const int dim = std::max(p.d, p.dv);
+  if (packed)
+    return dim <= 64    ? launch_f32<64, true>(p, a, s)
+           : dim <= 128 ? launch_f32<128, true>(p, a, s)
+                        : launch_f32<256, true>(p, a, s);
+  return dim <= 64    ? launch_f32<64, false>(p, a, s)
+         : dim <= 128 ? launch_f32<128, false>(p, a, s)
+                      : launch_f32<256, false>(p, a, s);
 }
 
 template <typename T, int DP, bool PACKED>
@@ -975,25 +1201,8 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
   const int sms = bio_host::sm_count(a->device);
   if (sms <= 0) return BIO_ERR_LAUNCH;
   bio::WindowJobs w;
-  const int64_t group = p.group;
-  w.hblocks = static_cast<int>((group + 15) / 16);  // up to 16 heads of a group in a tile
-  w.gh = static_cast<int>((group + w.hblocks - 1) / w.hblocks);
-  w.tok = 128 / w.gh;
-  const int64_t span = L::NT * w.tok, tiles = a->kv_heads * w.hblocks;
-  const int64_t qblocks = (p.lq + span - 1) / span + (packed ? p.nseq : 0);
-  const int64_t jobs = qblocks * tiles * (packed ? 1 : p.batch);
-  if (qblocks > kMaxGrid || jobs > (1 << 30)) return BIO_ERR_SHAPE;
-  w.qblocks = static_cast<int>(qblocks);
-  w.jobs = static_cast<int>(jobs);
-  w.by_qblocks = fixed_div(qblocks);
-  w.by_tiles = fixed_div(tiles);
-  w.by_hblocks = fixed_div(w.hblocks);
-  w.window = static_cast<int>(std::min<int64_t>(p.window, 1 << 30));
-  w.sinks = static_cast<int>(std::min<int64_t>(p.sinks, 1 << 30));
-  w.negate = p.scale < 0.f;
-  // a scale of 0 weighs every visible key alike; hidden ones stay at -inf
-  const float scale = (w.negate ? -p.scale : p.scale) * 1.4426950408889634f;
-  w.scale_log2 = scale == 0.f ? 1.17549435e-38f : scale;
+  const int st = plan_jobs(p, a, PACKED, 128, L::NT, &w);
+  if (st != BIO_OK) return st;
   const uint64_t out_bits = reinterpret_cast<uint64_t>(p.o) |
                             2 * static_cast<uint64_t>(p.o_sb | p.o_sh | p.o_st | p.dv);
   w.vec_out = out_bits % 32 == 0 ? 2 : out_bits % 16 == 0 ? 1 : 0;
@@ -1008,7 +1217,7 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
       !bio_host::map_of<T>(&v, none ? p.q : p.v, p.dv, none ? 1 : p.lk, a->kv_heads, batch, p.v_st,
                            p.v_sh, p.v_sb, L::BN))
     return BIO_ERR_ALIGN;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(jobs, sms));
+  const unsigned grid = static_cast<unsigned>(std::min(w.jobs, sms));
   bio::window_tc_kernel<T, DP, PACKED><<<grid, L::kThreads, L::kBytes, s>>>(q, k, v, p, w);
   return bio_host::launch_status(cudaGetLastError());
 }
@@ -1063,7 +1272,7 @@ int run_window(const bio_attn_args* a, int64_t window, int64_t sinks, bool packe
   p.status = bio_host::status_word(a->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
-    case BIO_F32: return launch_rows<float>(p, packed, s);
+    case BIO_F32: return launch_float(p, a, packed, s);
     case BIO_F16: return launch_half<__half>(p, a, packed, s);
     case BIO_BF16: return launch_half<__nv_bfloat16>(p, a, packed, s);
     default: return BIO_ERR_DTYPE;
