@@ -13,7 +13,9 @@ tensor or host synchronisation is needed.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 
 import torch
 
@@ -218,19 +220,36 @@ def varlen(q, k, v, cu_q, cu_k, *, is_causal, causal_name, scale):
     return out
 
 
-def _window_args(q, k, v, out, q_s, k_s, v_s, o_s, batch, heads, kv_heads, lq, lk, d, dv, scale):
-    a = _AttnArgs()
-    a.dtype = _lib.DTYPE_CODE[q.dtype]
-    a.device = q.device.index
-    a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.q_sb, a.q_sh, a.q_st = q_s
-    a.k_sb, a.k_sh, a.k_st = k_s
-    a.v_sb, a.v_sh, a.v_st = v_s
-    a.o_sb, a.o_sh, a.o_st = o_s
-    a.batch, a.heads, a.kv_heads = batch, heads, kv_heads
-    a.lq, a.lk, a.d, a.dv = lq, lk, d, dv
-    a.scale = scale if scale is not None else 1.0 / math.sqrt(d)
-    return a
+# bio_attn_args packed into bytes: what the sliding-window entries read of it, zeros elsewhere
+_WINDOW_ARGS = struct.Struct("@ii4P17qiifiiiP4qPPiqP")
+
+
+@functools.lru_cache(maxsize=1024)
+def _tma_strides(shape, stride) -> bool:
+    """Whether every stride that is used is a multiple of 16 bytes of 16-bit elements."""
+    return stride[-1] == 1 and all(n < 2 or s % 8 == 0 for n, s in zip(shape[:-1], stride[:-1]))
+
+
+def _window_operand(t, lead):
+    """`t` as [B, H, L, D] with D contiguous, packed where TMA needs it."""
+    if len(lead) != 1:
+        t = t.reshape(math.prod(lead), *t.shape[-3:])
+    if t.dtype == torch.float32:
+        return _dim_contiguous(t)
+    if t.data_ptr() % 16 == 0 and _tma_strides(t.shape, t.stride()):
+        return t
+    return _tma_ready(_dim_contiguous(t))
+
+
+def _window_args(q, k, v, out, strides, batch, heads, kv_heads, lq, lk, d, dv, scale,
+                 cu_q=None, cu_k=None):
+    many = (0, 0, 0, 0) if cu_q is None else (
+        cu_q.data_ptr(), cu_k.data_ptr(), 1 if cu_q.dtype == torch.int64 else 0, cu_q.numel() - 1)
+    return _WINDOW_ARGS.pack(
+        _lib.DTYPE_CODE[q.dtype], q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        out.data_ptr(), *strides, batch, heads, kv_heads, lq, lk, d, dv,
+        scale if scale is not None else 1.0 / math.sqrt(d), 0, MASK_NONE, 0, 0, 0, 0, 0, 0,
+        *many, 0)
 
 
 def window(q, k, v, window, sinks, scale):
@@ -239,26 +258,29 @@ def window(q, k, v, window, sinks, scale):
     h, lq, d = q.shape[-3:]
     hkv, lk, dv = k.shape[-3], k.shape[-2], v.shape[-1]
     nb = math.prod(lead)
-    q4 = _dim_contiguous(q.reshape(nb, h, lq, d))
-    k4 = _dim_contiguous(k.reshape(nb, hkv, lk, d))
-    v4 = _dim_contiguous(v.reshape(nb, hkv, lk, dv))
-    if q.dtype != torch.float32:
-        q4, k4, v4 = _tma_ready(q4), _tma_ready(k4), _tma_ready(v4)
+    q4, k4, v4 = _window_operand(q, lead), _window_operand(k, lead), _window_operand(v, lead)
     # token-major like the output of sdpa
-    out = torch.empty((nb, lq, h, dv), device=q.device, dtype=q.dtype).transpose(1, 2)
+    out = q.new_empty((nb, lq, h, dv)).transpose(1, 2)
+    result = out if len(lead) == 1 else out.reshape(*lead, h, lq, dv)
     if out.numel() == 0:
-        return out.reshape(*lead, h, lq, dv)
-    a = _window_args(q4, k4, v4, out, q4.stride()[:3], k4.stride()[:3], v4.stride()[:3],
-                     out.stride()[:3], nb, h, hkv, lq, lk, d, dv, scale)
-    seen = min(lk, window + sinks)
-    with tracing.span("window_attention", f"bio_attention_window [B={nb}, H={h}/{hkv}, Lq={lq}, "
-                      f"Lk={lk}, D={d}/{dv}, window={window}, sinks={sinks}]",
-                      2.0 * nb * h * lq * seen * (d + dv),
-                      q.element_size() * (q4.numel() + k4.numel() + v4.numel() + out.numel()),
-                      q.element_size()):
-        _lib.check(_lib.load().bio_attention_window(ctypes.byref(a), window, sinks,
-                                                    _lib.stream_of(q)), "bio_attention_window")
-    return out.reshape(*lead, h, lq, dv)
+        return result
+    args = _window_args(q4, k4, v4, out, (*q4.stride()[:3], *k4.stride()[:3], *v4.stride()[:3],
+                                          *out.stride()[:3]), nb, h, hkv, lq, lk, d, dv, scale)
+    pushed = False
+    if tracing.active():
+        seen = min(lk, window + sinks)
+        pushed = tracing.note(
+            "window_attention", f"bio_attention_window [B={nb}, H={h}/{hkv}, Lq={lq}, "
+            f"Lk={lk}, D={d}/{dv}, window={window}, sinks={sinks}]",
+            2.0 * nb * h * lq * seen * (d + dv),
+            q.element_size() * (q4.numel() + k4.numel() + v4.numel() + out.numel()),
+            q.element_size())
+    try:
+        _lib.check(_lib.load().bio_attention_window(args, window, sinks, _lib.stream_of(q)),
+                   "bio_attention_window")
+    finally:
+        tracing.done(pushed)
+    return result
 
 
 def window_varlen(q, k, v, cu_q, cu_k, window, sinks, scale):
@@ -277,16 +299,14 @@ def window_varlen(q, k, v, cu_q, cu_k, window, sinks, scale):
     cu_k = cu_k.to(cu_q.dtype) if cu_k.dtype != cu_q.dtype else cu_k
     cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
     by_token = lambda t: (0, t.stride(1), t.stride(0))  # noqa: E731
-    a = _window_args(q3, k3, v3, out, by_token(q3), by_token(k3), by_token(v3), by_token(out[0]),
-                     1, h, hkv, tq, tk, d, dv, scale)
-    a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
-    a.cu_is64 = 1 if cu_q.dtype == torch.int64 else 0
-    a.nseq = cu_q.numel() - 1
+    args = _window_args(q3, k3, v3, out, (*by_token(q3), *by_token(k3), *by_token(v3),
+                                          *by_token(out[0])),
+                        1, h, hkv, tq, tk, d, dv, scale, cu_q, cu_k)
     with tracing.span("window_attention", f"bio_attention_window_varlen [T={tq}/{tk}, H={h}/{hkv}, "
                       f"window={window}, sinks={sinks}]", 0,
                       q.element_size() * (q3.numel() + k3.numel() + v3.numel() + out.numel()),
                       q.element_size()):
-        _lib.check(_lib.load().bio_attention_window_varlen(ctypes.byref(a), window, sinks,
+        _lib.check(_lib.load().bio_attention_window_varlen(args, window, sinks,
                                                            _lib.stream_of(q)),
                    "bio_attention_window_varlen")
     return out

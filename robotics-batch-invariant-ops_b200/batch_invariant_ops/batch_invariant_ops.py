@@ -11,6 +11,7 @@ reference file.
 from __future__ import annotations
 
 import contextlib
+import functools
 from collections import namedtuple
 from typing import Any
 
@@ -420,25 +421,31 @@ def varlen_scaled_dot_product_attention_batch_invariant(
 # ---------------------------------------------------------------------------
 # Sliding-window attention (not in the reference)
 # ---------------------------------------------------------------------------
-def _check_window(query, key, value, window, sinks, heads_dim, tokens_dim):
-    if query.dtype != key.dtype or query.dtype != value.dtype:
+@functools.lru_cache(maxsize=1024)
+def _check_window_shapes(query, key, value, dtypes, heads_dim, tokens_dim):
+    """What depends on shapes and types alone, checked once for each of them."""
+    if dtypes[0] != dtypes[1] or dtypes[0] != dtypes[2]:
         raise ValueError("query, key, and value must have the same dtype")
-    if query.dtype not in _FLOAT_TYPES:
-        raise ValueError(f"unsupported sliding-window attention dtype: {query.dtype}")
-    if key.shape[heads_dim] != value.shape[heads_dim] or (
-            key.shape[tokens_dim] != value.shape[tokens_dim]):
+    if dtypes[0] not in _FLOAT_TYPES:
+        raise ValueError(f"unsupported sliding-window attention dtype: {dtypes[0]}")
+    if key[heads_dim] != value[heads_dim] or key[tokens_dim] != value[tokens_dim]:
         raise ValueError("key and value token and head dimensions must match")
-    if query.shape[-1] != key.shape[-1]:
+    if query[-1] != key[-1]:
         raise ValueError("query and key head dimensions must match")
-    if query.shape[-1] == 0 or value.shape[-1] == 0:
+    if query[-1] == 0 or value[-1] == 0:
         raise ValueError("head dimensions must not be zero")
-    if key.shape[heads_dim] == 0 or query.shape[heads_dim] % key.shape[heads_dim]:
+    if key[heads_dim] == 0 or query[heads_dim] % key[heads_dim]:
         raise ValueError("query heads must be divisible by key/value heads")
+    _attn._check_head_dims(query[-1], value[-1])
+
+
+def _check_window(query, key, value, window, sinks, heads_dim, tokens_dim):
+    _check_window_shapes(query.shape, key.shape, value.shape,
+                         (query.dtype, key.dtype, value.dtype), heads_dim, tokens_dim)
     if not 1 <= window <= 2147483647:
         raise ValueError("window must be at least 1 and fit in 32 bits")
     if not 0 <= sinks <= 2147483647:
         raise ValueError("sinks must not be negative and fit in 32 bits")
-    _attn._check_head_dims(query.shape[-1], value.shape[-1])
 
 
 def sliding_window_attention_batch_invariant(

@@ -25,8 +25,10 @@ are only known to the device, which skips what is out of range and sets
 
 from __future__ import annotations
 
+import functools
 import math
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -40,22 +42,55 @@ _POOL = struct.Struct("@iiPP4q4q4q2q")  # bio_kv_pool
 _TABLE = struct.Struct("@PqqqPPqqii")  # bio_kv_table
 
 
-def _on_one_device(first: torch.Tensor, *others: torch.Tensor) -> None:
-    assert first.is_cuda, "Input must be a CUDA tensor"
-    device = first.device
-    for t in others:
-        if t.device != device:
+# A call costs about as much on the host as its kernels take at the small end (a
+# single token), so what follows from shapes, strides, types and devices alone --
+# the checks and the integers of the C structs -- is worked out once per geometry.
+# Nothing here depends on an address or on what a tensor holds.
+_plan = functools.lru_cache(maxsize=1024)
+
+
+class _Geometry(NamedTuple):
+    shape: torch.Size
+    stride: tuple
+    dtype: torch.dtype
+    device: int  # -1 for the CPU
+
+    @property
+    def ndim(self) -> int:
+        return len(self.shape)
+
+    def contiguous(self) -> bool:
+        """For one dimension."""
+        return self.shape[0] < 2 or self.stride[0] == 1
+
+
+def _geo(t: torch.Tensor) -> tuple:
+    """A tensor's ``_Geometry`` as the plain tuple that plans are looked up by."""
+    return t.shape, t.stride(), t.dtype, t.get_device()
+
+
+def _geometries(*geos) -> list:
+    return [None if g is None else _Geometry(*g) for g in geos]
+
+
+def _on_one_device(first: _Geometry, *others: _Geometry) -> None:
+    assert first.device >= 0, "Input must be a CUDA tensor"
+    for g in others:
+        if g.device != first.device:
             raise ValueError("all tensors must be on the same CUDA device")
 
 
-def _index(t: torch.Tensor, what: str) -> torch.Tensor:
-    """A 1-D int32 tensor the kernels can read in place."""
-    if t.dtype != torch.int32 or t.ndim != 1:
+def _check_index(g: _Geometry, what: str) -> None:
+    """A 1-D int32 tensor; ``_in_place`` makes it one the kernels can read."""
+    if g.dtype != torch.int32 or g.ndim != 1:
         raise ValueError(f"{what} must be a 1-D int32 tensor")
-    return t if t.is_contiguous() else t.contiguous()
 
 
-def _check_pages(key_pages: torch.Tensor, value_pages: torch.Tensor, ndim: int) -> None:
+def _in_place(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _check_pages(key_pages: _Geometry, value_pages: _Geometry, ndim: int) -> None:
     if key_pages.ndim != ndim or value_pages.ndim != ndim:
         raise ValueError(f"key_pages and value_pages must have {ndim} dimensions")
     if key_pages.shape[:-1] != value_pages.shape[:-1]:
@@ -64,52 +99,98 @@ def _check_pages(key_pages: torch.Tensor, value_pages: torch.Tensor, ndim: int) 
         raise ValueError("key_pages and value_pages must share float32, float16 or bfloat16")
     if 0 in key_pages.shape[-3:] or value_pages.shape[-1] == 0:
         raise ValueError("pages need at least one head, one slot and one column")
-    if key_pages.stride(-1) != 1 or value_pages.stride(-1) != 1:
+    if key_pages.stride[-1] != 1 or value_pages.stride[-1] != 1:
         raise ValueError("pages must be contiguous in their last dimension")
 
 
-def _check_table(page_table: torch.Tensor, seq_lens=None, ref_counts=None, pages=None) -> None:
+def _check_table(page_table: _Geometry, seq_lens=None, ref_counts=None, pages=None) -> None:
     if page_table.ndim != 2 or page_table.dtype != torch.int32:
         raise ValueError("page_table must be a 2-D int32 tensor")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+    if page_table.shape[1] > 1 and page_table.stride[1] != 1:
         raise ValueError("page_table must be contiguous in its last dimension")
-    if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
+    if page_table.shape[0] > 1 and page_table.stride[0] < page_table.shape[1]:
         raise ValueError("the rows of page_table must not overlap")
     if seq_lens is not None and (seq_lens.dtype != torch.int32
                                  or seq_lens.shape != page_table.shape[:1]
-                                 or not seq_lens.is_contiguous()):
+                                 or not seq_lens.contiguous()):
         raise ValueError("seq_lens must be a contiguous int32 tensor with one entry per table row")
     if ref_counts is not None and (ref_counts.dtype != torch.int32 or ref_counts.ndim != 1
-                                   or not ref_counts.is_contiguous()
+                                   or not ref_counts.contiguous()
                                    or (pages is not None and ref_counts.shape[0] != pages)):
         raise ValueError("ref_counts must be a contiguous int32 tensor with one entry per page")
 
 
-def _pool_args(key_pages: torch.Tensor, value_pages: torch.Tensor) -> bytes:
-    ks, vs = key_pages.stride(), value_pages.stride()
-    shape = key_pages.shape
+def _pool_ints(key_pages: _Geometry, value_pages: _Geometry) -> tuple:
+    ks, vs, shape = tuple(key_pages.stride), tuple(value_pages.stride), tuple(key_pages.shape)
     if key_pages.ndim == 4:
         ks, vs, shape = (0, *ks), (0, *vs), (1, *shape)
-    return _POOL.pack(_lib.DTYPE_CODE[key_pages.dtype], key_pages.device.index,
-                      key_pages.data_ptr(), value_pages.data_ptr(), *shape[:4], *ks[:4], *vs[:4],
-                      shape[4], value_pages.shape[-1])
+    return ((_lib.DTYPE_CODE[key_pages.dtype], key_pages.device),
+            (*shape[:4], *ks[:4], *vs[:4], shape[4], value_pages.shape[-1]))
 
 
-def _table_args(page_table, seq_lens, ref_counts, pages: int, page_size: int) -> bytes:
-    rows, width = page_table.shape
-    return _TABLE.pack(page_table.data_ptr(), page_table.stride(0), rows, width,
+def _pool_args(ints: tuple, key_pages: torch.Tensor, value_pages: torch.Tensor) -> bytes:
+    return _POOL.pack(*ints[0], key_pages.data_ptr(), value_pages.data_ptr(), *ints[1])
+
+
+def _table_ints(page_table: _Geometry, pages: int, page_size: int) -> tuple:
+    return ((page_table.stride[0], *page_table.shape), (pages, page_size, page_table.device, 0))
+
+
+def _table_args(ints: tuple, page_table: torch.Tensor, seq_lens=None, ref_counts=None) -> bytes:
+    return _TABLE.pack(page_table.data_ptr(), *ints[0],
                        0 if seq_lens is None else seq_lens.data_ptr(),
-                       0 if ref_counts is None else ref_counts.data_ptr(),
-                       pages, page_size, page_table.device.index, 0)
+                       0 if ref_counts is None else ref_counts.data_ptr(), *ints[1])
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _call(name: str, note, *args) -> None:
+    """One call of the library, recorded when launches are (``note()`` says as what)."""
+    pushed = tracing.note(*note()) if note is not None and tracing.active() else False
+    try:
+        _lib.check(getattr(_lib.load(), name)(*args), name)
+    finally:
+        tracing.done(pushed)
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
+@_plan
+def _decode_plan(query, key_pages, value_pages, page_table, seq_lens, rows):
+    query, key_pages, value_pages, page_table, seq_lens, rows = _geometries(
+        query, key_pages, value_pages, page_table, seq_lens, rows)
+    if query.ndim != 3:
+        raise ValueError("query must be [batch, heads, head_dim]")
+    _check_pages(key_pages, value_pages, 4)
+    _check_table(page_table, seq_lens)
+    batch, heads, d = query.shape
+    pages, kv_heads, page_size, kd = key_pages.shape
+    dv = value_pages.shape[3]
+    if query.dtype != key_pages.dtype:
+        raise ValueError("query and pages must have the same dtype")
+    if d != kd:
+        raise ValueError("query and key head dimensions must match")
+    if d > MAX_HEAD_DIM or dv > MAX_HEAD_DIM:
+        raise ValueError(f"head dimensions above {MAX_HEAD_DIM} are not supported (got {d}, {dv})")
+    if heads == 0 or heads % kv_heads:
+        raise ValueError("query heads must be divisible by key/value heads")
+    if rows is not None:
+        _check_index(rows, "rows")
+        if rows.shape[0] != batch:
+            raise ValueError("rows must have one entry per query")
+    elif page_table.shape[0] != batch:
+        raise ValueError("page_table must have one row per query (or give rows)")
+    _on_one_device(query, key_pages, value_pages, page_table, seq_lens,
+                   *([] if rows is None else [rows]))
+    return ((_lib.DTYPE_CODE[query.dtype], query.device),
+            (*key_pages.stride[:3], *value_pages.stride[:3], heads * dv, dv, batch, heads,
+             kv_heads, pages, page_size), (page_table.stride[0], *page_table.shape),
+            (d, dv), (batch, heads, dv), d ** -0.5)
+
+
 def paged_attention_decode_batch_invariant(
     query: torch.Tensor,
     key_pages: torch.Tensor,
@@ -131,75 +212,72 @@ def paged_attention_decode_batch_invariant(
     Returns ``[B, H, Dv]``; rows of length 0 give zeros.  Slots beyond a row's
     length never reach the result, whatever they hold.
 
-    A row's cache is cut into pieces whose size depends on its own length
-    alone, so its bits do not depend on the other rows of the call.
+    A row's cache is cut into pieces whose size depends on its own length and
+    the window alone, so its bits do not depend on the other rows of the call.
     """
-    if query.ndim != 3:
-        raise ValueError("query must be [batch, heads, head_dim]")
-    _check_pages(key_pages, value_pages, 4)
-    _check_table(page_table, seq_lens)
-    batch, heads, d = query.shape
-    pages, kv_heads, page_size, kd = key_pages.shape
-    dv = value_pages.shape[3]
-    if query.dtype != key_pages.dtype:
-        raise ValueError("query and pages must have the same dtype")
-    if d != kd:
-        raise ValueError("query and key head dimensions must match")
-    if d > MAX_HEAD_DIM or dv > MAX_HEAD_DIM:
-        raise ValueError(f"head dimensions above {MAX_HEAD_DIM} are not supported (got {d}, {dv})")
-    if heads == 0 or heads % kv_heads:
-        raise ValueError("query heads must be divisible by key/value heads")
     if window is not None and window < 1:
         raise ValueError("window must be at least 1")
     if sinks < 0:
         raise ValueError("sinks must not be negative")
-    if rows is not None:
-        rows = _index(rows, "rows")
-        if rows.shape[0] != batch:
-            raise ValueError("rows must have one entry per query")
-        _on_one_device(query, key_pages, value_pages, page_table, seq_lens, rows)
-    else:
-        if page_table.shape[0] != batch:
-            raise ValueError("page_table must have one row per query (or give rows)")
-        _on_one_device(query, key_pages, value_pages, page_table, seq_lens)
-    if query.stride(2) != 1:
-        query = query.contiguous()
-    out = torch.empty((batch, heads, dv), dtype=query.dtype, device=query.device)
-    if batch == 0:
+    kind, shape, table, dims, out_shape, usual = _decode_plan(
+        _geo(query), _geo(key_pages), _geo(value_pages), _geo(page_table), _geo(seq_lens),
+        None if rows is None else _geo(rows))
+    query = _in_place(query)
+    out = query.new_empty(out_shape)
+    if out_shape[0] == 0:
         return out
-    lib = _lib.load()
-    qs, ks, vs = query.stride(), key_pages.stride(), value_pages.stride()
+    if rows is not None:
+        rows = _in_place(rows)
+    qs = query.stride()
     args = _ATTN_ARGS.pack(
-        _lib.DTYPE_CODE[query.dtype], query.device.index,
-        query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), out.data_ptr(),
-        qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], heads * dv, dv,
-        batch, heads, kv_heads, pages, page_size,
-        page_table.data_ptr(), page_table.stride(0), *page_table.shape, seq_lens.data_ptr(),
+        *kind, query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), out.data_ptr(),
+        qs[0], qs[1], *shape, page_table.data_ptr(), *table, seq_lens.data_ptr(),
         0 if rows is None else rows.data_ptr(),
         0 if window is None else min(window, 2147483647), min(sinks, 2147483647),
-        d, dv, d ** -0.5 if scale is None else scale, 0)
-    nbytes = lib.bio_paged_attention_workspace(args)
-    workspace = _workspace(nbytes, query.device) if nbytes else None
-    pushed = False
-    if tracing.active():
-        most = page_table.shape[1] * page_size
+        *dims, usual if scale is None else scale, 0)
+    nbytes = _lib.load().bio_paged_attention_workspace(args)
+    workspace = _workspace(nbytes, out.device) if nbytes else None
+
+    def note():
+        batch, heads, dv = out_shape
+        d, kv_heads, size = dims[0], shape[-3], query.element_size()
+        most = table[2] * shape[-1]
         most = most if window is None else min(most, window + sinks)
-        pushed = tracing.note(
-            "paged_attention", f"bio_paged_attention [B={batch}, H={heads}/{kv_heads}, "
-            f"tokens<={most}, D={d}/{dv}]", 2.0 * batch * heads * most * (d + dv),
-            query.element_size() * batch * (most * kv_heads * (d + dv) + heads * (d + dv)),
-            query.element_size())
-    try:
-        _lib.check(lib.bio_paged_attention(args, workspace.data_ptr() if nbytes else None, nbytes,
-                                           _lib.stream_of(query)), "bio_paged_attention")
-    finally:
-        tracing.done(pushed)
+        return ("paged_attention", f"bio_paged_attention [B={batch}, H={heads}/{kv_heads}, "
+                f"tokens<={most}, D={d}/{dv}]", 2.0 * batch * heads * most * (d + dv),
+                size * batch * (most * kv_heads * (d + dv) + heads * (d + dv)), size)
+
+    _call("bio_paged_attention", note, args, workspace.data_ptr() if nbytes else None, nbytes,
+          _lib.stream_of(out))
     return out
 
 
 # ---------------------------------------------------------------------------
 # pages
 # ---------------------------------------------------------------------------
+@_plan
+def _append_plan(key_pages, value_pages, key, value, page_table, rows, positions):
+    key_pages, value_pages, key, value, page_table, rows, positions = _geometries(
+        key_pages, value_pages, key, value, page_table, rows, positions)
+    _check_pages(key_pages, value_pages, 4)
+    _check_table(page_table)
+    if key.ndim != 3 or value.ndim != 3:
+        raise ValueError("key and value must be [tokens, kv_heads, head_dim]")
+    pages, kv_heads, page_size, d = key_pages.shape
+    tokens = key.shape[0]
+    if tuple(key.shape[1:]) != (kv_heads, d) or tuple(value.shape) != (
+            tokens, kv_heads, value_pages.shape[3]):
+        raise ValueError("key and value must match the heads and columns of the pages")
+    if key.dtype != key_pages.dtype or value.dtype != key_pages.dtype:
+        raise ValueError("key, value and pages must have the same dtype")
+    _check_index(rows, "rows")
+    _check_index(positions, "positions")
+    if rows.shape[0] != tokens or positions.shape[0] != tokens:
+        raise ValueError("rows and positions must have one entry per token")
+    _on_one_device(key, value, key_pages, value_pages, page_table, rows, positions)
+    return _pool_ints(key_pages, value_pages), _table_ints(page_table, pages, page_size)
+
+
 def paged_kv_append(
     key_pages: torch.Tensor,
     value_pages: torch.Tensor,
@@ -215,37 +293,36 @@ def paged_kv_append(
     to position ``positions[t]`` of table row ``rows[t]`` (both int32); a negative
     position is skipped (padding).  Slices of a fused projection are read in
     place."""
-    _check_pages(key_pages, value_pages, 4)
-    _check_table(page_table)
-    if key.ndim != 3 or value.ndim != 3:
-        raise ValueError("key and value must be [tokens, kv_heads, head_dim]")
-    pages, kv_heads, page_size, d = key_pages.shape
+    pool, table = _append_plan(_geo(key_pages), _geo(value_pages), _geo(key), _geo(value),
+                               _geo(page_table), _geo(rows), _geo(positions))
     tokens = key.shape[0]
-    if tuple(key.shape[1:]) != (kv_heads, d) or tuple(value.shape) != (
-            tokens, kv_heads, value_pages.shape[3]):
-        raise ValueError("key and value must match the heads and columns of the pages")
-    if key.dtype != key_pages.dtype or value.dtype != key_pages.dtype:
-        raise ValueError("key, value and pages must have the same dtype")
-    rows, positions = _index(rows, "rows"), _index(positions, "positions")
-    if rows.shape[0] != tokens or positions.shape[0] != tokens:
-        raise ValueError("rows and positions must have one entry per token")
-    _on_one_device(key, value, key_pages, value_pages, page_table, rows, positions)
-    if key.stride(2) != 1:
-        key = key.contiguous()
-    if value.stride(2) != 1:
-        value = value.contiguous()
     if tokens == 0:
         return
-    with tracing.span("kv_append", f"bio_kv_append [T={tokens}, H={kv_heads}, D={d}]", 0,
-                      2 * key.element_size() * (key.numel() + value.numel()), key.element_size()):
-        _lib.check(
-            _lib.load().bio_kv_append(
-                _pool_args(key_pages, value_pages),
-                _table_args(page_table, None, None, pages, page_size),
-                key.data_ptr(), key.stride(0), key.stride(1),
-                value.data_ptr(), value.stride(0), value.stride(1),
-                rows.data_ptr(), positions.data_ptr(), tokens, _lib.stream_of(key)),
-            "bio_kv_append")
+    key, value, rows, positions = map(_in_place, (key, value, rows, positions))
+    k_stride, v_stride = key.stride(), value.stride()
+    _call("bio_kv_append",
+          lambda: ("kv_append", f"bio_kv_append [T={tokens}, H={key.shape[1]}, D={key.shape[2]}]",
+                   0, 2 * key.element_size() * (key.numel() + value.numel()), key.element_size()),
+          _pool_args(pool, key_pages, value_pages), _table_args(table, page_table),
+          key.data_ptr(), k_stride[0], k_stride[1], value.data_ptr(), v_stride[0], v_stride[1],
+          rows.data_ptr(), positions.data_ptr(), tokens, _lib.stream_of(key))
+
+
+@_plan
+def _rows_plan(page_table, seq_lens, ref_counts, rows, new_lens, page_size):
+    page_table, seq_lens, ref_counts, rows, new_lens = _geometries(
+        page_table, seq_lens, ref_counts, rows, new_lens)
+    _check_table(page_table, seq_lens, ref_counts)
+    _check_index(rows, "rows")
+    if new_lens is not None:
+        _check_index(new_lens, "new_lens")
+        if rows.shape[0] != new_lens.shape[0]:
+            raise ValueError("rows and new_lens must have the same length")
+    if page_size < 1:
+        raise ValueError("page_size must be at least 1")
+    _on_one_device(page_table, seq_lens, ref_counts, rows,
+                   *([] if new_lens is None else [new_lens]))
+    return _table_ints(page_table, ref_counts.shape[0], page_size)
 
 
 def paged_kv_extend(
@@ -260,19 +337,14 @@ def paged_kv_extend(
     lowest free pages go to the rows in order.  A length that is not larger
     leaves its row as it is; when the pool runs out a row ends with the pages
     that it got (``BIO_DEV_PAGES``)."""
-    _check_table(page_table, seq_lens, ref_counts)
-    rows, new_lens = _index(rows, "rows"), _index(new_lens, "new_lens")
-    if rows.shape[0] != new_lens.shape[0]:
-        raise ValueError("rows and new_lens must have the same length")
-    if page_size < 1:
-        raise ValueError("page_size must be at least 1")
-    _on_one_device(page_table, seq_lens, ref_counts, rows, new_lens)
-    lib, n, pages = _lib.load(), rows.shape[0], ref_counts.shape[0]
-    nbytes = lib.bio_kv_workspace(n, 0)
+    table = _rows_plan(_geo(page_table), _geo(seq_lens), _geo(ref_counts), _geo(rows),
+                       _geo(new_lens), int(page_size))
+    rows, new_lens, n = _in_place(rows), _in_place(new_lens), rows.shape[0]
+    nbytes = _lib.load().bio_kv_workspace(n, 0)
     workspace = _workspace(nbytes, page_table.device)
-    _lib.check(lib.bio_kv_extend(_table_args(page_table, seq_lens, ref_counts, pages, page_size),
-                                 rows.data_ptr(), new_lens.data_ptr(), n, workspace.data_ptr(),
-                                 nbytes, _lib.stream_of(page_table)), "bio_kv_extend")
+    _call("bio_kv_extend", None, _table_args(table, page_table, seq_lens, ref_counts),
+          rows.data_ptr(), new_lens.data_ptr(), n, workspace.data_ptr(), nbytes,
+          _lib.stream_of(page_table))
 
 
 def paged_kv_free(
@@ -282,12 +354,10 @@ def paged_kv_free(
     rows: torch.Tensor,
 ) -> None:
     """Release every page of ``rows`` (int32, in place) and set their lengths to 0."""
-    _check_table(page_table, seq_lens, ref_counts)
-    rows = _index(rows, "rows")
-    _on_one_device(page_table, seq_lens, ref_counts, rows)
-    _lib.check(_lib.load().bio_kv_free(
-        _table_args(page_table, seq_lens, ref_counts, ref_counts.shape[0], 1), rows.data_ptr(),
-        rows.shape[0], _lib.stream_of(page_table)), "bio_kv_free")
+    table = _rows_plan(_geo(page_table), _geo(seq_lens), _geo(ref_counts), _geo(rows), None, 1)
+    rows = _in_place(rows)
+    _call("bio_kv_free", None, _table_args(table, page_table, seq_lens, ref_counts),
+          rows.data_ptr(), rows.shape[0], _lib.stream_of(page_table))
 
 
 def paged_kv_evict(
@@ -302,19 +372,32 @@ def paged_kv_evict(
     """Release the pages of ``rows`` that no token within ``window`` or ``sinks``
     of the newest one lies in (int32, in place).  Lengths stay; attention with
     this window and these sinks gives the same bits before and after."""
-    _check_table(page_table, seq_lens, ref_counts)
-    rows = _index(rows, "rows")
     if window < 1:
         raise ValueError("window must be at least 1")
     if sinks < 0:
         raise ValueError("sinks must not be negative")
-    if page_size < 1:
-        raise ValueError("page_size must be at least 1")
-    _on_one_device(page_table, seq_lens, ref_counts, rows)
-    _lib.check(_lib.load().bio_kv_evict(
-        _table_args(page_table, seq_lens, ref_counts, ref_counts.shape[0], page_size),
-        rows.data_ptr(), rows.shape[0], min(window, 2147483647), min(sinks, 2147483647),
-        _lib.stream_of(page_table)), "bio_kv_evict")
+    table = _rows_plan(_geo(page_table), _geo(seq_lens), _geo(ref_counts), _geo(rows), None,
+                       int(page_size))
+    rows = _in_place(rows)
+    _call("bio_kv_evict", None, _table_args(table, page_table, seq_lens, ref_counts),
+          rows.data_ptr(), rows.shape[0], min(window, 2147483647), min(sinks, 2147483647),
+          _lib.stream_of(page_table))
+
+
+
+@_plan
+def _fork_plan(key_pages, value_pages, page_table, seq_lens, ref_counts, src, dst):
+    key_pages, value_pages, page_table, seq_lens, ref_counts, src, dst = _geometries(
+        key_pages, value_pages, page_table, seq_lens, ref_counts, src, dst)
+    _check_pages(key_pages, value_pages, 5)
+    _, pages, _, page_size, _ = key_pages.shape
+    _check_table(page_table, seq_lens, ref_counts, pages)
+    _check_index(src, "src")
+    _check_index(dst, "dst")
+    if src.shape[0] != dst.shape[0]:
+        raise ValueError("src and dst must have the same length")
+    _on_one_device(key_pages, value_pages, page_table, seq_lens, ref_counts, src, dst)
+    return _pool_ints(key_pages, value_pages), _table_ints(page_table, pages, page_size)
 
 
 def paged_kv_fork(
@@ -331,23 +414,44 @@ def paged_kv_fork(
     released, whole pages are shared, the tokens of a last partial page are
     copied into the lowest free page, and the length is taken over.  No row may
     appear twice in ``dst`` or in both lists (``BIO_DEV_INDEX``, skipped)."""
-    _check_pages(key_pages, value_pages, 5)
-    layers, pages, _, page_size, _ = key_pages.shape
-    _check_table(page_table, seq_lens, ref_counts, pages)
-    src, dst = _index(src, "src"), _index(dst, "dst")
-    if src.shape[0] != dst.shape[0]:
-        raise ValueError("src and dst must have the same length")
-    _on_one_device(key_pages, value_pages, page_table, seq_lens, ref_counts, src, dst)
-    lib, n = _lib.load(), src.shape[0]
-    nbytes = lib.bio_kv_workspace(n, 0)
+    pool, table = _fork_plan(_geo(key_pages), _geo(value_pages), _geo(page_table), _geo(seq_lens),
+                             _geo(ref_counts), _geo(src), _geo(dst))
+    src, dst, n = _in_place(src), _in_place(dst), src.shape[0]
+    nbytes = _lib.load().bio_kv_workspace(n, 0)
     workspace = _workspace(nbytes, key_pages.device)
-    with tracing.span("kv_fork", f"bio_kv_fork [n={n}, layers={layers}]", 0, 0,
-                      key_pages.element_size()):
-        _lib.check(
-            lib.bio_kv_fork(_pool_args(key_pages, value_pages),
-                            _table_args(page_table, seq_lens, ref_counts, pages, page_size),
-                            src.data_ptr(), dst.data_ptr(), n, workspace.data_ptr(), nbytes,
-                            _lib.stream_of(key_pages)), "bio_kv_fork")
+    _call("bio_kv_fork",
+          lambda: ("kv_fork", f"bio_kv_fork [n={n}, layers={key_pages.shape[0]}]", 0, 0,
+                   key_pages.element_size()),
+          _pool_args(pool, key_pages, value_pages),
+          _table_args(table, page_table, seq_lens, ref_counts), src.data_ptr(), dst.data_ptr(), n,
+          workspace.data_ptr(), nbytes, _lib.stream_of(key_pages))
+
+
+@_plan
+def _compact_plan(key_pages, value_pages, page_table, ref_counts, out_key_pages, out_value_pages,
+                  out_page_table, out_ref_counts):
+    (key_pages, value_pages, page_table, ref_counts, out_key_pages, out_value_pages,
+     out_page_table, out_ref_counts) = _geometries(
+         key_pages, value_pages, page_table, ref_counts, out_key_pages, out_value_pages,
+         out_page_table, out_ref_counts)
+    _check_pages(key_pages, value_pages, 5)
+    _check_pages(out_key_pages, out_value_pages, 5)
+    pages, out_pages = key_pages.shape[1], out_key_pages.shape[1]
+    page_size = key_pages.shape[3]
+    _check_table(page_table, None, ref_counts, pages)
+    _check_table(out_page_table, None, out_ref_counts, out_pages)
+    if key_pages.dtype != out_key_pages.dtype:
+        raise ValueError("both pools must have the same dtype")
+    for a, b in ((key_pages, out_key_pages), (value_pages, out_value_pages)):
+        if (a.shape[0], *a.shape[2:]) != (b.shape[0], *b.shape[2:]):
+            raise ValueError("the pools must agree in all but their number of pages")
+    if page_table.shape != out_page_table.shape:
+        raise ValueError("the page tables must have the same shape")
+    _on_one_device(key_pages, value_pages, page_table, ref_counts, out_key_pages, out_value_pages,
+                   out_page_table, out_ref_counts)
+    return (_pool_ints(key_pages, value_pages), _table_ints(page_table, pages, page_size),
+            _pool_ints(out_key_pages, out_value_pages),
+            _table_ints(out_page_table, out_pages, page_size))
 
 
 def paged_kv_compact(
@@ -365,36 +469,22 @@ def paged_kv_compact(
     D]``, and write the table and the counts that go with them.  The pools may
     differ in their number of pages and must not overlap; pages that the other
     pool has no room for are dropped (``BIO_DEV_PAGES``)."""
-    _check_pages(key_pages, value_pages, 5)
-    _check_pages(out_key_pages, out_value_pages, 5)
-    pages, out_pages = key_pages.shape[1], out_key_pages.shape[1]
-    page_size = key_pages.shape[3]
-    _check_table(page_table, None, ref_counts, pages)
-    _check_table(out_page_table, None, out_ref_counts, out_pages)
-    if key_pages.dtype != out_key_pages.dtype:
-        raise ValueError("both pools must have the same dtype")
-    for a, b in ((key_pages, out_key_pages), (value_pages, out_value_pages)):
-        if (a.shape[0], *a.shape[2:]) != (b.shape[0], *b.shape[2:]):
-            raise ValueError("the pools must agree in all but their number of pages")
-    if page_table.shape != out_page_table.shape:
-        raise ValueError("the page tables must have the same shape")
-    _on_one_device(key_pages, value_pages, page_table, ref_counts, out_key_pages, out_value_pages,
-                   out_page_table, out_ref_counts)
-    lib = _lib.load()
-    nbytes = lib.bio_kv_workspace(0, pages)
+    pool, table, out_pool, out_table = _compact_plan(
+        _geo(key_pages), _geo(value_pages), _geo(page_table), _geo(ref_counts),
+        _geo(out_key_pages), _geo(out_value_pages), _geo(out_page_table), _geo(out_ref_counts))
+    nbytes = _lib.load().bio_kv_workspace(0, key_pages.shape[1])
     workspace = _workspace(nbytes, key_pages.device)
-    with tracing.span("kv_compact", f"bio_kv_compact [pages={pages}, out={out_pages}]", 0,
-                      2 * key_pages.element_size() * (out_key_pages.numel()
-                                                      + out_value_pages.numel()),
-                      key_pages.element_size()):
-        _lib.check(
-            lib.bio_kv_compact(_pool_args(key_pages, value_pages),
-                               _table_args(page_table, None, ref_counts, pages, page_size),
-                               _pool_args(out_key_pages, out_value_pages),
-                               _table_args(out_page_table, None, out_ref_counts, out_pages,
-                                           page_size),
-                               workspace.data_ptr(), nbytes, _lib.stream_of(key_pages)),
-            "bio_kv_compact")
+    _call("bio_kv_compact",
+          lambda: ("kv_compact",
+                   f"bio_kv_compact [pages={key_pages.shape[1]}, out={out_key_pages.shape[1]}]", 0,
+                   2 * key_pages.element_size() * (out_key_pages.numel()
+                                                   + out_value_pages.numel()),
+                   key_pages.element_size()),
+          _pool_args(pool, key_pages, value_pages),
+          _table_args(table, page_table, None, ref_counts),
+          _pool_args(out_pool, out_key_pages, out_value_pages),
+          _table_args(out_table, out_page_table, None, out_ref_counts), workspace.data_ptr(),
+          nbytes, _lib.stream_of(key_pages))
 
 
 class PagedKVCache:

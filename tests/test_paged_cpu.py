@@ -210,6 +210,24 @@ def test_argument_structs_have_the_c_sizes():
     assert paged._TABLE.size == 8 * (1 + 3 + 2 + 2 + 1)
 
 
+def test_window_arguments_land_in_the_fields_of_the_c_struct():
+    from batch_invariant_ops import _attn
+
+    t = torch.zeros(2, 3, 4, 8)
+    cu = torch.zeros(6, dtype=torch.int64)
+    strides = tuple(range(11, 23))
+    raw = _attn._window_args(t, t[:1], t[1:], t[1:, 1:], strides, 2, 6, 3, 4, 5, 8, 7, 0.25, cu,
+                             cu[1:])
+    a = _attn._AttnArgs.from_buffer_copy(raw)
+    assert [getattr(a, n) for n in ("q", "k", "v", "o")] == [
+        x.data_ptr() for x in (t, t[:1], t[1:], t[1:, 1:])]
+    assert tuple(getattr(a, f"{n}_{s}") for n in "qkvo" for s in ("sb", "sh", "st")) == strides
+    assert (a.dtype, a.batch, a.heads, a.kv_heads, a.lq, a.lk, a.d, a.dv, a.scale) == (
+        0, 2, 6, 3, 4, 5, 8, 7, 0.25)
+    assert (a.causal, a.mask_kind, a.mask, a.workspace) == (0, 0, None, None)
+    assert (a.cu_q, a.cu_k, a.cu_is64, a.nseq) == (cu.data_ptr(), cu[1:].data_ptr(), 1, 5)
+
+
 def attention_args(**change):
     a = dict(dtype=2, device=0, batch=4, heads=8, kv_heads=2, pages=64, page_size=16, rows=4,
              width=8, window=0, sinks=0, d=64, dv=64)
