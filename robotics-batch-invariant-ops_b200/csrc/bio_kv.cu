@@ -8,7 +8,9 @@
 // the order of their numbers by one block that scans the counts.
 //
 // Not in the reference, which keeps no cache between calls.
-#include "bio_common.cuh"
+#include <algorithm>
+
+#include "bio_tile.cuh"
 
 namespace bio {
 
@@ -54,7 +56,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
     kv_append_kernel(const KvPool pool, const KvTable tb, const char* __restrict__ k, int64_t k_st,
                      int64_t k_sh, const char* __restrict__ v, int64_t v_st, int64_t v_sh,
                      const int32_t* __restrict__ rows, const int32_t* __restrict__ positions,
-                     int64_t tokens) {
+                     int64_t tokens, const FixedDiv by_vk, const FixedDiv by_vv) {
   const int lane = threadIdx.x & 31;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
   if (t >= tokens) return;
@@ -67,7 +69,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
     if (lane == 0) raise_status(tb.status, BIO_DEV_INDEX);
     return;
   }
-  const unsigned vk = pool.k_row / sizeof(V), vv = pool.v_row / sizeof(V);
+  const unsigned vk = by_vk.n, vv = by_vv.n;  // vectors of one head
   const unsigned nk = vk * pool.heads, n = nk + vv * pool.heads;
   const char* ks = k + t * k_st;
   const char* vs = v + t * v_st;
@@ -84,7 +86,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32)
       if (i >= n) continue;
       const bool key = i < nk;
       const unsigned j = key ? i : i - nk, w = key ? vk : vv;
-      const unsigned h = j / w, c = (j - h * w) * sizeof(V);
+      const unsigned h = key ? by_vk.quotient(j) : by_vv.quotient(j), c = (j - h * w) * sizeof(V);
       val[u] = *reinterpret_cast<const V*>((key ? ks + h * k_sh : vs + h * v_sh) + c);
       to[u] = (key ? kd + h * pool.k_sh : vd + h * pool.v_sh) + c;
     }
@@ -377,25 +379,35 @@ __global__ void __launch_bounds__(kScanThreads)
   for (int64_t p = moved + threadIdx.x; p < out_pages; p += kScanThreads) out_refs[p] = 0;
 }
 
-// compact, second kernel: the table, then the pages.  A block copies pieces of
-// U * kRowThreads vectors; piece x belongs to page x / pieces of one layer's K
-// or V.  `runs` contiguous runs of `run` vectors make a page.
+// compact, second kernel: the table, then the pages.  Block (x, y, z) copies
+// pieces z, z + gridDim.z, ... of U * kRowThreads vectors of pages x, x +
+// gridDim.x, ... of one layer's K or V (y, y + gridDim.y, ...): no division to
+// find a page, and none inside it where its bytes lie together (FLAT).  DRAM
+// bounds it.  Divisions per vector instead: 1476 us for 2500 pages of 16 layers
+// (5.2 GB moved), instruction issue was the limit.
 struct KvCopySide {
   const char* from;
   char* to;
   int64_t from_sl, from_sp, from_s1, from_s2, to_sl, to_sp, to_s1, to_s2;  // bytes
-  unsigned n1, n2, run;  // a page: n1 x n2 runs of `run` vectors
+  unsigned per;               // vectors of a page: runs of by_run.n vectors in groups of by_n2.n
+  FixedDiv by_run, by_n2;
 };
 
-template <typename V>
-__global__ void __launch_bounds__(kRowThreads)
+__device__ __forceinline__ uint4 load_once(const uint4* p) { return __ldcs(p); }
+__device__ __forceinline__ uint2 load_once(const uint2* p) { return __ldcs(p); }
+__device__ __forceinline__ unsigned load_once(const unsigned* p) { return __ldcs(p); }
+__device__ __forceinline__ unsigned short load_once(const unsigned short* p) { return __ldcs(p); }
+
+template <typename V, bool FLAT>
+__global__ void __launch_bounds__(kRowThreads, 4)
     kv_compact_kernel(const KvCopySide ks, const KvCopySide vs, int64_t layers, const KvTable tb,
                       const KvTable out, const int32_t* __restrict__ rank_of,
                       const int32_t* __restrict__ in_use) {
   chain_wait();
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * kRowThreads;
-  for (int64_t x = static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x;
-       x < tb.rows * tb.width; x += threads) {
+  const int64_t block = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x +
+                        blockIdx.x;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z * kRowThreads;
+  for (int64_t x = block * kRowThreads + threadIdx.x; x < tb.rows * tb.width; x += threads) {
     const int64_t r = x / tb.width, c = x - r * tb.width;
     const int page = tb.table[r * tb.t_sr + c];
     if (page >= tb.pages) raise_status(tb.status, BIO_DEV_INDEX);
@@ -403,35 +415,32 @@ __global__ void __launch_bounds__(kRowThreads)
   }
   constexpr int U = 8;
   constexpr unsigned kPiece = U * kRowThreads;
-  const int64_t moved = in_use[0];
+  const int moved = in_use[0];
+  for (int64_t y = blockIdx.y; y < 2 * layers; y += gridDim.y) {
+    const KvCopySide& c = (y & 1) == 0 ? ks : vs;
+    const unsigned per = c.per;
+    auto offset = [&](unsigned v, int64_t s1, int64_t s2) -> int64_t {
+      if (FLAT) return static_cast<int64_t>(v) * sizeof(V);
+      const int r = c.by_run.quotient(v), i1 = c.by_n2.quotient(r);
+      return i1 * s1 + (r - i1 * static_cast<int>(c.by_n2.n)) * s2 +
+             static_cast<int64_t>(v - r * c.by_run.n) * sizeof(V);
+    };
+    for (int64_t rank = blockIdx.x; rank < moved; rank += gridDim.x) {
+      const char* from = c.from + (y >> 1) * c.from_sl + in_use[1 + rank] * c.from_sp;
+      char* to = c.to + (y >> 1) * c.to_sl + rank * c.to_sp;
+      for (unsigned at = blockIdx.z * kPiece; at < per; at += gridDim.z * kPiece) {
+        V val[U];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const KvCopySide& c = side == 0 ? ks : vs;
-    const unsigned per = c.n1 * c.n2 * c.run;  // vectors of a page
-    const unsigned pieces = (per + kPiece - 1) / kPiece;
-    const int64_t work = layers * moved * pieces;
-    for (int64_t x = blockIdx.x; x < work; x += gridDim.x) {
-      const int64_t pg = x / pieces;
-      const unsigned at = static_cast<unsigned>(x - pg * pieces) * kPiece;
-      const int64_t layer = pg / moved, rank = pg - layer * moved;
-      const char* from = c.from + layer * c.from_sl + in_use[1 + rank] * c.from_sp;
-      char* to = c.to + layer * c.to_sl + rank * c.to_sp;
-      V val[U];
+        for (int u = 0; u < U; ++u) {
+          const unsigned v = at + u * kRowThreads + threadIdx.x;
+          if (v < per)
+            val[u] = load_once(reinterpret_cast<const V*>(from + offset(v, c.from_s1, c.from_s2)));
+        }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const unsigned y = at + u * kRowThreads + threadIdx.x;
-        if (y >= per) continue;
-        const unsigned r = y / c.run, i1 = r / c.n2, i2 = r - i1 * c.n2;
-        val[u] = *reinterpret_cast<const V*>(from + i1 * c.from_s1 + i2 * c.from_s2 +
-                                             (y - r * c.run) * sizeof(V));
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const unsigned y = at + u * kRowThreads + threadIdx.x;
-        if (y >= per) continue;
-        const unsigned r = y / c.run, i1 = r / c.n2, i2 = r - i1 * c.n2;
-        *reinterpret_cast<V*>(to + i1 * c.to_s1 + i2 * c.to_s2 + (y - r * c.run) * sizeof(V)) =
-            val[u];
+        for (int u = 0; u < U; ++u) {
+          const unsigned v = at + u * kRowThreads + threadIdx.x;
+          if (v < per) __stcs(reinterpret_cast<V*>(to + offset(v, c.to_s1, c.to_s2)), val[u]);
+        }
       }
     }
   }
@@ -517,10 +526,10 @@ struct Width {
 // Launch that may overlap the end of the kernel before it on the stream; the
 // kernel waits for that one itself (chain_wait).
 template <typename... P, typename... A>
-int launch_chained(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t s,
+int launch_chained(void (*kernel)(P...), dim3 grid, unsigned block, cudaStream_t s,
                    A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.stream = s;
   cudaLaunchAttribute attr;
@@ -571,7 +580,8 @@ int bio_kv_append(const bio_kv_pool* pool, const bio_kv_table* table, const void
     using V = decltype(vec);
     bio::kv_append_kernel<V><<<static_cast<unsigned>(blocks), bio::kAppendWarps * 32, 0, s>>>(
         p, t, static_cast<const char*>(k), k_st * e, k_sh * e, static_cast<const char*>(v),
-        v_st * e, v_sh * e, rows, positions, tokens);
+        v_st * e, v_sh * e, rows, positions, tokens, bio_host::fixed_div(p.k_row / sizeof(V)),
+        bio_host::fixed_div(p.v_row / sizeof(V)));
     return bio_host::launch_status(cudaGetLastError());
   });
 }
@@ -701,21 +711,31 @@ int bio_kv_compact(const bio_kv_pool* pool, const bio_kv_table* table, const bio
       c.from_s1 = key ? p.k_sh : p.v_sh; c.to_s1 = key ? q.k_sh : q.v_sh;
       c.from_s2 = key ? p.k_st : p.v_st; c.to_s2 = key ? q.k_st : q.v_st;
       const int64_t row = key ? p.k_row : p.v_row;
-      c.n1 = p.heads;
-      c.n2 = p.page_size;
-      c.run = static_cast<unsigned>(row / sizeof(V));
+      int64_t n1 = p.heads, n2 = p.page_size, run = row / sizeof(V);
       if (c.from_s2 == row && c.to_s2 == row) {  // a head's tokens lie together
-        c.run *= c.n2;
-        c.n2 = 1;
+        run *= n2;
+        n2 = 1;
         if (c.from_s1 == row * p.page_size && c.to_s1 == c.from_s1) {  // and the heads do
-          c.run *= c.n1;
-          c.n1 = 1;
+          run *= n1;
+          n1 = 1;
         }
       }
+      c.per = static_cast<unsigned>(n1 * n2 * run);
+      c.by_run = bio_host::fixed_div(run);
+      c.by_n2 = bio_host::fixed_div(n2);
       return c;
     };
-    return launch_chained(bio::kv_compact_kernel<V>, static_cast<unsigned>(sms * 4),
-                          bio::kRowThreads, s, side(true), side(false), p.layers, t, o,
+    const bio::KvCopySide key = side(true), value = side(false);
+    constexpr unsigned kPiece = 8 * bio::kRowThreads;
+    const unsigned most = std::max(key.per, value.per);
+    dim3 grid;
+    grid.y = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(2 * p.layers, 1), 65535));
+    grid.z = std::min((most + kPiece - 1) / kPiece, 64u);
+    const int64_t wide = (static_cast<int64_t>(sms) * 8 + grid.y * grid.z - 1) / (grid.y * grid.z);
+    grid.x = static_cast<unsigned>(std::max<int64_t>(std::min(wide, q.pages), 1));
+    const bool flat = key.by_run.n == key.per && value.by_run.n == value.per;
+    auto kernel = flat ? bio::kv_compact_kernel<V, true> : bio::kv_compact_kernel<V, false>;
+    return launch_chained(kernel, grid, bio::kRowThreads, s, key, value, p.layers, t, o,
                           static_cast<const int32_t*>(rank_of),
                           static_cast<const int32_t*>(in_use));
   });

@@ -77,6 +77,16 @@ __device__ __forceinline__ bool parked_wait(uint32_t a, uint32_t parity,
   return false;
 }
 
+// Division of 0 <= x < 2^31 by a fixed n >= 1: (mulhi(x, mul) + x) >> shift with
+// 2^(shift-1) < n <= 2^shift and mul = floor(2^32 (2^shift - n) / n) + 1.
+struct FixedDiv {
+  unsigned mul, shift, n;
+  __device__ __forceinline__ int quotient(int x) const {
+    return static_cast<int>((__umulhi(static_cast<unsigned>(x), mul) + static_cast<unsigned>(x)) >>
+                            shift);
+  }
+};
+
 }  // namespace bio
 
 namespace bio_host {
@@ -103,6 +113,15 @@ inline bool map_of(CUtensorMap* map, const void* ptr, int64_t cols, int64_t n1, 
              4, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+inline bio::FixedDiv fixed_div(int64_t n) {
+  bio::FixedDiv d;
+  d.n = static_cast<unsigned>(n);
+  d.shift = 0;
+  while ((1ull << d.shift) < static_cast<uint64_t>(n)) ++d.shift;
+  d.mul = static_cast<unsigned>(((1ull << 32) * ((1ull << d.shift) - d.n)) / d.n + 1);
+  return d;
 }
 
 }  // namespace bio_host

@@ -141,16 +141,6 @@ __device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb,
 // neighbouring packed sequence are zeroed in shared memory instead, so that
 // they cannot even change a row's bits.
 // ---------------------------------------------------------------------------
-// Division of 0 <= x < 2^31 by a fixed n: (mulhi(x, mul) + x) >> shift with
-// 2^(shift-1) < n <= 2^shift and mul = floor(2^32 (2^shift - n) / n) + 1.
-struct FixedDiv {
-  unsigned mul, shift, n;
-  __device__ __forceinline__ int quotient(int x) const {
-    return static_cast<int>((__umulhi(static_cast<unsigned>(x), mul) + static_cast<unsigned>(x)) >>
-                            shift);
-  }
-};
-
 struct WindowJobs {
   int gh, tok, hblocks;  // heads and tokens of a tile, tiles across a group
   int qblocks;           // dense: blocks of NT * tok tokens per sequence; packed: at most
@@ -1119,15 +1109,6 @@ namespace {
 
 constexpr int64_t kMaxGrid = 2147483647;
 
-bio::FixedDiv fixed_div(int64_t n) {
-  bio::FixedDiv d;
-  d.n = static_cast<unsigned>(n);
-  d.shift = 0;
-  while ((1ull << d.shift) < static_cast<uint64_t>(n)) ++d.shift;
-  d.mul = static_cast<unsigned>(((1ull << 32) * ((1ull << d.shift) - d.n)) / d.n + 1);
-  return d;
-}
-
 // Tiles of `rows` query rows, `tiles_per_job` of them in a job.
 int plan_jobs(const bio::WindowParams& p, const bio_attn_args* a, bool packed, int rows,
               int tiles_per_job, bio::WindowJobs* w) {
@@ -1142,9 +1123,9 @@ int plan_jobs(const bio::WindowParams& p, const bio_attn_args* a, bool packed, i
   if (qblocks > kMaxGrid || jobs > (1 << 30)) return BIO_ERR_SHAPE;
   w->qblocks = static_cast<int>(qblocks);
   w->jobs = static_cast<int>(jobs);
-  w->by_qblocks = fixed_div(qblocks);
-  w->by_tiles = fixed_div(tiles);
-  w->by_hblocks = fixed_div(w->hblocks);
+  w->by_qblocks = bio_host::fixed_div(qblocks);
+  w->by_tiles = bio_host::fixed_div(tiles);
+  w->by_hblocks = bio_host::fixed_div(w->hblocks);
   w->window = static_cast<int>(std::min<int64_t>(p.window, 1 << 30));
   w->sinks = static_cast<int>(std::min<int64_t>(p.sinks, 1 << 30));
   w->negate = p.scale < 0.f;
