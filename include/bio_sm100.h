@@ -380,8 +380,10 @@ BIO_API int bio_attention_varlen(const bio_attn_args* args, void* stream);
  * position p = i + (lk - lq) (the last query at the last key); it sees key j
  * iff j <= p and (j > p - window or j < sinks).  window >= 1, sinks >= 0.
  * Rows that see no key produce zeros.  Operands, strides, grouped-query
- * sharing, alignment and batch invariance as bio_attention (causal and mask
- * fields must be 0); work grows with lq * (window + sinks), not lq * lk.  Keys
+ * sharing and batch invariance as bio_attention (causal and mask fields must
+ * be 0); 16-bit operands whose base or strides are not multiples of 16 bytes
+ * return BIO_ERR_ALIGN (bio_pack_rows makes such a copy), fp32 takes any
+ * stride.  Work grows with lq * (window + sinks), not lq * lk.  Keys
  * and values that a row does not see never reach it, whatever they hold.  No
  * counterpart in the reference (its SDPA, batch_invariant_ops.py:1148-1213,
  * would need the mask as a tensor and visits every key). */
@@ -486,11 +488,13 @@ BIO_API int bio_kv_compact(const bio_kv_pool* pool, const bio_kv_table* table,
  * give zeros.  Slots beyond the length and tokens outside the window never
  * reach the result, whatever they hold.
  *
- * Split: the n visible tokens of a row are cut into pieces whose size is a
- * function of n alone; each piece gives a maximum, a sum and an unnormalised
- * output in fp32, which are joined in the order of the pieces.  A row's bits
- * therefore depend on its own length and values only.  d, dv <= 256; strides
- * in elements, the innermost dimension contiguous. */
+ * Split: the tiles of 32 tokens that hold a visible token are cut into pieces
+ * of a length that is a function of their number alone; each piece gives a
+ * maximum, a sum and an unnormalised output in fp32, which are joined in the
+ * order of the pieces.  A row's bits therefore depend on its own length,
+ * window and values only.  d, dv <= 256; strides in elements, the innermost
+ * dimension contiguous.  16-bit pages and queries whose rows start on 16-byte
+ * borders run on the tensor cores, others (and fp32) on the CUDA cores. */
 typedef struct bio_paged_attn_args {
   int32_t dtype, device;
   const void* q;

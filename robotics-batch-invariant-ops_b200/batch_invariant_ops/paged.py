@@ -146,6 +146,11 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+@_plan
+def _kv_workspace(n: int, pages: int) -> int:
+    return _lib.load().bio_kv_workspace(n, pages)
+
+
 def _call(name: str, note, *args) -> None:
     """One call of the library, recorded when launches are (``note()`` says as what)."""
     pushed = tracing.note(*note()) if note is not None and tracing.active() else False
@@ -340,7 +345,7 @@ def paged_kv_extend(
     table = _rows_plan(_geo(page_table), _geo(seq_lens), _geo(ref_counts), _geo(rows),
                        _geo(new_lens), int(page_size))
     rows, new_lens, n = _in_place(rows), _in_place(new_lens), rows.shape[0]
-    nbytes = _lib.load().bio_kv_workspace(n, 0)
+    nbytes = _kv_workspace(n, 0)
     workspace = _workspace(nbytes, page_table.device)
     _call("bio_kv_extend", None, _table_args(table, page_table, seq_lens, ref_counts),
           rows.data_ptr(), new_lens.data_ptr(), n, workspace.data_ptr(), nbytes,
@@ -417,7 +422,7 @@ def paged_kv_fork(
     pool, table = _fork_plan(_geo(key_pages), _geo(value_pages), _geo(page_table), _geo(seq_lens),
                              _geo(ref_counts), _geo(src), _geo(dst))
     src, dst, n = _in_place(src), _in_place(dst), src.shape[0]
-    nbytes = _lib.load().bio_kv_workspace(n, 0)
+    nbytes = _kv_workspace(n, 0)
     workspace = _workspace(nbytes, key_pages.device)
     _call("bio_kv_fork",
           lambda: ("kv_fork", f"bio_kv_fork [n={n}, layers={key_pages.shape[0]}]", 0, 0,
@@ -472,7 +477,7 @@ def paged_kv_compact(
     pool, table, out_pool, out_table = _compact_plan(
         _geo(key_pages), _geo(value_pages), _geo(page_table), _geo(ref_counts),
         _geo(out_key_pages), _geo(out_value_pages), _geo(out_page_table), _geo(out_ref_counts))
-    nbytes = _lib.load().bio_kv_workspace(0, key_pages.shape[1])
+    nbytes = _kv_workspace(0, key_pages.shape[1])
     workspace = _workspace(nbytes, key_pages.device)
     _call("bio_kv_compact",
           lambda: ("kv_compact",

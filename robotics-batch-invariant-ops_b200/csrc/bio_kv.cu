@@ -299,42 +299,47 @@ __global__ void __launch_bounds__(kScanThreads)
   }
 }
 
-// fork, last kernel: block (i, layer, K or V) copies the tokens of the partial page.
+// fork, last kernel: the tokens of the partial page.  Block (i, x) copies them
+// for branch i in K or V of a layer (unit u = x, x + parts, ... of 2 * layers), so
+// that the chain of loads that finds the pages is walked once for all its units.
 template <typename V>
 __global__ void __launch_bounds__(kRowThreads)
     kv_fork_copy_kernel(const KvPool pool, const KvTable tb, const int32_t* __restrict__ src,
-                        const int32_t* __restrict__ dst, const int32_t* __restrict__ want) {
+                        const int32_t* __restrict__ dst, const int32_t* __restrict__ want,
+                        unsigned parts, const FixedDiv by_vk, const FixedDiv by_vv) {
   chain_wait();
-  const int64_t per = 2 * pool.layers;
-  const int64_t i = blockIdx.x / per, layer = (blockIdx.x % per) >> 1;
-  const bool key = (blockIdx.x % per & 1) == 0;
+  const unsigned i = blockIdx.x / parts;
   if (want[i] <= 0) return;
   const int s = src[i], d = dst[i];
   const int len = tb.lens[s], part = len % pool.page_size;
   if (tb.lens[d] != len) return;  // the pool had no page left
   const int64_t full = len / pool.page_size;
   const int64_t from = tb.table[s * tb.t_sr + full], to = tb.table[d * tb.t_sr + full];
-  const int64_t sl = key ? pool.k_sl : pool.v_sl, sp = key ? pool.k_sp : pool.v_sp;
-  const int64_t sh = key ? pool.k_sh : pool.v_sh, st = key ? pool.k_st : pool.v_st;
-  char* base = (key ? pool.k : pool.v) + layer * sl;
-  const unsigned w = (key ? pool.k_row : pool.v_row) / sizeof(V);
-  const unsigned run = w * part, n = run * pool.heads;
   constexpr int U = 4;
-  for (unsigned i0 = threadIdx.x; i0 < n; i0 += kRowThreads * U) {
-    V val[U];
-    int64_t off[U];
+  for (int64_t u0 = blockIdx.x - i * parts; u0 < 2 * pool.layers; u0 += parts) {
+    const bool key = (u0 & 1) == 0;
+    const int64_t sh = key ? pool.k_sh : pool.v_sh, st = key ? pool.k_st : pool.v_st;
+    char* base = key ? pool.k + (u0 >> 1) * pool.k_sl : pool.v + (u0 >> 1) * pool.v_sl;
+    const char* read = base + from * (key ? pool.k_sp : pool.v_sp);
+    char* write = base + to * (key ? pool.k_sp : pool.v_sp);
+    const FixedDiv by_w = key ? by_vk : by_vv;  // vectors of a token of a head
+    const unsigned n = by_w.n * part * pool.heads;
+    for (unsigned i0 = threadIdx.x; i0 < n; i0 += kRowThreads * U) {
+      V val[U];
+      int64_t off[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned x = i0 + kRowThreads * u;
-      off[u] = -1;
-      if (x >= n) continue;
-      const unsigned h = x / run, y = x - h * run, slot = y / w;
-      off[u] = h * sh + slot * st + (y - slot * w) * sizeof(V);
-      val[u] = *reinterpret_cast<const V*>(base + from * sp + off[u]);
+      for (int u = 0; u < U; ++u) {
+        const unsigned x = i0 + kRowThreads * u;
+        off[u] = -1;
+        if (x >= n) continue;
+        const int row = by_w.quotient(x), h = static_cast<unsigned>(row) / static_cast<unsigned>(part);
+        off[u] = h * sh + (row - h * part) * st + (x - row * by_w.n) * sizeof(V);
+        val[u] = *reinterpret_cast<const V*>(read + off[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (off[u] >= 0) *reinterpret_cast<V*>(write + off[u]) = val[u];
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (off[u] >= 0) *reinterpret_cast<V*>(base + to * sp + off[u]) = val[u];
   }
 }
 
@@ -580,8 +585,8 @@ int bio_kv_append(const bio_kv_pool* pool, const bio_kv_table* table, const void
     using V = decltype(vec);
     bio::kv_append_kernel<V><<<static_cast<unsigned>(blocks), bio::kAppendWarps * 32, 0, s>>>(
         p, t, static_cast<const char*>(k), k_st * e, k_sh * e, static_cast<const char*>(v),
-        v_st * e, v_sh * e, rows, positions, tokens, bio_host::fixed_div(p.k_row / sizeof(V)),
-        bio_host::fixed_div(p.v_row / sizeof(V)));
+        v_st * e, v_sh * e, rows, positions, tokens, bio::fixed_div(p.k_row / sizeof(V)),
+        bio::fixed_div(p.v_row / sizeof(V)));
     return bio_host::launch_status(cudaGetLastError());
   });
 }
@@ -647,6 +652,8 @@ int bio_kv_fork(const bio_kv_pool* pool, const bio_kv_table* table, const int32_
   if (workspace_bytes < 4 * (2 * n + 1)) return BIO_ERR_SCRATCH;
   st = bio_host::ensure_device(pool->device);
   if (st != BIO_OK) return st;
+  const int sms = bio_host::sm_count(pool->device);
+  if (sms <= 0) return BIO_ERR_LAUNCH;
   const bio::KvPool p = pool_view(pool);
   const bio::KvTable t = table_view(table);
   int32_t* ws = static_cast<int32_t*>(workspace);
@@ -662,8 +669,12 @@ int bio_kv_fork(const bio_kv_pool* pool, const bio_kv_table* table, const int32_
   w.add(p);
   return with_width(w.bytes(), [&](auto vec) {
     using V = decltype(vec);
-    return launch_chained(bio::kv_fork_copy_kernel<V>, static_cast<unsigned>(2 * n * p.layers),
-                          bio::kRowThreads, s, p, t, src, dst, ws);
+    // as many blocks as run at once, and a unit for each at least
+    const int64_t parts =
+        std::max<int64_t>(1, std::min(2 * p.layers, (static_cast<int64_t>(sms) * 8 + n - 1) / n));
+    return launch_chained(bio::kv_fork_copy_kernel<V>, static_cast<unsigned>(n * parts),
+                          bio::kRowThreads, s, p, t, src, dst, ws, static_cast<unsigned>(parts),
+                          bio::fixed_div(p.k_row / sizeof(V)), bio::fixed_div(p.v_row / sizeof(V)));
   });
 }
 
@@ -721,8 +732,8 @@ int bio_kv_compact(const bio_kv_pool* pool, const bio_kv_table* table, const bio
         }
       }
       c.per = static_cast<unsigned>(n1 * n2 * run);
-      c.by_run = bio_host::fixed_div(run);
-      c.by_n2 = bio_host::fixed_div(n2);
+      c.by_run = bio::fixed_div(run);
+      c.by_n2 = bio::fixed_div(n2);
       return c;
     };
     const bio::KvCopySide key = side(true), value = side(false);

@@ -87,6 +87,15 @@ struct FixedDiv {
   }
 };
 
+__host__ __device__ inline FixedDiv fixed_div(int64_t n) {
+  FixedDiv d;
+  d.n = static_cast<unsigned>(n);
+  d.shift = 0;
+  while ((1ull << d.shift) < static_cast<uint64_t>(n)) ++d.shift;
+  d.mul = static_cast<unsigned>(((1ull << 32) * ((1ull << d.shift) - d.n)) / d.n + 1);
+  return d;
+}
+
 }  // namespace bio
 
 namespace bio_host {
@@ -113,15 +122,6 @@ inline bool map_of(CUtensorMap* map, const void* ptr, int64_t cols, int64_t n1, 
              4, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-inline bio::FixedDiv fixed_div(int64_t n) {
-  bio::FixedDiv d;
-  d.n = static_cast<unsigned>(n);
-  d.shift = 0;
-  while ((1ull << d.shift) < static_cast<uint64_t>(n)) ++d.shift;
-  d.mul = static_cast<unsigned>(((1ull << 32) * ((1ull << d.shift) - d.n)) / d.n + 1);
-  return d;
 }
 
 }  // namespace bio_host

@@ -1123,9 +1123,9 @@ int plan_jobs(const bio::WindowParams& p, const bio_attn_args* a, bool packed, i
   if (qblocks > kMaxGrid || jobs > (1 << 30)) return BIO_ERR_SHAPE;
   w->qblocks = static_cast<int>(qblocks);
   w->jobs = static_cast<int>(jobs);
-  w->by_qblocks = bio_host::fixed_div(qblocks);
-  w->by_tiles = bio_host::fixed_div(tiles);
-  w->by_hblocks = bio_host::fixed_div(w->hblocks);
+  w->by_qblocks = bio::fixed_div(qblocks);
+  w->by_tiles = bio::fixed_div(tiles);
+  w->by_hblocks = bio::fixed_div(w->hblocks);
   w->window = static_cast<int>(std::min<int64_t>(p.window, 1 << 30));
   w->sinks = static_cast<int>(std::min<int64_t>(p.sinks, 1 << 30));
   w->negate = p.scale < 0.f;
