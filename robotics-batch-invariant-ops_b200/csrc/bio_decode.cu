@@ -294,7 +294,11 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
 // Measured on 128 rows of 1..8192 tokens (32 heads on 8, d 128, 2.15 GB): lanes
 // copying 16-token tiles by cp.async 636 us, TMA 614 us, both with four warps
 // on an item joining through shared memory; a warp per item 450 us, then bound
-// by the serial chain of one warp's instructions, which 32-token tiles halve.
+// by the serial chain of one warp's instructions, which 32-token tiles halve:
+// 413 us.  No divisions and two sums per product chain: 398 us.  This kernel now
+// runs 354 us of the 379 (6.1 TB/s read).  No gain from three stages and four
+// warps (437 us) or from keys and values in slots of their own and eight warps
+// (401 us, two waits a tile instead of one).
 // ---------------------------------------------------------------------------
 constexpr int kListRows = 512;   // rows whose piece counts fit in shared memory
 
@@ -761,20 +765,56 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Joins the pieces of one (row, head): weights e^(m_i - max m), eight warps
-// take the pieces i = warp, warp + 8, ... and are added in order.
+// Joins the pieces of every (row, head): weights e^(m_i - max m); pieces i = j,
+// j + 8, ... make sum j, and the eight sums are added in order.  With SPREAD, the
+// eight warps of a block make the sums of one head; without, a warp makes all of
+// them, eight loads in flight, and a block joins eight heads.  Bits are the same.
+// Latency bounds it: up to 32 pieces of 4096 heads (67 MB) took 25 us with a block
+// per head and take 16 with a warp; 256 pieces of 64 heads want the block, since 64
+// warps would leave most of the SMs idle.
 // ---------------------------------------------------------------------------
 constexpr int kJoinWarps = 8;
+constexpr int kSpreadPieces = 64;  // more pieces than this: a block per head
 
-template <typename T>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p) {
-  __shared__ float4 part[kJoinWarps][64];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+__device__ __forceinline__ void add_scaled(float4& y, const float4& a, float f) {
+  y.x = fmaf(a.x, f, y.x);
+  y.y = fmaf(a.y, f, y.y);
+  y.z = fmaf(a.z, f, y.z);
+  y.w = fmaf(a.w, f, y.w);
+}
+
+// G: 128-column groups of an output row
+template <typename T, int G, bool SPREAD>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedParams p,
+                                                                     int64_t outputs) {
+  constexpr int U = kJoinWarps;
+  __shared__ float4 part[SPREAD ? kJoinWarps : 1][32 * G];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads;
+  const int64_t bh = SPREAD ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp;
+  if (bh >= outputs) return;  // only without SPREAD
+  const int64_t b = bh / p.heads, h = bh - b * p.heads;
+  // lengths were there before the kernel that this one waits for began
   const int pieces = pieces_of(visible_of(p, row_of(p, b)).tiles);
   if (pieces <= 1) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const float2* ml = p.ml + bh * p.max_pieces;
+  const int groups = p.dvp / 4;  // four-float groups of an output row
+  const float4* acc = reinterpret_cast<const float4*>(p.acc + bh * p.max_pieces * p.dvp);
+  // round r, load u: piece 8 r + u of all sums, or piece 8 (8 r + u) + warp of the warp's
+  auto piece_of = [&](int r, int u) { return SPREAD ? (r * U + u) * kJoinWarps + warp : r * U + u; };
+  float4 a[U][G];
+  auto load = [&](int r) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int i = piece_of(r, u);
+        a[u][g] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < pieces && lane + 32 * g < groups)
+          a[u][g] = acc[static_cast<int64_t>(i) * groups + lane + 32 * g];
+      }
+  };
+  load(0);
   float top = -INFINITY;
   bool bad = false;
   for (int i = lane; i < pieces; i += 32) {
@@ -790,34 +830,53 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
 
-  const int groups = p.dvp / 4;  // four-float groups of an output row, <= 64
-  const float4* acc = reinterpret_cast<const float4*>(p.acc + bh * p.max_pieces * p.dvp);
-  float4 y[2];
-  y[0] = y[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = warp; i < pieces; i += kJoinWarps) {
-    const float f = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - top);
+  constexpr int Y = SPREAD ? 1 : U;
+  float4 y[Y][G];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      if (lane + 32 * g >= groups) continue;
-      const float4 a = acc[static_cast<int64_t>(i) * groups + lane + 32 * g];
-      y[g].x = fmaf(a.x, f, y[g].x);
-      y[g].y = fmaf(a.y, f, y[g].y);
-      y[g].z = fmaf(a.z, f, y[g].z);
-      y[g].w = fmaf(a.w, f, y[g].w);
+  for (int j = 0; j < Y; ++j)
+#pragma unroll
+    for (int g = 0; g < G; ++g) y[j][g] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r = 0; piece_of(r, 0) < pieces; ++r) {
+    if (r > 0) load(r);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = piece_of(r, u);
+      if (i >= pieces) break;
+      const float f = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - top);
+#pragma unroll
+      for (int g = 0; g < G; ++g) add_scaled(y[SPREAD ? 0 : u][g], a[u][g], f);
     }
   }
-#pragma unroll
-  for (int g = 0; g < 2; ++g)
-    if (lane + 32 * g < groups) part[warp][lane + 32 * g] = y[g];
-  __syncthreads();
   T* out = static_cast<T*>(p.o) + b * p.o_sb + h * p.o_sh;
-  const float* flat = reinterpret_cast<const float*>(part);
-  for (int e = threadIdx.x; e < p.dv; e += blockDim.x) {
-    float a = 0.f;
+  const bool none = bad || sum == 0.f;
+  if constexpr (SPREAD) {
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) a += flat[w * 256 + e];
-    out[e] = from_f32<T>(bad || sum == 0.f ? 0.f : a / sum);
+    for (int g = 0; g < G; ++g) part[warp][lane + 32 * g] = y[0][g];
+    __syncthreads();
+    const float* flat = reinterpret_cast<const float*>(part);
+    for (int e = threadIdx.x; e < p.dv; e += blockDim.x) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) x += flat[w * 128 * G + e];
+      out[e] = from_f32<T>(none ? 0.f : x / sum);
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < Y; ++j) {
+        x[0] += y[j][g].x;
+        x[1] += y[j][g].y;
+        x[2] += y[j][g].z;
+        x[3] += y[j][g].w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = (lane + 32 * g) * 4 + e;
+        if (c < p.dv) out[c] = from_f32<T>(none ? 0.f : x[e] / sum);
+      }
+    }
   }
 }
 
@@ -953,8 +1012,11 @@ int run(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
     if (st == BIO_ERR_ALIGN) st = dispatch_simt<T, false>(p, batch, s);
   }
   if (st != BIO_OK || p.max_pieces == 1) return st;
+  const bool spread = p.max_pieces > bio::kSpreadPieces, wide = p.dvp > 128;
+  const int64_t outputs = batch * p.heads;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(batch * p.heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(
+      spread ? outputs : (outputs + bio::kJoinWarps - 1) / bio::kJoinWarps));
   cfg.blockDim = dim3(bio::kJoinWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute attr;
@@ -962,7 +1024,10 @@ int run(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return bio_host::launch_status(cudaLaunchKernelEx(&cfg, bio::paged_join_kernel<T>, p));
+  auto join = spread ? (wide ? bio::paged_join_kernel<T, 2, true> : bio::paged_join_kernel<T, 1, true>)
+                     : (wide ? bio::paged_join_kernel<T, 2, false>
+                             : bio::paged_join_kernel<T, 1, false>);
+  return bio_host::launch_status(cudaLaunchKernelEx(&cfg, join, p, outputs));
 }
 
 }  // namespace
