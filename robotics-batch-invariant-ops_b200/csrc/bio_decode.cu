@@ -100,6 +100,10 @@ __device__ __forceinline__ Visible visible_of(const PagedParams& p, int2 row_len
 // CUDA-core kernel: fp32, and 16-bit pages whose rows are not 16-byte aligned.
 // LPK lanes share one key (16 dims each), so a warp handles 32 / LPK keys at
 // once for HB query heads; q waits in shared memory.
+// HBM bounds it with one query head per KV head (fp32, 32 rows of 4000 tokens, 8
+// heads of 128: 167 us, 6.3 TB/s), the instructions per key and head with more (32
+// heads on 8: 261 us, 4.0 TB/s; without the loads ahead and with each head's chain
+// by itself 289 us; 16 heads of 256 on one, 4 rows of 30000: 294 -> 209 us).
 // ---------------------------------------------------------------------------
 constexpr int kSimtWarps = 4;
 constexpr int kLaneDims = 16;
@@ -182,43 +186,88 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
   const T* kb = static_cast<const T*>(p.k) + hk * p.k_sh;
   const T* vb = static_cast<const T*>(p.v) + hk * p.v_sh;
   const int t0 = static_cast<int>(piece) * c, left = min(c, z.tiles - t0) * kTile;
-  for (int x0 = warp * kKeys; x0 < left; x0 += kSimtWarps * kKeys) {
+  // Two keys ahead: the page of key i + 2 and the key and value of i + 1 are on
+  // their way while key i is worked on.
+  constexpr int kStep = kSimtWarps * kKeys;
+  struct Place {
+    int page, slot;
+    bool on;
+  };
+  auto place_of = [&](int x0) {
+    Place w{0, 0, false};
+    if (x0 >= left) return w;
     const int x1 = x0 + sub;  // kKeys divides the tile: all of them lie in one
     const int pos = z.base(t0 + x1 / kTile) + x1 % kTile;
     const int col = page_of(p, pos);
-    bool on = z.sees(pos);
-    const int page = on ? p.table[z.row * p.t_sr + col] : 0;
-    if (page < 0 || page >= p.pages) {
+    w.on = z.sees(pos);
+    if (w.on) w.page = p.table[z.row * p.t_sr + col];
+    w.slot = pos - col * p.page_size;
+    return w;
+  };
+  auto load = [&](Place w, float (&kx)[kLaneDims], float (&vx)[kLaneDims]) {
+    if (w.page < 0 || w.page >= p.pages) {
       bad = 1;
-      on = false;
+      w.on = false;
     }
-    const int slot = pos - col * p.page_size;
-    float kx[kLaneDims], vx[kLaneDims];
-    load_dims<T, LPK, VEC>(kb + page * p.k_sp + slot * p.k_st, li, p.d, on, kx);
-    load_dims<T, LPK, VEC>(vb + page * p.v_sp + slot * p.v_st, li, p.dv, on, vx);
+    load_dims<T, LPK, VEC>(kb + w.page * p.k_sp + w.slot * p.k_st, li, p.d, w.on, kx);
+    load_dims<T, LPK, VEC>(vb + w.page * p.v_sp + w.slot * p.v_st, li, p.dv, w.on, vx);
+    return w.on;
+  };
+  auto take = [&](const float (&kx)[kLaneDims], const float (&vx)[kLaneDims], bool on) {
+    float s[HB];
 #pragma unroll
     for (int h = 0; h < HB; ++h) {
-      float s = 0.f;
+      float a = 0.f, b = 0.f;  // two chains
 #pragma unroll
-      for (int e = 0; e < kLaneDims; ++e) s = fmaf(qs[h][lane_dim<LPK, VEC>(li, e)], kx[e], s);
+      for (int e = 0; e < kLaneDims; e += 2) {
+        a = fmaf(qs[h][lane_dim<LPK, VEC>(li, e)], kx[e], a);
+        b = fmaf(qs[h][lane_dim<LPK, VEC>(li, e + 1)], kx[e + 1], b);
+      }
+      s[h] = a + b;
+    }
 #pragma unroll
-      for (int w = LPK / 2; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-      if (!on) s = -INFINITY;
-      const float top = fmaxf(m[h], s);
-      if (top > m[h]) {
-        const float f = exp2f(m[h] - top);
+    for (int w = LPK / 2; w > 0; w >>= 1)
+#pragma unroll
+      for (int h = 0; h < HB; ++h) s[h] += __shfl_xor_sync(0xffffffffu, s[h], w);
+    bool up = false;
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+      if (!on) s[h] = -INFINITY;
+      up |= s[h] > m[h];
+    }
+    if (__any_sync(0xffffffffu, up)) {  // a factor of 1 changes nothing
+#pragma unroll
+      for (int h = 0; h < HB; ++h) {
+        const float top = fmaxf(m[h], s[h]);
+        const float f = top > m[h] ? exp2f(m[h] - top) : 1.f;
         l[h] *= f;
 #pragma unroll
         for (int e = 0; e < kLaneDims; ++e) o[h][e] *= f;
         m[h] = top;
       }
-      const float w = s == -INFINITY ? 0.f : exp2f(s - top);
-      l[h] += w;
-      if (on) {
-#pragma unroll
-        for (int e = 0; e < kLaneDims; ++e) o[h][e] = fmaf(w, vx[e], o[h][e]);
-      }
     }
+#pragma unroll
+    for (int h = 0; h < HB; ++h) {
+      const float w = s[h] == -INFINITY ? 0.f : exp2f(s[h] - m[h]);
+      l[h] += w;
+      // the values of a key out of sight were loaded as zeros
+#pragma unroll
+      for (int e = 0; e < kLaneDims; ++e) o[h][e] = fmaf(w, vx[e], o[h][e]);
+    }
+  };
+  float kx[2][kLaneDims], vx[2][kLaneDims];
+  bool on[2];
+  int x0 = warp * kKeys;
+  on[0] = load(place_of(x0), kx[0], vx[0]);
+  Place then = place_of(x0 + kStep);
+  for (; x0 < left; x0 += 2 * kStep) {
+    on[1] = load(then, kx[1], vx[1]);
+    then = place_of(x0 + 2 * kStep);
+    take(kx[0], vx[0], on[0]);
+    if (x0 + kStep >= left) break;
+    on[0] = load(then, kx[0], vx[0]);
+    then = place_of(x0 + 3 * kStep);
+    take(kx[1], vx[1], on[1]);
   }
 
   // join the warp's key lanes (a fixed tree), then the warps in order
