@@ -276,3 +276,17 @@ def test_streams_and_graphs():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held, bio.paged_attention_decode_batch_invariant(*args))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 128, 256))
+def test_a_wide_table_changes_nothing(d, dtype):
+    """The pieces of a row are joined by a warp or by a block, depending on how
+    many pieces the table has room for; the bits do not depend on it."""
+    args = make([3000, 31, 0, 700, 9000], 8, 2, d, dtype=dtype, seed=d)
+    q, kp, vp, table, lens = args
+    out = bio.paged_attention_decode_batch_invariant(*args)
+    check(out, args)
+    wide = torch.full((5, 5000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    assert torch.equal(bio.paged_attention_decode_batch_invariant(q, kp, vp, wide, lens), out)

@@ -182,6 +182,40 @@ def test_fork_without_a_free_page_ends_at_the_last_whole_page():
     _lib.clear_device_status()
 
 
+@pytest.mark.parametrize("heads,d,dv,page", [(2, 64, 64, 16), (3, 33, 72, 7)])
+def test_many_branches_in_many_layers(heads, d, dv, page):
+    """More branches and layers than blocks run at once."""
+    c = cache(40, 200, page, heads, d, dv, rows=80, max_tokens=4 * page, dtype=torch.bfloat16)
+    lens = [page - 1, 2 * page, 3 * page - 2, 1]
+    c.extend(i32(0, 1, 2, 3), i32(*lens))
+    book, keys, values = book_of(c), c.key_pages.clone(), c.value_pages.clone()
+    src, dst = [i % 4 for i in range(64)], list(range(10, 74))
+    c.fork(i32(*src), i32(*dst))
+    for s, r in zip(src, dst):
+        book.fork([s], [r])
+    same(c, book)
+    for s, r in zip(src, dst):
+        for n in range(0, lens[s], page):
+            have = min(page, lens[s] - n)
+            a, b = c.page_table[s, n // page].item(), c.page_table[r, n // page].item()
+            assert torch.equal(c.key_pages[:, b, :, :have], keys[:, a, :, :have])
+            assert torch.equal(c.value_pages[:, b, :, :have], values[:, a, :, :have])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,d,dv,page", [(8, 128, 256, 64), (2, 256, 64, 256)])
+def test_compact_of_large_pages(heads, d, dv, page, dtype):
+    """Pages of more bytes than a block copies at once."""
+    c = cache(3, 30, page, heads, d, dv, rows=4, max_tokens=12 * page, dtype=dtype)
+    c.extend(i32(0, 1, 2), i32(4 * page, 5 * page - 3, 9 * page))
+    c.free(i32(1))
+    book = book_of(c)
+    out, live = c.compact(16), book.compact(16)
+    same(out, book)
+    assert torch.equal(out.key_pages[:, :len(live)], c.key_pages[:, live])
+    assert torch.equal(out.value_pages[:, :len(live)], c.value_pages[:, live])
+
+
 def test_free_ignores_repeated_rows():
     c = cache(1, 10, 4, 1, 8, rows=3, max_tokens=16)
     c.extend(i32(0, 1), i32(9, 9))
