@@ -224,63 +224,84 @@ def varlen(q, k, v, cu_q, cu_k, *, is_causal, causal_name, scale):
 _WINDOW_ARGS = struct.Struct("@ii4P17qiifiiiP4qPPiqP")
 
 
-@functools.lru_cache(maxsize=1024)
-def _tma_strides(shape, stride) -> bool:
-    """Whether every stride that is used is a multiple of 16 bytes of 16-bit elements."""
-    return stride[-1] == 1 and all(n < 2 or s % 8 == 0 for n, s in zip(shape[:-1], stride[:-1]))
-
-
 def _window_operand(t, lead):
     """`t` as [B, H, L, D] with D contiguous, packed where TMA needs it."""
     if len(lead) != 1:
         t = t.reshape(math.prod(lead), *t.shape[-3:])
-    if t.dtype == torch.float32:
-        return _dim_contiguous(t)
-    if t.data_ptr() % 16 == 0 and _tma_strides(t.shape, t.stride()):
-        return t
-    return _tma_ready(_dim_contiguous(t))
+    t = _dim_contiguous(t)
+    return t if t.dtype == torch.float32 else _tma_ready(t)
 
 
-def _window_args(q, k, v, out, strides, batch, heads, kv_heads, lq, lk, d, dv, scale,
-                 cu_q=None, cu_k=None):
-    many = (0, 0, 0, 0) if cu_q is None else (
-        cu_q.data_ptr(), cu_k.data_ptr(), 1 if cu_q.dtype == torch.int64 else 0, cu_q.numel() - 1)
-    return _WINDOW_ARGS.pack(
-        _lib.DTYPE_CODE[q.dtype], q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        out.data_ptr(), *strides, batch, heads, kv_heads, lq, lk, d, dv,
-        scale if scale is not None else 1.0 / math.sqrt(d), 0, MASK_NONE, 0, 0, 0, 0, 0, 0,
-        *many, 0)
+def geometry(t: torch.Tensor) -> tuple:
+    return t.shape, t.stride(), t.dtype, t.get_device()
 
 
-def window(q, k, v, window, sinks, scale):
+class WindowPlan:
+    """What a dense call needs to know about its operands' geometry."""
+
+    def __init__(self, q, k, v):
+        (qs, q_stride, dtype, device), (ks, k_stride, _, _), (vs, v_stride, _, _) = q, k, v
+        self.lead = qs[:-3]
+        nb = math.prod(self.lead)
+        h, lq, d = qs[-3:]
+        hkv, lk, dv = ks[-3], ks[-2], vs[-1]
+        self.kind = (_lib.DTYPE_CODE[dtype], device)
+        self.sizes = (nb, h, hkv, lq, lk, d, dv)
+        self.out_shape = (nb, lq, h, dv)  # token-major like the output of sdpa
+        self.empty = 0 in self.out_shape
+        self.out_strides = (lq * h * dv, dv, h * dv)
+        self.scale = 1.0 / math.sqrt(d)
+        # operands that are read where they lie: 16-byte strides for the 16-bit types
+        half = dtype != torch.float32
+        self.in_place = len(qs) == 4 and all(
+            stride[-1] == 1 and (not half or all(n < 2 or s % 8 == 0
+                                                 for n, s in zip(shape[:-1], stride[:-1])))
+            for shape, stride in ((qs, q_stride), (ks, k_stride), (vs, v_stride)))
+        self.align = 16 if half else 4
+        self.strides = (*q_stride[-4:-1], *k_stride[-4:-1], *v_stride[-4:-1])
+
+
+_NO_MASK = (0, MASK_NONE, 0, 0, 0, 0, 0, 0)
+
+
+def window(q, k, v, window, sinks, scale, plan):
     """q [..., H, Lq, D], k [..., Hkv, Lk, D], v [..., Hkv, Lk, Dv] -> [..., H, Lq, Dv]."""
-    lead = q.shape[:-3]
-    h, lq, d = q.shape[-3:]
-    hkv, lk, dv = k.shape[-3], k.shape[-2], v.shape[-1]
-    nb = math.prod(lead)
-    q4, k4, v4 = _window_operand(q, lead), _window_operand(k, lead), _window_operand(v, lead)
-    # token-major like the output of sdpa
-    out = q.new_empty((nb, lq, h, dv)).transpose(1, 2)
-    result = out if len(lead) == 1 else out.reshape(*lead, h, lq, dv)
-    if out.numel() == 0:
+    out = q.new_empty(plan.out_shape).transpose(1, 2)
+    result = out if len(plan.lead) == 1 else out.reshape(*plan.lead, *out.shape[1:])
+    if plan.empty:
         return result
-    args = _window_args(q4, k4, v4, out, (*q4.stride()[:3], *k4.stride()[:3], *v4.stride()[:3],
-                                          *out.stride()[:3]), nb, h, hkv, lq, lk, d, dv, scale)
+    strides, where = plan.strides, (q.data_ptr(), k.data_ptr(), v.data_ptr())
+    if not plan.in_place or (where[0] | where[1] | where[2]) % plan.align:
+        q, k, v = (_window_operand(t, plan.lead) for t in (q, k, v))
+        strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        where = (q.data_ptr(), k.data_ptr(), v.data_ptr())
+    args = _WINDOW_ARGS.pack(*plan.kind, *where, out.data_ptr(), *strides, *plan.out_strides,
+                             *plan.sizes, plan.scale if scale is None else scale, *_NO_MASK,
+                             0, 0, 0, 0, 0)
     pushed = False
     if tracing.active():
+        nb, h, hkv, lq, lk, d, dv = plan.sizes
         seen = min(lk, window + sinks)
         pushed = tracing.note(
             "window_attention", f"bio_attention_window [B={nb}, H={h}/{hkv}, Lq={lq}, "
             f"Lk={lk}, D={d}/{dv}, window={window}, sinks={sinks}]",
             2.0 * nb * h * lq * seen * (d + dv),
-            q.element_size() * (q4.numel() + k4.numel() + v4.numel() + out.numel()),
-            q.element_size())
+            q.element_size() * nb * (h * lq * (d + dv) + hkv * lk * (d + dv)), q.element_size())
     try:
         _lib.check(_lib.load().bio_attention_window(args, window, sinks, _lib.stream_of(q)),
                    "bio_attention_window")
     finally:
         tracing.done(pushed)
     return result
+
+
+def _window_args(q, k, v, out, strides, batch, heads, kv_heads, lq, lk, d, dv, scale, cu_q, cu_k):
+    return _WINDOW_ARGS.pack(
+        _lib.DTYPE_CODE[q.dtype], q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        out.data_ptr(), *strides, batch, heads, kv_heads, lq, lk, d, dv,
+        scale if scale is not None else 1.0 / math.sqrt(d), *_NO_MASK,
+        cu_q.data_ptr(), cu_k.data_ptr(), 1 if cu_q.dtype == torch.int64 else 0,
+        cu_q.numel() - 1, 0)
 
 
 def window_varlen(q, k, v, cu_q, cu_k, window, sinks, scale):

@@ -439,13 +439,27 @@ def _check_window_shapes(query, key, value, dtypes, heads_dim, tokens_dim):
     _attn._check_head_dims(query[-1], value[-1])
 
 
-def _check_window(query, key, value, window, sinks, heads_dim, tokens_dim):
-    _check_window_shapes(query.shape, key.shape, value.shape,
-                         (query.dtype, key.dtype, value.dtype), heads_dim, tokens_dim)
+def _check_window(window, sinks):
     if not 1 <= window <= 2147483647:
         raise ValueError("window must be at least 1 and fit in 32 bits")
     if not 0 <= sinks <= 2147483647:
         raise ValueError("sinks must not be negative and fit in 32 bits")
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_plan(query, key, value):
+    """Checks and sizes of a dense call, worked out once per geometry."""
+    q, k, v = query[0], key[0], value[0]
+    if len(q) < 3 or len(k) != len(q) or len(v) != len(q):
+        raise ValueError("query, key, and value must be [..., heads, tokens, head_dim]")
+    if q[:-3] != k[:-3] or q[:-3] != v[:-3]:
+        raise ValueError("query, key, and value batch dimensions must match")
+    _check_window_shapes(q, k, v, (query[2], key[2], value[2]), -3, -2)
+    if min(query[3], key[3], value[3]) < 0:
+        raise AssertionError("batch-invariant operators require CUDA tensors")
+    if query[3] != key[3] or query[3] != value[3]:
+        raise ValueError("query, key, and value must be on the same CUDA device")
+    return _attn.WindowPlan(query, key, value)
 
 
 def sliding_window_attention_batch_invariant(
@@ -468,13 +482,9 @@ def sliding_window_attention_batch_invariant(
     sinks).  A row's bits depend on its own query, keys and values only.  An
     addition: the reference's SDPA (:1148-1213) would need the mask as a tensor
     and visits every key."""
-    if query.ndim < 3 or key.ndim != query.ndim or value.ndim != query.ndim:
-        raise ValueError("query, key, and value must be [..., heads, tokens, head_dim]")
-    if query.shape[:-3] != key.shape[:-3] or query.shape[:-3] != value.shape[:-3]:
-        raise ValueError("query, key, and value batch dimensions must match")
-    _check_window(query, key, value, window, sinks, -3, -2)
-    _require_cuda(query, key, value)
-    return _attn.window(query, key, value, window, sinks, scale)
+    _check_window(window, sinks)
+    plan = _window_plan(_attn.geometry(query), _attn.geometry(key), _attn.geometry(value))
+    return _attn.window(query, key, value, window, sinks, scale, plan)
 
 
 def varlen_sliding_window_attention_batch_invariant(
@@ -497,7 +507,9 @@ def varlen_sliding_window_attention_batch_invariant(
         raise ValueError("varlen attention expects rank-4 query, key, and value")
     if query.shape[0] != 1 or key.shape[0] != 1 or value.shape[0] != 1:
         raise ValueError("varlen attention expects sequence-packed batch size 1")
-    _check_window(query, key, value, window, sinks, 2, 1)
+    _check_window_shapes(query.shape, key.shape, value.shape,
+                         (query.dtype, key.dtype, value.dtype), 2, 1)
+    _check_window(window, sinks)
     if cumulative_seqlen_q.ndim != 1 or cumulative_seqlen_kv.ndim != 1:
         raise ValueError("cumulative sequence lengths must be rank 1")
     integer_dtypes = {torch.int32, torch.int64}
