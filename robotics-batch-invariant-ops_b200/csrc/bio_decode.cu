@@ -38,6 +38,7 @@ struct PagedParams {
   unsigned page_mul, page_shift;  // position / page size = (mulhi(position, mul) + position) >> shift
   float scale_log2;
   int64_t max_pieces;  // most pieces that any row can have
+  int least;           // tiles of a piece at least: 1, or kSimtTiles
   int dvp;             // floats between partial outputs
   float* acc;          // [batch * heads][max_pieces][dvp]
   float2* ml;          // [batch * heads][max_pieces]: maximum, sum (-1: refused)
@@ -48,13 +49,14 @@ constexpr int kTile = 32;  // tokens of a tile
 
 // Tiles of a piece of a row of n tiles.  Short pieces spread one sequence over
 // the SMs; long rows take longer ones, since every piece costs a write and a
-// read of its fp32 output.
-__host__ __device__ __forceinline__ int piece_tiles(int n) {
-  return n <= 32 ? 1 : n <= 64 ? 2 : n <= 256 ? 8 : 16;
+// read of its fp32 output.  `least` is what the kernel's way of working asks for.
+__host__ __device__ __forceinline__ int piece_tiles(int n, int least) {
+  const int c = n <= 32 ? 1 : n <= 64 ? 2 : n <= 256 ? 8 : 16;
+  return c > least ? c : least;
 }
 
-__host__ __device__ __forceinline__ int pieces_of(int tiles) {
-  const int c = piece_tiles(tiles);
+__host__ __device__ __forceinline__ int pieces_of(int tiles, int least) {
+  const int c = piece_tiles(tiles, least);
   return (tiles + c - 1) / c;
 }
 
@@ -101,11 +103,15 @@ __device__ __forceinline__ Visible visible_of(const PagedParams& p, int2 row_len
 // LPK lanes share one key (16 dims each), so a warp handles 32 / LPK keys at
 // once for HB query heads; q waits in shared memory.
 // HBM bounds it with one query head per KV head (fp32, 32 rows of 4000 tokens, 8
-// heads of 128: 167 us, 6.3 TB/s), the instructions per key and head with more (32
-// heads on 8: 261 us, 4.0 TB/s; without the loads ahead and with each head's chain
-// by itself 289 us; 16 heads of 256 on one, 4 rows of 30000: 294 -> 209 us).
+// heads of 128: 166 us, 6.3 TB/s), the instructions per key and head with more (32
+// heads on 8: 252 us, 4.2 TB/s; without the loads ahead and with each head's chain
+// by itself 289 us; 16 heads of 256 on one, 4 rows of 30000: 294 -> 208 us).  A
+// block's start and its warps' join cost as much as some hundred keys, so a piece
+// has kSimtTiles tiles at least, and 64 columns take 4 lanes, not 8 (128 heads on
+// 8, 20 rows of 1108: 275 -> 153 us).
 // ---------------------------------------------------------------------------
 constexpr int kSimtWarps = 4;
+constexpr int kSimtTiles = 4;  // a tile for each warp of a piece's block at least
 constexpr int kLaneDims = 16;
 
 // Dim of element e of lane li: four-float groups (VEC) or single elements.
@@ -162,7 +168,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
   const int nh = min(HB, p.group - hb * HB);
 
   const Visible z = visible_of(p, row_of(p, b));
-  const int c = piece_tiles(z.tiles), pieces = pieces_of(z.tiles);
+  const int c = piece_tiles(z.tiles, p.least), pieces = pieces_of(z.tiles, p.least);
   if (piece > 0 && piece >= pieces) return;
   int bad = z.row < 0;
 
@@ -478,7 +484,7 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
       int mine = 0;
       if (b < batch) {
         rows[b] = row_of(p, b);
-        mine = max(1, pieces_of(visible_of(p, rows[b]).tiles)) * hgs;
+        mine = max(1, pieces_of(visible_of(p, rows[b]).tiles, 1)) * hgs;
       }
       int inc = mine;
 #pragma unroll
@@ -530,8 +536,8 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
     it.h0 = it.hk * p.group + before;
     it.nh = min(HB, p.group - before);
     it.z = visible_of(p, row);
-    const int c = piece_tiles(it.z.tiles);
-    it.pieces = max(1, pieces_of(it.z.tiles));
+    const int c = piece_tiles(it.z.tiles, 1);
+    it.pieces = max(1, pieces_of(it.z.tiles, 1));
     it.t0 = it.piece * c;
     it.tiles = max(0, min(c, it.z.tiles - it.t0));
   };
@@ -843,7 +849,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
   if (bh >= outputs) return;  // only without SPREAD
   const int64_t b = bh / p.heads, h = bh - b * p.heads;
   // lengths were there before the kernel that this one waits for began
-  const int pieces = pieces_of(visible_of(p, row_of(p, b)).tiles);
+  const int pieces = pieces_of(visible_of(p, row_of(p, b)).tiles, p.least);
   if (pieces <= 1) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float2* ml = p.ml + bh * p.max_pieces;
@@ -936,17 +942,18 @@ namespace {
 constexpr int64_t kMaxGrid = 2147483647;
 
 // Most pieces that a row of up to `most` tiles can have.
-int64_t most_pieces(int64_t most) {
+int64_t most_pieces(int64_t most, int least) {
   int64_t pieces = 1;
   for (int64_t top : {static_cast<int64_t>(32), static_cast<int64_t>(64),
                       static_cast<int64_t>(256), most}) {
-    const int64_t k = bio::pieces_of(static_cast<int>(top < most ? top : most));
+    const int64_t k = bio::pieces_of(static_cast<int>(top < most ? top : most), least);
     if (k > pieces) pieces = k;
   }
   return pieces;
 }
 
 struct Split {
+  int64_t most;    // tiles that any row can have
   int64_t pieces;
   int dvp;
   int64_t acc_bytes, bytes;
@@ -965,7 +972,8 @@ int split_of(const bio_paged_attn_args* a, Split* s) {
   int64_t most = (a->table_width * a->page_size + T - 1) / T;
   if (a->window > 0)  // the window's tiles, one more where it starts inside one, the sinks'
     most = std::min(most, (a->window + T - 1) / T + 1 + (a->sinks + T - 1) / T);
-  s->pieces = most_pieces(most);
+  s->most = most;
+  s->pieces = most_pieces(most, 1);  // longer pieces need less
   s->dvp = (a->dv + 3) / 4 * 4;
   if (a->batch > kMaxGrid / a->heads || a->batch * a->heads > kMaxGrid / s->pieces)
     return BIO_ERR_SHAPE;
@@ -983,14 +991,22 @@ int launch_simt(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
   return bio_host::launch_status(cudaGetLastError());
 }
 
-template <typename T, bool VEC>
+template <typename T, int LPK, bool VEC>
 int dispatch_simt(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
-  const bool wide = p.d > 128 || p.dv > 128;
-  if (p.group >= 3)
-    return wide ? launch_simt<T, 4, 16, VEC>(p, batch, s) : launch_simt<T, 4, 8, VEC>(p, batch, s);
-  if (p.group == 2)
-    return wide ? launch_simt<T, 2, 16, VEC>(p, batch, s) : launch_simt<T, 2, 8, VEC>(p, batch, s);
-  return wide ? launch_simt<T, 1, 16, VEC>(p, batch, s) : launch_simt<T, 1, 8, VEC>(p, batch, s);
+  if (p.group >= 3) return launch_simt<T, 4, LPK, VEC>(p, batch, s);
+  if (p.group == 2) return launch_simt<T, 2, LPK, VEC>(p, batch, s);
+  return launch_simt<T, 1, LPK, VEC>(p, batch, s);
+}
+
+// As many lanes per key as its columns fill.
+template <typename T, bool VEC>
+int run_simt(bio::PagedParams* p, int64_t batch, int64_t most, cudaStream_t s) {
+  p->least = bio::kSimtTiles;
+  p->max_pieces = most_pieces(most, p->least);
+  const int dim = std::max(p->d, p->dv);
+  return dim > 128  ? dispatch_simt<T, 16, VEC>(*p, batch, s)
+         : dim > 64 ? dispatch_simt<T, 8, VEC>(*p, batch, s)
+                    : dispatch_simt<T, 4, VEC>(*p, batch, s);
 }
 
 template <typename T, int DP, int NH>
@@ -1043,14 +1059,15 @@ int dispatch_mma(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
 }
 
 template <typename T>
-int run(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
+int run(bio::PagedParams p, int64_t batch, int64_t most, cudaStream_t s) {
   int st;
+  p.least = 1;
   if constexpr (sizeof(T) == 4) {
     const uint64_t bits = reinterpret_cast<uint64_t>(p.k) | reinterpret_cast<uint64_t>(p.v) |
                           4 * static_cast<uint64_t>(p.k_sp | p.k_sh | p.k_st | p.v_sp | p.v_sh |
                                                     p.v_st | p.d | p.dv);
-    st = bits % 16 == 0 ? dispatch_simt<T, true>(p, batch, s)
-                        : dispatch_simt<T, false>(p, batch, s);
+    st = bits % 16 == 0 ? run_simt<T, true>(&p, batch, most, s)
+                        : run_simt<T, false>(&p, batch, most, s);
   } else {
     const uint64_t bits = reinterpret_cast<uint64_t>(p.q) | reinterpret_cast<uint64_t>(p.k) |
                           reinterpret_cast<uint64_t>(p.v) |
@@ -1058,7 +1075,7 @@ int run(const bio::PagedParams& p, int64_t batch, cudaStream_t s) {
                                                     p.v_sp | p.v_sh | p.v_st | p.d | p.dv);
     st = bits % 16 == 0 ? dispatch_mma<T>(p, batch, s) : BIO_ERR_ALIGN;
     // rows off a 16-byte boundary, or strides that no tensor map takes
-    if (st == BIO_ERR_ALIGN) st = dispatch_simt<T, false>(p, batch, s);
+    if (st == BIO_ERR_ALIGN) st = run_simt<T, false>(&p, batch, most, s);
   }
   if (st != BIO_OK || p.max_pieces == 1) return st;
   const bool spread = p.max_pieces > bio::kSpreadPieces, wide = p.dvp > 128;
@@ -1136,9 +1153,9 @@ int bio_paged_attention(const bio_paged_attn_args* a, void* workspace, int64_t w
   p.status = bio_host::status_word(a->device);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
-    case BIO_F32: return run<float>(p, a->batch, cs);
-    case BIO_F16: return run<__half>(p, a->batch, cs);
-    case BIO_BF16: return run<__nv_bfloat16>(p, a->batch, cs);
+    case BIO_F32: return run<float>(p, a->batch, s.most, cs);
+    case BIO_F16: return run<__half>(p, a->batch, s.most, cs);
+    case BIO_BF16: return run<__nv_bfloat16>(p, a->batch, s.most, cs);
     default: return BIO_ERR_DTYPE;
   }
 }
