@@ -13,7 +13,6 @@ tensor or host synchronisation is needed.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 import struct
 
