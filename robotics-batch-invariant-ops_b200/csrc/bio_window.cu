@@ -12,6 +12,7 @@
 // need the mask as a tensor and visits every key.
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "bio_tile.cuh"
 
@@ -907,10 +908,18 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
 // the 16 threads of a row share its maximum and sum by shuffles, the weights go
 // through shared memory, and it accumulates 4 rows x 4 columns per 64 columns of
 // O.  V of a block and K of the next one are copied (cp.async) while the
-// products before them run.  FFMA bounds it: 64 products per 8 shared loads of
-// 16 bytes in S, 128 per 12 in PV.  Rows that come out not finite are computed
-// once more from their visible keys alone, as above.
+// products before them run.  FFMA and the shared loads that feed it bound it: 64
+// products per 8 loads of 16 bytes in S, 128 per 12 in PV.  Columns that no row of
+// the tile sees are skipped 32 at a time.  Rows that come out not finite are
+// computed once more from their visible keys alone, as above.
+// Measured: 94 us for 1024 queries, 8 heads over 2 of 128, window 512 (17 TFLOP/s;
+// one warp per row, with K read from L2 for every row, ran at 1).  A window of 31
+// keys (4 x 10198 queries, 8 heads of 128) wastes most of its blocks: 1074 us, and
+// 1609 with whole blocks and with queries and outputs moved by words.
 // ---------------------------------------------------------------------------
+// what lies on 16-byte borders
+constexpr int kVecKv = 1, kVecQ = 2, kVecO = 4;
+
 template <int DP>
 struct WinF32 {
   static constexpr int BN = DP == 256 ? 32 : 64;
@@ -931,21 +940,21 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int by
                  : "memory");
 }
 
-// rows x cols floats of `src` (row stride in elements) into dst [rows][pitch]; rows
-// from `have` on and columns from cols to DP are zeros.
+// Rows [r0, r1) of `src` (row stride in elements, cols floats) into dst [..][pitch];
+// rows from `have` on and columns from cols to DP are zeros.
 template <int DP>
-__device__ __forceinline__ void copy_tile(float* dst, int pitch, int rows, const float* src,
+__device__ __forceinline__ void copy_tile(float* dst, int pitch, int r0, int r1, const float* src,
                                           int64_t stride, int have, int cols, bool vec) {
   const uint32_t d = smem_u32(dst);
   if (vec) {
-    for (int x = threadIdx.x; x < rows * (DP / 4); x += 256) {
-      const int r = x / (DP / 4), c = x % (DP / 4) * 4;
+    for (int x = threadIdx.x; x < (r1 - r0) * (DP / 4); x += 256) {
+      const int r = r0 + x / (DP / 4), c = x % (DP / 4) * 4;
       const bool on = r < have && c < cols;
       copy_async(d + (r * pitch + c) * 4, on ? src + r * stride + c : src, 16, on);
     }
   } else {
-    for (int x = threadIdx.x; x < rows * DP; x += 256) {
-      const int r = x / DP, c = x % DP;
+    for (int x = threadIdx.x; x < (r1 - r0) * DP; x += 256) {
+      const int r = r0 + x / DP, c = x % DP;
       const bool on = r < have && c < cols;
       copy_async(d + (r * pitch + c) * 4, on ? src + r * stride + c : src, 4, on);
     }
@@ -977,15 +986,19 @@ __global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, c
   if (threadIdx.x < 2) redo[threadIdx.x] = 0;
 
   // queries: row r is head r / tok, token r % tok
-  for (int x = threadIdx.x; x < 64 * DP; x += 256) {
-    const int r = x / DP, c = x % DP, h = r / w.tok, t = r - h * w.tok;
-    sq[r * L::kPitch + c] =
-        h < j.nh && t < tile.n && c < p.d ? q[h * p.q_sh + t * p.q_st + c] : 0.f;
+  const int wide_q = vec & kVecQ ? 4 : 1;
+  for (int x = threadIdx.x; x < 64 * DP / wide_q; x += 256) {
+    const int r = x * wide_q / DP, c = x * wide_q % DP, h = r / w.tok, t = r - h * w.tok;
+    const bool on = h < j.nh && t < tile.n && c < p.d;
+    copy_async(smem_u32(sq + r * L::kPitch + c), on ? q + h * p.q_sh + t * p.q_st + c : q,
+               4 * wide_q, on);
   }
   auto first_of = [&](int i) { return (i < j.head ? i : i + j.jump) * BN; };
   auto load = [&](float* dst, const float* src, int64_t stride, int i, int cols) {
     const int at = first_of(i);
-    copy_tile<DP>(dst, L::kPitch, BN, src + at * stride, stride, min(BN, j.lk - at), cols, vec);
+    const int2 span = window_span<BN>(j, tile, i);
+    copy_tile<DP>(dst, L::kPitch, span.x, span.y, src + at * stride, stride, min(BN, j.lk - at),
+                  cols, (vec & kVecKv) != 0);
   };
   float m[4], l[4], acc[4][NO][4];
 #pragma unroll
@@ -1007,25 +1020,37 @@ __global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, c
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int c = 0; c < NC; ++c) s[a][c] = 0.f;
+    // the 32-key columns that some row sees
+    const int2 span = window_span<BN>(j, tile, i);
+    auto scores = [&](auto from, auto to) {
+      constexpr int C0 = decltype(from)::value, C1 = decltype(to)::value;
 #pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
-      float4 x[4], y[NC];
+      for (int d = 0; d < DP; d += 4) {
+        float4 x[4], y[NC];
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
-        x[a] = *reinterpret_cast<const float4*>(sq + (ty * 4 + a) * L::kPitch + d);
+        for (int a = 0; a < 4; ++a)
+          x[a] = *reinterpret_cast<const float4*>(sq + (ty * 4 + a) * L::kPitch + d);
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        y[c] = *reinterpret_cast<const float4*>(sk + (tx + 16 * c) * L::kPitch + d);
+        for (int c = C0; c < C1; ++c)
+          y[c] = *reinterpret_cast<const float4*>(sk + (tx + 16 * c) * L::kPitch + d);
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < 4; ++a)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          s[a][c] = fmaf(x[a].x, y[c].x, s[a][c]);
-          s[a][c] = fmaf(x[a].y, y[c].y, s[a][c]);
-          s[a][c] = fmaf(x[a].z, y[c].z, s[a][c]);
-          s[a][c] = fmaf(x[a].w, y[c].w, s[a][c]);
-        }
-    }
+          for (int c = C0; c < C1; ++c) {
+            s[a][c] = fmaf(x[a].x, y[c].x, s[a][c]);
+            s[a][c] = fmaf(x[a].y, y[c].y, s[a][c]);
+            s[a][c] = fmaf(x[a].z, y[c].z, s[a][c]);
+            s[a][c] = fmaf(x[a].w, y[c].w, s[a][c]);
+          }
+      }
+    };
+    using std::integral_constant;
+    if (BN == 32 || span.y - span.x > 32)
+      scores(integral_constant<int, 0>{}, integral_constant<int, NC>{});
+    else if (span.x == 0)
+      scores(integral_constant<int, 0>{}, integral_constant<int, 2>{});
+    else
+      scores(integral_constant<int, NC - 2>{}, integral_constant<int, NC>{});
     const int key0 = first_of(i);
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -1063,7 +1088,7 @@ __global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, c
     __syncthreads();                                       // and nobody needs the keys any more
     if (i + 1 < j.blocks) load(sk, k, p.k_st, i + 1, p.d);
 #pragma unroll 2
-    for (int n = 0; n < BN; n += 4) {
+    for (int n = span.x; n < span.y; n += 4) {
       float4 x[4];
 #pragma unroll
       for (int a = 0; a < 4; ++a)
@@ -1087,21 +1112,30 @@ __global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, c
     }
     __syncthreads();  // the values and the weights may be overwritten
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  asm volatile("cp.async.wait_all;" ::: "memory");  // a job without keys, too
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
     const int r = ty * 4 + a, h = r / w.tok, t = r - h * w.tok;
     if (h >= j.nh || t >= tile.n) continue;
     float odd = 0.f;
+    float* row = o + h * p.o_sh + t * p.o_st;
 #pragma unroll
-    for (int c = 0; c < NO; ++c)
+    for (int c = 0; c < NO; ++c) {
+      const int col = c * 64 + tx * 4;
+      float y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int col = c * 64 + tx * 4 + e;
-        const float y = l[a] == 0.f ? 0.f : acc[a][c][e] / l[a];
-        odd = fmaf(y, 0.f, odd);
-        if (col < p.dv) o[h * p.o_sh + t * p.o_st + col] = y;
+        y[e] = l[a] == 0.f ? 0.f : acc[a][c][e] / l[a];
+        odd = fmaf(y[e], 0.f, odd);
       }
+      if ((vec & kVecO) != 0 && col < p.dv) {
+        *reinterpret_cast<float4*>(row + col) = make_float4(y[0], y[1], y[2], y[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < p.dv) row[col + e] = y[e];
+      }
+    }
     if (!(odd == 0.f)) atomicOr(&redo[r >> 5], 1u << (r & 31));
   }
   __syncthreads();
@@ -1159,11 +1193,16 @@ int launch_f32(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t 
   bio::WindowJobs w;
   const int st = plan_jobs(p, a, PACKED, 64, 1, &w);
   if (st != BIO_OK) return st;
-  const uint64_t bits = reinterpret_cast<uint64_t>(p.k) | reinterpret_cast<uint64_t>(p.v) |
-                        4 * static_cast<uint64_t>(p.k_sb | p.k_sh | p.k_st | p.v_sb | p.v_sh |
-                                                  p.v_st | p.d | p.dv);
-  bio::window_f32_kernel<DP, PACKED><<<static_cast<unsigned>(w.jobs), 256, L::kBytes, s>>>(
-      p, w, bits % 16 == 0 ? 1 : 0);
+  auto on16 = [](const void* x, int64_t strides) {
+    return (reinterpret_cast<uint64_t>(x) | 4 * static_cast<uint64_t>(strides)) % 16 == 0;
+  };
+  int vec = 0;
+  if (on16(p.k, p.k_sb | p.k_sh | p.k_st | p.d) && on16(p.v, p.v_sb | p.v_sh | p.v_st | p.dv))
+    vec |= bio::kVecKv;
+  if (on16(p.q, p.q_sb | p.q_sh | p.q_st | p.d)) vec |= bio::kVecQ;
+  if (on16(p.o, p.o_sb | p.o_sh | p.o_st | p.dv)) vec |= bio::kVecO;
+  bio::window_f32_kernel<DP, PACKED><<<static_cast<unsigned>(w.jobs), 256, L::kBytes, s>>>(p, w,
+                                                                                           vec);
   return bio_host::launch_status(cudaGetLastError());
 }
 
