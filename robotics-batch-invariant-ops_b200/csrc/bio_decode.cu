@@ -846,12 +846,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
   __shared__ float4 part[SPREAD ? kJoinWarps : 1][32 * G];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t bh = SPREAD ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp;
-  if (bh >= outputs) return;  // only without SPREAD
-  const int64_t b = bh / p.heads, h = bh - b * p.heads;
+  const int64_t b = min(bh, outputs - 1) / p.heads, h = bh - b * p.heads;
   // lengths were there before the kernel that this one waits for began
   const int pieces = pieces_of(visible_of(p, row_of(p, b)).tiles, p.least);
-  if (pieces <= 1) return;
+  // Every thread waits, also where nothing is left to join: what comes next on the
+  // stream waits for this grid alone, and rows of one piece are written by the other.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (bh >= outputs || pieces <= 1) return;  // bh: only without SPREAD
   const float2* ml = p.ml + bh * p.max_pieces;
   const int groups = p.dvp / 4;  // four-float groups of an output row
   const float4* acc = reinterpret_cast<const float4*>(p.acc + bh * p.max_pieces * p.dvp);

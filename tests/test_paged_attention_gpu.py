@@ -290,3 +290,25 @@ def test_a_wide_table_changes_nothing(d, dtype):
     wide = torch.full((5, 5000), -1, dtype=torch.int32, device="cuda")
     wide[:, :table.shape[1]] = table
     assert torch.equal(bio.paged_attention_decode_batch_invariant(q, kp, vp, wide, lens), out)
+
+
+@pytest.mark.parametrize("dtype,longest", [(torch.bfloat16, 32), (torch.float16, 32),
+                                           (torch.float32, 128)])
+def test_rows_of_one_piece_are_written_before_the_next_kernel_reads(dtype, longest):
+    """A table with room for many pieces whose rows have one each: nothing is left
+    to join, and what follows in the graph or on the stream reads finished rows."""
+    lens = [longest] * 200 + [0, 1, longest - 1, longest]
+    q, kp, vp, table, ln = make(lens, 32, 2, 128, dtype=dtype, width=256)
+    want = bio.paged_attention_decode_batch_invariant(q, kp, vp, table[:, :longest // 16], ln)
+    check(want[-6:], (q[-6:], kp, vp, table[-6:], ln[-6:]))
+    given, read = torch.zeros_like(q), torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        read.copy_(bio.paged_attention_decode_batch_invariant(given, kp, vp, table, ln))
+    given.copy_(q)
+    for turn in range(100):
+        read.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(read, want), f"replay {turn}"
+        got = bio.paged_attention_decode_batch_invariant(q, kp, vp, table, ln) + 0
+        assert torch.equal(got, want), f"call {turn}"
