@@ -1239,13 +1239,15 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
   CUtensorMap q, k, v;
   const int64_t batch = packed ? 1 : p.batch;
   // without keys nothing is read through K and V: any operand will do for their maps
-  const bool none = p.lk == 0;
+  auto keys_map = [&](CUtensorMap* map, const void* x, int64_t cols, int64_t st, int64_t sh,
+                      int64_t sb) {
+    return p.lk == 0 ? bio_host::map_of<T>(map, p.q, p.d, 1, 1, 1, 0, 0, 0, L::BN)
+                     : bio_host::map_of<T>(map, x, cols, p.lk, a->kv_heads, batch, st, sh, sb, L::BN);
+  };
   if (!bio_host::map_of<T>(&q, p.q, p.d, p.lq, p.heads, batch, p.q_st, p.q_sh, p.q_sb, w.tok,
                            w.gh) ||
-      !bio_host::map_of<T>(&k, none ? p.q : p.k, p.d, none ? 1 : p.lk, a->kv_heads, batch, p.k_st,
-                           p.k_sh, p.k_sb, L::BN) ||
-      !bio_host::map_of<T>(&v, none ? p.q : p.v, p.dv, none ? 1 : p.lk, a->kv_heads, batch, p.v_st,
-                           p.v_sh, p.v_sb, L::BN))
+      !keys_map(&k, p.k, p.d, p.k_st, p.k_sh, p.k_sb) ||
+      !keys_map(&v, p.v, p.dv, p.v_st, p.v_sh, p.v_sb))
     return BIO_ERR_ALIGN;
   const unsigned grid = static_cast<unsigned>(std::min(w.jobs, sms));
   bio::window_tc_kernel<T, DP, PACKED><<<grid, L::kThreads, L::kBytes, s>>>(q, k, v, p, w);
@@ -1254,10 +1256,15 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
 
 template <typename T>
 int launch_half(const bio::WindowParams& p, const bio_attn_args* a, bool packed, cudaStream_t s) {
-  const uint64_t bits = reinterpret_cast<uint64_t>(p.q) | reinterpret_cast<uint64_t>(p.k) |
-                        reinterpret_cast<uint64_t>(p.v) |
-                        2 * static_cast<uint64_t>(p.q_sb | p.q_sh | p.q_st | p.k_sb | p.k_sh |
-                                                  p.k_st | p.v_sb | p.v_sh | p.v_st);
+  // the stride of a dimension of one element is never used
+  const int64_t batch = packed ? 1 : p.batch;
+  auto used = [](int64_t n, int64_t stride) { return 2 * static_cast<uint64_t>(n > 1 ? stride : 0); };
+  uint64_t bits = reinterpret_cast<uint64_t>(p.q) | used(batch, p.q_sb) | used(p.heads, p.q_sh) |
+                  used(p.lq, p.q_st);
+  if (p.lk > 0)
+    bits |= reinterpret_cast<uint64_t>(p.k) | reinterpret_cast<uint64_t>(p.v) |
+            used(batch, p.k_sb | p.v_sb) | used(a->kv_heads, p.k_sh | p.v_sh) |
+            used(p.lk, p.k_st | p.v_st);
   if (bits % 16 != 0) return BIO_ERR_ALIGN;
   const int dim = std::max(p.d, p.dv);
   if (packed)

@@ -241,3 +241,65 @@ def test_streams_and_graphs():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held, want)
+
+
+def one_token(d, heads, dtype, gen, step):
+    """[1, heads, 1, d] whose batch and token strides are `heads * step`, off the
+    16-byte borders that only a dimension of several elements has to keep."""
+    x = torch.zeros(1, 1, heads, step, dtype=dtype, device="cuda")
+    x[..., :d] = torch.randn(1, 1, heads, d, generator=gen, device="cuda").to(dtype)
+    return x[..., :d].transpose(1, 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (1, 8, 33, 36, 64, 100, 250))
+@pytest.mark.parametrize("h,step", [(1, 0), (3, 0), (1, 3), (1, 5)])
+def test_one_token_of_any_stride(h, step, d, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(d + h)
+    q, k, v = (one_token(d, n, dtype, gen, d + step) for n in (h, 1, 1))
+    out = bio.sliding_window_attention_batch_invariant(q, k, v, 4)
+    assert torch.equal(out, v.expand_as(out))  # one key: its value
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    packed = bio.varlen_sliding_window_attention_batch_invariant(
+        *(t.transpose(1, 2) for t in (q, k, v)), cu, cu, 4)
+    assert torch.equal(packed.transpose(1, 2), out)
+    # the last token of a longer sequence, alone: strides of the whole
+    q, k, v = make(1, h, 1, 9, 9, d, dtype=dtype, seed=d)
+    whole = bio.sliding_window_attention_batch_invariant(q, k, v, 5, 1)
+    last = bio.sliding_window_attention_batch_invariant(q[:, :, 8:], k, v, 5, 1)
+    assert torch.equal(last, whole[:, :, 8:])
+    first = bio.sliding_window_attention_batch_invariant(q[:, :, :1], k[:, :, :1], v[:, :, :1], 5, 1)
+    assert torch.equal(first, whole[:, :, :1])
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hk,d", [(1, 33), (2, 33), (2, 64), (4, 36)])
+def test_no_key_with_any_stride(hk, d, dtype):
+    q, k, v = make(2, 4, hk, 5, 0, d, dtype=dtype)
+    for x in (k, k.contiguous()):
+        out = bio.sliding_window_attention_batch_invariant(q, x, x, 4)
+        assert torch.equal(out, torch.zeros_like(out))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 100, 256))
+def test_keys_expanded_over_batch_and_heads(d, dtype):
+    """One prefix under several prompts, or one head's keys under all of them: strides of 0."""
+    q, _, _ = make(3, 4, 2, 70, 70, d, dtype=dtype)
+    _, k, v = make(1, 4, 2, 70, 90, d, dtype=dtype, seed=1)
+    want = bio.sliding_window_attention_batch_invariant(
+        q, k.repeat(3, 1, 1, 1), v.repeat(3, 1, 1, 1), 40, 4)
+    got = bio.sliding_window_attention_batch_invariant(
+        q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1), 40, 4)
+    assert torch.equal(got, want)
+    k, v = k[:, :1], v[:, :1]
+    want = bio.sliding_window_attention_batch_invariant(
+        q[:1], k.repeat(1, 2, 1, 1), v.repeat(1, 2, 1, 1), 40, 4)
+    got = bio.sliding_window_attention_batch_invariant(
+        q[:1], k.expand(-1, 2, -1, -1), v.expand(-1, 2, -1, -1), 40, 4)
+    assert torch.equal(got, want)
+    same = q[:1, :, :1].expand(-1, -1, 70, -1)  # one query at every position
+    got = bio.sliding_window_attention_batch_invariant(same, k, v, 40, 4)
+    want = bio.sliding_window_attention_batch_invariant(same.contiguous(), k, v, 40, 4)
+    assert torch.equal(got, want)
