@@ -303,3 +303,30 @@ def test_keys_expanded_over_batch_and_heads(d, dtype):
     got = bio.sliding_window_attention_batch_invariant(same, k, v, 40, 4)
     want = bio.sliding_window_attention_batch_invariant(same.contiguous(), k, v, 40, 4)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 128, 256, 72))
+@pytest.mark.parametrize("window,sinks", [(1, 0), (50, 4), (128, 0), (300, 140), (90, 700),
+                                          (5000, 3)])
+def test_chunks_equal_the_whole_prompt(d, window, sinks, dtype):
+    """Chunks behind the tokens before them, cut anywhere, dense and packed."""
+    n = 1000
+    q, k, v = make(1, 6, 2, n, n, d, dtype=dtype, seed=window)
+    whole = bio.sliding_window_attention_batch_invariant(q, k, v, window, sinks)
+    cuts = [0, 1, 32, 97, 128, 129, 255, 500, 501, 777, n]
+    for a, b in [*zip(cuts, cuts[1:]), (0, 501), (129, 777), (3, n)]:
+        got = bio.sliding_window_attention_batch_invariant(
+            q[:, :, a:b], k[:, :, :b], v[:, :, :b], window, sinks)
+        assert torch.equal(got, whole[:, :, a:b]), (a, b)
+    pairs = [(97, 255), (0, 33), (501, n)]
+    cu_q, cu_k = ([0, *torch.tensor(x).cumsum(0).tolist()] for x in (
+        [b - a for a, b in pairs], [b for _, b in pairs]))
+    packed = bio.varlen_sliding_window_attention_batch_invariant(
+        torch.cat([q[:, :, a:b] for a, b in pairs], 2).transpose(1, 2),
+        torch.cat([k[:, :, :b] for _, b in pairs], 2).transpose(1, 2),
+        torch.cat([v[:, :, :b] for _, b in pairs], 2).transpose(1, 2),
+        torch.tensor(cu_q, dtype=torch.int32, device="cuda"),
+        torch.tensor(cu_k, dtype=torch.int32, device="cuda"), window, sinks)
+    for (a, b), got in zip(pairs, packed.split([b - a for a, b in pairs], 1)):
+        assert torch.equal(got.transpose(1, 2), whole[:, :, a:b]), (a, b)
