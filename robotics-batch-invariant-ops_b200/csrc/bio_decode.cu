@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
     return w;
   };
   auto load = [&](Place w, float (&kx)[kLaneDims], float (&vx)[kLaneDims]) {
-    if (w.page < 0 || w.page >= p.pages) {
+    if (w.on && (w.page < 0 || w.page >= p.pages)) {
       bad = 1;
       w.on = false;
     }

@@ -312,3 +312,18 @@ def test_rows_of_one_piece_are_written_before_the_next_kernel_reads(dtype, longe
         assert torch.equal(read, want), f"replay {turn}"
         got = bio.paged_attention_decode_batch_invariant(q, kp, vp, table, ln) + 0
         assert torch.equal(got, want), f"call {turn}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 33))
+def test_an_empty_pool_under_empty_rows_raises_nothing(d, dtype):
+    q, kp, vp, table, ln = make([3, 40], 4, 2, d, dtype=dtype)
+    for t in (table, table[:, :0]):
+        out = bio.paged_attention_decode_batch_invariant(q, kp[:0], vp[:0], t, ln * 0)
+        assert torch.equal(out, torch.zeros_like(out))
+        assert _lib.device_status() == 0
+    # a token in a pool without pages is still refused
+    out = bio.paged_attention_decode_batch_invariant(q, kp[:0], vp[:0], table, ln)
+    assert torch.equal(out, torch.zeros_like(out))
+    assert _lib.device_status() == _lib.BIO_DEV_INDEX
+    _lib.clear_device_status()
