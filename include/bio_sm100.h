@@ -484,9 +484,9 @@ BIO_API int bio_kv_compact(const bio_kv_pool* pool, const bio_kv_table* table,
  * Query b [heads][d] attends to the first seq_lens[r] tokens of row r = rows[b]
  * (r = b without rows); with window > 0 only to tokens j with j >= len -
  * window or j < sinks.  Output [batch][heads][dv].  Rows of length 0 give
- * zeros.  Rows, lengths or page numbers out of range raise BIO_DEV_INDEX and
- * give zeros.  Slots beyond the length and tokens outside the window never
- * reach the result, whatever they hold.
+ * zeros.  Rows, lengths (above the table's or 2^31 - 65) or page numbers out of
+ * range raise BIO_DEV_INDEX and give zeros.  Slots beyond the length and tokens
+ * outside the window never reach the result, whatever they hold.
  *
  * Split: the tiles of 32 tokens that hold a visible token are cut into pieces
  * of a length that is a function of their number alone; each piece gives a

@@ -32,7 +32,7 @@ struct PagedParams {
   const int32_t* lens;
   const int32_t* rows;
   int window, sinks;   // window 0: everything is visible
-  int max_len;         // tokens that a row of the table can hold
+  int max_len;         // tokens that a row may have: its columns', below 2^31 by two tiles
   int box_rows;        // tokens of a TMA box: gcd(page size, tile)
   int group_shift;     // log2 of the boxes along a tile
   unsigned page_mul, page_shift;  // position / page size = (mulhi(position, mul) + position) >> shift
@@ -67,7 +67,7 @@ __device__ __forceinline__ int page_of(const PagedParams& p, int pos) {
 
 // What a row sees: token j with j < len and (j < sinks or j >= start).  Tile t
 // of the row is the tile t < head ? t : t + jump of its tokens.  Positions fit
-// in 32 bits: the table's width times the page size does.
+// in 32 bits, those of a last tile's hidden tokens too: max_len leaves room.
 struct Visible {
   int row;  // row of the table, -1 if refused
   int len, sinks, start;
@@ -941,6 +941,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
 namespace {
 
 constexpr int64_t kMaxGrid = 2147483647;
+// The kernels count positions in 32 bits, up to the end of a row's last tile and
+// of the tile after it.
+constexpr int64_t kMaxTokens = kMaxGrid - 2 * bio::kTile;
 
 // Most pieces that a row of up to `most` tiles can have.
 int64_t most_pieces(int64_t most, int least) {
@@ -1136,7 +1139,7 @@ int bio_paged_attention(const bio_paged_attn_args* a, void* workspace, int64_t w
   p.table = a->page_table; p.lens = a->seq_lens; p.rows = a->rows;
   p.window = static_cast<int>(a->window);
   p.sinks = static_cast<int>(a->sinks);
-  p.max_len = static_cast<int>(a->table_width * a->page_size);
+  p.max_len = static_cast<int>(std::min(a->table_width * a->page_size, kMaxTokens));
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.box_rows = std::gcd(p.page_size, bio::kTile);
   p.group_shift = 0;

@@ -327,3 +327,42 @@ def test_an_empty_pool_under_empty_rows_raises_nothing(d, dtype):
     assert torch.equal(out, torch.zeros_like(out))
     assert _lib.device_status() == _lib.BIO_DEV_INDEX
     _lib.clear_device_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", (127, 64))
+def test_lengths_up_to_the_last_position(page, dtype):
+    """Positions next to 2^31: the longest row that is taken, and rows beyond it."""
+    most, window, sinks = 2**31 - 65, 100, 40
+    width = (2**31 - 1) // page
+    lens = [most, most - 1, most - 33, most + 1, width * page]
+    gen = torch.Generator(device="cuda").manual_seed(page)
+    # pages 0.. hold the first tokens, the ones after them the last
+    first, last = range(sinks // page + 1), range((most - 200) // page, width)
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, :len(first)] = torch.arange(len(first))
+    table[0, last[0]:] = len(first) + torch.arange(len(last))
+    pages = len(first) + len(last)
+    kp, vp = (torch.randn(pages, 2, page, 64, generator=gen, device="cuda").to(dtype)
+              for _ in range(2))
+    q = torch.randn(1, 8, 64, generator=gen, device="cuda").to(dtype)
+    for n in lens:
+        ln = torch.tensor([n], dtype=torch.int32, device="cuda")
+        out = bio.paged_attention_decode_batch_invariant(q, kp, vp, table, ln, window=window,
+                                                         sinks=sinks)
+        if n > most:
+            assert torch.equal(out, torch.zeros_like(out))
+            assert _lib.device_status() == _lib.BIO_DEV_INDEX
+            _lib.clear_device_status()
+            continue
+        assert _lib.device_status() == 0
+        # the same tokens in a short cache of their own
+        keys = torch.cat([torch.arange(sinks), torch.arange(n - window, n)]).cuda()
+        p, s = table[0, keys // page].long(), keys % page
+        short = -(-keys.numel() // page)
+        own = [torch.zeros(short, 2, page, 64, dtype=dtype, device="cuda") for _ in range(2)]
+        t = torch.arange(keys.numel(), device="cuda")
+        for mine, theirs in zip(own, (kp, vp)):
+            mine[t // page, :, t % page] = theirs[p, :, s]
+        check(out, (q, *own, torch.arange(short, dtype=torch.int32, device="cuda")[None],
+                    torch.tensor([keys.numel()], dtype=torch.int32, device="cuda")))
