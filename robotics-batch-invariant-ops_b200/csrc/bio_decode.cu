@@ -941,6 +941,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
 namespace {
 
 constexpr int64_t kMaxGrid = 2147483647;
+// Items are counted in 32 bits, up to one step (a warp of every SM) past the last.
+constexpr int64_t kMaxItems = kMaxGrid - 65536;
 // The kernels count positions in 32 bits, up to the end of a row's last tile and
 // of the tile after it.
 constexpr int64_t kMaxTokens = kMaxGrid - 2 * bio::kTile;
@@ -979,7 +981,7 @@ int split_of(const bio_paged_attn_args* a, Split* s) {
   s->most = most;
   s->pieces = most_pieces(most, 1);  // longer pieces need less
   s->dvp = (a->dv + 3) / 4 * 4;
-  if (a->batch > kMaxGrid / a->heads || a->batch * a->heads > kMaxGrid / s->pieces)
+  if (a->batch > kMaxGrid / a->heads || a->batch * a->heads > kMaxItems / s->pieces)
     return BIO_ERR_SHAPE;
   const int64_t parts = s->pieces > 1 ? a->batch * a->heads * s->pieces : 0;
   s->acc_bytes = parts * s->dvp * 4;

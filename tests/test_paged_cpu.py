@@ -332,3 +332,18 @@ def test_oracle_page_book():
     book.free([0])
     assert book.compact(3) == [0, 1, 3] and book.refs == [1, 1, 1]
     assert book.table == [[-1, -1, -1], [0, 1, -1], [-1, 2, -1]]
+
+
+def test_items_leave_room_for_a_step_past_the_last():
+    """Pieces of all heads are walked in steps of some thousand with 32-bit numbers:
+    2^31 of them, less one step, are refused."""
+    need = _lib.load().bio_paged_attention_workspace
+    sizes = dict(heads=1, kv_heads=1, width=64, d=4, dv=4)  # 1024 tokens: 32 pieces a row
+    pieces = need(attention_args(batch=1, rows=1, **sizes)) // (4 * 4 + 8)
+    assert pieces == 32
+    most = (2**31 - 1) // pieces
+    assert need(attention_args(batch=most - 4096, **sizes)) == (most - 4096) * pieces * 24
+    for batch in (most - 10, most):
+        assert need(attention_args(batch=batch, **sizes)) == 0
+        assert _lib.load().bio_paged_attention(attention_args(batch=batch, **sizes), None, 0,
+                                               None) == _lib.BIO_ERR_SHAPE
