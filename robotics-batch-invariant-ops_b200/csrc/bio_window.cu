@@ -148,7 +148,8 @@ __device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb,
 //
 // A hidden key in a visited block has weight 0, but 0 * Inf or 0 * NaN in V
 // would still reach the row: a row whose output is not finite is computed once
-// more, by its warp, from its visible keys alone (window_row).  Keys of a
+// more, by its warp, from its visible keys alone (window_row), after the block's
+// last job, since a long row can take longer than the waits of the other warps.  Keys of a
 // neighbouring packed sequence are zeroed in shared memory instead, so that
 // they cannot even change a row's bits.
 // ---------------------------------------------------------------------------
@@ -380,6 +381,27 @@ __device__ __forceinline__ uint32_t pack_two<__half>(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+
+// Two values of type T in a word: a + 0 * y, which is NaN from the first y that is
+// not finite on.
+template <typename T>
+__device__ __forceinline__ uint32_t note_odd(uint32_t a, uint32_t y);
+template <>
+__device__ __forceinline__ uint32_t note_odd<__nv_bfloat16>(uint32_t a, uint32_t y) {
+  const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&y),
+                                   __floats2bfloat162_rn(0.f, 0.f),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&a));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t note_odd<__half>(uint32_t a, uint32_t y) {
+  const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&y), __floats2half2_rn(0.f, 0.f),
+                            *reinterpret_cast<const __half2*>(&a));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Bits of a value of type T that are all set in infinities and NaN.
+template <typename T>
+constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
 
 // The lowest x bits of a word, x anywhere.
 __device__ __forceinline__ uint32_t low_bits(int x) {
@@ -689,7 +711,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     const int rh = r / w.tok, rt = r - rh * w.tok;
     const uint64_t scale2 = pair_of(w.scale_log2, w.scale_log2);
     int base = 0, s_used = 0, jobs_done = 0;  // ring position of the job's first K
-    bool ok = true;
+    bool ok = true, odd = false;              // odd: an output of the warp is not finite
     for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
       WinJob j;
       if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
@@ -828,7 +850,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const uint64_t inv2 = pair_of(inv, inv);
-      uint64_t odd2 = 0;  // becomes NaN with the first output that is not finite
+      uint32_t odd2 = 0;
 #pragma unroll 1
       for (int c = 0; c < vc * 2; ++c) {
         uint32_t v[32];
@@ -846,10 +868,10 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         for (int e = 0; e < 16; ++e) {
           const uint64_t o2 = fma_pair(
               pair_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), inv2, 0);
-          odd2 = fma_pair(o2, 0, odd2);
           float lo, hi;
           split_pair(o2, lo, hi);
           y[e] = pack_two<T>(lo, hi);
+          odd2 = note_odd<T>(odd2, y[e]);
         }
         if (w.vec_out == 2) {  // whole 32-byte sectors
 #pragma unroll
@@ -875,23 +897,31 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         }
       }
       tc_fence_before();  // the next job's PV overwrites O after this row's next P
-      float odd, odd_hi;
-      split_pair(odd2, odd, odd_hi);
-      odd += odd_hi;
-      __syncwarp();
-      unsigned again = __ballot_sync(0xffffffffu, valid && !(odd == 0.f));
-      while (again != 0) {
+      odd |= __any_sync(0xffffffffu, (odd2 & 0x7fff7fffu) != 0u);  // zeros keep their sign
+    }
+    // Rows that are not finite, from their visible keys alone: a warp's job is one
+    // row, and nobody waits for this one any more.  The output tells which they are.
+    for (int number = blockIdx.x; ok && odd && number < w.jobs; number += gridDim.x) {
+      WinJob j;
+      if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
+      WinTile tile = j.tile[0];
+      if (NT == 2 && t == 1) tile = j.tile[NT - 1];
+      const int64_t first = j.qt + j.q0 + t * w.tok;  // the tile's first token
+      T* out = static_cast<T*>(p.o) + j.b * p.o_sb + j.h0 * p.o_sh + first * p.o_st;
+      bool bad = false;
+      if (rh < j.nh && rt < tile.n) {
+        const uint16_t* row = reinterpret_cast<const uint16_t*>(out + rh * p.o_sh + rt * p.o_st);
+        for (int c = 0; c < p.dv; ++c) bad |= (row[c] & kExponent<T>) == kExponent<T>;
+      }
+      for (unsigned again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1) {
         const int y = __ffs(again) - 1;
-        again &= again - 1;
-        const int xh = j.h0 + __shfl_sync(0xffffffffu, rh, y);
-        const int xt = __shfl_sync(0xffffffffu, rt, y);
-        const int64_t xtok = j.qt + j.q0 + t * w.tok + xt;
+        const int xh = __shfl_sync(0xffffffffu, rh, y), xt = __shfl_sync(0xffffffffu, rt, y);
         window_row<T>(
-            static_cast<const T*>(p.q) + j.b * p.q_sb + xh * p.q_sh + xtok * p.q_st,
+            static_cast<const T*>(p.q) + j.b * p.q_sb + (j.h0 + xh) * p.q_sh + (first + xt) * p.q_st,
             static_cast<const T*>(p.k) + j.b * p.k_sb + j.hk * p.k_sh + j.kt * p.k_st,
             static_cast<const T*>(p.v) + j.b * p.v_sb + j.hk * p.v_sh + j.kt * p.v_st,
-            static_cast<T*>(p.o) + j.b * p.o_sb + xh * p.o_sh + xtok * p.o_st, p.k_st, p.v_st, p.d,
-            p.dv, p.scale, p.window, p.sinks, tile.pf + xt);
+            out + xh * p.o_sh + xt * p.o_st, p.k_st, p.v_st, p.d, p.dv, p.scale, p.window, p.sinks,
+            tile.pf + xt);
       }
     }
   }

@@ -330,3 +330,26 @@ def test_chunks_equal_the_whole_prompt(d, window, sinks, dtype):
         torch.tensor(cu_k, dtype=torch.int32, device="cuda"), window, sinks)
     for (a, b), got in zip(pairs, packed.split([b - a for a, b in pairs], 1)):
         assert torch.equal(got.transpose(1, 2), whole[:, :, a:b]), (a, b)
+
+
+def test_rows_computed_again_hold_nobody_up():
+    """Rows of 200000 visible keys that come out not finite take seconds to compute
+    again: longer than the waits of a block's other warps, whose next sequences
+    must not notice."""
+    dtype, n = torch.bfloat16, 200000
+    lens_q, lens_k = [32] + [2] * 400, [n] + [5] * 400
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (torch.randn(1, x, 1, 64, generator=gen, device="cuda").to(dtype)
+               for x in (sum(lens_q), sum(lens_k), sum(lens_k)))
+    off = lambda x: torch.tensor([0, *x], device="cuda").cumsum(0)  # noqa: E731
+    cu = off(lens_q), off(lens_k)
+    clean = bio.varlen_sliding_window_attention_batch_invariant(q, k, v, *cu, 2**31 - 1)
+    v[:, 7, :, 3] = float("nan")
+    out = bio.varlen_sliding_window_attention_batch_invariant(q, k, v, *cu, 2**31 - 1)
+    assert _lib.device_status() == 0
+    assert torch.equal(out[:, 32:], clean[:, 32:])
+    assert torch.isnan(out[:, :32, :, 3]).all()
+    rest = torch.arange(64, device="cuda") != 3
+    # a mean of so many values is small beside them: within the weights' rounding of |v| <= 6
+    err = (out[:, :32, :, rest].double() - clean[:, :32, :, rest].double()).abs().max().item()
+    assert err <= 2 * 6 * (4 * UNIT[dtype] + 2.0**-24 * (2 * 64 * 50 + 2 * n + 8))
