@@ -147,11 +147,14 @@ __device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb,
 // rounded to the operand type, as the product needs, l sums it unrounded.
 //
 // A hidden key in a visited block has weight 0, but 0 * Inf or 0 * NaN in V
-// would still reach the row: a row whose output is not finite is computed once
-// more, by its warp, from its visible keys alone (window_row), after the block's
-// last job, since a long row can take longer than the waits of the other warps.  Keys of a
-// neighbouring packed sequence are zeroed in shared memory instead, so that
-// they cannot even change a row's bits.
+// would still reach the row.  A block whose rows all came out finite is done.  One
+// that wrote anything else goes through its jobs once more, with the values of
+// every key that holds an Inf or NaN zeroed in shared memory: rows that do not see
+// such a key get the bits that they have beside finite values, since it adds
+// exactly 0 either way.  Rows that see one, or are not finite for another reason,
+// are computed by their warp from their visible keys alone (window_row) after the
+// last job, since a long row can take longer than the waits of the other warps.
+// Keys of a neighbouring packed sequence are zeroed in shared memory at once.
 // ---------------------------------------------------------------------------
 struct WindowJobs {
   int gh, tok, hblocks;  // heads and tokens of a tile, tiles across a group
@@ -408,6 +411,42 @@ __device__ __forceinline__ uint32_t low_bits(int x) {
   return __funnelshift_lc(0xffffffffu, 0u, max(x, 0));
 }
 
+// Which of the keys a .. a + 31 a query at position `at` sees.
+__device__ __forceinline__ uint32_t window_sees(const WindowJobs& w, int at, int a) {
+  return (low_bits(at + 1 - a) & ~low_bits(at - w.window + 1 - a)) |
+         low_bits(min(w.sinks, at + 1) - a);
+}
+
+// Zeroes the values of the keys of a block (BN rows of 128 bytes per 64 columns)
+// that are not finite and says which keys these are.  Every warp that is going to
+// use the block calls it: each finds such a key itself or, where another warp was
+// faster, finds its bit in `shared`, which is set before the zeros are written.
+template <typename T, int BN>
+__device__ __noinline__ void clean_values(uint8_t* v, uint32_t* shared, int chunks,
+                                          uint32_t (&bad)[BN / 32]) {
+  constexpr uint32_t e = kExponent<T>;
+  const int lane = threadIdx.x & 31;
+  auto odd = [](uint32_t x) { return (x & e) == e || (x >> 16 & e) == e; };
+  for (int n = lane; n < BN; n += 32) {
+    bool found = false;
+    for (int x = 0; x < chunks * 8; ++x) {
+      const uint4 y = *reinterpret_cast<const uint4*>(v + (x >> 3) * (BN * 128) + n * 128 +
+                                                      (((x ^ n) & 7) << 4));
+      found |= odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w);
+    }
+    if (!found) continue;
+    atomicOr(shared + (n >> 5), 1u << (n & 31));
+    __threadfence_block();
+    for (int x = 0; x < chunks * 8; ++x)
+      *reinterpret_cast<uint4*>(v + (x >> 3) * (BN * 128) + n * 128 + ((x & 7) << 4)) =
+          make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();  // the products read what is left
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < BN / 32; ++c) bad[c] = *const_cast<volatile uint32_t*>(shared + c);
+}
+
 // 32 lanes x 8 columns of TMEM, the load waited for.
 __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile(
@@ -460,6 +499,8 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
   const WinBars bar{smem_u32(tail)};
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 260);
+  volatile int* odd_rows = reinterpret_cast<volatile int*>(tail + 264);
+  uint32_t* bad_keys = reinterpret_cast<uint32_t*>(tail + 272);  // [NS][4], clean turn only
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kc = (p.d + 63) / 64, vc = (p.dv + 63) / 64;
 
@@ -467,6 +508,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     uint64_t* b = reinterpret_cast<uint64_t*>(tail);
     for (int i = 0; i < 28; ++i) mbar_init(b + i, i == 22 || i == 23 ? 4 : 1);  // p_ready: 4 warps
     *abort_flag = 0;
+    *odd_rows = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -498,81 +540,93 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     return __all_sync(0xffffffffu, spin_wait(at, parity & 1u, abort_flag, p.status));
   };
 
-  // 384 threads start with 168 registers each, 128 of them go on with 56 and
-  // 256 with 216: 62464 of the 64512
+  // Every warp of the block comes here once, after its last job or after a wait that
+  // ran out: whether a row was not finite, so that all jobs are done again, clean.
+  auto clean_turn = [&]() -> bool {
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(L::kThreads) : "memory");
+    return *odd_rows != 0 && *abort_flag == 0;
+  };
+
+  // 384 threads start with 168 registers each, 128 of them go on with 72 and
+  // 256 with 216: the same 64512
   constexpr bool kShift = NT == 2;
   if (warp < 4) {
-    if (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
       // -------------------------------------------------------------- producer
       int slot = 0, count = 0;              // ring position, blocks loaded so far
       uint32_t turn = 0;
       int q_used[2] = {0, 0};
       bool ok = true;
-      for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
-        WinJob j;
-        if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
-        const int n = j.blocks;
-        if (n == 0) continue;
-        auto load = [&](const CUtensorMap* map, int chunks, int i) {
-          if (lane == 0) {
-            const int row = j.kt + (i < j.head ? i : i + j.jump) * BN;
-            expect_bytes(bar.full(slot), chunks * (BN * 128));
-            for (int c = 0; c < chunks; ++c)
-              load_box(ring32 + slot * L::kSlot + c * (BN * 128), map, bar.full(slot), c * 64, row,
-                       j.hk, j.b);
+      for (int again = 0; again < 2 && (again == 0 || clean_turn()); ++again) {
+        for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+          WinJob j;
+          if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
+          const int n = j.blocks;
+          if (n == 0) continue;
+          auto load = [&](const CUtensorMap* map, int chunks, int i) {
+            if (lane == 0) {
+              // whoever looked at the slot's last block has done so: it was empty
+              if (again) *reinterpret_cast<uint4*>(bad_keys + slot * 4) = make_uint4(0, 0, 0, 0);
+              const int row = j.kt + (i < j.head ? i : i + j.jump) * BN;
+              expect_bytes(bar.full(slot), chunks * (BN * 128));
+              for (int c = 0; c < chunks; ++c)
+                load_box(ring32 + slot * L::kSlot + c * (BN * 128), map, bar.full(slot), c * 64,
+                         row, j.hk, j.b);
+            }
+            ++count;
+            if (++slot == NS) {
+              slot = 0;
+              turn ^= 1u;
+            }
+          };
+          ok = wait(bar.empty(slot), turn ^ 1u);
+          if (!ok) break;
+          load(&tmK, kc, 0);
+          {  // the next job's queries on their way into L2, behind this job's first keys
+            WinJob then;
+            const int at = number + static_cast<int>(gridDim.x);
+            if (at < w.jobs && window_job<NT, BN, PACKED>(p, w, at, then) && lane < NT * kc) {
+              const int t = lane / kc;
+              prefetch_box(&tmQ, (lane - t * kc) * 64, then.qt + then.q0 + t * w.tok, then.h0,
+                           then.b);
+            }
           }
-          ++count;
-          if (++slot == NS) {
-            slot = 0;
-            turn ^= 1u;
-          }
-        };
-        ok = wait(bar.empty(slot), turn ^ 1u);
-        if (!ok) break;
-        load(&tmK, kc, 0);
-        {  // the next job's queries on their way into L2, behind this job's first keys
-          WinJob then;
-          const int at = number + static_cast<int>(gridDim.x);
-          if (at < w.jobs && window_job<NT, BN, PACKED>(p, w, at, then) && lane < NT * kc) {
-            const int t = lane / kc;
-            prefetch_box(&tmQ, (lane - t * kc) * 64, then.qt + then.q0 + t * w.tok, then.h0,
-                         then.b);
-          }
-        }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (j.tile[t].last < 0 || !ok) continue;
-          ok = wait(bar.q_empty(t), q_used[t] ^ 1);
-          if (!ok) break;
-          if (lane == 0) {
-            expect_bytes(bar.q_full(t), kc * w.gh * w.tok * 128);
-            for (int c = 0; c < kc; ++c)
-              load_box(q32 + t * L::kQ + c * 16384, &tmQ, bar.q_full(t), c * 64,
-                       j.qt + j.q0 + t * w.tok, j.h0, j.b);
+          for (int t = 0; t < NT; ++t) {
+            if (j.tile[t].last < 0 || !ok) continue;
+            ok = wait(bar.q_empty(t), q_used[t] ^ 1);
+            if (!ok) break;
+            if (lane == 0) {
+              expect_bytes(bar.q_full(t), kc * w.gh * w.tok * 128);
+              for (int c = 0; c < kc; ++c)
+                load_box(q32 + t * L::kQ + c * 16384, &tmQ, bar.q_full(t), c * 64,
+                         j.qt + j.q0 + t * w.tok, j.h0, j.b);
+            }
+            ++q_used[t];
           }
-          ++q_used[t];
+          for (int i = 1; ok && i <= n; ++i) {
+            const bool key = i < n;           // K of block i, then V of block i - 1
+            const int slot2 = slot + 1 == NS ? 0 : slot + 1;
+            const uint32_t turn2 = slot + 1 == NS ? turn ^ 1u : turn;
+            const uint32_t e1 = bar.empty(slot), e2 = key ? bar.empty(slot2) : e1;
+            ok = wait_all(e1, turn ^ 1u, e2, (key ? turn2 : turn) ^ 1u, e1, turn ^ 1u);
+            if (!ok) break;
+            if (key) load(&tmK, kc, i);
+            load(&tmV, vc, i - 1);
+          }
         }
-        for (int i = 1; ok && i <= n; ++i) {
-          const bool key = i < n;           // K of block i, then V of block i - 1
-          const int slot2 = slot + 1 == NS ? 0 : slot + 1;
-          const uint32_t turn2 = slot + 1 == NS ? turn ^ 1u : turn;
-          const uint32_t e1 = bar.empty(slot), e2 = key ? bar.empty(slot2) : e1;
-          ok = wait_all(e1, turn ^ 1u, e2, (key ? turn2 : turn) ^ 1u, e1, turn ^ 1u);
-          if (!ok) break;
-          if (key) load(&tmK, kc, i);
-          load(&tmV, vc, i - 1);
+        // every copy has to land before the block's shared memory goes
+        if (lane == 0) {
+          for (int i = max(0, count - NS); i < count; ++i)
+            if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + i % NS, (i / NS) & 1))
+              raise_status(p.status, BIO_DEV_TIMEOUT);
+          for (int t = 0; t < NT; ++t)
+            if (q_used[t] > 0 &&
+                !mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 16 + t, (q_used[t] - 1) & 1))
+              raise_status(p.status, BIO_DEV_TIMEOUT);
         }
-      }
-      // every copy has to land before the block's shared memory goes
-      if (lane == 0) {
-        for (int i = max(0, count - NS); i < count; ++i)
-          if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + i % NS, (i / NS) & 1))
-            raise_status(p.status, BIO_DEV_TIMEOUT);
-        for (int t = 0; t < NT; ++t)
-          if (q_used[t] > 0 &&
-              !mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 16 + t, (q_used[t] - 1) & 1))
-            raise_status(p.status, BIO_DEV_TIMEOUT);
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------------- MMA
@@ -588,118 +642,122 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
           turn ^= 1u;
         }
       };
-      for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
-        WinJob j;
-        if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
-        const int n = j.blocks;
-        if (n == 0) continue;
-        int2 open[NT], held[NT];            // whole blocks; columns of the P that waits
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          open[t] = window_whole<BN>(w, j, j.tile[t]);
-          held[t] = make_int2(0, 0);
-        }
-        uint32_t begun = 0;                 // bit t: O_t holds something
-        // S of block i, whose keys are at ring position `at`
-        auto products_s = [&](int t, int i, int at, int2 s) {
-          tc_fence_after();
-          const int x = NT == 2 ? t : s_used[t] & 1;
-          const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
-          const uint64_t qd = smem_desc_sw128(q32 + t * L::kQ, 16, 1024);
-          const uint64_t kd = smem_desc_sw128(ring32 + at * L::kSlot + s.x * 128, 16, 1024);
-          const uint32_t to = tmem + x * 128 + s.x;
-          if (elect_leader()) {
-            // 16 columns are 32 bytes, 2 units of a descriptor; 64 columns a chunk
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k)
-              if (DP == 64 || (k >> 2) < kc)
-                umma_f16(to, qd + (k >> 2) * 1024 + (k & 3) * 2,
-                         kd + (k >> 2) * (BN * 8) + (k & 3) * 2, idesc, k > 0 ? 1u : 0u);
-            commit_to(bar.s_full(x));
-            if (i == j.tile[t].last) commit_to(bar.q_empty(t));
-          }
-          __syncwarp();
-          ++s_used[t];
-          if (i == j.tile[t].last) ++q_used[t];
-        };
-        // PV of block i, whose values are at ring position `at`
-        auto products_pv = [&](int t, int i, int at) {
-          tc_fence_after();
-          const int x = NT == 2 ? t : p_used[t] & 1;
-          const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
-          // 16 keys are 2048 bytes of V and 8 columns of P
-          const uint64_t vd = smem_desc_sw128(ring32 + at * L::kSlot, BN * 128, 1024);
-          const uint32_t pa = tmem + x * 128, to = tmem + 256 + t * 128;
-          const bool on = (begun >> t) & 1u;
-          if (elect_leader()) {
-#pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
-              if (k * 16 >= held[t].x && k * 16 < held[t].y)
-                umma_f16_ts(to, pa + k * 8, vd + k * 128, idesc,
-                            on || k * 16 > held[t].x ? 1u : 0u);
-            if (NT == 1) commit_to(bar.pv_done());
-            if (i == j.tile[t].last) commit_to(bar.o_done(t));
-          }
-          __syncwarp();
-          begun |= 1u << t;
-          ++p_used[t];
-        };
-        auto p_bar = [&](int t) { return bar.p_ready(NT == 2 ? t : p_used[t] & 1); };
-        auto p_turn = [&](int t) {
-          return static_cast<uint32_t>(NT == 2 ? p_used[t] : p_used[t] >> 1);
-        };
-        for (int i = 0; ok && i <= n; ++i) {
-          const bool key = i < n, value = i > 0;
-          const int k_at = slot;
-          const uint32_t k_turn = turn;
-          if (key) next();
-          const int v_at = slot;
-          const uint32_t v_turn = turn;
-          if (value) next();
-          int2 now[NT];
+      for (int again = 0; again < 2 && (again == 0 || clean_turn()); ++again) {
+        for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+          WinJob j;
+          if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
+          const int n = j.blocks;
+          if (n == 0) continue;
+          int2 open[NT], held[NT];            // whole blocks; columns of the P that waits
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            now[t] = make_int2(0, 0);
-            if (key)
-              now[t] = i >= open[t].x && i < open[t].y ? make_int2(0, BN)
-                                                       : window_span<BN>(j, j.tile[t], i);
+            open[t] = window_whole<BN>(w, j, j.tile[t]);
+            held[t] = make_int2(0, 0);
           }
-          const bool p0 = held[0].x < held[0].y;
-          // the block's keys, the values of the one before, and with two tiles the
-          // first tile's P; queries with a job's first keys
-          const uint32_t b0 = key ? bar.full(k_at) : bar.full(v_at), t0 = key ? k_turn : v_turn;
-          uint32_t b2 = b0, t2 = t0;
-          if (NT == 2 && p0) {
-            b2 = p_bar(0);
-            t2 = p_turn(0);
-          }
-          ok = wait_all(b0, t0, value ? bar.full(v_at) : b0, value ? v_turn : t0, b2, t2);
+          uint32_t begun = 0;                 // bit t: O_t holds something
+          // S of block i, whose keys are at ring position `at`
+          auto products_s = [&](int t, int i, int at, int2 s) {
+            tc_fence_after();
+            const int x = NT == 2 ? t : s_used[t] & 1;
+            const uint32_t idesc = idesc_f16(kFmt, 128, s.y - s.x, false, false);
+            const uint64_t qd = smem_desc_sw128(q32 + t * L::kQ, 16, 1024);
+            const uint64_t kd = smem_desc_sw128(ring32 + at * L::kSlot + s.x * 128, 16, 1024);
+            const uint32_t to = tmem + x * 128 + s.x;
+            if (elect_leader()) {
+              // 16 columns are 32 bytes, 2 units of a descriptor; 64 columns a chunk
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-            if (ok && i == 0 && j.tile[t].last >= 0) ok = wait(bar.q_full(t), q_used[t]);
-          if (!ok) break;
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const bool s_on = now[t].x < now[t].y, p_on = held[t].x < held[t].y;
-            if (NT == 1 && s_on) products_s(t, i, k_at, now[t]);
-            if (p_on && ok) {
-              if (NT == 1 || t > 0) ok = wait(p_bar(t), p_turn(t));
-              if (ok) products_pv(t, i - 1, v_at);
+              for (int k = 0; k < DP / 16; ++k)
+                if (DP == 64 || (k >> 2) < kc)
+                  umma_f16(to, qd + (k >> 2) * 1024 + (k & 3) * 2,
+                           kd + (k >> 2) * (BN * 8) + (k & 3) * 2, idesc, k > 0 ? 1u : 0u);
+              commit_to(bar.s_full(x));
+              if (i == j.tile[t].last) commit_to(bar.q_empty(t));
             }
-            if (NT == 2 && s_on && ok) products_s(t, i, k_at, now[t]);
-            held[t] = now[t];
+            __syncwarp();
+            ++s_used[t];
+            if (i == j.tile[t].last) ++q_used[t];
+          };
+          // PV of block i, whose values are at ring position `at`
+          auto products_pv = [&](int t, int i, int at) {
+            tc_fence_after();
+            const int x = NT == 2 ? t : p_used[t] & 1;
+            const uint32_t idesc = idesc_f16(kFmt, 128, vc * 64, false, true);
+            // 16 keys are 2048 bytes of V and 8 columns of P
+            const uint64_t vd = smem_desc_sw128(ring32 + at * L::kSlot, BN * 128, 1024);
+            const uint32_t pa = tmem + x * 128, to = tmem + 256 + t * 128;
+            const bool on = (begun >> t) & 1u;
+            if (elect_leader()) {
+#pragma unroll
+              for (int k = 0; k < BN / 16; ++k)
+                if (k * 16 >= held[t].x && k * 16 < held[t].y)
+                  umma_f16_ts(to, pa + k * 8, vd + k * 128, idesc,
+                              on || k * 16 > held[t].x ? 1u : 0u);
+              if (NT == 1) commit_to(bar.pv_done());
+              if (i == j.tile[t].last) commit_to(bar.o_done(t));
+            }
+            __syncwarp();
+            begun |= 1u << t;
+            ++p_used[t];
+          };
+          auto p_bar = [&](int t) { return bar.p_ready(NT == 2 ? t : p_used[t] & 1); };
+          auto p_turn = [&](int t) {
+            return static_cast<uint32_t>(NT == 2 ? p_used[t] : p_used[t] >> 1);
+          };
+          for (int i = 0; ok && i <= n; ++i) {
+            const bool key = i < n, value = i > 0;
+            const int k_at = slot;
+            const uint32_t k_turn = turn;
+            if (key) next();
+            const int v_at = slot;
+            const uint32_t v_turn = turn;
+            if (value) next();
+            int2 now[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              now[t] = make_int2(0, 0);
+              if (key)
+                now[t] = i >= open[t].x && i < open[t].y ? make_int2(0, BN)
+                                                         : window_span<BN>(j, j.tile[t], i);
+            }
+            const bool p0 = held[0].x < held[0].y;
+            // the block's keys, the values of the one before, and with two tiles the
+            // first tile's P; queries with a job's first keys
+            const uint32_t b0 = key ? bar.full(k_at) : bar.full(v_at), t0 = key ? k_turn : v_turn;
+            uint32_t b2 = b0, t2 = t0;
+            if (NT == 2 && p0) {
+              b2 = p_bar(0);
+              t2 = p_turn(0);
+            }
+            ok = wait_all(b0, t0, value ? bar.full(v_at) : b0, value ? v_turn : t0, b2, t2);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              if (ok && i == 0 && j.tile[t].last >= 0) ok = wait(bar.q_full(t), q_used[t]);
+            if (!ok) break;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              const bool s_on = now[t].x < now[t].y, p_on = held[t].x < held[t].y;
+              if (NT == 1 && s_on) products_s(t, i, k_at, now[t]);
+              if (p_on && ok) {
+                if (NT == 1 || t > 0) ok = wait(p_bar(t), p_turn(t));
+                if (ok) products_pv(t, i - 1, v_at);
+              }
+              if (NT == 2 && s_on && ok) products_s(t, i, k_at, now[t]);
+              held[t] = now[t];
+            }
+            // what the products issued so far have read is free once they are done
+            if (ok && elect_leader()) {
+              if (key) commit_to(bar.empty(k_at));
+              if (value) commit_to(bar.empty(v_at));
+            }
+            __syncwarp();
           }
-          // what the products issued so far have read is free once they are done
-          if (ok && elect_leader()) {
-            if (key) commit_to(bar.empty(k_at));
-            if (value) commit_to(bar.empty(v_at));
-          }
-          __syncwarp();
         }
+        if (elect_leader()) commit_to(bar.all_done());
+        if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 27, again))
+          raise_status(p.status, BIO_DEV_TIMEOUT);
       }
-      if (elect_leader()) commit_to(bar.all_done());
-      if (!mbar_wait_drain(reinterpret_cast<uint64_t*>(tail) + 27, 0))
-        raise_status(p.status, BIO_DEV_TIMEOUT);
+    } else {
+      clean_turn();
     }
   } else {
     if (kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -712,193 +770,213 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
     const uint64_t scale2 = pair_of(w.scale_log2, w.scale_log2);
     int base = 0, s_used = 0, jobs_done = 0;  // ring position of the job's first K
     bool ok = true, odd = false;              // odd: an output of the warp is not finite
-    for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
-      WinJob j;
-      if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
-      WinTile tile = j.tile[0];
-      if (NT == 2 && t == 1) tile = j.tile[NT - 1];
-      const bool valid = rh < j.nh && rt < tile.n;
-      const int at = tile.pf + rt;                     // position of the row
-      const int2 open = window_whole<BN>(w, j, tile);
-      float m = -INFINITY, l = 0.f;
-      bool first = true;
-      for (int i = 0; i <= tile.last; ++i) {
-        const bool whole = i >= open.x && i < open.y;
-        int2 s = make_int2(0, BN);
-        if (!whole) s = window_span<BN>(j, tile, i);
-        if (s.x >= s.y) continue;
-        const int x = NT == 2 ? t : s_used & 1;
-        ok = wait(bar.s_full(x), NT == 2 ? s_used : s_used >> 1);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t s_at = tmem + lanes + x * 128;
-        uint32_t f[NC][32];
+    // a copy for each turn, so that the first does not pay for the other
+    auto all_jobs = [&](auto turn) {
+      constexpr bool kClean = decltype(turn)::value;
+      for (int number = blockIdx.x; ok && number < w.jobs; number += gridDim.x) {
+        WinJob j;
+        if (!window_job<NT, BN, PACKED>(p, w, number, j)) continue;
+        WinTile tile = j.tile[0];
+        if (NT == 2 && t == 1) tile = j.tile[NT - 1];
+        const bool valid = rh < j.nh && rt < tile.n;
+        const int at = tile.pf + rt;                     // position of the row
+        const int2 open = window_whole<BN>(w, j, tile);
+        float m = -INFINITY, l = 0.f;
+        bool first = true, dirty = false;  // dirty: the row sees a key that was cleaned
+        for (int i = 0; i <= tile.last; ++i) {
+          const bool whole = i >= open.x && i < open.y;
+          int2 s = make_int2(0, BN);
+          if (!whole) s = window_span<BN>(j, tile, i);
+          if (s.x >= s.y) continue;
+          const int x = NT == 2 ? t : s_used & 1;
+          ok = wait(bar.s_full(x), NT == 2 ? s_used : s_used >> 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t s_at = tmem + lanes + x * 128;
+          uint32_t f[NC][32];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
+          for (int c = 0; c < NC; ++c) tmem_ld_32x32b_x32(s_at + c * 32, f[c]);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) tmem_ld_wait_tied(f[c]);
-        if (!whole) {
-          const uint32_t flip = w.negate ? 0x80000000u : 0u;
+          for (int c = 0; c < NC; ++c) tmem_ld_wait_tied(f[c]);
+          if (!whole) {
+            const uint32_t flip = w.negate ? 0x80000000u : 0u;
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            // keys a + e: inside the window, or one of the sinks; trimmed columns hold
-            // what was there before
-            const int a = (i < j.head ? i : i + j.jump) * BN + c * 32;
-            uint32_t sees = (low_bits(at + 1 - a) & ~low_bits(at - w.window + 1 - a)) |
-                            low_bits(min(w.sinks, at + 1) - a);
-            if (!valid || c * 32 < s.x || c * 32 >= s.y) sees = 0u;
-            if (flip != 0u || !__all_sync(0xffffffffu, sees == 0xffffffffu)) {
+            for (int c = 0; c < NC; ++c) {
+              // keys a + e: inside the window, or one of the sinks; trimmed columns hold
+              // what was there before
+              const int a = (i < j.head ? i : i + j.jump) * BN + c * 32;
+              uint32_t sees = window_sees(w, at, a);
+              if (!valid || c * 32 < s.x || c * 32 >= s.y) sees = 0u;
+              if (flip != 0u || !__all_sync(0xffffffffu, sees == 0xffffffffu)) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                f[c][e] = sees & (1u << e) ? f[c][e] ^ flip : 0xff800000u;  // -inf
+                for (int e = 0; e < 32; ++e)
+                  f[c][e] = sees & (1u << e) ? f[c][e] ^ flip : 0xff800000u;  // -inf
+              }
             }
           }
-        }
-        float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+          float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            a0 = max3(a0, __uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1]));
-            a1 = max3(a1, __uint_as_float(f[c][e + 2]), __uint_as_float(f[c][e + 3]));
-            a2 = max3(a2, __uint_as_float(f[c][e + 4]), __uint_as_float(f[c][e + 5]));
-            a3 = max3(a3, __uint_as_float(f[c][e + 6]), __uint_as_float(f[c][e + 7]));
-          }
-        const float top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
-        const float scaled = top == -INFINITY ? top : top * w.scale_log2;
-        const bool move = scaled > m + 8.f;
-        const float alpha = move ? pow2(m - scaled) : 1.f;
-        if (move) m = scaled;
-        l *= alpha;
-        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // S of this block was issued after the PV before it (two tiles), or that
-          // one has to be waited for (one tile)
-          if (NT == 1) {
-            ok = wait(bar.pv_done(), s_used - 1);
-            if (!ok) break;
-            tc_fence_after();
-          }
+            for (int e = 0; e < 32; e += 8) {
+              a0 = max3(a0, __uint_as_float(f[c][e]), __uint_as_float(f[c][e + 1]));
+              a1 = max3(a1, __uint_as_float(f[c][e + 2]), __uint_as_float(f[c][e + 3]));
+              a2 = max3(a2, __uint_as_float(f[c][e + 4]), __uint_as_float(f[c][e + 5]));
+              a3 = max3(a3, __uint_as_float(f[c][e + 6]), __uint_as_float(f[c][e + 7]));
+            }
+          const float top = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3));
+          const float scaled = top == -INFINITY ? top : top * w.scale_log2;
+          const bool move = scaled > m + 8.f;
+          const float alpha = move ? pow2(m - scaled) : 1.f;
+          if (move) m = scaled;
+          l *= alpha;
+          if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
+            // S of this block was issued after the PV before it (two tiles), or that
+            // one has to be waited for (one tile)
+            if (NT == 1) {
+              ok = wait(bar.pv_done(), s_used - 1);
+              if (!ok) break;
+              tc_fence_after();
+            }
 #pragma unroll 1
-          for (int c = 0; c < vc * 8; ++c) {  // 8 columns at a time: few registers
-            uint32_t v[8];
-            tmem_ld_x8(o_at + c * 8, v);
+            for (int c = 0; c < vc * 8; ++c) {  // 8 columns at a time: few registers
+              uint32_t v[8];
+              tmem_ld_x8(o_at + c * 8, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-            tmem_st_x8(o_at + c * 8, v);
+              for (int e = 0; e < 8; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+              tmem_st_x8(o_at + c * 8, v);
+            }
           }
-        }
-        first = false;
-        const float ref = m == -INFINITY ? 0.f : m;
-        const uint64_t ref2 = pair_of(-ref, -ref);
-        uint64_t sum2 = 0, sum3 = 0;
+          first = false;
+          const float ref = m == -INFINITY ? 0.f : m;
+          const uint64_t ref2 = pair_of(-ref, -ref);
+          uint64_t sum2 = 0, sum3 = 0;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if (!whole && (c * 32 < s.x || c * 32 >= s.y)) continue;
-          uint32_t packed[16];
+          for (int c = 0; c < NC; ++c) {
+            if (!whole && (c * 32 < s.x || c * 32 >= s.y)) continue;
+            uint32_t packed[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float a, bb;
-            split_pair(fma_pair(pair_of(__uint_as_float(f[c][2 * e]),
-                                        __uint_as_float(f[c][2 * e + 1])),
-                                scale2, ref2),
-                       a, bb);
-            a = pow2(a);
-            bb = pow2(bb);
-            packed[e] = pack_two<T>(a, bb);
-            if (e & 1)
-              sum3 = add_pair(sum3, pair_of(a, bb));
-            else
-              sum2 = add_pair(sum2, pair_of(a, bb));
+            for (int e = 0; e < 16; ++e) {
+              float a, bb;
+              split_pair(fma_pair(pair_of(__uint_as_float(f[c][2 * e]),
+                                          __uint_as_float(f[c][2 * e + 1])),
+                                  scale2, ref2),
+                         a, bb);
+              a = pow2(a);
+              bb = pow2(bb);
+              packed[e] = pack_two<T>(a, bb);
+              if (e & 1)
+                sum3 = add_pair(sum3, pair_of(a, bb));
+              else
+                sum2 = add_pair(sum2, pair_of(a, bb));
+            }
+            tmem_st_32x32b_x16(s_at + c * 16, packed);
           }
-          tmem_st_32x32b_x16(s_at + c * 16, packed);
-        }
-        float s0, s1;
-        split_pair(add_pair(sum2, sum3), s0, s1);
-        l += s0 + s1;
-        if (PACKED) {
-          const int from = (i < j.head ? i : i + j.jump) * BN;
-          if (from + s.y > j.lk) {
-            // the block's last columns may be another sequence's tokens
+          float s0, s1;
+          split_pair(add_pair(sum2, sum3), s0, s1);
+          l += s0 + s1;
+          if constexpr (kClean) {
             const int pos = base + ring_of_v(i, j.blocks);
             ok = wait(bar.full(pos % NS), pos / NS);
             if (!ok) break;
-            uint8_t* v = ring + pos % NS * L::kSlot;
-            for (int row = max(0, j.lk - from); row < s.y; ++row)
-              for (int c = r; c < vc * 8; c += 128)
-                *reinterpret_cast<uint4*>(v + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
-                    make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
+            uint32_t bad[NC];
+            clean_values<T, BN>(ring + pos % NS * L::kSlot, bad_keys + pos % NS * 4, vc, bad);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const int a = (i < j.head ? i : i + j.jump) * BN + c * 32;
+              dirty |= (bad[c] & window_sees(w, at, a)) != 0u;
+            }
+          }
+          if (PACKED) {
+            const int from = (i < j.head ? i : i + j.jump) * BN;
+            if (from + s.y > j.lk) {
+              // the block's last columns may be another sequence's tokens
+              const int pos = base + ring_of_v(i, j.blocks);
+              ok = wait(bar.full(pos % NS), pos / NS);
+              if (!ok) break;
+              uint8_t* v = ring + pos % NS * L::kSlot;
+              for (int row = max(0, j.lk - from); row < s.y; ++row)
+                for (int c = r; c < vc * 8; c += 128)
+                  *reinterpret_cast<uint4*>(v + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
+                      make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(bar.p_ready(x));
+          ++s_used;
+        }
+        base += 2 * j.blocks;
+        if (!ok) continue;
+        // ------------------------------------------------------------- the output
+        const int tok = j.qt + j.q0 + t * w.tok + rt;
+        T* out = valid ? static_cast<T*>(p.o) + j.b * p.o_sb + (j.h0 + rh) * p.o_sh + tok * p.o_st
+                       : nullptr;
+        if (tile.last >= 0) {
+          ok = wait(bar.o_done(t), jobs_done);
+          if (!ok) continue;
+          ++jobs_done;
+          tc_fence_after();
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const uint64_t inv2 = pair_of(inv, inv);
+        uint32_t odd2 = 0;
+#pragma unroll 1
+        for (int c = 0; c < vc * 2; ++c) {
+          uint32_t v[32];
+          if (tile.last >= 0) {
+            tmem_ld_32x32b_x32(o_at + c * 32, v);
+            tmem_ld_wait_tied(v);
+          }
+          if (l == 0.f || tile.last < 0) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0;
+          }
+          if (!valid) continue;
+          uint32_t y[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t o2 = fma_pair(
+                pair_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), inv2, 0);
+            float lo, hi;
+            split_pair(o2, lo, hi);
+            y[e] = kClean && dirty ? 0x7fff7fffu : pack_two<T>(lo, hi);  // NaN: again below
+            odd2 = note_odd<T>(odd2, y[e]);
+          }
+          if (w.vec_out == 2) {  // whole 32-byte sectors
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              if (c * 32 + 2 * e < p.dv)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
+                                 out + c * 32 + 2 * e),
+                             "r"(y[e]), "r"(y[e + 1]), "r"(y[e + 2]), "r"(y[e + 3]), "r"(y[e + 4]),
+                             "r"(y[e + 5]), "r"(y[e + 6]), "r"(y[e + 7])
+                             : "memory");
+          } else if (w.vec_out == 1) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              if (c * 32 + 2 * e < p.dv)
+                *reinterpret_cast<uint4*>(out + c * 32 + 2 * e) =
+                    make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e < p.dv)
+                reinterpret_cast<uint16_t*>(out)[c * 32 + e] =
+                    static_cast<uint16_t>(y[e >> 1] >> (16 * (e & 1)));
           }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive(bar.p_ready(x));
-        ++s_used;
-      }
-      base += 2 * j.blocks;
-      if (!ok) break;
-      // ------------------------------------------------------------- the output
-      const int tok = j.qt + j.q0 + t * w.tok + rt;
-      T* out = valid ? static_cast<T*>(p.o) + j.b * p.o_sb + (j.h0 + rh) * p.o_sh + tok * p.o_st
-                     : nullptr;
-      if (tile.last >= 0) {
-        ok = wait(bar.o_done(t), jobs_done);
-        if (!ok) break;
-        ++jobs_done;
-        tc_fence_after();
-      }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const uint64_t inv2 = pair_of(inv, inv);
-      uint32_t odd2 = 0;
-#pragma unroll 1
-      for (int c = 0; c < vc * 2; ++c) {
-        uint32_t v[32];
-        if (tile.last >= 0) {
-          tmem_ld_32x32b_x32(o_at + c * 32, v);
-          tmem_ld_wait_tied(v);
-        }
-        if (l == 0.f || tile.last < 0) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0;
-        }
-        if (!valid) continue;
-        uint32_t y[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint64_t o2 = fma_pair(
-              pair_of(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), inv2, 0);
-          float lo, hi;
-          split_pair(o2, lo, hi);
-          y[e] = pack_two<T>(lo, hi);
-          odd2 = note_odd<T>(odd2, y[e]);
-        }
-        if (w.vec_out == 2) {  // whole 32-byte sectors
-#pragma unroll
-          for (int e = 0; e < 16; e += 8)
-            if (c * 32 + 2 * e < p.dv)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
-                               out + c * 32 + 2 * e),
-                           "r"(y[e]), "r"(y[e + 1]), "r"(y[e + 2]), "r"(y[e + 3]), "r"(y[e + 4]),
-                           "r"(y[e + 5]), "r"(y[e + 6]), "r"(y[e + 7])
-                           : "memory");
-        } else if (w.vec_out == 1) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (c * 32 + 2 * e < p.dv)
-              *reinterpret_cast<uint4*>(out + c * 32 + 2 * e) =
-                  make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (c * 32 + e < p.dv)
-              reinterpret_cast<uint16_t*>(out)[c * 32 + e] =
-                  static_cast<uint16_t>(y[e >> 1] >> (16 * (e & 1)));
+        tc_fence_before();  // the next job's PV overwrites O after this row's next P
+        if (__any_sync(0xffffffffu, (odd2 & 0x7fff7fffu) != 0u)) {  // zeros keep their sign
+          odd = true;
+          if (lane == 0) *odd_rows = 1;
         }
       }
-      tc_fence_before();  // the next job's PV overwrites O after this row's next P
-      odd |= __any_sync(0xffffffffu, (odd2 & 0x7fff7fffu) != 0u);  // zeros keep their sign
-    }
+    };
+    all_jobs(std::false_type{});
+    if (clean_turn()) all_jobs(std::true_type{});
     // Rows that are not finite, from their visible keys alone: a warp's job is one
     // row, and nobody waits for this one any more.  The output tells which they are.
     for (int number = blockIdx.x; ok && odd && number < w.jobs; number += gridDim.x) {
@@ -917,7 +995,8 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
         const int y = __ffs(again) - 1;
         const int xh = __shfl_sync(0xffffffffu, rh, y), xt = __shfl_sync(0xffffffffu, rt, y);
         window_row<T>(
-            static_cast<const T*>(p.q) + j.b * p.q_sb + (j.h0 + xh) * p.q_sh + (first + xt) * p.q_st,
+            static_cast<const T*>(p.q) + j.b * p.q_sb + (j.h0 + xh) * p.q_sh +
+                (first + xt) * p.q_st,
             static_cast<const T*>(p.k) + j.b * p.k_sb + j.hk * p.k_sh + j.kt * p.k_st,
             static_cast<const T*>(p.v) + j.b * p.v_sb + j.hk * p.v_sh + j.kt * p.v_st,
             out + xh * p.o_sh + xt * p.o_st, p.k_st, p.v_st, p.d, p.dv, p.scale, p.window, p.sinks,
@@ -940,8 +1019,8 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
 // O.  V of a block and K of the next one are copied (cp.async) while the
 // products before them run.  FFMA and the shared loads that feed it bound it: 64
 // products per 8 loads of 16 bytes in S, 128 per 12 in PV.  Columns that no row of
-// the tile sees are skipped 32 at a time.  Rows that come out not finite are
-// computed once more from their visible keys alone, as above.
+// the tile sees are skipped 32 at a time.  A tile with a row that is not finite is
+// gone through once more with such values zeroed, as above.
 // Measured: 94 us for 1024 queries, 8 heads over 2 of 128, window 512 (17 TFLOP/s;
 // one warp per row, with K read from L2 for every row, ran at 1).  A window of 31
 // keys (4 x 10198 queries, 8 heads of 128) wastes most of its blocks: 1074 us, and
@@ -1002,7 +1081,8 @@ __global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, c
   float* sk = sq + 64 * L::kPitch;
   float* sv = sk + BN * L::kPitch;
   float* sp = sv + BN * L::kPitch;
-  uint32_t* redo = reinterpret_cast<uint32_t*>(sp + 64 * L::kP);  // [2] rows to compute again
+  uint32_t* redo = reinterpret_cast<uint32_t*>(sp + 64 * L::kP);  // [2] rows that are not finite
+  uint32_t* bad_keys = redo + 2;                                  // [2] keys of a block
   WinJob j;
   if (!window_job<1, BN, PACKED>(p, w, blockIdx.x, j)) return;  // the same for every warp
   const WinTile tile = j.tile[0];
@@ -1013,7 +1093,7 @@ __global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, c
   float* o = static_cast<float*>(p.o) + j.b * p.o_sb + j.h0 * p.o_sh +
              static_cast<int64_t>(j.qt + j.q0) * p.o_st;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  if (threadIdx.x < 2) redo[threadIdx.x] = 0;
+  if (threadIdx.x < 4) redo[threadIdx.x] = 0;  // bad_keys too
 
   // queries: row r is head r / tok, token r % tok
   const int wide_q = vec & kVecQ ? 4 : 1;
@@ -1030,145 +1110,176 @@ __global__ void __launch_bounds__(256) window_f32_kernel(const WindowParams p, c
     copy_tile<DP>(dst, L::kPitch, span.x, span.y, src + at * stride, stride, min(BN, j.lk - at),
                   cols, (vec & kVecKv) != 0);
   };
-  float m[4], l[4], acc[4][NO][4];
-#pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    m[a] = -INFINITY;
-    l[a] = 0.f;
-#pragma unroll
-    for (int c = 0; c < NO; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[a][c][e] = 0.f;
-  }
-  if (j.blocks > 0) load(sk, k, p.k_st, 0, p.d);
-  for (int i = 0; i < j.blocks; ++i) {
-    load(sv, v, p.v_st, i, p.dv);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys
-    __syncthreads();
-    float s[4][NC];
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) s[a][c] = 0.f;
-    // the 32-key columns that some row sees
-    const int2 span = window_span<BN>(j, tile, i);
-    auto scores = [&](auto from, auto to) {
-      constexpr int C0 = decltype(from)::value, C1 = decltype(to)::value;
-#pragma unroll 4
-      for (int d = 0; d < DP; d += 4) {
-        float4 x[4], y[NC];
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-          x[a] = *reinterpret_cast<const float4*>(sq + (ty * 4 + a) * L::kPitch + d);
-#pragma unroll
-        for (int c = C0; c < C1; ++c)
-          y[c] = *reinterpret_cast<const float4*>(sk + (tx + 16 * c) * L::kPitch + d);
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-          for (int c = C0; c < C1; ++c) {
-            s[a][c] = fmaf(x[a].x, y[c].x, s[a][c]);
-            s[a][c] = fmaf(x[a].y, y[c].y, s[a][c]);
-            s[a][c] = fmaf(x[a].z, y[c].z, s[a][c]);
-            s[a][c] = fmaf(x[a].w, y[c].w, s[a][c]);
-          }
-      }
-    };
-    using std::integral_constant;
-    if (BN == 32 || span.y - span.x > 32)
-      scores(integral_constant<int, 0>{}, integral_constant<int, NC>{});
-    else if (span.x == 0)
-      scores(integral_constant<int, 0>{}, integral_constant<int, 2>{});
-    else
-      scores(integral_constant<int, NC - 2>{}, integral_constant<int, NC>{});
-    const int key0 = first_of(i);
+  auto whole_tile = [&](auto turn) {
+    constexpr bool kClean = decltype(turn)::value;
+    float m[4], l[4], acc[4][NO][4];
+    uint32_t dirty = 0;  // bit a: row a of the thread sees a key that was cleaned
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const int r = ty * 4 + a, h = r / w.tok, t = r - h * w.tok, at = tile.pf + t;
-      const bool valid = h < j.nh && t < tile.n;
-      float top = m[a];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int key = key0 + tx + 16 * c;
-        const bool sees = valid && key <= at && (key > at - w.window || key < w.sinks);
-        s[a][c] = sees ? s[a][c] * p.scale : -INFINITY;
-        top = fmaxf(top, s[a][c]);
-      }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float f = expf(m[a] - ref);
-      m[a] = top;
-      float sum = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const float e = expf(s[a][c] - ref);
-        sum += e;
-        sp[r * L::kP + tx + 16 * c] = e;
-      }
-#pragma unroll
-      for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      l[a] = l[a] * f + sum;
+      m[a] = -INFINITY;
+      l[a] = 0.f;
 #pragma unroll
       for (int c = 0; c < NO; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[a][c][e] *= f;
+        for (int e = 0; e < 4; ++e) acc[a][c][e] = 0.f;
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");  // the values
-    __syncthreads();                                       // and nobody needs the keys any more
-    if (i + 1 < j.blocks) load(sk, k, p.k_st, i + 1, p.d);
-#pragma unroll 2
-    for (int n = span.x; n < span.y; n += 4) {
-      float4 x[4];
+    if (j.blocks > 0) load(sk, k, p.k_st, 0, p.d);
+    for (int i = 0; i < j.blocks; ++i) {
+      load(sv, v, p.v_st, i, p.dv);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys
+      __syncthreads();
+      float s[4][NC];
 #pragma unroll
       for (int a = 0; a < 4; ++a)
-        x[a] = *reinterpret_cast<const float4*>(sp + (ty * 4 + a) * L::kP + n);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+        for (int c = 0; c < NC; ++c) s[a][c] = 0.f;
+      // the 32-key columns that some row sees
+      const int2 span = window_span<BN>(j, tile, i);
+      auto scores = [&](auto from, auto to) {
+        constexpr int C0 = decltype(from)::value, C1 = decltype(to)::value;
+#pragma unroll 4
+        for (int d = 0; d < DP; d += 4) {
+          float4 x[4], y[NC];
 #pragma unroll
-        for (int c = 0; c < NO; ++c) {
-          const float4 y =
-              *reinterpret_cast<const float4*>(sv + (n + u) * L::kPitch + c * 64 + tx * 4);
+          for (int a = 0; a < 4; ++a)
+            x[a] = *reinterpret_cast<const float4*>(sq + (ty * 4 + a) * L::kPitch + d);
 #pragma unroll
-          for (int a = 0; a < 4; ++a) {
-            const float e = u == 0 ? x[a].x : u == 1 ? x[a].y : u == 2 ? x[a].z : x[a].w;
-            acc[a][c][0] = fmaf(e, y.x, acc[a][c][0]);
-            acc[a][c][1] = fmaf(e, y.y, acc[a][c][1]);
-            acc[a][c][2] = fmaf(e, y.z, acc[a][c][2]);
-            acc[a][c][3] = fmaf(e, y.w, acc[a][c][3]);
+          for (int c = C0; c < C1; ++c)
+            y[c] = *reinterpret_cast<const float4*>(sk + (tx + 16 * c) * L::kPitch + d);
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int c = C0; c < C1; ++c) {
+              s[a][c] = fmaf(x[a].x, y[c].x, s[a][c]);
+              s[a][c] = fmaf(x[a].y, y[c].y, s[a][c]);
+              s[a][c] = fmaf(x[a].z, y[c].z, s[a][c]);
+              s[a][c] = fmaf(x[a].w, y[c].w, s[a][c]);
+            }
+        }
+      };
+      using std::integral_constant;
+      if (BN == 32 || span.y - span.x > 32)
+        scores(integral_constant<int, 0>{}, integral_constant<int, NC>{});
+      else if (span.x == 0)
+        scores(integral_constant<int, 0>{}, integral_constant<int, 2>{});
+      else
+        scores(integral_constant<int, NC - 2>{}, integral_constant<int, NC>{});
+      const int key0 = first_of(i);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const int r = ty * 4 + a, h = r / w.tok, t = r - h * w.tok, at = tile.pf + t;
+        const bool valid = h < j.nh && t < tile.n;
+        float top = m[a];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int key = key0 + tx + 16 * c;
+          const bool sees = valid && key <= at && (key > at - w.window || key < w.sinks);
+          s[a][c] = sees ? s[a][c] * p.scale : -INFINITY;
+          top = fmaxf(top, s[a][c]);
+        }
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float f = expf(m[a] - ref);
+        m[a] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float e = expf(s[a][c] - ref);
+          sum += e;
+          sp[r * L::kP + tx + 16 * c] = e;
+        }
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        l[a] = l[a] * f + sum;
+#pragma unroll
+        for (int c = 0; c < NO; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[a][c][e] *= f;
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");  // the values
+      __syncthreads();                                       // and nobody needs the keys any more
+      if constexpr (kClean) {
+        // the clean turn, as above: keys whose values are not finite, which rows see them,
+        // and zeros in their place
+        constexpr int kParts = 256 / BN;
+        const int n = threadIdx.x / kParts, part = threadIdx.x % kParts;
+        const bool on = n >= span.x && n < span.y;
+        bool found = false;
+        for (int c = part; on && c < DP; c += kParts) found |= !isfinite(sv[n * L::kPitch + c]);
+        if (found) atomicOr(&bad_keys[n >> 5], 1u << (n & 31));
+        __syncthreads();
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int r = ty * 4 + a, at = tile.pf + r % w.tok;
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c)
+            if (bad_keys[c] & window_sees(w, at, key0 + c * 32)) dirty |= 1u << a;
+        }
+        for (int c = part; on && ((bad_keys[n >> 5] >> (n & 31)) & 1u) && c < DP; c += kParts)
+          sv[n * L::kPitch + c] = 0.f;
+        __syncthreads();
+        if (threadIdx.x < 2) bad_keys[threadIdx.x] = 0;
+      }
+      if (i + 1 < j.blocks) load(sk, k, p.k_st, i + 1, p.d);
+#pragma unroll 2
+      for (int n = span.x; n < span.y; n += 4) {
+        float4 x[4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          x[a] = *reinterpret_cast<const float4*>(sp + (ty * 4 + a) * L::kP + n);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+          for (int c = 0; c < NO; ++c) {
+            const float4 y =
+                *reinterpret_cast<const float4*>(sv + (n + u) * L::kPitch + c * 64 + tx * 4);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+              const float e = u == 0 ? x[a].x : u == 1 ? x[a].y : u == 2 ? x[a].z : x[a].w;
+              acc[a][c][0] = fmaf(e, y.x, acc[a][c][0]);
+              acc[a][c][1] = fmaf(e, y.y, acc[a][c][1]);
+              acc[a][c][2] = fmaf(e, y.z, acc[a][c][2]);
+              acc[a][c][3] = fmaf(e, y.w, acc[a][c][3]);
+            }
           }
         }
       }
+      __syncthreads();  // the values and the weights may be overwritten
     }
-    __syncthreads();  // the values and the weights may be overwritten
-  }
-  asm volatile("cp.async.wait_all;" ::: "memory");  // a job without keys, too
+    asm volatile("cp.async.wait_all;" ::: "memory");  // a job without keys, too
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    const int r = ty * 4 + a, h = r / w.tok, t = r - h * w.tok;
-    if (h >= j.nh || t >= tile.n) continue;
-    float odd = 0.f;
-    float* row = o + h * p.o_sh + t * p.o_st;
+    for (int a = 0; a < 4; ++a) {
+      const int r = ty * 4 + a, h = r / w.tok, t = r - h * w.tok;
+      if (h >= j.nh || t >= tile.n) continue;
+      float odd = 0.f;
+      float* row = o + h * p.o_sh + t * p.o_st;
 #pragma unroll
-    for (int c = 0; c < NO; ++c) {
-      const int col = c * 64 + tx * 4;
-      float y[4];
+      for (int c = 0; c < NO; ++c) {
+        const int col = c * 64 + tx * 4;
+        float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = l[a] == 0.f ? 0.f : acc[a][c][e] / l[a];
-        odd = fmaf(y[e], 0.f, odd);
+        for (int e = 0; e < 4; ++e) {
+          y[e] = l[a] == 0.f ? 0.f : acc[a][c][e] / l[a];
+          odd = fmaf(y[e], 0.f, odd);
+        }
+        if ((vec & kVecO) != 0 && col < p.dv) {
+          *reinterpret_cast<float4*>(row + col) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < p.dv) row[col + e] = y[e];
+        }
       }
-      if ((vec & kVecO) != 0 && col < p.dv) {
-        *reinterpret_cast<float4*>(row + col) = make_float4(y[0], y[1], y[2], y[3]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < p.dv) row[col + e] = y[e];
-      }
+      if (!(odd == 0.f) || ((dirty >> a) & 1u)) atomicOr(&redo[r >> 5], 1u << (r & 31));
     }
-    if (!(odd == 0.f)) atomicOr(&redo[r >> 5], 1u << (r & 31));
-  }
+    __syncthreads();
+  };
+  whole_tile(std::false_type{});
+  if ((redo[0] | redo[1]) == 0u) return;
   __syncthreads();
+  if (threadIdx.x < 2) redo[threadIdx.x] = 0;
+  whole_tile(std::true_type{});
   for (int r = threadIdx.x >> 5; r < 64; r += 8) {
     if (!((redo[r >> 5] >> (r & 31)) & 1u)) continue;
     const int h = r / w.tok, t = r - h * w.tok;
@@ -1272,7 +1383,8 @@ int launch_tc(const bio::WindowParams& p, const bio_attn_args* a, cudaStream_t s
   auto keys_map = [&](CUtensorMap* map, const void* x, int64_t cols, int64_t st, int64_t sh,
                       int64_t sb) {
     return p.lk == 0 ? bio_host::map_of<T>(map, p.q, p.d, 1, 1, 1, 0, 0, 0, L::BN)
-                     : bio_host::map_of<T>(map, x, cols, p.lk, a->kv_heads, batch, st, sh, sb, L::BN);
+                     : bio_host::map_of<T>(map, x, cols, p.lk, a->kv_heads, batch, st, sh, sb,
+                                           L::BN);
   };
   if (!bio_host::map_of<T>(&q, p.q, p.d, p.lq, p.heads, batch, p.q_st, p.q_sh, p.q_sb, w.tok,
                            w.gh) ||
@@ -1288,7 +1400,9 @@ template <typename T>
 int launch_half(const bio::WindowParams& p, const bio_attn_args* a, bool packed, cudaStream_t s) {
   // the stride of a dimension of one element is never used
   const int64_t batch = packed ? 1 : p.batch;
-  auto used = [](int64_t n, int64_t stride) { return 2 * static_cast<uint64_t>(n > 1 ? stride : 0); };
+  auto used = [](int64_t n, int64_t stride) {
+    return 2 * static_cast<uint64_t>(n > 1 ? stride : 0);
+  };
   uint64_t bits = reinterpret_cast<uint64_t>(p.q) | used(batch, p.q_sb) | used(p.heads, p.q_sh) |
                   used(p.lq, p.q_st);
   if (p.lk > 0)

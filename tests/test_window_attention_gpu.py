@@ -353,3 +353,65 @@ def test_rows_computed_again_hold_nobody_up():
     # a mean of so many values is small beside them: within the weights' rounding of |v| <= 6
     err = (out[:, :32, :, rest].double() - clean[:, :32, :, rest].double()).abs().max().item()
     assert err <= 2 * 6 * (4 * UNIT[dtype] + 2.0**-24 * (2 * 64 * 50 + 2 * n + 8))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", (64, 128, 256, 72))
+@pytest.mark.parametrize("window,sinks", [(1, 0), (100, 0), (128, 4), (300, 140), (5000, 0)])
+@pytest.mark.parametrize("bads", [(333,), (0, 2, 128, 255, 256, 511), (699,),
+                                  tuple(range(40, 60)) + tuple(range(300, 460))])
+def test_hidden_values_do_not_change_a_bit(bads, window, sinks, d, dtype):
+    """Keys with infinities and NaN: rows that see none of them have the bits that
+    they have beside finite values, whole, in chunks and packed; rows that see one
+    show it where the oracle does."""
+    n = 700
+    q, k, v = make(1, 6, 2, n, n, d, dtype=dtype, seed=window + d)
+    clean = bio.sliding_window_attention_batch_invariant(q, k, v, window, sinks)
+    k, v = k.clone(), v.clone()
+    for x, bad in enumerate(bads):
+        v[:, x % 2, bad, (5 * x) % d] = (float("nan"), float("inf"), -float("inf"))[x % 3]
+        if x % 4 == 3:  # a NaN score, too
+            k[:, x % 2, bad, 0] = float("nan")
+    i, at = torch.arange(n, device="cuda")[:, None], torch.tensor(bads, device="cuda")
+    sees = (i >= at) & ((i < at + window) | (at < sinks))
+    head = torch.arange(len(bads), device="cuda") % 2
+    out = bio.sliding_window_attention_batch_invariant(q, k, v, window, sinks)
+    for hk in range(2):
+        hidden = ~sees[:, head == hk].any(1)
+        mine = slice(3 * hk, 3 * hk + 3)
+        assert torch.equal(out[0, mine][:, hidden], clean[0, mine][:, hidden])
+    ref = bio_oracle.window_attention(q, k, v, window, sinks)
+    got = out.double().cpu()
+    finite = torch.isfinite(ref)
+    assert torch.equal(torch.isfinite(got), finite)
+    assert torch.equal(got[~finite].nan_to_num(7.0), ref[~finite].nan_to_num(7.0))
+    assert (got[finite] - ref[finite]).abs().max().item() <= bound_of(q, k, v)
+    for a, b in [(0, 1), (1, 129), (129, 350), (350, n)]:
+        part = bio.sliding_window_attention_batch_invariant(
+            q[:, :, a:b], k[:, :, :b], v[:, :, :b], window, sinks)
+        assert torch.equal(part.nan_to_num(7.0), out[:, :, a:b].nan_to_num(7.0)), (a, b)
+    cu = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 60, 60 + n],
+                                                                      [0, 60, 60 + n])]
+    packed = bio.varlen_sliding_window_attention_batch_invariant(
+        *(torch.cat([t[:, :, :60], t], 2).transpose(1, 2) for t in (q, k, v)), *cu, window, sinks)
+    want = torch.cat([out[:, :, :60], out], 2).transpose(1, 2)
+    assert torch.equal(packed.nan_to_num(7.0), want.nan_to_num(7.0))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_hidden_values_beside_many_other_tiles(dtype):
+    """Blocks that go through several tiles again, one of them with a NaN."""
+    q, k, v = make(90, 4, 2, 300, 400, 128, dtype=dtype, seed=2)
+    clean = bio.sliding_window_attention_batch_invariant(q, k, v, 130, 4)
+    v = v.clone()
+    v[7, 1, 350] = float("nan")
+    v[50, 0, 9] = float("inf")
+    out = bio.sliding_window_attention_batch_invariant(q, k, v, 130, 4)
+    i = torch.arange(300, device="cuda") + 100
+    keep = torch.ones(90, 4, 300, dtype=torch.bool, device="cuda")
+    keep[7, 2:] = ~((i >= 350) & (i < 480))
+    keep[50, :2] = ~((i >= 9) & (i < 139))
+    assert torch.equal(out[keep], clean[keep])
+    assert not torch.isfinite(out[~keep]).any()
+    assert _lib.device_status() == 0
