@@ -366,3 +366,22 @@ def test_lengths_up_to_the_last_position(page, dtype):
             mine[t // page, :, t % page] = theirs[p, :, s]
         check(out, (q, *own, torch.arange(short, dtype=torch.int32, device="cuda")[None],
                     torch.tensor([keys.numel()], dtype=torch.int32, device="cuda")))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (4, 1, 256)])
+def test_more_rows_than_a_block_lists(heads, kv_heads, d, dtype):
+    """700 rows under a wide table: the pieces that rows lack are passed over, and a
+    row has the bits that it has among a few."""
+    gen = torch.Generator().manual_seed(d)
+    lens = torch.randint(0, 300, (700,), generator=gen)
+    lens[torch.tensor([5, 80, 444, 699])] = torch.tensor([9000, 1100, 0, 2500])
+    q, kp, vp, table, ln = make(lens.tolist(), heads, kv_heads, d, dtype=dtype, seed=d, width=640)
+    out = bio.paged_attention_decode_batch_invariant(q, kp, vp, table, ln, window=6000, sinks=3)
+    for some in (torch.arange(0, 12), torch.tensor([80, 444, 511, 512, 513, 698, 699])):
+        at = some.to(torch.int32).cuda()
+        few = bio.paged_attention_decode_batch_invariant(
+            q[some.cuda()], kp, vp, table, ln, rows=at, window=6000, sinks=3)
+        assert torch.equal(few, out[some.cuda()])
+        check(few, (q[some.cuda()], kp, vp, table, ln), 6000, 3, rows=at)
+    assert _lib.device_status() == 0
