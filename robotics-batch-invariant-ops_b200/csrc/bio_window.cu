@@ -143,8 +143,12 @@ __device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb,
 //
 // Scores, maxima and sums are fp32 in registers (128 scores a thread).  The
 // reference m of the exponentials moves only when a block's maximum exceeds it
-// by more than 8 (log2), so O is rarely rescaled and P stays below 2^8; P is
-// rounded to the operand type, as the product needs, l sums it unrounded.
+// by more than 8 (log2), so O is rarely rescaled and P stays below 2^8.  P is
+// rounded to the operand type, as the product needs; l sums it unrounded, since the
+// rounded values would have to be unpacked again: 95 instead of 86 us (512 tokens
+// behind 4096, D 64) and 827 instead of 771 us (the case above), for an error that
+// is 1 % smaller (bf16, 1500 tokens, window 1024: 2.05e-3 instead of 2.07e-3 of the
+// output's norm, 1.61e-3 of it the rounding of the output).
 //
 // A hidden key in a visited block has weight 0, but 0 * Inf or 0 * NaN in V
 // would still reach the row.  A block whose rows all came out finite is done.  One
