@@ -232,6 +232,7 @@ def _window_operand(t, lead):
 
 
 def geometry(t: torch.Tensor) -> tuple:
+    """What plans are looked up by: nothing of an address or of what `t` holds."""
     return t.shape, t.stride(), t.dtype, t.get_device()
 
 

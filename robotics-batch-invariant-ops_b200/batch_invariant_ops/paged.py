@@ -33,6 +33,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, tracing
+from ._attn import geometry as _geo
 
 MAX_HEAD_DIM = 256
 
@@ -62,11 +63,6 @@ class _Geometry(NamedTuple):
     def contiguous(self) -> bool:
         """For one dimension."""
         return self.shape[0] < 2 or self.stride[0] == 1
-
-
-def _geo(t: torch.Tensor) -> tuple:
-    """A tensor's ``_Geometry`` as the plain tuple that plans are looked up by."""
-    return t.shape, t.stride(), t.dtype, t.get_device()
 
 
 def _geometries(*geos) -> list:

@@ -35,7 +35,7 @@ struct PagedParams {
   int max_len;         // tokens that a row may have: its columns', below 2^31 by two tiles
   int box_rows;        // tokens of a TMA box: gcd(page size, tile)
   int group_shift;     // log2 of the boxes along a tile
-  unsigned page_mul, page_shift;  // position / page size = (mulhi(position, mul) + position) >> shift
+  FixedDiv by_page;    // position -> column of the table
   float scale_log2;
   int64_t max_pieces;  // most pieces that any row can have
   int least;           // tiles of a piece at least: 1, or kSimtTiles
@@ -58,11 +58,6 @@ __host__ __device__ __forceinline__ int piece_tiles(int n, int least) {
 __host__ __device__ __forceinline__ int pieces_of(int tiles, int least) {
   const int c = piece_tiles(tiles, least);
   return (tiles + c - 1) / c;
-}
-
-__device__ __forceinline__ int page_of(const PagedParams& p, int pos) {
-  return static_cast<int>((__umulhi(static_cast<unsigned>(pos), p.page_mul) +
-                           static_cast<unsigned>(pos)) >> p.page_shift);
 }
 
 // What a row sees: token j with j < len and (j < sinks or j >= start).  Tile t
@@ -204,7 +199,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Paged
     if (x0 >= left) return w;
     const int x1 = x0 + sub;  // kKeys divides the tile: all of them lie in one
     const int pos = z.base(t0 + x1 / kTile) + x1 % kTile;
-    const int col = page_of(p, pos);
+    const int col = p.by_page.quotient(pos);
     w.on = z.sees(pos);
     if (w.on) w.page = p.table[z.row * p.t_sr + col];
     w.slot = pos - col * p.page_size;
@@ -568,7 +563,7 @@ __global__ void __launch_bounds__(PagedSmem<DP, NH>::kWarps * 32, 1)
       // visible in [pos, pos + box_rows): before the sinks' end, or from start to the length
       in_held = pos < in.z.sinks || (pos < in.z.len && pos + p.box_rows > in.z.start);
       if (in_held) {
-        const int col = page_of(p, pos);
+        const int col = p.by_page.quotient(pos);
         in_slot = pos - col * p.page_size;
         // not looked at before the next fetch, so that nobody waits for it here
         in_page = p.table[in.z.row * p.t_sr + col];
@@ -1146,12 +1141,7 @@ int bio_paged_attention(const bio_paged_attn_args* a, void* workspace, int64_t w
   p.box_rows = std::gcd(p.page_size, bio::kTile);
   p.group_shift = 0;
   while ((p.box_rows << p.group_shift) < bio::kTile) ++p.group_shift;
-  // Division of a position (below 2^31) by the page size n with 2^(s-1) < n <= 2^s:
-  // floor(2^32 (2^s - n) / n) + 1 is the 33-bit reciprocal's low word.
-  p.page_shift = 0;
-  while ((1u << p.page_shift) < static_cast<unsigned>(p.page_size)) ++p.page_shift;
-  p.page_mul = static_cast<unsigned>(((1ull << 32) * ((1ull << p.page_shift) - p.page_size)) /
-                                     p.page_size + 1);
+  p.by_page = bio::fixed_div(p.page_size);
   p.max_pieces = s.pieces;
   p.dvp = s.dvp;
   p.acc = static_cast<float*>(workspace);

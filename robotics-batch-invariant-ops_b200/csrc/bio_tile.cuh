@@ -78,7 +78,9 @@ __device__ __forceinline__ bool parked_wait(uint32_t a, uint32_t parity,
 }
 
 // Division of 0 <= x < 2^31 by a fixed n >= 1: (mulhi(x, mul) + x) >> shift with
-// 2^(shift-1) < n <= 2^shift and mul = floor(2^32 (2^shift - n) / n) + 1.
+// 2^(shift-1) < n <= 2^shift and mul = floor(2^32 (2^shift - n) / n) + 1
+// (Granlund and Montgomery, "Division by invariant integers using multiplication",
+// 1994).
 struct FixedDiv {
   unsigned mul, shift, n;
   __device__ __forceinline__ int quotient(int x) const {
