@@ -143,7 +143,9 @@ __device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb,
 //
 // Scores, maxima and sums are fp32 in registers (128 scores a thread).  The
 // reference m of the exponentials moves only when a block's maximum exceeds it
-// by more than 8 (log2), so O is rarely rescaled and P stays below 2^8.  P is
+// by more than 8 (log2), so O is rarely rescaled and P stays below 2^8.  In fp16 P
+// is kept 2^7 times larger (below 2^15): weights under 2^-25 of the largest would be
+// rounded to nothing, and some 100000 of them are worth more than a rounding.  P is
 // rounded to the operand type, as the product needs; l sums it unrounded, since the
 // rounded values would have to be unpacked again: 95 instead of 86 us (512 tokens
 // behind 4096, D 64) and 827 instead of 771 us (the case above), for an error that
@@ -494,6 +496,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
   using L = WinSmem<DP>;
   constexpr int NT = L::NT, BN = L::BN, NS = L::kSlots, NC = BN / 32;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+  constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;  // log2
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -852,7 +855,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
             }
           }
           first = false;
-          const float ref = m == -INFINITY ? 0.f : m;
+          const float ref = m == -INFINITY ? 0.f : m - kLift;
           const uint64_t ref2 = pair_of(-ref, -ref);
           uint64_t sum2 = 0, sum3 = 0;
 #pragma unroll

@@ -415,3 +415,19 @@ def test_hidden_values_beside_many_other_tiles(dtype):
     assert torch.equal(out[keep], clean[keep])
     assert not torch.isfinite(out[~keep]).any()
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_small_weights_beside_a_large_one(dtype):
+    """A sink that outweighs every other key by 2^25, and 300000 other keys that
+    together weigh 0.6 % of it: none of them may be rounded away."""
+    n, d = 300000, 64
+    q, k, v = (torch.zeros(1, 1, x, d, dtype=dtype, device="cuda") for x in (3, n, n))
+    q[..., 0], k[:, :, 0, 0], v[:, :, 1:] = 1, 17.75, 1
+    out = bio.sliding_window_attention_batch_invariant(q, k, v, n, 0, scale=1.0)
+    rest = torch.arange(n - 3, n, dtype=torch.float64)  # keys beside the sink
+    ref = rest / (rest + torch.tensor(17.75, dtype=torch.float64).exp())
+    # relative to their own sum: weights and output rounded (4 u), an fp16 weight of
+    # 2^-18.6 kept to half of 2^-24 (2^-6), 18750 sums of 16 keys (2^-9)
+    err = ((out.double().cpu() - ref[None, None, :, None]) / ref.max()).abs().max().item()
+    assert err <= 4 * UNIT[dtype] + 2.0**-6 + 2.0**-9
