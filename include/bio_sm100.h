@@ -518,8 +518,11 @@ typedef struct bio_paged_attn_args {
 } bio_paged_attn_args;
 
 /* Workspace bytes that bio_paged_attention needs for these sizes (pure; the
- * pointers are not looked at).  The workspace is 16-byte aligned device
- * memory; it may be NULL when 0 bytes are needed. */
+ * pointers are not looked at).  It grows with batch * heads and the pieces that
+ * a row of table_width pages (or of the window) can have, whatever the lengths
+ * are: a table of fewer columns, t_sr as before, needs less and gives the same
+ * bits.  The workspace is 16-byte aligned device memory; it may be NULL when 0
+ * bytes are needed. */
 BIO_API int64_t bio_paged_attention_workspace(const bio_paged_attn_args* args);
 BIO_API int bio_paged_attention(const bio_paged_attn_args* args, void* workspace,
                                 int64_t workspace_bytes, void* stream);

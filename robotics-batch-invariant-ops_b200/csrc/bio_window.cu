@@ -126,7 +126,7 @@ __device__ __noinline__ void window_row(const T* qrow, const T* kb, const T* vb,
 // nobody has to wait, so barriers that are due together are looked at together
 // (one per lane), and a TMA box about 50, so blocks are loaded whole.
 //
-// Measured, 32768 tokens, 32 heads on 8, D 128, window 1024: 775 us, 700 TFLOP/s
+// Measured, 32768 tokens, 32 heads on 8, D 128, window 1024: 770 us, 705 TFLOP/s
 // of visible products; window 16384 runs at 1050, so the two blocks that a window
 // cuts, the sinks' block, refill and output cost a job about 10 of its 28 us.
 // Steps: one thread issuing everything in a divergent branch 1073 us, an elected
@@ -1028,7 +1028,7 @@ __global__ void __launch_bounds__(WinSmem<DP>::kThreads, 1)
 // products per 8 loads of 16 bytes in S, 128 per 12 in PV.  Columns that no row of
 // the tile sees are skipped 32 at a time.  A tile with a row that is not finite is
 // gone through once more with such values zeroed, as above.
-// Measured: 94 us for 1024 queries, 8 heads over 2 of 128, window 512 (17 TFLOP/s;
+// Measured: 99 us for 1024 queries, 8 heads over 2 of 128, window 512 (16 TFLOP/s;
 // one warp per row, with K read from L2 for every row, ran at 1).  A window of 31
 // keys (4 x 10198 queries, 8 heads of 128) wastes most of its blocks: 1074 us, and
 // 1609 with whole blocks and with queries and outputs moved by words.
